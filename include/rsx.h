@@ -31,6 +31,10 @@ extern "C" {
 #define RSX_ABI_VERSION 8
 
 #define RSX_OK 0
+/* element types of the calls that take more than fp32 */
+#define RSX_F32 0
+#define RSX_BF16 1
+
 #define RSX_E_INVALID (-1)   /* bad argument (null pointer, unsupported d, K ...) */
 #define RSX_E_HIP (-2)       /* a HIP runtime call failed                         */
 #define RSX_E_WORKSPACE (-3) /* caller-provided workspace too small               */
@@ -199,6 +203,25 @@ int rsx_bpr_grad(const float *P, const float *Q, float *GP, float *GQ, int64_t n
                  int64_t batch, int d, float inv_batch, float *loss_acc, rsx_stream_t stream);
 int rsx_adam_apply(float *W, float *M, float *V, float *G, int64_t n, double lr, double beta1,
                    double beta2, double eps, int64_t t, rsx_stream_t stream);
+
+/* ---- orthogonalised updates ---------------------------------------------------------------
+ * rsx_orthogonalize: Newton-Schulz iteration of X [rows x d] towards its nearest matrix with orthonormal columns,
+ *   X_0 = X / (|X|_F + eps);   X_{k+1} = a X_k + X_k (b A_k + c A_k^2),  A_k = X_k^T X_k,   out = X_steps.
+ *   dtype RSX_F32 or RSX_BF16 (of X and out; the Gram matrix and everything [d x d] is held in 64 bits, the last product in
+ *   fp32).  out may be X.  steps in [0, 32].  An all-zero X gives zeros where eps > 0.  Bit-reproducible.
+ *   A column of zeros stays one (padded widths).
+ * rsx_muon_apply: the optimizer step built on it, beside rsx_adam_apply and in its manner (one call per table and step, G = 0 after it):
+ *   M = momentum M + G;  U = nesterov ? G + momentum M : M;
+ *   W = (1 - lr weight_decay) W - lr update_scale orthogonalize(U);   G = 0
+ *   W, M fp32; G of g_dtype.  update_scale is the caller's, sqrt(max(1, rows / width)) by custom.
+ * ws: rsx_orthogonalize_workspace(rows, d) bytes of scratch, contents irrelevant, one per concurrent call.  Rows 16-byte aligned.
+ * No host synchronisation: the calls can be captured into a graph.                                                              */
+int64_t rsx_orthogonalize_workspace(int64_t rows, int d);
+int rsx_orthogonalize(const void *X, void *out, int64_t rows, int d, int dtype, int steps, double a, double b, double c,
+                      double eps, void *ws, int64_t ws_bytes, rsx_stream_t stream);
+int rsx_muon_apply(float *W, float *M, void *G, int64_t rows, int d, int g_dtype, double lr, double momentum, int nesterov,
+                   int steps, double a, double b, double c, double eps, double weight_decay, double update_scale, void *ws,
+                   int64_t ws_bytes, rsx_stream_t stream);
 
 /* rsx_pointwise_grad: the POINTWISE branch of the reference model (models/MF.py:99-102 with hparams['pointwise'] = True;
  * "widening" row beyond SURVEY section 8f).  Batch of n (user, item, rating) entries -- users and items repeat, as in the

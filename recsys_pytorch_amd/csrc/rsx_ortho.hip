@@ -1,0 +1,631 @@
+// rsx_ortho.hip -- Newton-Schulz orthogonalisation of a tall [rows x d] matrix and the optimizer step built on it, for gfx950 (MI355X).
+//
+//   X_0 = X / (|X|_F + eps);   X_{k+1} = a X_k + X_k (b A_k + c A_k^2),   A_k = X_k^T X_k          (`steps` times)
+//
+// Every X_k is X times a polynomial of G = X^T X, so only the first Gram matrix and the last product touch the rows:
+//   with s = 1 / (|X|_F + eps), A_0 = s^2 G, M_0 = s I:   T = a I + b A + c A^2,   M <- M T,   A <- T A T = (A T) T,   X_steps = X M.
+// All these matrices are symmetric and commute.  |X|_F^2 is the trace of G: it costs no pass of its own.
+//
+// The [d x d] part is held in 64 bits.  A step amplifies A's small eigenvalues by a^2 (about 12): noise of 2^-24 |A| in G would have
+// grown to 12^4 * 6e-8 = 1e-3 by the fifth step, and decide the small directions of X.  v_mfma_f64_16x16x4_f64 does the products.
+//
+// Four launches of row work and [d x d] work:
+//   gram_kernel    rows -> partial Gram matrices (upper triangle of 16 x 16 blocks), with the momentum update of the optimizer step
+//   gram_reduce    partials in a fixed order -> G
+//   ns_*           the iteration in [d x d]
+//   project_kernel rows times M (fp32 MFMA), with the weight update of the optimizer step
+#include "rsx_common.h"
+
+namespace {
+
+typedef double f64x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int kGramWaves = 4;
+
+__device__ __forceinline__ float bf16_f32(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
+// round to nearest even; NaN stays NaN
+__device__ __forceinline__ uint16_t f32_bf16(float v)
+{
+    const uint32_t u = __float_as_uint(v);
+    if ((u & 0x7FFFFFFFu) > 0x7F800000u) return (uint16_t)((u >> 16) | 0x40u);
+    return (uint16_t)((u + 0x7FFFu + ((u >> 16) & 1u)) >> 16);
+}
+
+// four consecutive elements of a row, in fp32
+template <typename T>
+__device__ __forceinline__ float4 load4(const T *p);
+template <>
+__device__ __forceinline__ float4 load4<float>(const float *p) { return *reinterpret_cast<const float4 *>(p); }
+template <>
+__device__ __forceinline__ float4 load4<uint16_t>(const uint16_t *p)
+{
+    const ushort4 h = *reinterpret_cast<const ushort4 *>(p);
+    return make_float4(bf16_f32(h.x), bf16_f32(h.y), bf16_f32(h.z), bf16_f32(h.w));
+}
+
+// what is orthogonalised: X itself, or the optimizer's momentum (M <- mu M + G, U = G + mu M or M)
+template <typename T, bool MUON>
+struct Rows {
+    const T *X;       // X, or the gradient G
+    float *M;         // MUON: the momentum
+    float mu;
+    int nesterov;
+    // UPDATE: this is the pass that advances M (it reads the old one and stores the new one)
+    template <bool UPDATE>
+    __device__ __forceinline__ float4 get(int64_t at) const
+    {
+        float4 g = load4<T>(X + at);
+        if constexpr (MUON) {
+            float4 m = *reinterpret_cast<const float4 *>(M + at);
+            if constexpr (UPDATE) {
+                m = make_float4(fmaf(mu, m.x, g.x), fmaf(mu, m.y, g.y), fmaf(mu, m.z, g.z), fmaf(mu, m.w, g.w));
+                *reinterpret_cast<float4 *>(M + at) = m;
+            }
+            if (!nesterov) return m;
+            g = make_float4(fmaf(mu, m.x, g.x), fmaf(mu, m.y, g.y), fmaf(mu, m.z, g.z), fmaf(mu, m.w, g.w));
+        }
+        return g;
+    }
+};
+
+// ---- the Gram matrix -------------------------------------------------------------------------------------------------------------
+// Column groups of 16: group b = 4 q + j of a row holds the columns 64 q + 4 m + j, m = 0..15 (d = 32: 8-lane halves, see below) -- what
+// one float4 load per lane and 64 columns delivers, without a transpose.  group_col maps (group, m) back to the column.
+__host__ __device__ constexpr int n_groups(int D) { return D / 16; }
+__device__ __forceinline__ int group_col(int D, int b, int m) { return D == 32 ? 4 * (m & 7) + 2 * (m >> 3) + b : 64 * (b >> 2) + 4 * m + (b & 3); }
+__host__ __device__ constexpr int n_blocks(int D) { return n_groups(D) * (n_groups(D) + 1) / 2; }
+__host__ __device__ constexpr int block_at(int D, int p, int q) { return p * n_groups(D) - p * (p - 1) / 2 + (q - p); }   // q >= p
+
+// one wavefront, rows r0 + (lane >> 4), all blocks: D <= 128 (36 blocks of 8 registers at D = 128, one wavefront per SIMD).
+// Bound by the fp64 matrix rate: 36 instructions of 64 cycles per four rows.  Row loads of the next four rows fly under them.
+template <int D, typename T, bool MUON>
+__global__ __launch_bounds__(64 * kGramWaves, 1) void gram_kernel(Rows<T, MUON> in, int64_t rows, double *__restrict__ part)
+{
+    constexpr int NG = n_groups(D), NB = n_blocks(D), NQ = D < 64 ? 1 : D / 64;
+    constexpr int RPI = D == 32 ? 8 : 4;            // rows a wavefront's load instruction covers (D = 32: 8 lanes of float4 a row)
+    __shared__ __attribute__((aligned(16))) double red[NB * 256];
+    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+    f64x4 acc[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) acc[b] = f64x4{0.0, 0.0, 0.0, 0.0};
+    const int64_t stride = (int64_t)gridDim.x * kGramWaves * RPI;
+    const int64_t first = ((int64_t)blockIdx.x * kGramWaves + wid) * RPI;
+    const int lrow = D == 32 ? lane >> 3 : lane >> 4, lcol = D == 32 ? 4 * (lane & 7) : 4 * (lane & 15);
+    float4 nxt[NQ];
+    auto fetch = [&](int64_t r0) {
+        const int64_t r = r0 + lrow;
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
+            nxt[q] = r < rows ? in.template get<true>(r * D + 64 * q + lcol) : make_float4(0.f, 0.f, 0.f, 0.f);
+    };
+    if (first < rows) fetch(first);
+    for (int64_t r0 = first; r0 < rows; r0 += stride) {
+        float4 cur[NQ];
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) cur[q] = nxt[q];
+        if (r0 + stride < rows) fetch(r0 + stride);
+        if constexpr (D == 32) {
+            // lane l holds columns 4 (l & 7) .. + 3 of row l >> 3.  The instruction wants 16 columns of four rows: lane l of the fragment is
+            // (m = l & 15, k = l >> 4) -> row k (then k + 4) is lanes 8 k .., column pair by m >> 3.
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int src = 8 * ((lane >> 4) + 4 * h) + (lane & 7);
+                const bool up = (lane >> 3) & 1;
+                const float x0 = __shfl(cur[0].x, src, 64), x1 = __shfl(cur[0].y, src, 64), x2 = __shfl(cur[0].z, src, 64), x3 = __shfl(cur[0].w, src, 64);
+                const double v[2] = {(double)(up ? x2 : x0), (double)(up ? x3 : x1)};
+#pragma unroll
+                for (int p = 0; p < NG; ++p)
+#pragma unroll
+                    for (int q = p; q < NG; ++q)
+                        acc[block_at(D, p, q)] = __builtin_amdgcn_mfma_f64_16x16x4f64(v[p], v[q], acc[block_at(D, p, q)], 0, 0, 0);
+            }
+        } else {
+            double v[NG];
+#pragma unroll
+            for (int q = 0; q < NQ; ++q) { v[4 * q] = cur[q].x; v[4 * q + 1] = cur[q].y; v[4 * q + 2] = cur[q].z; v[4 * q + 3] = cur[q].w; }
+#pragma unroll
+            for (int p = 0; p < NG; ++p)
+#pragma unroll
+                for (int q = p; q < NG; ++q)
+                    acc[block_at(D, p, q)] = __builtin_amdgcn_mfma_f64_16x16x4f64(v[p], v[q], acc[block_at(D, p, q)], 0, 0, 0);
+        }
+    }
+    // the four wavefronts' sums, one after the other (a fixed order), then the workgroup's partial
+    // (f64 result layout: register pair i of lane l is row 4 i + (l >> 4), column l & 15)
+    for (int w = 0; w < kGramWaves; ++w) {
+        if (wid == w) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    double *cell = red + b * 256 + (4 * i + (lane >> 4)) * 16 + (lane & 15);
+                    *cell = w == 0 ? acc[b][i] : *cell + acc[b][i];
+                }
+        }
+        __syncthreads();
+    }
+    double *dst = part + (size_t)blockIdx.x * (NB * 256);
+    for (int t = threadIdx.x; t < NB * 256; t += 64 * kGramWaves) dst[t] = red[t];
+}
+
+// D = 256: 136 blocks are four wavefronts' registers.  The workgroup stages 16 rows in LDS; wavefronts 0..2 take two 64 x 64 squares off
+// the diagonal each (32 blocks), wavefront 3 the four on it (40 blocks).
+template <int JOB, typename F>
+__device__ __forceinline__ void gram256_blocks(F f)     // f(index of the accumulator, column group p, column group q)
+{
+    constexpr int sq[3][2][2] = {{{0, 1}, {0, 2}}, {{0, 3}, {1, 3}}, {{1, 2}, {2, 3}}};
+    if constexpr (JOB < 3) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) f(s * 16 + i * 4 + j, 4 * sq[JOB][s][0] + i, 4 * sq[JOB][s][1] + j);
+    } else {
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            int n = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = i; j < 4; ++j) f(s * 10 + n++, 4 * s + i, 4 * s + j);
+        }
+    }
+}
+
+constexpr int kG256Rows = 16;
+
+template <int JOB, typename T, bool MUON>
+__device__ __forceinline__ void gram256_body(const Rows<T, MUON> &in, int64_t rows, double *__restrict__ part, float (*tile)[kG256Rows * 256])
+{
+    constexpr int NA = JOB < 3 ? 32 : 40;
+    const int tid = threadIdx.x, lane = tid & 63;
+    f64x4 acc[NA];
+#pragma unroll
+    for (int b = 0; b < NA; ++b) acc[b] = f64x4{0.0, 0.0, 0.0, 0.0};
+    const int64_t stride = (int64_t)gridDim.x * kG256Rows, first = (int64_t)blockIdx.x * kG256Rows;
+    float4 nxt[4];
+    auto fetch = [&](int64_t r0) {
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            const int64_t r = r0 + 4 * n + (tid >> 6);
+            nxt[n] = r < rows ? in.template get<true>(r * 256 + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+    };
+    if (first < rows) fetch(first);
+    int par = 0;
+    for (int64_t r0 = first; r0 < rows; r0 += stride, par ^= 1) {
+        float *t = tile[par];               // (two tiles: a slow wavefront still reads the last one while this one is filled)
+#pragma unroll
+        for (int n = 0; n < 4; ++n) *reinterpret_cast<float4 *>(t + (4 * n + (tid >> 6)) * 256 + 4 * lane) = nxt[n];
+        __syncthreads();
+        if (r0 + stride < rows) fetch(r0 + stride);
+#pragma unroll 1
+        for (int k = 0; k < kG256Rows; k += 4) {
+            double v[16];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const float4 x = *reinterpret_cast<const float4 *>(t + (k + (lane >> 4)) * 256 + 64 * q + 4 * (lane & 15));
+                v[4 * q] = x.x; v[4 * q + 1] = x.y; v[4 * q + 2] = x.z; v[4 * q + 3] = x.w;
+            }
+            gram256_blocks<JOB>([&](int a, int p, int q) { acc[a] = __builtin_amdgcn_mfma_f64_16x16x4f64(v[p], v[q], acc[a], 0, 0, 0); });
+        }
+    }
+    double *dst = part + (size_t)blockIdx.x * (n_blocks(256) * 256);
+    gram256_blocks<JOB>([&](int a, int p, int q) {
+        double *blk = dst + (size_t)block_at(256, p, q) * 256;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) blk[(4 * i + (lane >> 4)) * 16 + (lane & 15)] = acc[a][i];
+    });
+}
+
+template <typename T, bool MUON>
+__global__ __launch_bounds__(256, 1) void gram256_kernel(Rows<T, MUON> in, int64_t rows, double *__restrict__ part)
+{
+    __shared__ __attribute__((aligned(16))) float tile[2][kG256Rows * 256];
+    switch (__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) {      // (every wavefront runs the same number of rounds and barriers)
+    case 0: gram256_body<0, T, MUON>(in, rows, part, tile); break;
+    case 1: gram256_body<1, T, MUON>(in, rows, part, tile); break;
+    case 2: gram256_body<2, T, MUON>(in, rows, part, tile); break;
+    default: gram256_body<3, T, MUON>(in, rows, part, tile); break;
+    }
+}
+
+// partials -> the full symmetric matrix in column order.  16 elements x 16 slices of the partials per workgroup.
+template <int D>
+__global__ __launch_bounds__(256) void gram_reduce_kernel(const double *__restrict__ part, int n_part, double *__restrict__ G)
+{
+    constexpr int NB = n_blocks(D);
+    __shared__ double s[16][17];
+    const int e = threadIdx.x & 15, sl = threadIdx.x >> 4;
+    const int at = blockIdx.x * 16 + e;                       // element of [NB][16][16]
+    double sum = 0.0;
+    for (int p = sl; p < n_part; p += 16) sum += part[(size_t)p * (NB * 256) + at];
+    s[sl][e] = sum;
+    __syncthreads();
+    if (sl == 0) {
+        double v = 0.0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v += s[i][e];
+        const int blk = at >> 8;
+        int p = 0;
+        while (p + 1 < n_groups(D) && block_at(D, p + 1, p + 1) <= blk) ++p;
+        const int q = p + blk - block_at(D, p, p);
+        const int r = group_col(D, p, (at >> 4) & 15), c = group_col(D, q, at & 15);
+        G[(size_t)r * D + c] = v;
+        G[(size_t)c * D + r] = v;
+    }
+}
+
+// ---- the iteration in [d x d] ------------------------------------------------------------------------------------------------------
+struct Coeffs { double a, b, c, eps; };
+
+// 1 / (|X|_F + eps): every workgroup sums the diagonal in the same order
+__device__ __forceinline__ double norm_scale(const double *G, int D, double eps, double *lds)
+{
+    if (threadIdx.x < 64) {
+        double t = 0.0;
+        for (int i = threadIdx.x; i < D; i += 64) t += G[(size_t)i * D + i];
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o, 64);
+        if (threadIdx.x == 0) *lds = 1.0 / (sqrt(t) + eps);
+    }
+    __syncthreads();
+    return *lds;
+}
+
+// one 16 x 16 block of X Y (both symmetric): four wavefronts share the contraction.  Operands are read as rows k, columns of the block.
+template <int D, typename FX, typename FY>
+__device__ __forceinline__ double ns_block(FX fx, FY fy, int p, int q, double (*red)[64][4])
+{
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    constexpr int KS = D / 16;
+    double x[KS], y[KS];
+#pragma unroll
+    for (int i = 0; i < KS; ++i) {
+        const int k = w * (D / 4) + 4 * i + (lane >> 4);
+        x[i] = fx(k, 16 * p + (lane & 15));
+        y[i] = fy(k, 16 * q + (lane & 15));
+    }
+    f64x4 acc = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+    for (int i = 0; i < KS; ++i) acc = __builtin_amdgcn_mfma_f64_16x16x4f64(x[i], y[i], acc, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) red[w][lane][i] = acc[i];
+    __syncthreads();
+    const int r = threadIdx.x >> 4, c = threadIdx.x & 15, l = (r & 3) * 16 + c;
+    return red[0][l][r >> 2] + red[1][l][r >> 2] + red[2][l][r >> 2] + red[3][l][r >> 2];
+}
+
+template <int D>
+__device__ __forceinline__ void ns_pq(int b, int *p, int *q)
+{
+    int i = 0;
+    while (i + 1 < n_groups(D) && block_at(D, i + 1, i + 1) <= b) ++i;
+    *p = i; *q = i + b - block_at(D, i, i);
+}
+
+// both triangles from the upper one.  (On the diagonal X Y's (r, c) and (c, r) are sums of other roundings: one of them, always the same
+// one, stands for both.)
+template <int D, typename O>
+__device__ __forceinline__ void ns_store(O *out, int p, int q, double v)
+{
+    const int r = 16 * p + (threadIdx.x >> 4), c = 16 * q + (threadIdx.x & 15);
+    if (r > c) return;
+    out[(size_t)r * D + c] = (O)v;
+    out[(size_t)c * D + r] = (O)v;
+}
+
+// S = A A.  FIRST: A = s^2 G is formed here and stored
+template <int D, bool FIRST>
+__global__ __launch_bounds__(256) void ns_square_kernel(const double *__restrict__ G, double *__restrict__ A, double *__restrict__ S, double eps)
+{
+    __shared__ double red[4][64][4], s_norm;
+    int p, q;
+    ns_pq<D>(blockIdx.x, &p, &q);
+    double s2 = 1.0;
+    if constexpr (FIRST) { const double s = norm_scale(G, D, eps, &s_norm); s2 = s * s; }
+    auto f = [&](int k, int c) { const double v = G[(size_t)k * D + c]; return FIRST ? s2 * v : v; };
+    const double v = ns_block<D>(f, f, p, q, red);
+    ns_store<D>(S, p, q, v);
+    if constexpr (FIRST) ns_store<D>(A, p, q, s2 * G[(size_t)(16 * p + (threadIdx.x >> 4)) * D + 16 * q + (threadIdx.x & 15)]);
+}
+
+// blockIdx.y == 0: out_m = M T (FIRST: s T, no product);  1: W = A T
+template <int D, bool FIRST, typename O>
+__global__ __launch_bounds__(256) void ns_times_t_kernel(const double *__restrict__ G, const double *__restrict__ A, const double *__restrict__ S,
+                                                         const double *__restrict__ M, O *__restrict__ out_m, double *__restrict__ W, Coeffs k)
+{
+    __shared__ double red[4][64][4], s_norm;
+    int p, q;
+    ns_pq<D>(blockIdx.x, &p, &q);
+    auto t = [&](int r, int c) { const size_t at = (size_t)r * D + c; return fma(k.c, S[at], fma(k.b, A[at], r == c ? k.a : 0.0)); };
+    if (blockIdx.y == 0) {
+        if constexpr (FIRST) {
+            const double s = norm_scale(G, D, k.eps, &s_norm);
+            ns_store<D>(out_m, p, q, s * t(16 * p + (threadIdx.x >> 4), 16 * q + (threadIdx.x & 15)));
+        } else {
+            ns_store<D>(out_m, p, q, ns_block<D>([&](int r, int c) { return M[(size_t)r * D + c]; }, t, p, q, red));
+        }
+    } else {
+        ns_store<D>(W, p, q, ns_block<D>([&](int r, int c) { return A[(size_t)r * D + c]; }, t, p, q, red));
+    }
+}
+
+// A' = W T
+template <int D>
+__global__ __launch_bounds__(256) void ns_next_kernel(const double *__restrict__ A, const double *__restrict__ S, const double *__restrict__ W,
+                                                      double *__restrict__ A2, Coeffs k)
+{
+    __shared__ double red[4][64][4];
+    int p, q;
+    ns_pq<D>(blockIdx.x, &p, &q);
+    auto t = [&](int r, int c) { const size_t at = (size_t)r * D + c; return fma(k.c, S[at], fma(k.b, A[at], r == c ? k.a : 0.0)); };
+    ns_store<D>(A2, p, q, ns_block<D>([&](int r, int c) { return W[(size_t)r * D + c]; }, t, p, q, red));
+}
+
+// d <= 64: the whole iteration in one workgroup, the four matrices in LDS (128 KB at d = 64), one 16 x 16 block per wavefront.
+// Odd rows swap neighbouring groups of 16 columns: the two rows of a half-wavefront's read fall on different halves of the banks.
+template <int D>
+__global__ __launch_bounds__(64 * (D / 16) * (D / 16)) void ns_small_kernel(const double *__restrict__ G, float *__restrict__ out, int steps, Coeffs k)
+{
+    constexpr int NG = D / 16, N = 64 * NG * NG;
+    __shared__ __attribute__((aligned(16))) double A[D * D], T[D * D], W[D * D], M[D * D];
+    __shared__ double s_norm;
+    auto el = [](int r, int c) { return r * D + (c ^ ((r & 1) << 4)); };
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, p = w / NG, q = w % NG;
+    const double s = norm_scale(G, D, k.eps, &s_norm);
+    for (int t = tid; t < D * D; t += N) {
+        const int r = t / D, c = t % D;
+        A[el(r, c)] = s * s * G[t];
+        M[el(r, c)] = r == c ? s : 0.0;
+    }
+    __syncthreads();
+    auto mul = [&](const double *x, const double *y) {
+        f64x4 acc = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll 4
+        for (int i = 0; i < D; i += 4)
+            acc = __builtin_amdgcn_mfma_f64_16x16x4f64(x[el(i + (lane >> 4), 16 * p + (lane & 15))], y[el(i + (lane >> 4), 16 * q + (lane & 15))], acc, 0, 0, 0);
+        return acc;
+    };
+    auto at = [&](int i) { return el(16 * p + 4 * i + (lane >> 4), 16 * q + (lane & 15)); };
+    for (int step = 0; step < steps; ++step) {
+        const f64x4 sq = mul(A, A);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = 16 * p + 4 * i + (lane >> 4), c = 16 * q + (lane & 15);
+            T[at(i)] = fma(k.c, sq[i], fma(k.b, A[at(i)], r == c ? k.a : 0.0));
+        }
+        __syncthreads();
+        const f64x4 m = mul(M, T);
+        f64x4 x = {0.0, 0.0, 0.0, 0.0};
+        if (step + 1 < steps) x = mul(A, T);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { M[at(i)] = m[i]; W[at(i)] = x[i]; }
+        __syncthreads();
+        if (step + 1 < steps) {
+            const f64x4 y = mul(W, T);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) A[at(i)] = y[i];      // (A was last read before the barrier above)
+            __syncthreads();
+        }
+    }
+    for (int t = tid; t < D * D; t += N) out[t] = (float)M[el(t / D, t % D)];
+}
+
+template <int D>
+__global__ __launch_bounds__(256) void ns_identity_kernel(const double *__restrict__ G, float *__restrict__ out, double eps)   // steps == 0
+{
+    __shared__ double s_norm;
+    const double s = norm_scale(G, D, eps, &s_norm);
+    for (int t = threadIdx.x; t < D * D; t += 256) out[t] = t / D == t % D ? (float)s : 0.0f;
+}
+
+// ---- rows times the [d x d] result ---------------------------------------------------------------------------------------------------
+// v_mfma_f32_32x32x2_f32, exact fp32 products.  A wavefront owns 32 output columns and keeps its 32 columns of the [d x d] matrix in registers
+// (d / 2 of them) for all its rows; rows pass through LDS.  The contraction index is permuted so that a lane reads its row four
+// elements at a time: step 4 j + e multiplies k = 8 j + 4 (lane >> 5) + e.
+template <int D>
+struct Proj {
+    static constexpr int WAVES = D == 256 ? 8 : 4, CG = D / 32, RG = WAVES / CG, TR = 32 * RG, LD = D + 4;
+};
+
+template <int D, typename T, bool MUON>
+__global__ __launch_bounds__(64 * Proj<D>::WAVES) void project_kernel(Rows<T, MUON> in, T *__restrict__ out, float *__restrict__ W, int64_t rows,
+                                                                        const float *__restrict__ Mt, float keep, float step)
+{
+    using C = Proj<D>;
+    __shared__ __attribute__((aligned(16))) float tile[C::TR * C::LD];
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, cg = w % C::CG, rg = w / C::CG, hi = lane >> 5, l31 = lane & 31;
+    float b[D / 2];
+#pragma unroll
+    for (int j = 0; j < D / 8; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) b[4 * j + e] = Mt[(8 * j + 4 * hi + e) * D + 32 * cg + l31];
+    for (int64_t r0 = (int64_t)blockIdx.x * C::TR; r0 < rows; r0 += (int64_t)gridDim.x * C::TR) {
+#pragma unroll
+        for (int t = tid; t < C::TR * (D / 4); t += 64 * C::WAVES) {
+            const int r = t / (D / 4), c = 4 * (t % (D / 4));
+            const float4 v = r0 + r < rows ? in.template get<false>((r0 + r) * D + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+            *reinterpret_cast<float4 *>(tile + r * C::LD + c) = v;
+        }
+        __syncthreads();
+        f32x16 acc;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[i] = 0.0f;
+        const float *a = tile + (32 * rg + l31) * C::LD + 4 * hi;
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j) {
+            const float4 x = *reinterpret_cast<const float4 *>(a + 8 * j);
+            acc = __builtin_amdgcn_mfma_f32_32x32x2f32(x.x, b[4 * j], acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f32_32x32x2f32(x.y, b[4 * j + 1], acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f32_32x32x2f32(x.z, b[4 * j + 2], acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f32_32x32x2f32(x.w, b[4 * j + 3], acc, 0, 0, 0);
+        }
+        __syncthreads();                // (every wavefront has read its rows, also before any of them is written where out == X)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int64_t r = r0 + 32 * rg + (i & 3) + 8 * (i >> 2) + 4 * hi;
+            if (r >= rows) continue;
+            const int64_t at = r * D + 32 * cg + l31;
+            if constexpr (MUON) {
+                W[at] = fmaf(-step, acc[i], keep * W[at]);
+                out[at] = (T)0;         // out is the gradient: zero for the next step
+            } else if constexpr (sizeof(T) == 2) {
+                out[at] = f32_bf16(acc[i]);
+            } else {
+                out[at] = acc[i];
+            }
+        }
+    }
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------------------------
+struct OrthoWs {
+    double *part, *G, *A, *A2, *S, *W, *M, *M2;
+    float *T;
+    int n_part;
+    int64_t bytes;
+};
+
+int gram_groups(int64_t rows, int d)
+{
+    // a workgroup for every 64 rows, at most one per CU (the accumulators are one wavefront per SIMD)
+    const int64_t per = d == 256 ? kG256Rows : kGramWaves * (d == 32 ? 8 : 4), want = (rows + 4 * per - 1) / (4 * per);
+    return (int)(want < 1 ? 1 : want > 256 ? 256 : want);
+}
+
+OrthoWs ortho_carve(void *ws, int64_t rows, int d)
+{
+    OrthoWs w;
+    char *base = (char *)ws;
+    int64_t off = 0;
+    auto take = [&](int64_t n) { char *q = base + off; off += (n + 255) / 256 * 256; return q; };
+    w.n_part = gram_groups(rows, d);
+    const int64_t mat = (int64_t)d * d * 8;
+    w.part = (double *)take((int64_t)w.n_part * n_blocks(d) * 2048);
+    w.G = (double *)take(mat); w.A = (double *)take(mat); w.A2 = (double *)take(mat); w.S = (double *)take(mat);
+    w.W = (double *)take(mat); w.M = (double *)take(mat); w.M2 = (double *)take(mat);
+    w.T = (float *)take(mat / 2);
+    w.bytes = off;
+    return w;
+}
+
+template <int D>
+void newton_schulz(const OrthoWs &w, int steps, const Coeffs &k, hipStream_t st)
+{
+    if (steps == 0) { hipLaunchKernelGGL(ns_identity_kernel<D>, dim3(1), dim3(256), 0, st, w.G, w.T, k.eps); return; }
+    if constexpr (D <= 64) {
+        hipLaunchKernelGGL(ns_small_kernel<D>, dim3(1), dim3(64 * (D / 16) * (D / 16)), 0, st, w.G, w.T, steps, k);
+    } else {
+        constexpr int NB = n_blocks(D);
+        double *A = w.A, *A2 = w.A2, *M = w.M, *M2 = w.M2;
+        for (int s = 0; s < steps; ++s) {
+            const bool last = s + 1 == steps;
+            if (s == 0) hipLaunchKernelGGL((ns_square_kernel<D, true>), dim3(NB), dim3(256), 0, st, w.G, A, w.S, k.eps);
+            else hipLaunchKernelGGL((ns_square_kernel<D, false>), dim3(NB), dim3(256), 0, st, A, (double *)nullptr, w.S, k.eps);
+            const dim3 grid(NB, last ? 1 : 2);
+            if (s == 0 && last) hipLaunchKernelGGL((ns_times_t_kernel<D, true, float>), grid, dim3(256), 0, st, w.G, A, w.S, M, w.T, w.W, k);
+            else if (s == 0) hipLaunchKernelGGL((ns_times_t_kernel<D, true, double>), grid, dim3(256), 0, st, w.G, A, w.S, M, M2, w.W, k);
+            else if (last) hipLaunchKernelGGL((ns_times_t_kernel<D, false, float>), grid, dim3(256), 0, st, w.G, A, w.S, M, w.T, w.W, k);
+            else hipLaunchKernelGGL((ns_times_t_kernel<D, false, double>), grid, dim3(256), 0, st, w.G, A, w.S, M, M2, w.W, k);
+            if (!last) hipLaunchKernelGGL(ns_next_kernel<D>, dim3(NB), dim3(256), 0, st, A, w.S, w.W, A2, k);
+            double *x = A; A = A2; A2 = x;
+            x = M; M = M2; M2 = x;
+        }
+    }
+}
+
+template <int D, typename T, bool MUON>
+void orthogonalize_d(const Rows<T, MUON> &in, T *out, float *W, int64_t rows, int steps, const Coeffs &k, float keep, float step, const OrthoWs &w, hipStream_t st)
+{
+    if constexpr (D == 256)
+        hipLaunchKernelGGL((gram256_kernel<T, MUON>), dim3(w.n_part), dim3(256), 0, st, in, rows, w.part);
+    else
+        hipLaunchKernelGGL((gram_kernel<D, T, MUON>), dim3(w.n_part), dim3(64 * kGramWaves), 0, st, in, rows, w.part);
+    hipLaunchKernelGGL(gram_reduce_kernel<D>, dim3(n_blocks(D) * 16), dim3(256), 0, st, w.part, w.n_part, w.G);
+    newton_schulz<D>(w, steps, k, st);
+    using C = Proj<D>;
+    const int64_t tiles = (rows + C::TR - 1) / C::TR;
+    const int64_t most = (int64_t)rsx_num_cus() * (D == 256 ? 2 : 4);
+    hipLaunchKernelGGL((project_kernel<D, T, MUON>), dim3((unsigned)(tiles < most ? tiles : most)), dim3(64 * C::WAVES), 0, st, in, out, W, rows, w.T, keep, step);
+}
+
+template <typename T, bool MUON>
+void orthogonalize_any(const Rows<T, MUON> &in, T *out, float *W, int64_t rows, int d, int steps, const Coeffs &k, float keep, float step, const OrthoWs &w,
+                       hipStream_t st)
+{
+    switch (d) {
+    case 32: orthogonalize_d<32, T, MUON>(in, out, W, rows, steps, k, keep, step, w, st); break;
+    case 64: orthogonalize_d<64, T, MUON>(in, out, W, rows, steps, k, keep, step, w, st); break;
+    case 128: orthogonalize_d<128, T, MUON>(in, out, W, rows, steps, k, keep, step, w, st); break;
+    default: orthogonalize_d<256, T, MUON>(in, out, W, rows, steps, k, keep, step, w, st); break;
+    }
+}
+
+bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+bool finite64(double v) { return v - v == 0.0; }
+
+}  // namespace
+
+RSX_API int64_t rsx_orthogonalize_workspace(int64_t rows, int d)
+{
+    if (rows < 0 || !rsx_dim_ok(d)) return RSX_E_INVALID;
+    return ortho_carve(nullptr, rows, d).bytes;
+}
+
+RSX_API int rsx_orthogonalize(const void *X, void *out, int64_t rows, int d, int dtype, int steps, double a, double b, double c, double eps, void *ws,
+                              int64_t ws_bytes, rsx_stream_t stream)
+{
+    RSX_CHECK_ARG(X && out, "null pointer");
+    RSX_CHECK_ARG(rsx_dim_ok(d), "d must be 32, 64, 128 or 256");
+    RSX_CHECK_ARG(rows >= 0, "bad shape");
+    RSX_CHECK_ARG(dtype == RSX_F32 || dtype == RSX_BF16, "dtype must be RSX_F32 or RSX_BF16");
+    RSX_CHECK_ARG(steps >= 0 && steps <= 32, "steps must be in [0, 32]");
+    RSX_CHECK_ARG(finite64(a) && finite64(b) && finite64(c) && finite64(eps) && eps >= 0.0, "coefficients must be finite, eps >= 0");
+    RSX_CHECK_ARG(aligned16(X) && aligned16(out), "rows must be 16-byte aligned");
+    if (rows == 0) return RSX_OK;
+    const OrthoWs w = ortho_carve(ws, rows, d);
+    if (ws == nullptr || ws_bytes < w.bytes || (reinterpret_cast<uintptr_t>(ws) & 7)) {
+        rsx_set_error("rsx_orthogonalize: workspace of %lld bytes (8-byte aligned) required, got %lld", (long long)w.bytes, (long long)ws_bytes);
+        return RSX_E_WORKSPACE;
+    }
+    const Coeffs k{a, b, c, eps};
+    hipStream_t st = (hipStream_t)stream;
+    if (dtype == RSX_F32)
+        orthogonalize_any<float, false>({(const float *)X, nullptr, 0.f, 0}, (float *)out, nullptr, rows, d, steps, k, 0.f, 0.f, w, st);
+    else
+        orthogonalize_any<uint16_t, false>({(const uint16_t *)X, nullptr, 0.f, 0}, (uint16_t *)out, nullptr, rows, d, steps, k, 0.f, 0.f, w, st);
+    RSX_CHECK_LAUNCH();
+    return RSX_OK;
+}
+
+RSX_API int rsx_muon_apply(float *W, float *M, void *G, int64_t rows, int d, int g_dtype, double lr, double momentum, int nesterov, int steps, double a,
+                           double b, double c, double eps, double weight_decay, double update_scale, void *ws, int64_t ws_bytes, rsx_stream_t stream)
+{
+    RSX_CHECK_ARG(W && M && G, "null pointer");
+    RSX_CHECK_ARG(rsx_dim_ok(d), "d must be 32, 64, 128 or 256");
+    RSX_CHECK_ARG(rows >= 0, "bad shape");
+    RSX_CHECK_ARG(g_dtype == RSX_F32 || g_dtype == RSX_BF16, "g_dtype must be RSX_F32 or RSX_BF16");
+    RSX_CHECK_ARG(steps >= 0 && steps <= 32, "steps must be in [0, 32]");
+    RSX_CHECK_ARG(finite64(a) && finite64(b) && finite64(c) && finite64(eps) && eps >= 0.0, "coefficients must be finite, eps >= 0");
+    RSX_CHECK_ARG(finite64(lr) && finite64(weight_decay) && finite64(update_scale) && momentum >= 0.0 && momentum < 1.0, "momentum must be in [0, 1), the rest finite");
+    RSX_CHECK_ARG(aligned16(W) && aligned16(M) && aligned16(G), "rows must be 16-byte aligned");
+    if (rows == 0) return RSX_OK;
+    const OrthoWs w = ortho_carve(ws, rows, d);
+    if (ws == nullptr || ws_bytes < w.bytes || (reinterpret_cast<uintptr_t>(ws) & 7)) {
+        rsx_set_error("rsx_muon_apply: workspace of %lld bytes (8-byte aligned) required, got %lld", (long long)w.bytes, (long long)ws_bytes);
+        return RSX_E_WORKSPACE;
+    }
+    const Coeffs k{a, b, c, eps};
+    const float keep = (float)(1.0 - lr * weight_decay), step = (float)(lr * update_scale);
+    hipStream_t st = (hipStream_t)stream;
+    if (g_dtype == RSX_F32)
+        orthogonalize_any<float, true>({(const float *)G, M, (float)momentum, nesterov}, (float *)G, W, rows, d, steps, k, keep, step, w, st);
+    else
+        orthogonalize_any<uint16_t, true>({(const uint16_t *)G, M, (float)momentum, nesterov}, (uint16_t *)G, W, rows, d, steps, k, keep, step, w, st);
+    RSX_CHECK_LAUNCH();
+    return RSX_OK;
+}

@@ -49,6 +49,9 @@ SIGNATURES = {
     "rsx_bpr_grad": (C.c_int, [_P, _P, _P, _P, _I64, _I64, _P, _P, _P, _I64, _I32, _F, _P, _P]),
     "rsx_pointwise_grad": (C.c_int, [_P, _P, _P, _P, _I64, _I64, _P, _P, _P, _I64, _I32, _F, _I32, _P, _P]),
     "rsx_adam_apply": (C.c_int, [_P, _P, _P, _P, _I64, _D, _D, _D, _D, _I64, _P]),
+    "rsx_orthogonalize_workspace": (_I64, [_I64, _I32]),
+    "rsx_orthogonalize": (C.c_int, [_P, _P, _I64, _I32, _I32, _I32, _D, _D, _D, _D, _P, _I64, _P]),
+    "rsx_muon_apply": (C.c_int, [_P, _P, _P, _I64, _I32, _I32, _D, _D, _I32, _I32, _D, _D, _D, _D, _D, _D, _P, _I64, _P]),
     "rsx_spmm_plan": (_I64, [_P, _I64, _I32, _P, _P, _P]),
     "rsx_spmm_csr": (C.c_int, [_P, _P, _P, _I64, _P, _P, _P, _P, _P, _P, _I64, _I32, _P]),
     "rsx_spmm_csr_sparse_rows": (C.c_int, [_P, _P, _P, _I64, _P, _P, _P, _P, _P, _P, _P, _I64, _I32, _P]),
@@ -266,6 +269,80 @@ def adam_apply(W, M, V, G, lr, t, beta1=0.9, beta2=0.999, eps=1e-8):
                                 _dev(V, torch.float32, "V"), _dev(G, torch.float32, "G"), W.numel(),
                                 float(lr), float(beta1), float(beta2), float(eps), int(t), _stream()),
            "rsx_adam_apply")
+
+
+# element types of include/rsx.h
+RSX_F32, RSX_BF16 = 0, 1
+_DTYPES = {torch.float32: RSX_F32, torch.bfloat16: RSX_BF16}
+MUON_COEFFS = (3.4445, -4.7750, 2.0315)
+
+
+def _dtype(t, name):
+    if not isinstance(t, torch.Tensor) or t.dtype not in _DTYPES:
+        raise RsxError(f"{name} must be a float32 or bfloat16 device tensor")
+    return _DTYPES[t.dtype]
+
+
+def _matrix(t, name, rows=None, d=None, dtype=None):
+    """pointer of a contiguous 2-D device tensor, its shape checked"""
+    if not isinstance(t, torch.Tensor) or t.dim() != 2 or (rows is not None and t.shape[0] != rows) or (d is not None and t.shape[1] != d):
+        raise RsxError(f"{name} must be a [{'rows' if rows is None else rows} x {'d' if d is None else d}] tensor")
+    return _dev(t, t.dtype if dtype is None else dtype, name)
+
+
+def _scratch(ws, need, device):
+    """`ws` where it is large enough, else a new tensor (one that a caller keeps must be on the call's device)"""
+    if ws is None or ws.numel() * ws.element_size() < need:
+        return torch.empty((max(need, 8) + 7) // 8, dtype=torch.int64, device=device)
+    if ws.device != device or not ws.is_contiguous():
+        raise RsxError(f"workspace must be a contiguous tensor on {device}")
+    return ws
+
+
+def _same_device(first, *others):
+    """everything on one device, which the launch is made on whatever the caller's current one is"""
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise RsxError(f"tensors on {first.device} and {t.device} in one call")
+    return torch.cuda.device(first.device)
+
+
+def orthogonalize_workspace(rows, d):
+    n = lib().rsx_orthogonalize_workspace(int(rows), int(d))
+    if n < 0:
+        raise RsxError("rsx_orthogonalize_workspace: invalid shape")
+    return n
+
+
+def orthogonalize(X, steps=5, coeffs=MUON_COEFFS, eps=1e-7, out=None, ws=None):
+    """Newton-Schulz iteration of a [rows x d] matrix (float32 or bfloat16) towards its nearest orthonormal columns
+    (include/rsx.h:rsx_orthogonalize); out may be X"""
+    ptr, dt = _matrix(X, "X"), _dtype(X, "X")
+    out = torch.empty_like(X) if out is None else out
+    po = _matrix(out, "out", X.shape[0], X.shape[1], X.dtype)
+    if X.shape[0] == 0:
+        return out
+    with _same_device(X, out):
+        ws = _scratch(ws, orthogonalize_workspace(*X.shape), X.device)
+        _check(lib().rsx_orthogonalize(ptr, po, X.shape[0], X.shape[1], dt, int(steps), *(float(c) for c in coeffs), float(eps),
+                                       C.c_void_p(ws.data_ptr()), ws.numel() * ws.element_size(), _stream()), "rsx_orthogonalize")
+    return out
+
+
+def muon_apply(W, M, G, lr, momentum=0.95, nesterov=True, steps=5, coeffs=MUON_COEFFS, eps=1e-7, weight_decay=0.0, update_scale=None, ws=None):
+    """one orthogonalised optimizer step over a whole table, then G = 0 (include/rsx.h:rsx_muon_apply); W, M float32, G float32 or
+    bfloat16; update_scale: sqrt(max(1, rows / d)) by default"""
+    pw, dt = _matrix(W, "W", dtype=torch.float32), _dtype(G, "G")
+    rows, d = W.shape
+    pm, pg = _matrix(M, "M", rows, d, torch.float32), _matrix(G, "G", rows, d)
+    if rows == 0:
+        return
+    scale = max(1.0, rows / d) ** 0.5 if update_scale is None else float(update_scale)
+    with _same_device(W, M, G):
+        ws = _scratch(ws, orthogonalize_workspace(rows, d), W.device)
+        _check(lib().rsx_muon_apply(pw, pm, pg, rows, d, dt, float(lr), float(momentum), int(bool(nesterov)), int(steps), *(float(c) for c in coeffs),
+                                    float(eps), float(weight_decay), scale, C.c_void_p(ws.data_ptr()), ws.numel() * ws.element_size(), _stream()),
+               "rsx_muon_apply")
 
 
 class SpmmHot(C.Structure):
