@@ -240,6 +240,27 @@ int rsx_pointwise_grad(const float *P, const float *Q, float *GP, float *GQ, int
 int rsx_pair_score(const float *P, const float *Q, const int32_t *u_dev, const int32_t *i_dev,
                    int64_t n, int d, float *r_out, rsx_stream_t stream);
 
+/* ---- softmax over the whole catalog -----------------------------------------------------------
+ * rsx_score_logprobs: with z_ri = scale <P[user_ids[r]], Q[i]> (-inf where i is in the CSR row of user_ids[r]: seen items),
+ *   lse_out[r]      = log sum_i exp z_ri                      (nullable; -inf for a row whose every item is masked)
+ *   entropy_out[r]  = -sum_i p_ri log p_ri, p = exp(z - lse)  (nullable; 0 for such a row)
+ *   logp_out[r, t]  = z_r,items[r, t] - lse[r]                (T per row, T = 0: none; -inf for a masked item)
+ *   topk_idx_out / topk_logp_out [num_rows x K]: the K most probable items in descending order and their log-probabilities
+ *                     (K = 0: none; K <= 128).  Ties go to the lowest id.  The order is that of the products in 64 bits.
+ *                     Fewer than K unmasked items: -1 and -inf.
+ * The scores are never stored.  P, Q: dtype RSX_F32 or RSX_BF16, both [. x d]; sums in fp32 and 64 bits.
+ * A position whose user id is outside [0, num_users) names no row (a padded batch): lse -inf, entropy 0, logp 0, no top items.
+ * An item id outside [0, num_items) names no item: its logp is 0.  mask_indptr: int64 [num_users + 1] (nullable with
+ * mask_indices); rows need not be sorted, ids outside the catalog are ignored.  What a masked cell's product would have been
+ * (infinities, NaN) does not matter.
+ * No call synchronises with the host: all can be captured into a graph.  ws: *_workspace bytes, 16-byte aligned, contents irrelevant,
+ * one per concurrent call.                                                                                                    */
+int64_t rsx_score_logprobs_workspace(int64_t num_rows, int64_t num_items, int d, int dtype, int masked, int K);
+int rsx_score_logprobs(const void *P, int64_t num_users, const int32_t *user_ids_dev, int64_t num_rows, const void *Q,
+                       int64_t num_items, int d, int dtype, const int64_t *mask_indptr_dev, const int32_t *mask_indices_dev,
+                       float scale, const int32_t *items_dev, int T, int K, float *logp_out, float *lse_out, float *entropy_out,
+                       int32_t *topk_idx_out, float *topk_logp_out, void *ws, int64_t ws_bytes, rsx_stream_t stream);
+
 /* ---- on-device triplet sampler ------------------------------------------------
  * Replaces data/generators.py:151-224 (PairwiseGenerator: host-side numpy
  * sampling + permutation + H2D copy).  Sampling semantics are BPR's, not the

@@ -1,0 +1,155 @@
+// rsx_logprob.h -- what the full-catalog log-probability (rsx_logprob.hip) and its gradient (rsx_logprob_grad.hip) share.
+//
+// fp32 tables go through the 16-bit matrix cores: v_mfma_f32_32x32x16_f16 does 16 times the products of v_mfma_f32_32x32x2_f32, and
+// x = hi + lo with hi = half(x), lo = half(x - hi) holds x to 2^-24 of itself (11 + 11 bits and a sign) as long as lo is not
+// subnormal.  x y = hi hi' + hi lo' + lo hi' (lo lo' is below 2^-24 |x y|): three instructions instead of sixteen.  A row of P, and
+// 32 rows of Q together, are scaled by a power of two that puts their largest element into [2^13, 2^14): elements down to 2^-27 of the
+// largest keep their 24 bits.  bf16 tables are multiplied as they are.
+#pragma once
+#include "rsx_common.h"
+
+namespace lp {
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr double kLn2 = 0.69314718055994530942;
+constexpr int kTile = 32;                 // items (or rows) of one matrix instruction
+
+// eight 16-bit elements, the operand of one lane
+union Frag {
+    half8 h;
+    bf16x8 b;
+    uint4 u;
+};
+
+template <bool F32>
+__device__ __forceinline__ f32x16 mfma32(const Frag &a, const Frag &b, f32x16 c)
+{
+    if constexpr (F32) return __builtin_amdgcn_mfma_f32_32x32x16_f16(a.h, b.h, c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.b, b.b, c, 0, 0, 0);
+}
+
+__device__ __forceinline__ float bf16_f32(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
+__device__ __forceinline__ uint16_t f32_bf16(float v)        // nearest even; NaN stays NaN
+{
+    const uint32_t u = __float_as_uint(v);
+    if ((u & 0x7FFFFFFFu) > 0x7F800000u) return (uint16_t)((u >> 16) | 0x40u);
+    return (uint16_t)((u + 0x7FFFu + ((u >> 16) & 1u)) >> 16);
+}
+
+// geometry of a [rows x d] operand as 16-bit planes: a row is hi[d] lo[d] (fp32) or [d] (bf16)
+template <int D, bool F32>
+struct Geo {
+    static constexpr int NP = F32 ? 2 : 1, ROWB = D * NP * 2, TILEB = kTile * ROWB, KS = D / 16;
+    // 16-byte slots of a row are XORed with this, so that the 16 rows a quarter of a fragment read touches fall on 16 different slots of
+    // the 256 bytes the LDS delivers a cycle (rows of 64 and 128 bytes: 4 and 2 of them share a line)
+    __device__ static __forceinline__ int swz(int row) { return ROWB >= 256 ? row & 15 : ROWB == 128 ? (row >> 1) & 7 : (row >> 2) & 3; }
+};
+
+// 64 lanes x 16 bytes from global memory straight into LDS (lane-linear from a wavefront-uniform base); the next barrier waits for it.
+// (a function of its own: called from a kernel's body, the builtin costs the kernel its host stub)
+__device__ __forceinline__ void copy_to_lds(const char *src, char *dst) { __builtin_amdgcn_global_load_lds(src, dst, 16, 0, 0); }
+
+// power of two that brings a largest magnitude m into [2^13, 2^14), and its inverse.  Below 2^-40 as for 2^-40: the product of two such
+// inverses stays a normal number, and what is lost there moves no score by 2^-40
+__device__ __forceinline__ void scale_for(float m, float *up, float *down)
+{
+    int e = (int)((__float_as_uint(m) >> 23) & 0xFF) - 126;      // m in [2^(e-1), 2^e)
+    e = e < -40 ? -40 : e;
+    *up = ldexpf(1.0f, 14 - e);
+    *down = ldexpf(1.0f, e - 14);
+}
+__device__ __forceinline__ float finite_abs(float v) { const float a = fabsf(v); return a < INFINITY ? a : 0.0f; }     // NaN and infinities: 0
+
+// eight scaled floats -> the two planes' fragments
+__device__ __forceinline__ void split8(const float *x, Frag *hi, Frag *lo)
+{
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const _Float16 h = (_Float16)x[j];
+        hi->h[j] = h;
+        lo->h[j] = (_Float16)(x[j] - (float)h);
+    }
+}
+
+// rows of the call: a position whose user id is outside the table names no row
+__device__ __forceinline__ bool row_ok(int32_t u, int64_t num_users) { return u >= 0 && u < num_users; }
+
+static __global__ __launch_bounds__(256) void fill_u32_kernel(uint4 *__restrict__ p, int64_t n16, uint32_t v)
+{
+    for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < n16; t += (int64_t)gridDim.x * 256) p[t] = make_uint4(v, v, v, v);
+}
+
+// words a row of the bit mask holds: four tiles of 32 items at a time
+__host__ __device__ __forceinline__ int64_t mask_words(int64_t num_items) { return (num_items + 127) / 128 * 4; }
+
+// seen items of a row as bits, [rows][words]: bit i & 31 of word i >> 5; one wavefront per row, the words zero before
+__device__ __forceinline__ void set_seen_bits(int32_t u, const int64_t *__restrict__ indptr, const int32_t *__restrict__ indices, int64_t num_items, uint32_t *row)
+{
+    const int64_t hi = indptr[u + 1];
+    for (int64_t p = indptr[u] + (threadIdx.x & 63); p < hi; p += 64) {
+        const int32_t i = indices[p];
+        if (i >= 0 && i < num_items) atomicOr(row + (i >> 5), 1u << (i & 31));
+    }
+}
+
+inline void launch_clear_bits(int64_t rows, int64_t num_items, uint32_t *bits, hipStream_t st)
+{
+    const int64_t n16 = rows * mask_words(num_items) / 4, most = (int64_t)rsx_num_cus() * 8;
+    const int64_t want = (n16 + 255) / 256;
+    hipLaunchKernelGGL(fill_u32_kernel, dim3((unsigned)(want < most ? want : most)), dim3(256), 0, st, (uint4 *)bits, n16, 0u);
+}
+
+// fp32 item rows -> scaled planes [tiles padded to a multiple of 4][32][hi d, lo d] and a factor per tile.  One workgroup per tile.
+// Rows behind the last item are zero.
+template <int D>
+__global__ __launch_bounds__(256) void split_items_kernel(const float *__restrict__ Q, int64_t num_items, uint4 *__restrict__ planes, float *__restrict__ factor)
+{
+    constexpr int TPR = D / 8, RPP = 256 / TPR, N = kTile / RPP > 0 ? kTile / RPP : 1;       // threads a row, rows a pass, passes
+    __shared__ float s_max[4];
+    const int tid = threadIdx.x;
+    const int64_t tile = blockIdx.x;
+    float x[N][8];
+    float m = 0.0f;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        const int r = n * RPP + tid / TPR;
+        const int64_t i = tile * kTile + r;
+        const bool live = r < kTile && i < num_items;
+        const float4 *src = reinterpret_cast<const float4 *>(Q + (size_t)(live ? i : 0) * D + 8 * (tid % TPR));
+        const float4 a = live ? src[0] : make_float4(0.f, 0.f, 0.f, 0.f), b = live ? src[1] : make_float4(0.f, 0.f, 0.f, 0.f);
+        x[n][0] = a.x; x[n][1] = a.y; x[n][2] = a.z; x[n][3] = a.w; x[n][4] = b.x; x[n][5] = b.y; x[n][6] = b.z; x[n][7] = b.w;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m = fmaxf(m, finite_abs(x[n][j]));
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    if ((tid & 63) == 0) s_max[tid >> 6] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
+    float up, down;
+    scale_for(m, &up, &down);
+    if (tid == 0) factor[tile] = down;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        const int r = n * RPP + tid / TPR;
+        if (r >= kTile) continue;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[n][j] *= up;
+        Frag h, l;
+        split8(x[n], &h, &l);
+        uint4 *dst = planes + (size_t)(tile * kTile + r) * (2 * TPR) + tid % TPR;
+        dst[0] = h.u;
+        dst[TPR] = l.u;
+    }
+}
+
+inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+inline int64_t a256(int64_t x) { return (x + 255) / 256 * 256; }
+
+}  // namespace lp

@@ -1,0 +1,876 @@
+// rsx_logprob.hip -- log-probabilities of given items under the softmax over the whole catalog, with entropy and the K most probable
+// items, for gfx950 (MI355X).
+//
+//   z_ri = scale <P[u_r], Q_i>  (-inf where masked),  lse_r = log sum_i exp z_ri,  logp_rt = z_r,items[r,t] - lse_r,
+//   H_r = lse_r - sum_i p_ri z_ri,  top = the K largest z_ri (ties: lowest id)
+//
+// The [rows x items] scores never exist in memory.  One pass over the catalog keeps, per row, a running reference m, the sum of
+// 2^(t - m) and the sum of (t - m) 2^(t - m) with t = z log2 e; they are rescaled only when a tile exceeds m by 2^16, so the common
+// path is one fused multiply-add, one v_exp_f32 and two accumulations per score.  The products are laid out so that a lane holds
+// scores of ONE row (items are the matrix instruction's rows, users its columns): all of this is lane-local.
+//
+// Top-K: the pass also stores the largest score of every 8 items as a half (relative to a score of the same row, so that halves
+// resolve it).  The K best items lie in chunks whose maximum is at least the K-th largest maximum; finish_kernel takes K + 8 chunks
+// and every tie, computes their items' products again in 64 bits and orders those.  What the fast products' rounding could swap is
+// decided by the 64-bit ones.
+//
+// Two forms of the pass:
+//   thin_kernel  few rows: the catalog is read once, straight into registers (v_mfma_f32_16x16x4_f32 / 16x16x32_bf16), bound by HBM
+//   wide_kernel  many rows: item tiles through LDS (asynchronous copies, two buffers), users' operands held in registers for the whole
+//                pass (up to 128 registers a lane), bound by the matrix cores (fp32: three f16 products, rsx_logprob.h) or, for bf16
+//                rows of 128, by the five vector instructions a score needs after its product
+#include "rsx_logprob.h"
+
+namespace {
+using namespace lp;
+
+constexpr int kMaxK = 128;
+constexpr float kNone = -3.0e38f;        // reference of a row that has met no score yet
+constexpr float kLazy = 16.0f;           // a tile's maximum may exceed the reference by this much before the sums are rescaled
+
+struct Shape {
+    const int32_t *user_ids;
+    int64_t rows, users, items;
+    float scale;
+};
+
+// running sums of one row, in units of log2
+struct Stat {
+    float m, sum, ent;
+};
+
+__device__ __forceinline__ void stat_lift(Stat &s, float top)      // new reference max(m, top)
+{
+    const float m = fmaxf(s.m, top);
+    const float r = __builtin_amdgcn_exp2f(s.m - m);
+    s.ent = s.sum > 0.0f ? r * fmaf(s.sum, s.m - m, s.ent) : s.ent;      // (0 * inf for a row that has met nothing: skipped.  NaN sums: kept)
+    s.sum = s.sum * r;
+    s.m = m;
+}
+
+// reference score of a row for the chunk maxima: the median of three items' scores, 0 if that is not finite
+__device__ __forceinline__ float pick_reference(float a, float b, float c)
+{
+    const float m = __builtin_amdgcn_fmed3f(a, b, c);
+    return fabsf(m) < 1.0e30f ? m : 0.0f;
+}
+
+__device__ __forceinline__ uint16_t half_bits(float v) { const _Float16 h = (_Float16)v; return __builtin_bit_cast(uint16_t, h); }
+
+// eight consecutive elements of a table row in fp32
+template <bool F32>
+__device__ __forceinline__ void load8(const void *base, int64_t at, float *x)
+{
+    if constexpr (F32) {
+        const float4 *p = reinterpret_cast<const float4 *>((const float *)base + at);
+        const float4 a = p[0], b = p[1];
+        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    } else {
+        const uint4 v = *reinterpret_cast<const uint4 *>((const uint16_t *)base + at);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { x[2 * j] = __uint_as_float(w[j] << 16); x[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u); }
+    }
+}
+
+// what a row needs before the pass: its seen items as bits, and the reference its chunk maxima are stored against (a score of its own, so that
+// an offset common to a row's scores does not eat the halves' eleven bits).  One wavefront per row.
+template <int D, bool F32>
+__global__ __launch_bounds__(256) void row_prep_kernel(const void *__restrict__ P, const void *__restrict__ Q, Shape sh, const int64_t *__restrict__ indptr,
+                                                       const int32_t *__restrict__ indices, uint32_t *__restrict__ bits, float *__restrict__ ref)
+{
+    const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (r >= sh.rows) return;
+    const int32_t u = sh.user_ids[r];
+    if (!row_ok(u, sh.users)) return;
+    if (ref != nullptr) {
+        float d[3] = {0.0f, 0.0f, 0.0f};
+        if (lane < D / 8) {
+            float x[8], q[8];
+            load8<F32>(P, (int64_t)u * D + 8 * lane, x);
+#pragma unroll
+            for (int n = 0; n < 3; ++n) {
+                load8<F32>(Q, (n == 0 ? 0 : n == 1 ? sh.items / 2 : sh.items - 1) * D + 8 * lane, q);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) d[n] = fmaf(x[j], q[j], d[n]);
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < 3; ++n)
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) d[n] += __shfl_xor(d[n], o, 64);
+        if (lane == 0) ref[r] = sh.scale * kLog2e * pick_reference(d[0], d[1], d[2]);
+    }
+    if (indptr != nullptr) set_seen_bits(u, indptr, indices, sh.items, bits + r * mask_words(sh.items));
+}
+
+// ---- many rows ------------------------------------------------------------------------------------------------------------------------
+template <int D, bool F32>
+struct WideGeo : Geo<D, F32> {
+    using G = Geo<D, F32>;
+    // 32-user blocks a wavefront holds: their operands take KS * NP * 4 registers each
+    static constexpr int UB = D * G::NP <= 256 ? 2 : 1, WGU = 128 * UB;
+    // item tiles of one of the two LDS buffers: 32 KB, so that two workgroups share a CU
+    static constexpr int ST = 32768 / G::TILEB >= 4 ? 4 : 32768 / G::TILEB;
+};
+
+// chunk maxima of a row, 16 halves per group of four tiles: [hi][tile & 3][h] holds items 32 tile + 16 h + 4 hi + {0..3, 8..11}
+__device__ __forceinline__ int64_t chunk_item0(int64_t c)
+{
+    return (4 * (c >> 4) + ((c >> 1) & 3)) * kTile + 16 * (c & 1) + 4 * ((c >> 3) & 1);
+}
+
+template <int D, bool F32, bool MASK, bool TOP>
+__global__ __launch_bounds__(256, 2) void wide_kernel(const void *__restrict__ P, const void *__restrict__ Qtab, const char *__restrict__ planes,
+                                                      const float *__restrict__ factor, Shape sh, const uint32_t *__restrict__ bits,
+                                                      const float *__restrict__ row_ref, int splits, float4 *__restrict__ part, uint4 *__restrict__ keys)
+{
+    using G = WideGeo<D, F32>;
+    constexpr int UB = G::UB, KS = G::KS, NP = G::NP, ST = G::ST;
+    __shared__ __attribute__((aligned(1024))) char lds[2][ST * G::TILEB];
+    const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, hi = lane >> 5, l31 = lane & 31;
+    const int64_t groups = (sh.items + 127) / 128;
+    const int64_t g0 = groups * blockIdx.x / splits, g1 = groups * (blockIdx.x + 1) / splits;
+    const int64_t row0 = (int64_t)blockIdx.y * G::WGU + wid * (32 * UB);
+
+    // this wavefront's users: operands, scale, reference
+    Frag b[UB][KS][NP];
+    float rowf[UB], ref[UB];
+    Stat st[UB];
+#pragma unroll
+    for (int ub = 0; ub < UB; ++ub) {
+        const int64_t r = row0 + 32 * ub + l31;
+        const int32_t u = sh.user_ids[r < sh.rows ? r : sh.rows - 1];
+        const bool ok = row_ok(u, sh.users);
+        const int64_t at = (int64_t)(ok ? u : 0) * D + 8 * hi;
+        float up = 1.0f, down = 1.0f;
+        if constexpr (F32) {
+            float m = 0.0f;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                float x[8];
+                load8<F32>(P, at + 16 * s, x);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) m = fmaxf(m, finite_abs(x[j]));
+            }
+            scale_for(fmaxf(m, __shfl_xor(m, 32, 64)), &up, &down);
+        }
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            if constexpr (F32) {
+                float x[8];
+                load8<F32>(P, at + 16 * s, x);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] *= up;
+                split8(x, &b[ub][s][0], &b[ub][s][NP - 1]);
+            } else {
+                b[ub][s][0].u = *reinterpret_cast<const uint4 *>((const uint16_t *)P + at + 16 * s);
+            }
+        }
+        rowf[ub] = ok ? down * sh.scale * kLog2e : 0.0f;
+        ref[ub] = TOP && ok ? row_ref[r < sh.rows ? r : sh.rows - 1] : 0.0f;
+        st[ub] = {kNone, 0.0f, 0.0f};
+    }
+
+    // copies of the next ST tiles: 1 KB a wavefront instruction, lane-linear in LDS, the swizzle in the source address
+    auto stage = [&](int64_t tile, int buf) {
+#pragma unroll
+        for (int n = 0; n < ST * G::TILEB / 4096; ++n) {
+            const int o = (n * 4 + wid) * 1024 + lane * 16, row = o / G::ROWB, c = (o % G::ROWB) / 16 ^ G::swz(row);
+            int64_t i = tile * kTile + row;
+            if constexpr (!F32) i = i < sh.items ? i : sh.items - 1;         // (the planes of fp32 tables are padded)
+            const char *src = F32 ? planes + (size_t)i * G::ROWB + 16 * c : (const char *)Qtab + (size_t)i * G::ROWB + 16 * c;
+            copy_to_lds(src, lds[buf] + (n * 4 + wid) * 1024);
+        }
+    };
+    const int64_t words = mask_words(sh.items);
+    const int sw = G::swz(l31) * 16;
+    if (g0 < g1) stage(4 * g0, 0);
+    int buf = 0;
+    for (int64_t g = g0; g < g1; ++g) {
+        uint4 seen[UB];
+        if constexpr (MASK) {
+#pragma unroll
+            for (int ub = 0; ub < UB; ++ub) {
+                const int64_t r = row0 + 32 * ub + l31;
+                seen[ub] = *reinterpret_cast<const uint4 *>(bits + (size_t)(r < sh.rows ? r : sh.rows - 1) * words + 4 * g);
+            }
+        }
+        uint32_t key[UB][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int64_t tile = 4 * g + j;
+            if (j % ST == 0) {
+                __syncthreads();         // this stage's copies have landed; everyone is done with the other buffer
+                if (j + ST < 4 || g + 1 < g1) stage(tile + ST, buf ^ 1);
+                buf ^= 1;
+            }
+            const char *t0 = lds[buf ^ 1] + (j % ST) * G::TILEB + l31 * G::ROWB;
+            f32x16 acc[UB];
+#pragma unroll
+            for (int ub = 0; ub < UB; ++ub)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[ub][i] = 0.0f;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                Frag a[NP];
+#pragma unroll
+                for (int p = 0; p < NP; ++p) a[p].u = *reinterpret_cast<const uint4 *>(t0 + ((16 * (p * (D / 8) + 2 * s + hi)) ^ sw));
+#pragma unroll
+                for (int ub = 0; ub < UB; ++ub) acc[ub] = mfma32<F32>(a[0], b[ub][s][0], acc[ub]);
+                if constexpr (F32) {
+#pragma unroll
+                    for (int ub = 0; ub < UB; ++ub) acc[ub] = mfma32<F32>(a[0], b[ub][s][1], acc[ub]);
+#pragma unroll
+                    for (int ub = 0; ub < UB; ++ub) acc[ub] = mfma32<F32>(a[1], b[ub][s][0], acc[ub]);
+                }
+            }
+            // scores of row l31 (of each block): register i is item 32 tile + (i & 3) + 8 (i >> 2) + 4 hi
+            const float tf = F32 ? factor[tile] : 1.0f;
+            const int64_t left = sh.items - tile * kTile;
+            const uint32_t none = left >= 32 ? 0u : left <= 0 ? 0xFFFFFFFFu : 0xFFFFFFFFu << left;
+#pragma unroll
+            for (int ub = 0; ub < UB; ++ub) {
+                const float f = rowf[ub] * tf;
+                uint32_t w = none;
+                if constexpr (MASK) w |= j == 0 ? seen[ub].x : j == 1 ? seen[ub].y : j == 2 ? seen[ub].z : seen[ub].w;
+                w >>= 4 * hi;
+                const bool any = __builtin_amdgcn_ballot_w64((w & 0x0F0F0F0Fu) != 0u) != 0ull;
+                if (any) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if ((w >> ((i & 3) + 8 * (i >> 2))) & 1u) acc[ub][i] = -INFINITY;
+                }
+                float c0 = acc[ub][0], c1 = acc[ub][8];
+#pragma unroll
+                for (int i = 1; i < 8; ++i) { c0 = fmaxf(c0, acc[ub][i]); c1 = fmaxf(c1, acc[ub][8 + i]); }
+                const float top = fmaxf(c0, c1) * f;
+                if constexpr (TOP)
+                    key[ub][j] = (uint32_t)half_bits(fmaf(c0, f, -ref[ub])) | ((uint32_t)half_bits(fmaf(c1, f, -ref[ub])) << 16);
+                if (__builtin_amdgcn_ballot_w64(top > st[ub].m + kLazy) != 0ull) {
+                    if (top > st[ub].m) stat_lift(st[ub], top);
+                }
+                const float m = st[ub].m;
+                float sum = st[ub].sum, ent = st[ub].ent;
+                if (any) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float t = acc[ub][i] == -INFINITY ? -1.0e4f : fmaf(acc[ub][i], f, -m);
+                        const float e = __builtin_amdgcn_exp2f(t);
+                        sum += e;
+                        ent = fmaf(e, t, ent);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float t = fmaf(acc[ub][i], f, -m);
+                        const float e = __builtin_amdgcn_exp2f(t);
+                        sum += e;
+                        ent = fmaf(e, t, ent);
+                    }
+                }
+                st[ub].sum = sum;
+                st[ub].ent = ent;
+            }
+        }
+        if constexpr (TOP) {
+#pragma unroll
+            for (int ub = 0; ub < UB; ++ub) {
+                const int64_t r = row0 + 32 * ub + l31;
+                if (r < sh.rows) keys[(size_t)r * (2 * groups) + 2 * g + hi] = make_uint4(key[ub][0], key[ub][1], key[ub][2], key[ub][3]);
+            }
+        }
+    }
+    // the two halves of a row, then the row's partial of this split
+#pragma unroll
+    for (int ub = 0; ub < UB; ++ub) {
+        Stat o = {__shfl_xor(st[ub].m, 32, 64), __shfl_xor(st[ub].sum, 32, 64), __shfl_xor(st[ub].ent, 32, 64)};
+        const float m = fmaxf(st[ub].m, o.m);
+        stat_lift(st[ub], m);
+        stat_lift(o, m);
+        const int64_t r = row0 + 32 * ub + l31;
+        if (hi == 0 && r < sh.rows) part[(size_t)r * splits + blockIdx.x] = make_float4(m, st[ub].sum + o.sum, st[ub].ent + o.ent, 0.0f);
+    }
+}
+
+// ---- few rows ---------------------------------------------------------------------------------------------------------------------------
+// A wavefront takes 32-item tiles in two halves of 16 rows.  Row m of half h of a tile is item 16 (m >> 3) + 4 ((m >> 2) & 1) + (m & 3) + 8 h:
+// lane (user l & 15, g = l >> 4) then holds, over both halves, exactly one chunk of wide_kernel's numbering (h = g >> 1, hi = g & 1).
+template <int D, bool F32, int UB, bool MASK, bool TOP>
+__global__ __launch_bounds__(256) void thin_kernel(const void *__restrict__ P, const void *__restrict__ Q, Shape sh, const uint32_t *__restrict__ bits,
+                                                   const float *__restrict__ row_ref, float4 *__restrict__ part, uint16_t *__restrict__ keys)
+{
+    constexpr int NL = F32 ? D / 16 : D / 32;              // 16-byte loads of a lane per item row
+    constexpr int EPL = F32 ? 4 : 8;                       // elements of one
+    __shared__ float4 s_part[4][16 * UB];
+    const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, g = lane >> 4, l15 = lane & 15;
+    const int64_t tiles = (sh.items + kTile - 1) / kTile;
+
+    auto load = [&](const void *t, int64_t row, int n) { return *reinterpret_cast<const u32x4 *>((const char *)t + (size_t)row * (D * (F32 ? 4 : 2)) + n * 64 + g * 16); };
+    u32x4 b[UB][NL];
+    float rowf[UB], ref[UB];
+    Stat st[UB];
+#pragma unroll
+    for (int ub = 0; ub < UB; ++ub) {
+        const int64_t r = 16 * ub + l15;
+        const int32_t u = sh.user_ids[r < sh.rows ? r : sh.rows - 1];
+        const bool ok = row_ok(u, sh.users);
+#pragma unroll
+        for (int n = 0; n < NL; ++n) b[ub][n] = load(P, ok ? u : 0, n);
+        rowf[ub] = ok ? sh.scale * kLog2e : 0.0f;
+        ref[ub] = TOP && ok ? row_ref[r < sh.rows ? r : sh.rows - 1] : 0.0f;
+        st[ub] = {kNone, 0.0f, 0.0f};
+    }
+    const int64_t words = mask_words(sh.items), groups = (sh.items + 127) / 128;
+    const int irow = 16 * (l15 >> 3) + 4 * ((l15 >> 2) & 1) + (l15 & 3);
+    const int64_t step = (int64_t)gridDim.x * 4;
+    const int64_t first = (int64_t)blockIdx.x * 4 + wid;
+    u32x4 a[2][NL];
+    auto fetch = [&](int64_t tile, int h) {
+        int64_t i = tile * kTile + irow + 8 * h;
+        i = i < sh.items ? i : sh.items - 1;
+#pragma unroll
+        for (int n = 0; n < NL; ++n) a[h][n] = load(Q, i, n);
+    };
+    if (first < tiles) { fetch(first, 0); fetch(first, 1); }
+    for (int64_t tile = first; tile < tiles; tile += step) {
+        uint32_t w[UB];
+        const int64_t left = sh.items - tile * kTile;
+        const uint32_t none = left >= 32 ? 0u : 0xFFFFFFFFu << left;
+#pragma unroll
+        for (int ub = 0; ub < UB; ++ub) {
+            w[ub] = none;
+            if constexpr (MASK) {
+                const int64_t r = 16 * ub + l15;
+                w[ub] |= bits[(size_t)(r < sh.rows ? r : sh.rows - 1) * words + tile];
+            }
+        }
+        f32x4 acc[2][UB];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int ub = 0; ub < UB; ++ub) acc[h][ub] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int n = 0; n < NL; ++n) {
+#pragma unroll
+                for (int ub = 0; ub < UB; ++ub) {
+                    if constexpr (F32) {
+#pragma unroll
+                        for (int e = 0; e < EPL; ++e)
+                            acc[h][ub] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[h][n][e]), __uint_as_float(b[ub][n][e]), acc[h][ub], 0, 0, 0);
+                    } else {
+                        acc[h][ub] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a[h][n]), __builtin_bit_cast(bf16x8, b[ub][n]), acc[h][ub], 0, 0, 0);
+                    }
+                }
+            }
+            if (tile + step < tiles) fetch(tile + step, h);        // (into the half that was just used up)
+        }
+#pragma unroll
+        for (int ub = 0; ub < UB; ++ub) {
+            const float f = rowf[ub];
+            // result layout of the 16 x 16 instruction: register i of lane l is row 4 (l >> 4) + i
+            const uint32_t ws = w[ub] >> (16 * (g >> 1) + 4 * (g & 1));
+            const bool any = __builtin_amdgcn_ballot_w64((ws & 0x0F0Fu) != 0u) != 0ull;
+            float x[8];
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[4 * h + i] = any && ((ws >> (8 * h + i)) & 1u) ? -INFINITY : acc[h][ub][i];
+            float c = x[0];
+#pragma unroll
+            for (int i = 1; i < 8; ++i) c = fmaxf(c, x[i]);
+            const float top = c * f;
+            if constexpr (TOP) {
+                const int64_t r = 16 * ub + l15;
+                if (r < sh.rows) keys[(size_t)r * (16 * groups) + 16 * (tile >> 2) + 8 * (g & 1) + 2 * (tile & 3) + (g >> 1)] = half_bits(fmaf(c, f, -ref[ub]));
+            }
+            if (__builtin_amdgcn_ballot_w64(top > st[ub].m + kLazy) != 0ull) {
+                if (top > st[ub].m) stat_lift(st[ub], top);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float t = x[i] == -INFINITY ? -1.0e4f : fmaf(x[i], f, -st[ub].m);
+                const float e = __builtin_amdgcn_exp2f(t);
+                st[ub].sum += e;
+                st[ub].ent = fmaf(e, t, st[ub].ent);
+            }
+        }
+    }
+    // four lanes and four wavefronts hold a row
+#pragma unroll
+    for (int ub = 0; ub < UB; ++ub) {
+#pragma unroll
+        for (int o = 16; o <= 32; o <<= 1) {
+            Stat q = {__shfl_xor(st[ub].m, o, 64), __shfl_xor(st[ub].sum, o, 64), __shfl_xor(st[ub].ent, o, 64)};
+            const float m = fmaxf(st[ub].m, q.m);
+            stat_lift(st[ub], m);
+            stat_lift(q, m);
+            st[ub].sum += q.sum;
+            st[ub].ent += q.ent;
+        }
+        if (g == 0) s_part[wid][16 * ub + l15] = make_float4(st[ub].m, st[ub].sum, st[ub].ent, 0.f);
+    }
+    __syncthreads();
+    if (tid < 16 * UB && tid < sh.rows) {
+        Stat s = {kNone, 0.f, 0.f};
+        float m = kNone;
+        for (int q = 0; q < 4; ++q) m = fmaxf(m, s_part[q][tid].x);
+        s.m = m;
+        for (int q = 0; q < 4; ++q) {
+            Stat o = {s_part[q][tid].x, s_part[q][tid].y, s_part[q][tid].z};
+            stat_lift(o, m);
+            s.sum += o.sum;
+            s.ent += o.ent;
+        }
+        part[(size_t)tid * gridDim.x + blockIdx.x] = make_float4(s.m, s.sum, s.ent, 0.f);
+    }
+    // chunk maxima behind the last tile of a group: none
+    if constexpr (TOP) {
+        if (blockIdx.x == 0) {
+            const int spare = (int)(4 * groups - tiles);
+            for (int64_t t = tid; t < sh.rows * spare * 4; t += 256) {
+                const int64_t r = t / (spare * 4), q = t % (spare * 4), tile = tiles + q / 4;
+                keys[(size_t)r * (16 * groups) + 16 * (tile >> 2) + 8 * (q & 1) + 2 * (tile & 3) + ((q >> 1) & 1)] = 0xFC00u;      // -inf
+            }
+        }
+    }
+}
+
+// ---- one workgroup per row: join the partials, the given items, the K best -------------------------------------------------------------
+constexpr int kFin = 256;
+constexpr int kMaxChunks = 256;                   // chunks whose items are computed again; more (ties by the thousand): the whole row is
+constexpr int kCand = 8 * kMaxChunks;
+constexpr int kListed = 4096;                     // chunks looked at more closely for that choice
+static_assert(kListed * 4 <= kCand * 8 && kListed * 2 <= kCand * 4, "the list of chunks lies in the candidates' memory");
+
+// (score, id) order: larger score first, then lower id
+__device__ __forceinline__ bool before(double sa, int32_t ia, double sb, int32_t ib) { return sa > sb || (sa == sb && ia < ib); }
+
+__device__ void sort_candidates(double *s, int32_t *id, int n)          // descending; n <= kCand entries, padded here to a power of two
+{
+    int n2 = 1;
+    while (n2 < n) n2 <<= 1;
+    for (int t = n + threadIdx.x; t < n2; t += kFin) { s[t] = -INFINITY; id[t] = 0x7FFFFFFF; }
+    __syncthreads();
+    for (int size = 2; size <= n2; size <<= 1)
+        for (int stride = size >> 1; stride > 0; stride >>= 1) {
+            for (int t = threadIdx.x; t < n2 / 2; t += kFin) {
+                const int lo = 2 * t - (t & (stride - 1)), hi = lo + stride;
+                const bool down = (lo & size) == 0;
+                if (before(s[hi], id[hi], s[lo], id[lo]) == down) {
+                    const double x = s[lo]; s[lo] = s[hi]; s[hi] = x;
+                    const int32_t y = id[lo]; id[lo] = id[hi]; id[hi] = y;
+                }
+            }
+            __syncthreads();
+        }
+}
+
+template <int D, bool F32>
+__global__ __launch_bounds__(kFin) void finish_kernel(const void *__restrict__ P, const void *__restrict__ Q, Shape sh, const uint32_t *__restrict__ bits,
+                                                      const float4 *__restrict__ part, int splits, const uint16_t *__restrict__ keys,
+                                                      const int32_t *__restrict__ given, int T, int K, float *__restrict__ logp, float *__restrict__ lse_out,
+                                                      float *__restrict__ ent_out, int32_t *__restrict__ top_idx, float *__restrict__ top_logp)
+{
+    constexpr int LPI = F32 ? D / 4 : D / 8, EPL = F32 ? 4 : 8, IPP = kFin / LPI;      // lanes an item's row takes, elements a lane, items a pass
+    __shared__ double c_s[kCand];
+    __shared__ int32_t c_id[kCand];
+    __shared__ double s_lse;
+    __shared__ double s_red[3][4];
+    __shared__ uint16_t s_max[kFin];
+    __shared__ int32_t s_list[kMaxChunks];
+    __shared__ int s_n, s_count;
+    __shared__ uint32_t s_tau;
+    const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+    const int64_t r = blockIdx.x;
+    const int32_t u = sh.user_ids[r];
+    if (!row_ok(u, sh.users)) {                    // no row: nothing is probable, nothing has a log-probability
+        for (int t = tid; t < T; t += kFin) logp[r * T + t] = 0.0f;
+        for (int t = tid; t < K; t += kFin) { top_idx[r * K + t] = -1; top_logp[r * K + t] = -INFINITY; }
+        if (tid == 0) { if (lse_out) lse_out[r] = -INFINITY; if (ent_out) ent_out[r] = 0.0f; }
+        return;
+    }
+    // the partials, in 64 bits
+    double m = kNone, sum = 0.0, ent = 0.0;
+    for (int s = tid; s < splits; s += kFin) m = fmax(m, (double)part[r * splits + s].x);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = fmax(m, __shfl_xor(m, o, 64));
+    if (lane == 0) s_red[0][wid] = m;
+    __syncthreads();
+    m = fmax(fmax(s_red[0][0], s_red[0][1]), fmax(s_red[0][2], s_red[0][3]));
+    for (int s = tid; s < splits; s += kFin) {
+        const float4 p = part[r * splits + s];
+        if (p.y == 0.0f) continue;                 // (met nothing; NaN sums are kept)
+        const double w = exp2((double)p.x - m);
+        sum += w * p.y;
+        ent += w * ((double)p.z + (double)p.y * ((double)p.x - m));
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) { sum += __shfl_xor(sum, o, 64); ent += __shfl_xor(ent, o, 64); }
+    if (lane == 0) { s_red[1][wid] = sum; s_red[2][wid] = ent; }
+    __syncthreads();
+    if (tid == 0) {
+        sum = s_red[1][0] + s_red[1][1] + s_red[1][2] + s_red[1][3];
+        ent = s_red[2][0] + s_red[2][1] + s_red[2][2] + s_red[2][3];
+        const double l2 = log2(sum);
+        const double lse = sum == 0.0 ? -INFINITY : kLn2 * (m + l2);
+        s_lse = lse;
+        if (lse_out) lse_out[r] = (float)lse;
+        if (ent_out) ent_out[r] = sum == 0.0 ? 0.0f : (float)(kLn2 * (l2 - ent / sum));
+    }
+    __syncthreads();
+    const double lse = s_lse;
+
+    // a lane's elements of the row's user, and its share of an item's product in 64 bits
+    const int li = tid % LPI;
+    double p[EPL];
+    auto elements = [&](const void *t, int64_t row, double *x) {
+        const uint4 v = *reinterpret_cast<const uint4 *>((const char *)t + (size_t)row * (D * (F32 ? 4 : 2)) + li * 16);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (F32) x[j] = (double)__uint_as_float(w[j]);
+            else { x[2 * j] = (double)__uint_as_float(w[j] << 16); x[2 * j + 1] = (double)__uint_as_float(w[j] & 0xFFFF0000u); }
+        }
+    };
+    elements(P, u, p);
+    const int64_t words = mask_words(sh.items);
+    const uint32_t *seen = bits ? bits + (size_t)r * words : nullptr;
+    auto masked = [&](int32_t i) { return seen != nullptr && ((seen[i >> 5] >> (i & 31)) & 1u); };
+    // four items at a time: their rows are on the way together
+    auto dots = [&](const int64_t (&i)[4], double (&z)[4]) {
+        double q[4][EPL];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) elements(Q, i[n], q[n]);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            z[n] = 0.0;
+#pragma unroll
+            for (int j = 0; j < EPL; ++j) z[n] = fma(p[j], q[n][j], z[n]);
+        }
+#pragma unroll
+        for (int o = LPI / 2; o > 0; o >>= 1)
+#pragma unroll
+            for (int n = 0; n < 4; ++n) z[n] += __shfl_xor(z[n], o, LPI);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) z[n] *= (double)sh.scale;
+    };
+    for (int t0 = tid / LPI; t0 < T; t0 += 4 * IPP) {
+        int64_t i[4];
+        double z[4];
+        bool ok[4];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            const int t = t0 + n * IPP;
+            i[n] = t < T ? given[r * T + t] : -1;
+            ok[n] = i[n] >= 0 && i[n] < sh.items;
+            i[n] = ok[n] ? i[n] : 0;
+        }
+        dots(i, z);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            const int t = t0 + n * IPP;
+            if (li == 0 && t < T) logp[r * T + t] = !ok[n] ? 0.0f : masked((int32_t)i[n]) ? -INFINITY : (float)(z[n] - lse);
+        }
+    }
+    if (K == 0) return;
+
+    // K + 8 chunks with the largest maxima, and all that equal the last of them: a lower bound of that maximum comes from 256 threads' own
+    const int64_t chunks = (sh.items + 127) / 128 * 16;
+    const uint16_t *key = keys + (size_t)r * chunks;
+    auto order = [](uint32_t h) { return (h & 0x8000u) ? (~h & 0xFFFFu) : (h | 0x8000u); };      // halves -> ordered integers (NaN above all)
+    const uint32_t lowest = order(0xFC00u);                                                         // -inf: nothing in the chunk
+    uint32_t mine = 0;
+    auto walk = [&](auto f) {            // every chunk once, 8 at a time where there are many
+        if (chunks > 16 * kFin) {
+            for (int64_t c = 8 * tid; c < chunks; c += 8 * kFin) {
+                const uint4 v = *reinterpret_cast<const uint4 *>(key + c);
+                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) { f(order(w[j] & 0xFFFFu), c + 2 * j); f(order(w[j] >> 16), c + 2 * j + 1); }
+            }
+        } else {
+            for (int64_t c = tid; c < chunks; c += kFin) f(order(key[c]), c);
+        }
+    };
+    walk([&](uint32_t k, int64_t) { mine = k > mine ? k : mine; });
+    s_max[tid] = (uint16_t)mine;
+    if (tid == 0) { s_n = 0; s_tau = lowest + 1; }
+    __syncthreads();
+    int above = 0;
+    for (int t = 0; t < kFin; ++t) above += s_max[t] > mine || (s_max[t] == mine && t < tid);
+    if (above == K + 7 && mine > lowest) s_tau = mine;
+    __syncthreads();
+    // the chunks from that bound up, with their maxima (in the candidates' memory); where the bound was loose -- the best items' chunks were
+    // few threads' -- the K + 8-th largest maximum among them is found bit by bit
+    int32_t *const l_chunk = reinterpret_cast<int32_t *>(c_s);
+    uint16_t *const l_key = reinterpret_cast<uint16_t *>(c_id);
+    const uint32_t bound = s_tau;
+    walk([&](uint32_t k, int64_t c) {
+        if (k >= bound) {
+            const int at = atomicAdd(&s_n, 1);
+            if (at < kListed) { l_chunk[at] = (int32_t)c; l_key[at] = (uint16_t)k; }
+        }
+    });
+    __syncthreads();
+    const int listed = s_n;
+    uint32_t tau = bound;
+    if (listed > kMaxChunks && listed <= kListed) {
+        tau = 0;
+        for (int bit = 15; bit >= 0; --bit) {
+            const uint32_t t = tau | (1u << bit);
+            if (tid == 0) s_count = 0;
+            __syncthreads();
+            int c = 0;
+            for (int q = tid; q < listed; q += kFin) c += l_key[q] >= t;
+            if (c) atomicAdd(&s_count, c);
+            __syncthreads();
+            if (s_count >= K + 8) tau = t;
+            __syncthreads();
+        }
+    }
+    if (tid == 0) s_n = listed <= kListed ? 0 : listed;
+    __syncthreads();
+    if (listed <= kListed) {
+        for (int q = tid; q < listed; q += kFin)
+            if (l_key[q] >= tau) {
+                const int at = atomicAdd(&s_n, 1);
+                if (at < kMaxChunks) s_list[at] = l_chunk[q];
+            }
+    }
+    __syncthreads();
+    int n;
+    if (s_n <= kMaxChunks) {
+        n = 8 * s_n;
+        for (int q0 = tid / LPI; q0 < n; q0 += 4 * IPP) {
+            int64_t i[4];
+            double z[4];
+            bool ok[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int q = q0 + k * IPP;
+                i[k] = q < n ? chunk_item0(s_list[q >> 3]) + (q & 3) + 2 * (q & 4) : sh.items;
+                ok[k] = i[k] < sh.items;
+                i[k] = ok[k] ? i[k] : 0;
+            }
+            dots(i, z);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int q = q0 + k * IPP;
+                if (li == 0 && q < n) {
+                    const bool in = ok[k] && z[k] == z[k] && !masked((int32_t)i[k]);
+                    c_s[q] = in ? z[k] : -INFINITY;
+                    c_id[q] = in ? (int32_t)i[k] : 0x7FFFFFFF;
+                }
+            }
+        }
+        __syncthreads();
+        sort_candidates(c_s, c_id, n);
+    } else {
+        // the row in blocks of half the list: what exceeds the K-th best so far is added, and the list cut to K when it is half full
+        __shared__ int s_m;
+        if (tid == 0) s_m = 0;
+        double floor_ = -INFINITY;
+        __syncthreads();
+        for (int64_t base = 0; base < sh.items; base += kCand / 2) {
+            const int64_t end = base + kCand / 2 < sh.items ? base + kCand / 2 : sh.items;
+            for (int64_t q0 = base + tid / LPI; q0 < base + kCand / 2; q0 += 4 * IPP) {      // (whole groups of lanes stay together)
+                int64_t i[4];
+                double z[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) i[k] = q0 + k * IPP < end ? q0 + k * IPP : 0;
+                dots(i, z);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    if (li == 0 && q0 + k * IPP < end && z[k] > floor_ && !masked((int32_t)i[k])) {
+                        const int at = atomicAdd(&s_m, 1);
+                        c_s[at] = z[k];
+                        c_id[at] = (int32_t)i[k];
+                    }
+                }
+            }
+            __syncthreads();
+            const int have = s_m;
+            __syncthreads();
+            if (have > kCand / 2 || end == sh.items) {
+                sort_candidates(c_s, c_id, have);
+                if (have >= K) floor_ = c_s[K - 1];
+                if (tid == 0) s_m = have < K ? have : K;
+                __syncthreads();
+            }
+        }
+        n = s_m;
+    }
+    for (int t = tid; t < K; t += kFin) {
+        const bool in = t < n && c_id[t] != 0x7FFFFFFF;
+        top_idx[r * K + t] = in ? c_id[t] : -1;
+        top_logp[r * K + t] = in ? (float)(c_s[t] - lse) : -INFINITY;
+    }
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------------------------------------
+int thin_rows(int d, int dtype)                // rows the thin form takes: operands of 16 rows cost d / 4 (fp32) or d / 8 registers
+{
+    const int ub = dtype == RSX_F32 ? 256 / d : 512 / d;
+    return 16 * (ub > 4 ? 4 : ub);
+}
+
+int thin_groups(int64_t items)
+{
+    const int64_t tiles = (items + kTile - 1) / kTile, want = (tiles + 3) / 4, most = (int64_t)rsx_num_cus() * 4;
+    return (int)(want < most ? want : most);
+}
+
+struct Ws {
+    char *planes;
+    float *factor;
+    uint32_t *bits;
+    float *ref;
+    float4 *part;
+    uint16_t *keys;
+    int64_t pass, bytes;      // rows of one pass over the catalog
+};
+
+int wide_users(int d, int dtype) { return d * (dtype == RSX_F32 ? 2 : 1) <= 256 ? 256 : 128; }
+
+int64_t wide_splits(int64_t rows, int64_t items, int d, int dtype)
+{
+    const int64_t slots = 2 * (int64_t)rsx_num_cus(), ut = (rows + wide_users(d, dtype) - 1) / wide_users(d, dtype), groups = (items + 127) / 128;
+    const int64_t s = slots / ut;
+    return s < 1 ? 1 : s > groups ? groups : s;
+}
+
+// a pass' bits and chunk maxima are held to 768 MB
+int64_t pass_rows(int64_t rows, int64_t items)
+{
+    const int64_t per = mask_words(items) * 4 + (items + 127) / 128 * 32;
+    int64_t most = (768ll << 20) / per / 256 * 256;
+    most = most < 256 ? 256 : most;
+    return rows < most ? rows : most;
+}
+
+Ws carve(void *ws, int64_t rows, int64_t items, int d, int dtype, bool mask, int K)
+{
+    Ws w;
+    char *base = (char *)ws;
+    int64_t off = 0;
+    auto take = [&](int64_t n) { char *q = base + off; off += a256(n); return q; };
+    const int64_t tiles4 = (items + 127) / 128 * 4;
+    const bool thin = rows <= thin_rows(d, dtype);
+    w.pass = pass_rows(rows, items);
+    const int64_t parts = thin ? thin_groups(items) : wide_splits(w.pass, items, d, dtype);
+    // (the last, shorter pass takes more splits over fewer rows: rows x splits never exceeds this)
+    const int64_t cells = thin ? rows * parts : w.pass * parts + 2 * (int64_t)rsx_num_cus() * wide_users(d, dtype);
+    w.planes = take(!thin && dtype == RSX_F32 ? tiles4 * kTile * (int64_t)d * 4 : 0);
+    w.factor = (float *)take(!thin && dtype == RSX_F32 ? tiles4 * 4 : 0);
+    w.bits = (uint32_t *)take(mask ? w.pass * mask_words(items) * 4 : 0);
+    w.ref = (float *)take(w.pass * 4);
+    w.part = (float4 *)take(cells * 16);
+    w.keys = (uint16_t *)take(K > 0 ? w.pass * ((items + 127) / 128) * 32 : 0);
+    w.bytes = off;
+    return w;
+}
+
+struct Call {
+    const void *P, *Q;
+    Shape sh;
+    const int64_t *indptr;
+    const int32_t *indices;
+    const int32_t *given;
+    int T, K;
+    float *logp, *lse, *ent;
+    int32_t *top_idx;
+    float *top_logp;
+};
+
+template <int D, bool F32, int UB>
+void launch_thin(const Call &c, const Shape &sh, const Ws &w, int groups, hipStream_t st)
+{
+#define RSX_LP_THIN(M_, T_) hipLaunchKernelGGL((thin_kernel<D, F32, UB, M_, T_>), dim3(groups), dim3(256), 0, st, c.P, c.Q, sh, w.bits, w.ref, w.part, w.keys)
+    if (c.indptr) { if (c.K) RSX_LP_THIN(true, true); else RSX_LP_THIN(true, false); }
+    else { if (c.K) RSX_LP_THIN(false, true); else RSX_LP_THIN(false, false); }
+#undef RSX_LP_THIN
+}
+
+template <int D, bool F32>
+void run(const Call &c, const Ws &w, hipStream_t st)
+{
+    const bool thin = c.sh.rows <= thin_rows(D, F32 ? RSX_F32 : RSX_BF16);
+    const int64_t items = c.sh.items, tiles4 = (items + 127) / 128 * 4;
+    if constexpr (F32)
+        if (!thin) hipLaunchKernelGGL(split_items_kernel<D>, dim3((unsigned)tiles4), dim3(256), 0, st, (const float *)c.Q, items, (uint4 *)w.planes, w.factor);
+    for (int64_t r0 = 0; r0 < c.sh.rows; r0 += w.pass) {
+        Shape sh = c.sh;
+        sh.user_ids += r0;
+        sh.rows = c.sh.rows - r0 < w.pass ? c.sh.rows - r0 : w.pass;
+        if (c.indptr) launch_clear_bits(sh.rows, items, w.bits, st);
+        if (c.indptr || c.K)
+            hipLaunchKernelGGL((row_prep_kernel<D, F32>), dim3((unsigned)((sh.rows + 3) / 4)), dim3(256), 0, st, c.P, c.Q, sh, c.indptr, c.indices, w.bits,
+                               c.K ? w.ref : (float *)nullptr);
+        int parts;
+        if (thin) {
+            parts = thin_groups(items);
+            constexpr int MOST = F32 ? 256 / D : 512 / D;
+            if (sh.rows <= 16) launch_thin<D, F32, 1>(c, sh, w, parts, st);
+            else if constexpr (MOST >= 2) {
+                if (sh.rows <= 32) launch_thin<D, F32, 2>(c, sh, w, parts, st);
+                else if constexpr (MOST >= 4) launch_thin<D, F32, 4>(c, sh, w, parts, st);
+            }
+        } else {
+            parts = (int)wide_splits(sh.rows, items, D, F32 ? RSX_F32 : RSX_BF16);
+            const dim3 grid((unsigned)parts, (unsigned)((sh.rows + WideGeo<D, F32>::WGU - 1) / WideGeo<D, F32>::WGU));
+#define RSX_LP_WIDE(M_, T_) hipLaunchKernelGGL((wide_kernel<D, F32, M_, T_>), grid, dim3(256), 0, st, c.P, c.Q, w.planes, w.factor, sh, w.bits, w.ref, parts, w.part, (uint4 *)w.keys)
+            if (c.indptr) { if (c.K) RSX_LP_WIDE(true, true); else RSX_LP_WIDE(true, false); }
+            else { if (c.K) RSX_LP_WIDE(false, true); else RSX_LP_WIDE(false, false); }
+#undef RSX_LP_WIDE
+        }
+        hipLaunchKernelGGL((finish_kernel<D, F32>), dim3((unsigned)sh.rows), dim3(kFin), 0, st, c.P, c.Q, sh, c.indptr ? w.bits : (const uint32_t *)nullptr, w.part,
+                           parts, w.keys, c.given + (c.T ? r0 * c.T : 0), c.T, c.K, c.logp + (c.T ? r0 * c.T : 0), c.lse ? c.lse + r0 : nullptr,
+                           c.ent ? c.ent + r0 : nullptr, c.top_idx + (c.K ? r0 * c.K : 0), c.top_logp + (c.K ? r0 * c.K : 0));
+    }
+}
+
+}  // namespace
+
+RSX_API int64_t rsx_score_logprobs_workspace(int64_t num_rows, int64_t num_items, int d, int dtype, int masked, int K)
+{
+    if (num_rows < 0 || num_items <= 0 || num_items >= (1ll << 31) - 128 || !rsx_dim_ok(d) || (dtype != RSX_F32 && dtype != RSX_BF16) || K < 0 || K > kMaxK)
+        return RSX_E_INVALID;
+    return carve(nullptr, num_rows < 1 ? 1 : num_rows, num_items, d, dtype, masked != 0, K).bytes;
+}
+
+RSX_API int rsx_score_logprobs(const void *P, int64_t num_users, const int32_t *user_ids_dev, int64_t num_rows, const void *Q, int64_t num_items, int d,
+                               int dtype, const int64_t *mask_indptr_dev, const int32_t *mask_indices_dev, float scale, const int32_t *items_dev, int T, int K,
+                               float *logp_out, float *lse_out, float *entropy_out, int32_t *topk_idx_out, float *topk_logp_out, void *ws, int64_t ws_bytes,
+                               rsx_stream_t stream)
+{
+    RSX_CHECK_ARG(P && Q && user_ids_dev, "null pointer");
+    RSX_CHECK_ARG(rsx_dim_ok(d), "d must be 32, 64, 128 or 256");
+    RSX_CHECK_ARG(dtype == RSX_F32 || dtype == RSX_BF16, "dtype must be RSX_F32 or RSX_BF16");
+    RSX_CHECK_ARG(num_rows >= 0 && num_users > 0 && num_items > 0 && num_items < (1ll << 31) - 128, "bad shape");
+    RSX_CHECK_ARG((mask_indptr_dev == nullptr) == (mask_indices_dev == nullptr), "mask needs both CSR arrays");
+    RSX_CHECK_ARG(scale > 0.0f && scale < INFINITY, "scale must be positive and finite");
+    RSX_CHECK_ARG(T >= 0 && (T == 0 || (items_dev && logp_out)), "T items per row need their ids and an output");
+    RSX_CHECK_ARG(K >= 0 && K <= kMaxK && K <= num_items && (K == 0 || (topk_idx_out && topk_logp_out)), "K must be in [0, min(128, num_items)], with both outputs");
+    RSX_CHECK_ARG(aligned16(P) && aligned16(Q), "table rows must be 16-byte aligned");
+    if (num_rows == 0) return RSX_OK;
+    const Ws w = carve(ws, num_rows, num_items, d, dtype, mask_indptr_dev != nullptr, K);
+    if (ws == nullptr || ws_bytes < w.bytes || !aligned16(ws)) {
+        rsx_set_error("rsx_score_logprobs: workspace of %lld bytes (16-byte aligned) required, got %lld", (long long)w.bytes, (long long)ws_bytes);
+        return RSX_E_WORKSPACE;
+    }
+    const Call c{P, Q, {user_ids_dev, num_rows, num_users, num_items, scale}, mask_indptr_dev, mask_indices_dev, items_dev, T, K,
+                 logp_out, lse_out, entropy_out, topk_idx_out, topk_logp_out};
+    hipStream_t st = (hipStream_t)stream;
+#define RSX_LP_RUN(D_) do { if (dtype == RSX_F32) run<D_, true>(c, w, st); else run<D_, false>(c, w, st); } while (0)
+    switch (d) {
+    case 32: RSX_LP_RUN(32); break;
+    case 64: RSX_LP_RUN(64); break;
+    case 128: RSX_LP_RUN(128); break;
+    default: RSX_LP_RUN(256); break;
+    }
+#undef RSX_LP_RUN
+    RSX_CHECK_LAUNCH();
+    return RSX_OK;
+}

@@ -6,6 +6,7 @@ library or a non-device tensor raises.
 """
 import ctypes as C
 import os
+from collections import namedtuple
 
 import torch
 
@@ -108,6 +109,8 @@ SIGNATURES = {
     "rsx_mesh_check": (C.c_int, [_P, _P]),
     "rsx_mesh_export_retries": (C.c_int, [_P]),
     "rsx_mesh_destroy": (None, [_P]),
+    "rsx_score_logprobs_workspace": (_I64, [_I64, _I64, _I32, _I32, _I32, _I32]),
+    "rsx_score_logprobs": (C.c_int, [_P, _I64, _P, _I64, _P, _I64, _I32, _I32, _P, _P, _F, _P, _I32, _I32, _P, _P, _P, _P, _P, _P, _I64, _P]),
     "rsx_score": (C.c_int, [_P, _P, _I64, _P, _I64, _I32, _P, _P, _P, _P]),
     "rsx_topk": (C.c_int, [_P, _I64, _I64, _I32, _P, _P, _P]),
     "rsx_score_topk_workspace": (_I64, [_I64, _I64]),
@@ -1117,3 +1120,48 @@ def score_topk(P, Q, user_ids, K, mask=None, want_values=False, ws=None):
         _dev(val, torch.float32, "val") if val is not None else None,
         C.c_void_p(ws.data_ptr()), ws.numel() * ws.element_size(), _stream()), "rsx_score_topk")
     return (idx, val) if want_values else idx
+
+
+LogProbs = namedtuple("LogProbs", "logp lse entropy top_idx top_logp")
+
+
+def score_logprobs_workspace(rows, num_items, d, dtype=torch.float32, masked=False, K=0):
+    n = lib().rsx_score_logprobs_workspace(int(rows), int(num_items), int(d), _DTYPES.get(dtype, -1), int(bool(masked)), int(K))
+    if n < 0:
+        raise RsxError("rsx_score_logprobs_workspace: invalid shape")
+    return n
+
+
+def _logprob_args(P, Q, user_ids, items, mask):
+    """checks what score_logprobs and its gradient share: (P, Q, ids, items pointers, dtype, rows, T, mask pointers)"""
+    dt = _dtype(P, "P")
+    pp, pq = _matrix(P, "P"), _matrix(Q, "Q", d=P.shape[1], dtype=P.dtype)
+    pu = _dev(user_ids, torch.int32, "user_ids")
+    rows = user_ids.numel()
+    if items is not None and (items.dim() != 2 or items.shape[0] != rows):
+        raise RsxError(f"items must be a [{rows} x T] tensor")
+    pi = _dev(items, torch.int32, "items") if items is not None else None
+    mp, mi = _mask_ptrs(mask)
+    if mask is not None and mask[0].numel() != P.shape[0] + 1:
+        raise RsxError(f"mask indptr must have {P.shape[0] + 1} entries, got {mask[0].numel()}")
+    return pp, pq, pu, pi, dt, rows, (items.shape[1] if items is not None else 0), mp, mi
+
+
+def score_logprobs(P, Q, user_ids, items=None, K=0, mask=None, scale=1.0, ws=None):
+    """log-softmax of S = scale * P[user_ids] @ Q.T over the catalog, without S (include/rsx.h:rsx_score_logprobs): LogProbs with
+    logp [n x T] of the given items (None without `items`), lse and entropy [n], the K most probable items and their
+    log-probabilities [n x K] (None for K = 0).  float32 or bfloat16 tables; mask: CSR of seen items by user id."""
+    pp, pq, pu, pi, dt, rows, T, mp, mi = _logprob_args(P, Q, user_ids, items, mask)
+    (num_users, d), num_items, K = P.shape, Q.shape[0], int(K)
+    new = lambda *s, dtype=torch.float32: torch.empty(s, dtype=dtype, device=P.device)
+    out = LogProbs(new(rows, T) if items is not None else None, new(rows), new(rows),
+                   new(rows, K, dtype=torch.int32) if K > 0 else None, new(rows, K) if K > 0 else None)
+    if rows == 0:
+        return out
+    ptr = lambda t: C.c_void_p(t.data_ptr()) if t is not None else None
+    with _same_device(P, Q, user_ids, items, *(mask or ())):
+        ws = _scratch(ws, score_logprobs_workspace(rows, num_items, d, P.dtype, mask is not None, K), P.device)
+        _check(lib().rsx_score_logprobs(pp, num_users, pu, rows, pq, num_items, d, dt, mp, mi, float(scale), pi, T, K, ptr(out.logp), ptr(out.lse),
+                                        ptr(out.entropy), ptr(out.top_idx), ptr(out.top_logp), ptr(ws), ws.numel() * ws.element_size(), _stream()),
+               "rsx_score_logprobs")
+    return out
