@@ -253,6 +253,15 @@ int rsx_pair_score(const float *P, const float *Q, const int32_t *u_dev, const i
  * An item id outside [0, num_items) names no item: its logp is 0.  mask_indptr: int64 [num_users + 1] (nullable with
  * mask_indices); rows need not be sorted, ids outside the catalog are ignored.  What a masked cell's product would have been
  * (infinities, NaN) does not matter.
+ * rsx_score_logprobs_grad: gradient of sum_rt g_logp[r, t] logp_rt + sum_r g_entropy[r] H_r with respect to the rows:
+ *   GP[r]  = sum_i dz_ri Q[i]  [num_rows x d],   GQ[i] = sum_r dz_ri P[user_ids[r]]  [num_items x d],   both overwritten, in dtype,
+ *   dz_ri  = scale (sum_t g_logp[r, t] ([i = items[r, t]] - p_ri) - g_entropy[r] p_ri (log p_ri + H_r))
+ *   over unmasked i and the items that are neither masked nor outside the catalog (a masked item's logp is the constant -inf).
+ *   An item listed twice counts twice.  lse, entropy: what rsx_score_logprobs returned for the same arguments (entropy and
+ *   g_entropy nullable together).  GP is per POSITION: add the rows of a user that stands in the batch more than once
+ *   (rsx_add_rows).  A position that names no row has a zero row.  Bit-reproducible (no floating atomics).
+ * rsx_add_rows: T[ids[r]] += R[r] for r = 0 .. n - 1, in this order for every row of T (T fp32 [table_rows x d]; R [n x d] of dtype);
+ *   ids outside [0, table_rows) are skipped.
  * No call synchronises with the host: all can be captured into a graph.  ws: *_workspace bytes, 16-byte aligned, contents irrelevant,
  * one per concurrent call.                                                                                                    */
 int64_t rsx_score_logprobs_workspace(int64_t num_rows, int64_t num_items, int d, int dtype, int masked, int K);
@@ -260,6 +269,14 @@ int rsx_score_logprobs(const void *P, int64_t num_users, const int32_t *user_ids
                        int64_t num_items, int d, int dtype, const int64_t *mask_indptr_dev, const int32_t *mask_indices_dev,
                        float scale, const int32_t *items_dev, int T, int K, float *logp_out, float *lse_out, float *entropy_out,
                        int32_t *topk_idx_out, float *topk_logp_out, void *ws, int64_t ws_bytes, rsx_stream_t stream);
+int64_t rsx_score_logprobs_grad_workspace(int64_t num_rows, int64_t num_items, int d, int dtype, int masked, int T);
+int rsx_score_logprobs_grad(const void *P, int64_t num_users, const int32_t *user_ids_dev, int64_t num_rows, const void *Q,
+                            int64_t num_items, int d, int dtype, const int64_t *mask_indptr_dev, const int32_t *mask_indices_dev,
+                            float scale, const int32_t *items_dev, int T, const float *lse_dev, const float *g_logp_dev,
+                            const float *entropy_dev, const float *g_entropy_dev, void *GP_out, void *GQ_out, void *ws,
+                            int64_t ws_bytes, rsx_stream_t stream);
+int rsx_add_rows(float *T, int64_t table_rows, int d, const int32_t *ids_dev, const void *R, int dtype, int64_t n,
+                 rsx_stream_t stream);
 
 /* ---- on-device triplet sampler ------------------------------------------------
  * Replaces data/generators.py:151-224 (PairwiseGenerator: host-side numpy

@@ -57,23 +57,45 @@ __device__ __forceinline__ void copy_to_lds(const char *src, char *dst) { __buil
 
 // power of two that brings a largest magnitude m into [2^13, 2^14), and its inverse.  Below 2^-40 as for 2^-40: the product of two such
 // inverses stays a normal number, and what is lost there moves no score by 2^-40
-__device__ __forceinline__ void scale_for(float m, float *up, float *down)
+__device__ __forceinline__ void scale_for(float m, float *up, float *down, int least = -40)
 {
     int e = (int)((__float_as_uint(m) >> 23) & 0xFF) - 126;      // m in [2^(e-1), 2^e)
-    e = e < -40 ? -40 : e;
+    e = e < least ? least : e;
     *up = ldexpf(1.0f, 14 - e);
     *down = ldexpf(1.0f, e - 14);
 }
 __device__ __forceinline__ float finite_abs(float v) { const float a = fabsf(v); return a < INFINITY ? a : 0.0f; }     // NaN and infinities: 0
+
+// a value the compiler does not look behind.  half(a * b) becomes one fused instruction that rounds the exact product once, and where the same half
+// is also needed in fp32 (to form its remainder) the unfused one is used beside it: at a tie of the two roundings hi and lo would not belong
+// to each other (errors of 2^-11 of an element, one in some thousand).
+__device__ __forceinline__ float opaque(float v)
+{
+    asm("" : "+v"(v));
+    return v;
+}
 
 // eight scaled floats -> the two planes' fragments
 __device__ __forceinline__ void split8(const float *x, Frag *hi, Frag *lo)
 {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        const _Float16 h = (_Float16)x[j];
+        const float v = opaque(x[j]);
+        const _Float16 h = (_Float16)v;
         hi->h[j] = h;
-        lo->h[j] = (_Float16)(x[j] - (float)h);
+        lo->h[j] = (_Float16)(v - (float)h);
+    }
+}
+
+// ... of x times k, the product not rounded before it is split
+__device__ __forceinline__ void split8_times(const float *x, double k, Frag *hi, Frag *lo)
+{
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const double y = (double)x[j] * k;
+        const _Float16 h = (_Float16)opaque((float)y);
+        hi->h[j] = h;
+        lo->h[j] = (_Float16)opaque((float)(y - (double)(float)h));
     }
 }
 

@@ -129,6 +129,7 @@ __global__ __launch_bounds__(256, 2) void wide_kernel(const void *__restrict__ P
     using G = WideGeo<D, F32>;
     constexpr int UB = G::UB, KS = G::KS, NP = G::NP, ST = G::ST;
     __shared__ __attribute__((aligned(1024))) char lds[2][ST * G::TILEB];
+    __shared__ float s_all[UB][3][256];
     const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, hi = lane >> 5, l31 = lane & 31;
     const int64_t groups = (sh.items + 127) / 128;
     const int64_t g0 = groups * blockIdx.x / splits, g1 = groups * (blockIdx.x + 1) / splits;
@@ -137,7 +138,7 @@ __global__ __launch_bounds__(256, 2) void wide_kernel(const void *__restrict__ P
     // this wavefront's users: operands, scale, reference
     Frag b[UB][KS][NP];
     float rowf[UB], ref[UB];
-    Stat st[UB];
+    Stat st[UB];                          // of the current group of tiles; of all before: s_all, this lane's own slots
 #pragma unroll
     for (int ub = 0; ub < UB; ++ub) {
         const int64_t r = row0 + 32 * ub + l31;
@@ -154,23 +155,23 @@ __global__ __launch_bounds__(256, 2) void wide_kernel(const void *__restrict__ P
 #pragma unroll
                 for (int j = 0; j < 8; ++j) m = fmaxf(m, finite_abs(x[j]));
             }
-            scale_for(fmaxf(m, __shfl_xor(m, 32, 64)), &up, &down);
+            scale_for(fmaxf(m, __shfl_xor(m, 32, 64)) * (sh.scale * kLog2e), &up, &down);
         }
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             if constexpr (F32) {
                 float x[8];
                 load8<F32>(P, at + 16 * s, x);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] *= up;
-                split8(x, &b[ub][s][0], &b[ub][s][NP - 1]);
+                split8_times(x, (double)sh.scale * 1.4426950408889634074 * up, &b[ub][s][0], &b[ub][s][NP - 1]);
             } else {
                 b[ub][s][0].u = *reinterpret_cast<const uint4 *>((const uint16_t *)P + at + 16 * s);
             }
         }
-        rowf[ub] = ok ? down * sh.scale * kLog2e : 0.0f;
+        rowf[ub] = !ok ? 0.0f : F32 ? down : sh.scale * kLog2e;      // (fp32: scale log2 e is in the operands, the factor a power of two)
         ref[ub] = TOP && ok ? row_ref[r < sh.rows ? r : sh.rows - 1] : 0.0f;
         st[ub] = {kNone, 0.0f, 0.0f};
+        s_all[ub][0][tid] = kNone;
+        s_all[ub][1][tid] = s_all[ub][2][tid] = 0.0f;
     }
 
     // copies of the next ST tiles: 1 KB a wavefront instruction, lane-linear in LDS, the swizzle in the source address
@@ -252,7 +253,7 @@ __global__ __launch_bounds__(256, 2) void wide_kernel(const void *__restrict__ P
                     if (top > st[ub].m) stat_lift(st[ub], top);
                 }
                 const float m = st[ub].m;
-                float sum = st[ub].sum, ent = st[ub].ent;
+                float sum = 0.0f, ent = 0.0f;         // of the tile; then of the group, then of all: each sum adds up few terms
                 if (any) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
@@ -270,9 +271,18 @@ __global__ __launch_bounds__(256, 2) void wide_kernel(const void *__restrict__ P
                         ent = fmaf(e, t, ent);
                     }
                 }
-                st[ub].sum = sum;
-                st[ub].ent = ent;
+                st[ub].sum += sum;
+                st[ub].ent += ent;
             }
+        }
+#pragma unroll
+        for (int ub = 0; ub < UB; ++ub) {
+            Stat all = {s_all[ub][0][tid], s_all[ub][1][tid], s_all[ub][2][tid]};
+            stat_lift(all, st[ub].m);
+            s_all[ub][0][tid] = all.m;
+            s_all[ub][1][tid] = all.sum + st[ub].sum;
+            s_all[ub][2][tid] = all.ent + st[ub].ent;
+            st[ub].sum = st[ub].ent = 0.0f;
         }
         if constexpr (TOP) {
 #pragma unroll
@@ -285,12 +295,13 @@ __global__ __launch_bounds__(256, 2) void wide_kernel(const void *__restrict__ P
     // the two halves of a row, then the row's partial of this split
 #pragma unroll
     for (int ub = 0; ub < UB; ++ub) {
-        Stat o = {__shfl_xor(st[ub].m, 32, 64), __shfl_xor(st[ub].sum, 32, 64), __shfl_xor(st[ub].ent, 32, 64)};
-        const float m = fmaxf(st[ub].m, o.m);
-        stat_lift(st[ub], m);
+        Stat all = {s_all[ub][0][tid], s_all[ub][1][tid], s_all[ub][2][tid]};
+        Stat o = {__shfl_xor(all.m, 32, 64), __shfl_xor(all.sum, 32, 64), __shfl_xor(all.ent, 32, 64)};
+        const float m = fmaxf(all.m, o.m);
+        stat_lift(all, m);
         stat_lift(o, m);
         const int64_t r = row0 + 32 * ub + l31;
-        if (hi == 0 && r < sh.rows) part[(size_t)r * splits + blockIdx.x] = make_float4(m, st[ub].sum + o.sum, st[ub].ent + o.ent, 0.0f);
+        if (hi == 0 && r < sh.rows) part[(size_t)r * splits + blockIdx.x] = make_float4(m, all.sum + o.sum, all.ent + o.ent, 0.0f);
     }
 }
 
@@ -388,13 +399,16 @@ __global__ __launch_bounds__(256) void thin_kernel(const void *__restrict__ P, c
             if (__builtin_amdgcn_ballot_w64(top > st[ub].m + kLazy) != 0ull) {
                 if (top > st[ub].m) stat_lift(st[ub], top);
             }
+            float sum = 0.0f, ent = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float t = x[i] == -INFINITY ? -1.0e4f : fmaf(x[i], f, -st[ub].m);
                 const float e = __builtin_amdgcn_exp2f(t);
-                st[ub].sum += e;
-                st[ub].ent = fmaf(e, t, st[ub].ent);
+                sum += e;
+                ent = fmaf(e, t, ent);
             }
+            st[ub].sum += sum;
+            st[ub].ent += ent;
         }
     }
     // four lanes and four wavefronts hold a row
@@ -615,6 +629,7 @@ __global__ __launch_bounds__(kFin) void finish_kernel(const void *__restrict__ P
     });
     __syncthreads();
     const int listed = s_n;
+    __syncthreads();                     // (s_n is counted anew below)
     uint32_t tau = bound;
     if (listed > kMaxChunks && listed <= kListed) {
         tau = 0;

@@ -1,0 +1,712 @@
+// rsx_logprob_grad.hip -- gradient of the full-catalog log-probabilities (rsx_logprob.hip) for gfx950 (MI355X).
+//
+//   dz_ri = scale (sum_t g_rt [i = items_rt] - p_ri (sum_t g_rt + h_r (log p_ri + H_r))),   p_ri = exp(z_ri - lse_r)
+//   GP_r = sum_i dz_ri Q_i,   GQ_i = sum_r dz_ri P_r
+//
+// Neither the scores nor dz exist in memory.  Two launches of one kernel, each recomputing the scores it needs:
+//   users stay, items stream   -> GP: the p part; the T rows of Q that the positions name are added when the partial sums are joined
+//   items stay, users stream   -> GQ, with the named items inside the tile
+// A wavefront keeps 32 columns (users or items) in registers: their operands for the scores and their d sums of the gradient.  Tiles of 32
+// streaming rows come through LDS in two forms, copied asynchronously: row-major for the scores, and in the operand order of the
+// second product (transposed once, before the pass).  The scores come out of the first product with a column in a lane, which is the
+// layout the second product takes its operand in: dz goes from one to the other in registers.  The order of the contraction that this
+// fixes (register i of half h is row (i & 3) + 8 (i >> 2) + 4 h) is built into the transposed tiles.
+//
+// 8 n I d operations instead of the 6 that a stored dz would take, against 3 n I of stored and twice read halves: recomputing is the
+// cheaper side from d = 128 down (4096 x 100 000 x 128: 0.4 TFLOP against 2.4 GB).  No atomics: every sum has one order.
+//
+// fp32: three products of halves (rsx_logprob.h) on both sides; dz is a half pair too.  |dz| <= about 5 of the row's weight w_r =
+// sum |g| + |h|; it is divided by w_r, multiplied by 2^12 and its lower end is 2^-24 (a half's), 2^-36 of w_r.  w_r goes to the joined sum
+// (GP) or into the streaming rows (GQ), whose common scale is the largest of w_r |P_r|.  bf16: dz is rounded to bf16, an error of a
+// term that is at most as large as that of rounding the result (the same where one term is all of it; sums of many average theirs out).
+#include <type_traits>
+
+#include "rsx_logprob.h"
+
+namespace {
+using namespace lp;
+
+constexpr float kFar = 1.0e30f;           // log-normaliser of a row without probabilities: every p is 0
+constexpr float kLift = 4096.0f;          // dz of fp32 tables is held times 2^12
+
+struct Args {
+    const void *P, *Q;
+    const int32_t *user_ids, *items;
+    const float *lse, *ent, *g, *h;
+    int64_t rows, users, cat;             // positions, user rows, items
+    int T;
+    float scale;
+};
+
+// per tile of 32 positions: [0] factor of its scores, [1] lse in log2, [2] [3] dz = p (A + B log2 p), the rest unused: 1 KB, one wavefront copy
+struct Prm {
+    float v[8][kTile];
+};
+
+// ---- what the passes need -------------------------------------------------------------------------------------------------------------
+// one wavefront per position (padded to 128): coefficients, named items with theirs, seen bits; the largest w |P| of all
+template <int D, bool F32>
+__global__ __launch_bounds__(256) void rows_kernel(Args a, const int64_t *__restrict__ indptr, const int32_t *__restrict__ indices, uint32_t *__restrict__ bits,
+                                                   int64_t padded, Prm *__restrict__ prm, float *__restrict__ weight, int32_t *__restrict__ named,
+                                                   float *__restrict__ coef, uint32_t *__restrict__ largest)
+{
+    const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (r >= padded) return;
+    const int32_t u = r < a.rows ? a.user_ids[r] : -1;
+    const bool ok = row_ok(u, a.users);
+    if (indptr != nullptr && r < a.rows) {
+        uint32_t *row = bits + r * mask_words(a.cat);
+        if (ok) set_seen_bits(u, indptr, indices, a.cat, row);
+        else for (int64_t k = lane; k < mask_words(a.cat); k += 64) row[k] = 0xFFFFFFFFu;      // nobody's row: nothing of it counts, whatever the products are
+    }
+    auto listed = [&](int32_t i) {           // is item i among the row's seen items?  (the bits are still being set: the list itself)
+        bool hit = false;
+        for (int64_t p = indptr[u] + lane; p < indptr[u + 1]; p += 64) hit |= indices[p] == i;
+        return __builtin_amdgcn_ballot_w64(hit) != 0ull;
+    };
+    // the row's weight: one order of summation, every lane the same
+    double sum = 0.0, mag = 0.0;
+    for (int t = 0; t < a.T && r < a.rows; ++t) {
+        const int32_t i = a.items[r * a.T + t];
+        const bool in = ok && i >= 0 && i < a.cat && !(indptr != nullptr && listed(i));
+        const float g = in ? a.g[r * a.T + t] : 0.0f;
+        sum += g;
+        mag += fabs((double)g);
+        if (lane == 0) { named[r * a.T + t] = in ? i : -1; coef[r * a.T + t] = g; }
+    }
+    const float h = ok && a.h != nullptr ? a.h[r] : 0.0f;
+    const float lse = ok ? a.lse[r] : -INFINITY;
+    const bool live = ok && lse != -INFINITY;
+    const float w = F32 ? (float)(mag + fabs((double)h)) : 1.0f;
+    const float inv = w > 0.0f ? 1.0f / w : w == w ? 0.0f : w;              // (NaN weights stay NaN)
+    float big = 0.0f, factor = live ? F32 ? 1.0f : a.scale * kLog2e : 0.0f;
+    if (ok && lane < D / 8) {
+        if constexpr (F32) {
+            const float4 *p = reinterpret_cast<const float4 *>((const float *)a.P + (int64_t)u * D + 8 * lane);
+            const float4 x = p[0], y = p[1];
+            big = fmaxf(fmaxf(fmaxf(finite_abs(x.x), finite_abs(x.y)), fmaxf(finite_abs(x.z), finite_abs(x.w))),
+                        fmaxf(fmaxf(finite_abs(y.x), finite_abs(y.y)), fmaxf(finite_abs(y.z), finite_abs(y.w))));
+        }
+    }
+    if constexpr (F32) {
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor(big, o, 64));
+        float up, down;
+        scale_for(big * (a.scale * kLog2e), &up, &down);
+        factor *= down;
+        if (lane == 0) atomicMax(largest, __float_as_uint(finite_abs(big * w)));
+    }
+    // lse in log2 is rounded to fp32 (half a step at 24 is 1e-6 of every p): what that changes goes into the coefficients
+    const double lse2 = (double)lse * 1.4426950408889634074;
+    const float l2 = (float)lse2;
+    const double fix = exp2((double)l2 - lse2) * inv;
+    if (lane == 0) {
+        Prm &t = prm[r / kTile];
+        const int c = (int)(r % kTile);
+        t.v[0][c] = factor;
+        t.v[1][c] = live ? l2 : kFar;
+        t.v[2][c] = live ? (float)(-(sum + (double)h * (a.ent != nullptr ? a.ent[r] : 0.0f)) * fix) : 0.0f;
+        t.v[3][c] = live ? (float)(-(double)h * kLn2 * fix) : 0.0f;
+#pragma unroll
+        for (int k = 4; k < 8; ++k) t.v[k][c] = 0.0f;
+        weight[r] = live ? w : 0.0f;
+    }
+    if constexpr (F32)
+        for (int t = 0; t < a.T && r < a.rows; ++t)
+            if (lane == 0) coef[r * a.T + t] *= inv;
+}
+
+// element order of a transposed tile: [plane][block of 32 columns][half of the rows][lane][8]: lane l, element j is column 32 kb + (l & 31) of
+// row (i & 3) + 8 (i >> 2) + 4 (l >> 5), i = 8 half + j
+template <int D>
+__device__ __forceinline__ int tile_row(int half, int hi, int j) { const int i = 8 * half + j; return (i & 3) + 8 * (i >> 2) + 4 * hi; }
+
+// one workgroup per tile of 32 rows: row-major planes and the transposed tile.  USERS: rows gathered by user id, each times scale log2 e and with its own
+// power of two in the row-major planes, times its weight and one common scale in the transposed ones.  Items: the tile's scale in both.
+template <int D, bool F32, bool USERS>
+__global__ __launch_bounds__(256) void tiles_kernel(Args a, const float *__restrict__ weight, const uint32_t *__restrict__ largest, uint4 *__restrict__ rowm,
+                                                    uint4 *__restrict__ tr, float *__restrict__ factor, uint32_t *__restrict__ top_factor)
+{
+    constexpr int TPR = D / 8, LD = D + 1;
+    using S = typename std::conditional<F32, float, uint16_t>::type;
+    __shared__ S x[kTile][LD];
+    __shared__ float s_max[4], s_mul[kTile];
+    const int tid = threadIdx.x;
+    const int64_t tile = blockIdx.x, n = USERS ? a.rows : a.cat;
+    float m = 0.0f;
+    for (int t = tid; t < kTile * TPR; t += 256) {
+        const int r = t / TPR, c = 8 * (t % TPR);
+        const int64_t at = tile * kTile + r;
+        int64_t row = at < n ? at : -1;
+        if constexpr (USERS) { const int32_t u = row >= 0 ? a.user_ids[row] : -1; row = row_ok(u, a.users) ? u : -1; }
+        const void *src = USERS ? a.P : a.Q;
+        if constexpr (F32) {
+            float v[8];
+            const float4 *p = reinterpret_cast<const float4 *>((const float *)src + (row < 0 ? 0 : row) * D + c);
+            const float4 y = p[0], z = p[1];
+            v[0] = y.x; v[1] = y.y; v[2] = y.z; v[3] = y.w; v[4] = z.x; v[5] = z.y; v[6] = z.z; v[7] = z.w;
+            float big = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) { v[j] = row < 0 ? 0.0f : v[j]; big = fmaxf(big, finite_abs(v[j])); x[r][c + j] = v[j]; }
+            m = fmaxf(m, big);
+            if constexpr (USERS) {            // the row's own scale: its TPR threads are neighbours (a power of two, at most 32)
+#pragma unroll
+                for (int o = TPR / 2; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor(big, o, TPR));
+                float up, down;
+                scale_for(big * (a.scale * kLog2e), &up, &down);
+                Frag h, l;
+                split8_times(v, (double)a.scale * 1.4426950408889634074 * up, &h, &l);
+                rowm[(size_t)at * (2 * TPR) + t % TPR] = h.u;
+                rowm[(size_t)at * (2 * TPR) + TPR + t % TPR] = l.u;
+            }
+        } else {
+            uint4 v = *reinterpret_cast<const uint4 *>((const uint16_t *)src + (row < 0 ? 0 : row) * D + c);
+            if (row < 0) v = make_uint4(0u, 0u, 0u, 0u);
+            if constexpr (USERS) rowm[(size_t)at * TPR + t % TPR] = v;
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { x[r][c + 2 * j] = (uint16_t)w[j]; x[r][c + 2 * j + 1] = (uint16_t)(w[j] >> 16); }
+        }
+    }
+    if constexpr (F32) {
+        if constexpr (USERS) {
+            float up, down;
+            scale_for(__uint_as_float(*largest), &up, &down, -100);      // (weights may be small)
+            if (tid < kTile) s_mul[tid] = weight[tile * kTile + tid] * up;
+            if (tile == 0 && tid == 0) factor[0] = down;
+        } else {
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+            if ((tid & 63) == 0) s_max[tid >> 6] = m;
+        }
+    }
+    __syncthreads();
+    if constexpr (F32 && !USERS) {
+        float up, down;
+        scale_for(fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3])), &up, &down);
+        if (tid == 0) { factor[tile] = down; atomicMax(top_factor, __float_as_uint(down)); }
+        if (tid < kTile) s_mul[tid] = up;
+        for (int t = tid; t < kTile * TPR; t += 256) {
+            const int r = t / TPR, c = 8 * (t % TPR);
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = x[r][c + j] * up;
+            Frag h, l;
+            split8(v, &h, &l);
+            rowm[(size_t)(tile * kTile + r) * (2 * TPR) + t % TPR] = h.u;
+            rowm[(size_t)(tile * kTile + r) * (2 * TPR) + TPR + t % TPR] = l.u;
+        }
+        __syncthreads();
+    }
+    // the second product multiplies by dz = 0 where a cell is masked: what is not finite is 0 there (where it is not masked, lse is NaN already)
+    constexpr int NF = D / 32 * 2 * 64;
+    uint4 *dst = tr + (size_t)tile * (NF * (F32 ? 2 : 1));
+    for (int t = tid; t < NF; t += 256) {
+        const int lane = t & 63, half = (t >> 6) & 1, kb = t >> 7, col = 32 * kb + (lane & 31);
+        Frag h, l;
+        if constexpr (F32) {
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int r = tile_row<D>(half, lane >> 5, j);
+                const float y = x[r][col];
+                v[j] = (fabsf(y) < INFINITY ? y : 0.0f) * s_mul[r];
+            }
+            split8(v, &h, &l);
+            dst[NF + t] = l.u;
+        } else {
+            uint16_t v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint16_t y = x[tile_row<D>(half, lane >> 5, j)][col];
+                v[j] = (y & 0x7F80u) == 0x7F80u ? (uint16_t)0 : y;
+            }
+            h.u = make_uint4(v[0] | ((uint32_t)v[1] << 16), v[2] | ((uint32_t)v[3] << 16), v[4] | ((uint32_t)v[5] << 16), v[6] | ((uint32_t)v[7] << 16));
+        }
+        dst[t] = h.u;
+    }
+}
+
+// ---- the pass -------------------------------------------------------------------------------------------------------------------------
+struct Pass {
+    const char *stay, *flow;              // row-major planes of what stays in registers and of what streams
+    const char *flow_t;                   // transposed tiles of what streams
+    const float *tile_factor;             // fp32: factor of an item tile
+    const uint32_t *top_factor;           // ... and the largest of them
+    const Prm *prm;
+    const uint32_t *bits;
+    const int32_t *named;
+    const float *coef;
+    int64_t stay_rows, flow_tiles;        // valid rows of what stays; tiles that stream
+    int64_t flow_valid;                   // valid rows of what streams
+    int64_t positions;                    // rows of named / coef / bits
+    int64_t cat;
+    int T;
+    int splits;
+    float *part;                          // [splits][padded rows that stay][d]
+    int64_t part_rows;
+};
+
+template <int D, bool F32>
+struct GradGeo : Geo<D, F32> {
+    using G = Geo<D, F32>;
+    static constexpr int KB = D / 32;
+    static constexpr int ST = 16384 / G::TILEB >= 4 ? 4 : 16384 / G::TILEB >= 1 ? 16384 / G::TILEB : 1;       // tiles of one LDS buffer
+    static constexpr int STAGE = ST * (2 * G::TILEB + 1024);
+    static constexpr int WGS = 2 * STAGE > 81920 ? 1 : 2;                                                      // workgroups a CU holds
+};
+
+template <int D, bool F32, bool ITEMS_STAY, bool MASK, bool ENT>
+__device__ __forceinline__ void grad_body(const Pass &a, char (*lds)[GradGeo<D, F32>::STAGE])
+{
+    using G = GradGeo<D, F32>;
+    constexpr int KS = G::KS, NP = G::NP, ST = G::ST, KB = G::KB;
+    const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, hi = lane >> 5, l31 = lane & 31;
+    const int64_t t0 = a.flow_tiles * blockIdx.x / a.splits, t1 = a.flow_tiles * (blockIdx.x + 1) / a.splits;
+    const int64_t col = (int64_t)blockIdx.y * 128 + wid * 32 + l31;            // this lane's column
+    const int64_t colc = col < a.stay_rows ? col : a.stay_rows - 1;
+
+    Frag b[KS][NP];
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int p = 0; p < NP; ++p) b[s][p].u = *reinterpret_cast<const uint4 *>(a.stay + (size_t)colc * G::ROWB + 16 * (p * (D / 8) + 2 * s + hi));
+    f32x16 out[KB];
+#pragma unroll
+    for (int k = 0; k < KB; ++k)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) out[k][i] = 0.0f;
+    float sf = 0.0f, slse = 0.0f, sA = 0.0f, sB = 0.0f, my_factor = 1.0f;      // users stay: this lane's row; items stay: its tile's factor
+    const float top = F32 ? __uint_as_float(*a.top_factor) : 1.0f;
+    if constexpr (!ITEMS_STAY) {
+        const Prm &p = a.prm[colc / kTile];
+        const int c = (int)(colc % kTile);
+        sf = p.v[0][c]; slse = p.v[1][c]; sA = p.v[2][c]; sB = p.v[3][c];
+    } else if constexpr (F32) {
+        my_factor = a.tile_factor[colc / kTile];
+    }
+    const int64_t words = mask_words(a.cat);
+    const int32_t my_block = (int32_t)(((int64_t)blockIdx.y * 128 + wid * 32) / kTile);       // items stay: the block of 32 this wavefront holds
+
+    auto stage = [&](int64_t tile, int buf) {
+#pragma unroll
+        for (int n = 0; n < (ST * (2 * G::TILEB / 1024 + 1) + 3) / 4; ++n) {
+            const int k = n * 4 + wid;                                           // 1 KB piece of the stage: ST row-major tiles, ST transposed, ST parameter blocks
+            if (k >= ST * (2 * G::TILEB / 1024 + 1)) break;
+            constexpr int per = G::TILEB / 1024;
+            char *dst = lds[buf] + k * 1024;
+            if (k < ST * per) {
+                const int o = k * 1024 + lane * 16, row = o / G::ROWB, c = (o % G::ROWB) / 16 ^ G::swz(row & 31);
+                int64_t i = tile * kTile + row;
+                const int64_t most = ITEMS_STAY || F32 ? a.flow_tiles * kTile - 1 : a.flow_valid - 1;    // (bf16 item rows are the table itself)
+                i = i < most ? i : most;
+                copy_to_lds(a.flow + (size_t)i * G::ROWB + 16 * c, dst);
+            } else if (k < 2 * ST * per) {
+                const int64_t last = a.flow_tiles * G::TILEB - 16;
+                int64_t o = tile * G::TILEB + (k - ST * per) * 1024 + lane * 16;
+                o = o < last ? o : last;
+                copy_to_lds(a.flow_t + o, dst);
+            } else if (ITEMS_STAY) {
+                int64_t t = tile + k - 2 * ST * per;
+                t = t < a.flow_tiles ? t : a.flow_tiles - 1;
+                copy_to_lds((const char *)(a.prm + t) + lane * 16, dst);
+            }
+        }
+    };
+    const int sw = G::swz(l31) * 16;
+    if (t0 < t1) stage(t0, 0);
+    int buf = 0;
+    for (int64_t s0 = t0; s0 < t1; s0 += ST) {
+        __syncthreads();
+        if (s0 + ST < t1) stage(s0 + ST, buf ^ 1);
+        for (int j = 0; j < ST && s0 + j < t1; ++j) {
+            const int64_t tile = s0 + j;
+            // what the tile's epilogue needs from memory, asked for early
+            uint32_t seen = 0u;
+            if constexpr (MASK) {
+                if constexpr (ITEMS_STAY) {
+                    const int64_t r = tile * kTile + l31;
+                    seen = r < a.positions && my_block < words ? a.bits[(size_t)r * words + my_block] : 0xFFFFFFFFu;
+                } else {
+                    seen = a.bits[(size_t)(colc < a.positions ? colc : a.positions - 1) * words + tile];
+                }
+            }
+            const float tf = !ITEMS_STAY && F32 ? a.tile_factor[tile] : my_factor;
+            const char *rm = lds[buf] + j * G::TILEB + l31 * G::ROWB;
+            const char *tr = lds[buf] + ST * G::TILEB + j * G::TILEB + lane * 16;
+            f32x16 acc;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[i] = 0.0f;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                Frag x[NP];
+#pragma unroll
+                for (int p = 0; p < NP; ++p) x[p].u = *reinterpret_cast<const uint4 *>(rm + ((16 * (p * (D / 8) + 2 * s + hi)) ^ sw));
+                acc = mfma32<F32>(x[0], b[s][0], acc);
+                if constexpr (F32) {
+                    acc = mfma32<F32>(x[0], b[s][NP - 1], acc);
+                    acc = mfma32<F32>(x[NP - 1], b[s][0], acc);
+                }
+            }
+            // dz of this lane's column and rows (i & 3) + 8 (i >> 2) + 4 hi of the tile
+            float v[16];
+            if constexpr (!ITEMS_STAY) {
+                const int64_t left = a.flow_valid - tile * kTile;
+                uint32_t w = left >= 32 ? 0u : 0xFFFFFFFFu << left;
+                if constexpr (MASK) w |= seen;
+                w >>= 4 * hi;
+                const bool any = __builtin_amdgcn_ballot_w64((w & 0x0F0F0F0Fu) != 0u) != 0ull;
+                const float f = sf * tf;
+                // items of a tile whose scale is below the largest count less by that: the tile's sums are over planes of its own scale
+                const float lift = F32 ? (float)(12 + (int)(__float_as_uint(tf) >> 23) - (int)(__float_as_uint(top) >> 23)) : 0.0f;
+                const float off = ENT ? -slse : lift - slse;             // (without the entropy's part log2 p itself is not needed)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    float t = fmaf(acc[i], f, off);
+                    if (any && ((w >> ((i & 3) + 8 * (i >> 2))) & 1u)) t = -1.0e4f;
+                    const float p = __builtin_amdgcn_exp2f(F32 && ENT ? t + lift : t);
+                    v[i] = ENT ? p * fmaf(sB, t, sA) : p * sA;
+                }
+            } else {
+                const Prm *prm = reinterpret_cast<const Prm *>(lds[buf] + 2 * ST * G::TILEB + j * 1024);
+                const bool any = MASK && __builtin_amdgcn_ballot_w64(seen != 0u) != 0ull;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int r0 = 8 * q + 4 * hi;
+                    const float4 f4 = *reinterpret_cast<const float4 *>(&prm->v[0][r0]), l4 = *reinterpret_cast<const float4 *>(&prm->v[1][r0]),
+                                 a4 = *reinterpret_cast<const float4 *>(&prm->v[2][r0]);
+                    float4 b4 = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if constexpr (ENT) b4 = *reinterpret_cast<const float4 *>(&prm->v[3][r0]);
+                    const float fs[4] = {f4.x, f4.y, f4.z, f4.w}, ls[4] = {l4.x, l4.y, l4.z, l4.w}, as[4] = {a4.x, a4.y, a4.z, a4.w}, bs[4] = {b4.x, b4.y, b4.z, b4.w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int i = 4 * q + e;
+                        float t = fmaf(acc[i], fs[e] * tf, F32 && !ENT ? 12.0f - ls[e] : -ls[e]);
+                        if (any) {
+                            const uint32_t w = __shfl(seen, r0 + e, 64);
+                            if ((w >> l31) & 1u) t = -1.0e4f;
+                        }
+                        const float p = __builtin_amdgcn_exp2f(F32 && ENT ? t + 12.0f : t);
+                        v[i] = ENT ? p * fmaf(bs[e], t, as[e]) : p * as[e];
+                    }
+                }
+                // named items of the tile's positions that are in this wavefront's block.
+                for (int t = 0; t < a.T; ++t) {
+                    const int64_t r = tile * kTile + l31;
+                    const int32_t it = r < a.positions ? a.named[r * a.T + t] : -1;
+                    const bool mine = hi == 0 && it >= 0 && it / kTile == my_block;
+                    unsigned long long hits = __builtin_amdgcn_ballot_w64(mine);
+                    if (hits == 0ull) continue;
+                    const float c = mine ? a.coef[r * a.T + t] * (F32 ? kLift : 1.0f) : 0.0f;
+                    while (hits) {
+                        const int row = __builtin_ctzll(hits);
+                        hits &= hits - 1;
+                        const int at = __builtin_amdgcn_readlane(it, row) & 31;
+                        const float add = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(c), row));
+                        const int reg = (row & 3) | ((row >> 3) << 2);
+                        const bool here = lane == at + 32 * ((row >> 2) & 1);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) v[i] += here && i == reg ? add : 0.0f;
+                    }
+                }
+            }
+            // second product: registers 8 h .. 8 h + 7 are the operand of its half h
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                Frag z[NP];
+                if constexpr (F32) {
+                    split8(v + 8 * h, &z[0], &z[NP - 1]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) z[0].b[e] = (__bf16)v[8 * h + e];
+                }
+#pragma unroll
+                for (int k = 0; k < KB; ++k) {
+                    Frag y[NP];
+#pragma unroll
+                    for (int p = 0; p < NP; ++p) y[p].u = *reinterpret_cast<const uint4 *>(tr + ((p * KB + k) * 2 + h) * 1024);
+                    out[k] = mfma32<F32>(y[0], z[0], out[k]);
+                    if constexpr (F32) {
+                        out[k] = mfma32<F32>(y[0], z[NP - 1], out[k]);
+                        out[k] = mfma32<F32>(y[NP - 1], z[0], out[k]);
+                    }
+                }
+            }
+        }
+        buf ^= 1;
+    }
+    float *dst = a.part + ((size_t)blockIdx.x * a.part_rows + col) * D + 4 * hi;
+#pragma unroll
+    for (int k = 0; k < KB; ++k)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<float4 *>(dst + 32 * k + 8 * q) = make_float4(out[k][4 * q], out[k][4 * q + 1], out[k][4 * q + 2], out[k][4 * q + 3]);
+}
+
+template <int D, bool F32, bool ITEMS_STAY, bool MASK, bool ENT>
+__global__ __launch_bounds__(256, (GradGeo<D, F32>::WGS)) void grad_kernel(Pass a)
+{
+    __shared__ __attribute__((aligned(1024))) char lds[2][GradGeo<D, F32>::STAGE];
+    grad_body<D, F32, ITEMS_STAY, MASK, ENT>(a, lds);
+}
+
+// ---- the partial sums -> the gradients ------------------------------------------------------------------------------------------------------
+// GP: four elements a thread; the partials in order, the row's weight, the named rows of Q
+template <int D, bool F32>
+__global__ __launch_bounds__(256) void join_rows_kernel(Args a, const float *__restrict__ part, int splits, int64_t part_rows, const float *__restrict__ weight,
+                                                        const uint32_t *__restrict__ top_factor, const int32_t *__restrict__ named, void *__restrict__ GP)
+{
+    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x, r = t / (D / 4);
+    const int c = 4 * (int)(t % (D / 4));
+    if (r >= a.rows) return;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int k = 0; k < splits && weight[r] != 0.0f; ++k) {          // (no weight, no gradient, whatever the products were)
+        const float4 p = *reinterpret_cast<const float4 *>(part + ((size_t)k * part_rows + r) * D + c);
+        s[0] += p.x; s[1] += p.y; s[2] += p.z; s[3] += p.w;
+    }
+    const float f = F32 ? __uint_as_float(*top_factor) * (1.0f / kLift) * weight[r] : weight[r];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[j] *= f;
+    for (int k = 0; k < a.T; ++k) {
+        const int32_t i = named[r * a.T + k];
+        if (i < 0) continue;
+        const float g = a.g[r * a.T + k];
+        if constexpr (F32) {
+            const float4 q = *reinterpret_cast<const float4 *>((const float *)a.Q + (size_t)i * D + c);
+            s[0] = fmaf(g, q.x, s[0]); s[1] = fmaf(g, q.y, s[1]); s[2] = fmaf(g, q.z, s[2]); s[3] = fmaf(g, q.w, s[3]);
+        } else {
+            const ushort4 q = *reinterpret_cast<const ushort4 *>((const uint16_t *)a.Q + (size_t)i * D + c);
+            s[0] = fmaf(g, bf16_f32(q.x), s[0]); s[1] = fmaf(g, bf16_f32(q.y), s[1]); s[2] = fmaf(g, bf16_f32(q.z), s[2]); s[3] = fmaf(g, bf16_f32(q.w), s[3]);
+        }
+    }
+    if constexpr (F32) *reinterpret_cast<float4 *>((float *)GP + r * D + c) = make_float4(s[0] * a.scale, s[1] * a.scale, s[2] * a.scale, s[3] * a.scale);
+    else *reinterpret_cast<ushort4 *>((uint16_t *)GP + r * D + c) = make_ushort4(f32_bf16(s[0] * a.scale), f32_bf16(s[1] * a.scale), f32_bf16(s[2] * a.scale), f32_bf16(s[3] * a.scale));
+}
+
+template <int D, bool F32>
+__global__ __launch_bounds__(256) void join_items_kernel(int64_t cat, const float *__restrict__ part, int splits, int64_t part_rows, const float *__restrict__ factor,
+                                                         int factor_every, float scale, void *__restrict__ GQ)
+{
+    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x, r = t / (D / 4);
+    const int c = 4 * (int)(t % (D / 4));
+    if (r >= cat) return;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int k = 0; k < splits; ++k) {
+        const float4 p = *reinterpret_cast<const float4 *>(part + ((size_t)k * part_rows + r) * D + c);
+        const float f = F32 ? factor[k / factor_every] * (scale / kLift) : scale;        // (a pass has its own scale of the positions' rows)
+        s[0] = fmaf(p.x, f, s[0]); s[1] = fmaf(p.y, f, s[1]); s[2] = fmaf(p.z, f, s[2]); s[3] = fmaf(p.w, f, s[3]);
+    }
+    if constexpr (F32) *reinterpret_cast<float4 *>((float *)GQ + r * D + c) = make_float4(s[0], s[1], s[2], s[3]);
+    else *reinterpret_cast<ushort4 *>((uint16_t *)GQ + r * D + c) = make_ushort4(f32_bf16(s[0]), f32_bf16(s[1]), f32_bf16(s[2]), f32_bf16(s[3]));
+}
+
+// ---- T[ids[r]] += R[r] in the order of r -----------------------------------------------------------------------------------------------
+// One wavefront per position of a block of kAddRows: the first of the block that names a row adds up all of the block's for it.
+constexpr int kAddRows = 16384;
+
+template <bool F32>
+__global__ __launch_bounds__(256) void add_rows_kernel(float *__restrict__ T, int64_t table_rows, int d, const int32_t *__restrict__ ids, const void *__restrict__ R, int n)
+{
+    const int r = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (r >= n) return;
+    const int32_t id = ids[r];
+    if (!row_ok(id, table_rows)) return;
+    for (int q = 0; q < r; q += 64)                     // somebody before me?
+        if (__builtin_amdgcn_ballot_w64(q + lane < r && ids[q + lane] == id) != 0ull) return;
+    float acc[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[j] = 64 * j + lane < d ? T[(size_t)id * d + 64 * j + lane] : 0.0f;
+    for (int q = r & ~63; q < n; q += 64) {
+        unsigned long long m = __builtin_amdgcn_ballot_w64(q + lane >= r && q + lane < n && ids[q + lane < n ? q + lane : n - 1] == id);
+        while (m) {
+            const int k = q + __builtin_ctzll(m);
+            m &= m - 1;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (64 * j + lane < d) {
+                    const size_t at = (size_t)k * d + 64 * j + lane;
+                    acc[j] += F32 ? ((const float *)R)[at] : bf16_f32(((const uint16_t *)R)[at]);
+                }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (64 * j + lane < d) T[(size_t)id * d + 64 * j + lane] = acc[j];
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------------------------------------
+constexpr int kTopFactor = 16;
+
+struct Ws {
+    char *user_rm, *user_t, *item_rm, *item_t;
+    float *tile_factor, *user_factor, *weight, *coef, *part_p, *part_q;
+    uint32_t *scalars;                    // [0] largest w |P| (per pass), [kTopFactor] largest item factor
+    Prm *prm;
+    int32_t *named;
+    uint32_t *bits;
+    int64_t pass, passes, splits_p, splits_q, pad_p, pad_q, bytes;
+};
+
+int64_t pad128(int64_t n) { return (n + 127) / 128 * 128; }
+
+int64_t grad_splits(int64_t stay, int64_t flow_tiles, int wgs, int st)
+{
+    const int64_t slots = (int64_t)wgs * rsx_num_cus(), s = slots / (pad128(stay) / 128), most = (flow_tiles + st - 1) / st;
+    return s < 1 ? 1 : s > most ? most : s;
+}
+
+// geometry the host needs of GradGeo
+void grad_geo(int d, bool f32, int *wgs, int *st)
+{
+    const int tileb = kTile * d * (f32 ? 4 : 2), s = 16384 / tileb;
+    *st = s >= 4 ? 4 : s >= 1 ? s : 1;
+    *wgs = 2 * *st * (2 * tileb + 1024) > 81920 ? 1 : 2;
+}
+
+Ws carve(void *ws, int64_t rows, int64_t cat, int d, int dtype, bool mask, int T)
+{
+    Ws w;
+    char *base = (char *)ws;
+    int64_t off = 0;
+    auto take = [&](int64_t n) { char *q = base + off; off += a256(n); return q; };
+    const bool f32 = dtype == RSX_F32;
+    const int rowb = d * (f32 ? 4 : 2);
+    int wgs, st;
+    grad_geo(d, f32, &wgs, &st);
+    // a pass' bits are held to 1 GB (without a mask: one pass)
+    int64_t most = (1ll << 30) / (mask_words(cat) * 4) / 128 * 128;
+    most = most < 128 ? 128 : most;
+    w.pass = mask && rows > most ? most : rows;
+    w.passes = (rows + w.pass - 1) / w.pass;
+    w.pad_p = pad128(w.pass);
+    w.pad_q = pad128(cat);
+    const int64_t item_tiles = w.pad_q / kTile, user_tiles = w.pad_p / kTile;
+    w.splits_p = grad_splits(w.pass, item_tiles, wgs, st);
+    w.splits_q = grad_splits(cat, user_tiles, wgs, st);
+    w.user_rm = take(w.pad_p * rowb);
+    w.user_t = take(w.pad_p * rowb);
+    w.item_rm = take(f32 ? w.pad_q * rowb : 0);
+    w.item_t = take(w.pad_q * rowb);
+    w.tile_factor = (float *)take(item_tiles * 4);
+    w.user_factor = (float *)take(w.passes * 4);
+    w.weight = (float *)take(w.pad_p * 4);
+    w.coef = (float *)take(w.pass * T * 4);
+    w.named = (int32_t *)take(w.pass * T * 4);
+    w.prm = (Prm *)take(user_tiles * (int64_t)sizeof(Prm));
+    w.scalars = (uint32_t *)take(256);
+    w.bits = (uint32_t *)take(mask ? w.pass * mask_words(cat) * 4 : 0);
+    w.part_p = (float *)take(w.splits_p * w.pad_p * d * 4);
+    w.part_q = (float *)take(w.passes * w.splits_q * w.pad_q * d * 4);
+    w.bytes = off;
+    return w;
+}
+
+template <int D, bool F32, bool ITEMS_STAY>
+void launch_pass(const Pass &p, bool mask, bool ent, hipStream_t st)
+{
+    const dim3 grid((unsigned)p.splits, (unsigned)(p.part_rows / 128));
+#define RSX_GRAD(M_, E_) hipLaunchKernelGGL((grad_kernel<D, F32, ITEMS_STAY, M_, E_>), grid, dim3(256), 0, st, p)
+    if (mask) { if (ent) RSX_GRAD(true, true); else RSX_GRAD(true, false); }
+    else { if (ent) RSX_GRAD(false, true); else RSX_GRAD(false, false); }
+#undef RSX_GRAD
+}
+
+template <int D, bool F32>
+void run(const Args &all, const int64_t *indptr, const int32_t *indices, const Ws &w, void *GP, void *GQ, hipStream_t st)
+{
+    const int64_t item_tiles = w.pad_q / kTile;
+    const int es = F32 ? 4 : 2;
+    hipLaunchKernelGGL(fill_u32_kernel, dim3(1), dim3(256), 0, st, (uint4 *)w.scalars, 16, 0u);
+    hipLaunchKernelGGL((tiles_kernel<D, F32, false>), dim3((unsigned)item_tiles), dim3(256), 0, st, all, (const float *)nullptr, (const uint32_t *)nullptr,
+                       (uint4 *)w.item_rm, (uint4 *)w.item_t, w.tile_factor, w.scalars + kTopFactor);
+    for (int64_t k = 0; k < w.passes; ++k) {
+        Args a = all;
+        const int64_t r0 = k * w.pass;
+        a.rows = all.rows - r0 < w.pass ? all.rows - r0 : w.pass;
+        a.user_ids += r0; a.lse += r0; a.g += r0 * a.T; a.items += r0 * a.T;
+        if (a.ent) a.ent += r0;
+        if (a.h) a.h += r0;
+        const int64_t pad = pad128(a.rows), user_tiles = pad / kTile;
+        if (k > 0) hipLaunchKernelGGL(fill_u32_kernel, dim3(1), dim3(256), 0, st, (uint4 *)w.scalars, 1, 0u);
+        if (indptr) launch_clear_bits(a.rows, a.cat, w.bits, st);
+        hipLaunchKernelGGL((rows_kernel<D, F32>), dim3((unsigned)(pad / 4)), dim3(256), 0, st, a, indptr, indices, w.bits, pad, w.prm, w.weight, w.named, w.coef, w.scalars);
+        hipLaunchKernelGGL((tiles_kernel<D, F32, true>), dim3((unsigned)user_tiles), dim3(256), 0, st, a, w.weight, w.scalars, (uint4 *)w.user_rm, (uint4 *)w.user_t,
+                           w.user_factor + k, (uint32_t *)nullptr);
+        Pass p;
+        p.tile_factor = w.tile_factor; p.top_factor = w.scalars + kTopFactor; p.prm = w.prm; p.bits = w.bits; p.named = w.named; p.coef = w.coef;
+        p.positions = a.rows; p.cat = a.cat; p.T = a.T;
+        p.stay = w.user_rm; p.flow = F32 ? w.item_rm : (const char *)a.Q; p.flow_t = w.item_t;
+        p.stay_rows = pad; p.flow_tiles = (a.cat + kTile - 1) / kTile; p.flow_valid = a.cat;
+        p.splits = (int)w.splits_p; p.part = w.part_p; p.part_rows = pad;
+        launch_pass<D, F32, false>(p, indptr != nullptr, a.h != nullptr, st);
+        hipLaunchKernelGGL((join_rows_kernel<D, F32>), dim3((unsigned)((a.rows * (D / 4) + 255) / 256)), dim3(256), 0, st, a, w.part_p, p.splits, pad, w.weight, w.scalars + kTopFactor,
+                           w.named, (char *)GP + r0 * D * es);
+        p.stay = F32 ? w.item_rm : (const char *)a.Q; p.flow = w.user_rm; p.flow_t = w.user_t;
+        p.stay_rows = F32 ? w.pad_q : a.cat; p.flow_tiles = user_tiles; p.flow_valid = a.rows;
+        p.splits = (int)w.splits_q; p.part = w.part_q + (size_t)k * w.splits_q * w.pad_q * D; p.part_rows = w.pad_q;
+        launch_pass<D, F32, true>(p, indptr != nullptr, a.h != nullptr, st);
+    }
+    hipLaunchKernelGGL((join_items_kernel<D, F32>), dim3((unsigned)((all.cat * (D / 4) + 255) / 256)), dim3(256), 0, st, all.cat, w.part_q, (int)(w.passes * w.splits_q), w.pad_q,
+                       w.user_factor, (int)w.splits_q, all.scale, GQ);
+}
+
+}  // namespace
+
+RSX_API int64_t rsx_score_logprobs_grad_workspace(int64_t num_rows, int64_t num_items, int d, int dtype, int masked, int T)
+{
+    if (num_rows < 0 || num_rows >= (1ll << 31) - 128 || num_items <= 0 || num_items >= (1ll << 31) - 128 || !rsx_dim_ok(d) || (dtype != RSX_F32 && dtype != RSX_BF16) || T < 0)
+        return RSX_E_INVALID;
+    return carve(nullptr, num_rows < 1 ? 1 : num_rows, num_items, d, dtype, masked != 0, T).bytes;
+}
+
+RSX_API int rsx_score_logprobs_grad(const void *P, int64_t num_users, const int32_t *user_ids_dev, int64_t num_rows, const void *Q, int64_t num_items, int d,
+                                    int dtype, const int64_t *mask_indptr_dev, const int32_t *mask_indices_dev, float scale, const int32_t *items_dev, int T,
+                                    const float *lse_dev, const float *g_logp_dev, const float *entropy_dev, const float *g_entropy_dev, void *GP_out,
+                                    void *GQ_out, void *ws, int64_t ws_bytes, rsx_stream_t stream)
+{
+    RSX_CHECK_ARG(P && Q && user_ids_dev && lse_dev && GP_out && GQ_out, "null pointer");
+    RSX_CHECK_ARG(rsx_dim_ok(d), "d must be 32, 64, 128 or 256");
+    RSX_CHECK_ARG(dtype == RSX_F32 || dtype == RSX_BF16, "dtype must be RSX_F32 or RSX_BF16");
+    RSX_CHECK_ARG(num_rows >= 1 && num_rows < (1ll << 31) - 128 && num_users > 0 && num_items > 0 && num_items < (1ll << 31) - 128, "bad shape");
+    RSX_CHECK_ARG((mask_indptr_dev == nullptr) == (mask_indices_dev == nullptr), "mask needs both CSR arrays");
+    RSX_CHECK_ARG((entropy_dev == nullptr) == (g_entropy_dev == nullptr), "the entropies and their gradients come together");
+    RSX_CHECK_ARG(scale > 0.0f && scale < INFINITY, "scale must be positive and finite");
+    RSX_CHECK_ARG(T >= 0 && (T == 0 || (items_dev && g_logp_dev)), "T items per row need their ids and gradients");
+    RSX_CHECK_ARG(T > 0 || g_entropy_dev != nullptr, "nothing to differentiate");
+    RSX_CHECK_ARG(aligned16(P) && aligned16(Q) && aligned16(GP_out) && aligned16(GQ_out), "table rows must be 16-byte aligned");
+    const Ws w = carve(ws, num_rows, num_items, d, dtype, mask_indptr_dev != nullptr, T);
+    if (ws == nullptr || ws_bytes < w.bytes || !aligned16(ws)) {
+        rsx_set_error("rsx_score_logprobs_grad: workspace of %lld bytes (16-byte aligned) required, got %lld", (long long)w.bytes, (long long)ws_bytes);
+        return RSX_E_WORKSPACE;
+    }
+    const Args a{P, Q, user_ids_dev, items_dev, lse_dev, entropy_dev, g_logp_dev, g_entropy_dev, num_rows, num_users, num_items, T, scale};
+    hipStream_t st = (hipStream_t)stream;
+#define RSX_GRAD_RUN(D_) do { if (dtype == RSX_F32) run<D_, true>(a, mask_indptr_dev, mask_indices_dev, w, GP_out, GQ_out, st); \
+                              else run<D_, false>(a, mask_indptr_dev, mask_indices_dev, w, GP_out, GQ_out, st); } while (0)
+    switch (d) {
+    case 32: RSX_GRAD_RUN(32); break;
+    case 64: RSX_GRAD_RUN(64); break;
+    case 128: RSX_GRAD_RUN(128); break;
+    default: RSX_GRAD_RUN(256); break;
+    }
+#undef RSX_GRAD_RUN
+    RSX_CHECK_LAUNCH();
+    return RSX_OK;
+}
+
+RSX_API int rsx_add_rows(float *T, int64_t table_rows, int d, const int32_t *ids_dev, const void *R, int dtype, int64_t n, rsx_stream_t stream)
+{
+    RSX_CHECK_ARG(T && ids_dev && R, "null pointer");
+    RSX_CHECK_ARG(rsx_dim_ok(d), "d must be 32, 64, 128 or 256");
+    RSX_CHECK_ARG(dtype == RSX_F32 || dtype == RSX_BF16, "dtype must be RSX_F32 or RSX_BF16");
+    RSX_CHECK_ARG(table_rows > 0 && n >= 0, "bad shape");
+    for (int64_t r0 = 0; r0 < n; r0 += kAddRows) {
+        const int m = (int)(n - r0 < kAddRows ? n - r0 : kAddRows);
+        const void *src = (const char *)R + (size_t)r0 * d * (dtype == RSX_F32 ? 4 : 2);
+        if (dtype == RSX_F32) hipLaunchKernelGGL(add_rows_kernel<true>, dim3((m + 3) / 4), dim3(256), 0, (hipStream_t)stream, T, table_rows, d, ids_dev + r0, src, m);
+        else hipLaunchKernelGGL(add_rows_kernel<false>, dim3((m + 3) / 4), dim3(256), 0, (hipStream_t)stream, T, table_rows, d, ids_dev + r0, src, m);
+    }
+    RSX_CHECK_LAUNCH();
+    return RSX_OK;
+}

@@ -111,6 +111,9 @@ SIGNATURES = {
     "rsx_mesh_destroy": (None, [_P]),
     "rsx_score_logprobs_workspace": (_I64, [_I64, _I64, _I32, _I32, _I32, _I32]),
     "rsx_score_logprobs": (C.c_int, [_P, _I64, _P, _I64, _P, _I64, _I32, _I32, _P, _P, _F, _P, _I32, _I32, _P, _P, _P, _P, _P, _P, _I64, _P]),
+    "rsx_score_logprobs_grad_workspace": (_I64, [_I64, _I64, _I32, _I32, _I32, _I32]),
+    "rsx_score_logprobs_grad": (C.c_int, [_P, _I64, _P, _I64, _P, _I64, _I32, _I32, _P, _P, _F, _P, _I32, _P, _P, _P, _P, _P, _P, _P, _I64, _P]),
+    "rsx_add_rows": (C.c_int, [_P, _I64, _I32, _P, _P, _I32, _I64, _P]),
     "rsx_score": (C.c_int, [_P, _P, _I64, _P, _I64, _I32, _P, _P, _P, _P]),
     "rsx_topk": (C.c_int, [_P, _I64, _I64, _I32, _P, _P, _P]),
     "rsx_score_topk_workspace": (_I64, [_I64, _I64]),
@@ -1165,3 +1168,49 @@ def score_logprobs(P, Q, user_ids, items=None, K=0, mask=None, scale=1.0, ws=Non
                                         ptr(out.entropy), ptr(out.top_idx), ptr(out.top_logp), ptr(ws), ws.numel() * ws.element_size(), _stream()),
                "rsx_score_logprobs")
     return out
+
+
+def score_logprobs_grad_workspace(rows, num_items, d, dtype=torch.float32, masked=False, T=1):
+    n = lib().rsx_score_logprobs_grad_workspace(int(rows), int(num_items), int(d), _DTYPES.get(dtype, -1), int(bool(masked)), int(T))
+    if n < 0:
+        raise RsxError("rsx_score_logprobs_grad_workspace: invalid shape")
+    return n
+
+
+def score_logprobs_grad(P, Q, user_ids, items, lse, g_logp, entropy=None, g_entropy=None, mask=None, scale=1.0, out=None, ws=None):
+    """(GP [n x d], GQ [I x d]), the gradient of sum(g_logp * logp) + sum(g_entropy * entropy) by the positions' rows and by the item
+    rows, in the tables' dtype (include/rsx.h:rsx_score_logprobs_grad); lse, entropy: score_logprobs' of the same arguments.
+    GP is per position (add_rows sums the positions of a user).  out: (GP, GQ) to write into."""
+    pp, pq, pu, pi, dt, rows, T, mp, mi = _logprob_args(P, Q, user_ids, items, mask)
+    (num_users, d), num_items = P.shape, Q.shape[0]
+    if (entropy is None) != (g_entropy is None):
+        raise RsxError("entropy and g_entropy come together")
+    vec = lambda t, n, name: _dev(t, torch.float32, name) if t.numel() == n else _shape_error(name, n)
+    pl = vec(lse, rows, "lse")
+    pg = vec(g_logp, rows * T, "g_logp") if items is not None else None
+    pe, ph = (vec(entropy, rows, "entropy"), vec(g_entropy, rows, "g_entropy")) if entropy is not None else (None, None)
+    GP, GQ = out if out is not None else (torch.empty((rows, d), dtype=P.dtype, device=P.device), torch.empty_like(Q))
+    po, qo = _matrix(GP, "GP", rows, d, P.dtype), _matrix(GQ, "GQ", num_items, d, P.dtype)
+    with _same_device(P, Q, user_ids, items, lse, g_logp, entropy, g_entropy, GP, GQ, *(mask or ())):
+        if rows == 0:
+            GQ.zero_()
+            return GP, GQ
+        ws = _scratch(ws, score_logprobs_grad_workspace(rows, num_items, d, P.dtype, mask is not None, T), P.device)
+        _check(lib().rsx_score_logprobs_grad(pp, num_users, pu, rows, pq, num_items, d, dt, mp, mi, float(scale), pi, T, pl, pg, pe, ph, po, qo,
+                                             C.c_void_p(ws.data_ptr()), ws.numel() * ws.element_size(), _stream()), "rsx_score_logprobs_grad")
+    return GP, GQ
+
+
+def _shape_error(name, n):
+    raise RsxError(f"{name} must have {n} entries")
+
+
+def add_rows(T, ids, R):
+    """T[ids[r]] += R[r], in the order of r for every row of T (include/rsx.h:rsx_add_rows): T float32, R float32 or bfloat16"""
+    pt, dt = _matrix(T, "T", dtype=torch.float32), _dtype(R, "R")
+    pr = _matrix(R, "R", ids.numel(), T.shape[1])
+    if ids.numel() == 0:
+        return T
+    with _same_device(T, ids, R):
+        _check(lib().rsx_add_rows(pt, T.shape[0], T.shape[1], _dev(ids, torch.int32, "ids"), pr, dt, ids.numel(), _stream()), "rsx_add_rows")
+    return T
