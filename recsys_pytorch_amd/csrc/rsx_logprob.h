@@ -54,6 +54,7 @@ struct Geo {
 // 64 lanes x 16 bytes from global memory straight into LDS (lane-linear from a wavefront-uniform base); the next barrier waits for it.
 // (a function of its own: called from a kernel's body, the builtin costs the kernel its host stub)
 __device__ __forceinline__ void copy_to_lds(const char *src, char *dst) { __builtin_amdgcn_global_load_lds(src, dst, 16, 0, 0); }
+__device__ __forceinline__ void copy4_to_lds(const char *src, char *dst) { __builtin_amdgcn_global_load_lds(src, dst, 4, 0, 0); }       // 64 lanes x 4 bytes
 
 // power of two that brings a largest magnitude m into [2^13, 2^14), and its inverse.  Below 2^-40 as for 2^-40: the product of two such
 // inverses stays a normal number, and what is lost there moves no score by 2^-40
@@ -110,21 +111,35 @@ static __global__ __launch_bounds__(256) void fill_u32_kernel(uint4 *__restrict_
 // words a row of the bit mask holds: four tiles of 32 items at a time
 __host__ __device__ __forceinline__ int64_t mask_words(int64_t num_items) { return (num_items + 127) / 128 * 4; }
 
-// seen items of a row as bits, [rows][words]: bit i & 31 of word i >> 5; one wavefront per row, the words zero before
-__device__ __forceinline__ void set_seen_bits(int32_t u, const int64_t *__restrict__ indptr, const int32_t *__restrict__ indices, int64_t num_items, uint32_t *row)
+// seen items of the call's rows as bits, [rows][words]: bit i & 31 of word i >> 5.  One workgroup per row builds 32 KB of it at a time in LDS and
+// writes it out whole: no clearing pass, no atomics on memory.  A position that names no row sees everything.
+constexpr int kBitWords = 8192;
+__device__ __forceinline__ void write_seen_bits(int32_t u, bool ok, const int64_t *__restrict__ indptr, const int32_t *__restrict__ indices, int64_t num_items,
+                                                uint32_t *__restrict__ row, uint32_t *lds)
 {
-    const int64_t hi = indptr[u + 1];
-    for (int64_t p = indptr[u] + (threadIdx.x & 63); p < hi; p += 64) {
-        const int32_t i = indices[p];
-        if (i >= 0 && i < num_items) atomicOr(row + (i >> 5), 1u << (i & 31));
+    const int64_t words = mask_words(num_items);
+    const int64_t lo = ok ? indptr[u] : 0, hi = ok ? indptr[u + 1] : 0;
+    for (int64_t w0 = 0; w0 < words; w0 += kBitWords) {
+        const int n = (int)(words - w0 < kBitWords ? words - w0 : kBitWords);             // (a multiple of four)
+        for (int t = threadIdx.x; t < n / 4; t += blockDim.x) reinterpret_cast<uint4 *>(lds)[t] = ok ? make_uint4(0u, 0u, 0u, 0u) : make_uint4(~0u, ~0u, ~0u, ~0u);
+        __syncthreads();
+        for (int64_t p = lo + threadIdx.x; p < hi; p += blockDim.x) {
+            const int32_t i = indices[p];
+            const int64_t w = (i >> 5) - w0;
+            if (i >= 0 && i < num_items && w >= 0 && w < n) atomicOr(lds + w, 1u << (i & 31));
+        }
+        __syncthreads();
+        for (int t = threadIdx.x; t < n / 4; t += blockDim.x) reinterpret_cast<uint4 *>(row + w0)[t] = reinterpret_cast<const uint4 *>(lds)[t];
+        __syncthreads();
     }
 }
 
-inline void launch_clear_bits(int64_t rows, int64_t num_items, uint32_t *bits, hipStream_t st)
+static __global__ __launch_bounds__(256) void seen_bits_kernel(const int32_t *__restrict__ user_ids, int64_t num_users, const int64_t *__restrict__ indptr,
+                                                               const int32_t *__restrict__ indices, int64_t num_items, uint32_t *__restrict__ bits)
 {
-    const int64_t n16 = rows * mask_words(num_items) / 4, most = (int64_t)rsx_num_cus() * 8;
-    const int64_t want = (n16 + 255) / 256;
-    hipLaunchKernelGGL(fill_u32_kernel, dim3((unsigned)(want < most ? want : most)), dim3(256), 0, st, (uint4 *)bits, n16, 0u);
+    __shared__ __attribute__((aligned(16))) uint32_t lds[kBitWords];
+    const int32_t u = user_ids[blockIdx.x];
+    write_seen_bits(u, row_ok(u, num_users), indptr, indices, num_items, bits + (size_t)blockIdx.x * mask_words(num_items), lds);
 }
 
 // fp32 item rows -> scaled planes [tiles padded to a multiple of 4][32][hi d, lo d] and a factor per tile.  One workgroup per tile.

@@ -25,6 +25,13 @@ namespace {
 using namespace lp;
 
 constexpr int kMaxK = 128;
+#ifndef RSX_LP_UB
+#define RSX_LP_UB(D_, F_) ((D_) * ((F_) ? 2 : 1) <= 256 ? 2 : 1)
+#define RSX_LP_OCC(D_, F_) 2
+#endif
+#ifndef RSX_LP_AHEAD
+#define RSX_LP_AHEAD 2
+#endif
 constexpr float kNone = -3.0e38f;        // reference of a row that has met no score yet
 constexpr float kLazy = 16.0f;           // a tile's maximum may exceed the reference by this much before the sums are rescaled
 
@@ -73,36 +80,32 @@ __device__ __forceinline__ void load8(const void *base, int64_t at, float *x)
     }
 }
 
-// what a row needs before the pass: its seen items as bits, and the reference its chunk maxima are stored against (a score of its own, so that
-// an offset common to a row's scores does not eat the halves' eleven bits).  One wavefront per row.
+// the reference a row's chunk maxima are stored against: a score of its own, so that an offset common to a row's scores does not eat the halves'
+// eleven bits.  One wavefront per row.
 template <int D, bool F32>
-__global__ __launch_bounds__(256) void row_prep_kernel(const void *__restrict__ P, const void *__restrict__ Q, Shape sh, const int64_t *__restrict__ indptr,
-                                                       const int32_t *__restrict__ indices, uint32_t *__restrict__ bits, float *__restrict__ ref)
+__global__ __launch_bounds__(256) void reference_kernel(const void *__restrict__ P, const void *__restrict__ Q, Shape sh, float *__restrict__ ref)
 {
     const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
     if (r >= sh.rows) return;
     const int32_t u = sh.user_ids[r];
     if (!row_ok(u, sh.users)) return;
-    if (ref != nullptr) {
-        float d[3] = {0.0f, 0.0f, 0.0f};
-        if (lane < D / 8) {
-            float x[8], q[8];
-            load8<F32>(P, (int64_t)u * D + 8 * lane, x);
+    float d[3] = {0.0f, 0.0f, 0.0f};
+    if (lane < D / 8) {
+        float x[8], q[8];
+        load8<F32>(P, (int64_t)u * D + 8 * lane, x);
 #pragma unroll
-            for (int n = 0; n < 3; ++n) {
-                load8<F32>(Q, (n == 0 ? 0 : n == 1 ? sh.items / 2 : sh.items - 1) * D + 8 * lane, q);
+        for (int n = 0; n < 3; ++n) {
+            load8<F32>(Q, (n == 0 ? 0 : n == 1 ? sh.items / 2 : sh.items - 1) * D + 8 * lane, q);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) d[n] = fmaf(x[j], q[j], d[n]);
-            }
+            for (int j = 0; j < 8; ++j) d[n] = fmaf(x[j], q[j], d[n]);
         }
-#pragma unroll
-        for (int n = 0; n < 3; ++n)
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) d[n] += __shfl_xor(d[n], o, 64);
-        if (lane == 0) ref[r] = sh.scale * kLog2e * pick_reference(d[0], d[1], d[2]);
     }
-    if (indptr != nullptr) set_seen_bits(u, indptr, indices, sh.items, bits + r * mask_words(sh.items));
+#pragma unroll
+    for (int n = 0; n < 3; ++n)
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) d[n] += __shfl_xor(d[n], o, 64);
+    if (lane == 0) ref[r] = sh.scale * kLog2e * pick_reference(d[0], d[1], d[2]);
 }
 
 // ---- many rows ------------------------------------------------------------------------------------------------------------------------
@@ -110,9 +113,9 @@ template <int D, bool F32>
 struct WideGeo : Geo<D, F32> {
     using G = Geo<D, F32>;
     // 32-user blocks a wavefront holds: their operands take KS * NP * 4 registers each
-    static constexpr int UB = D * G::NP <= 256 ? 2 : 1, WGU = 128 * UB;
-    // item tiles of one of the two LDS buffers: 32 KB, so that two workgroups share a CU
-    static constexpr int ST = 32768 / G::TILEB >= 4 ? 4 : 32768 / G::TILEB;
+    static constexpr int UB = RSX_LP_UB(D, F32), WGU = 128 * UB, OCC = RSX_LP_OCC(D, F32);
+    // item tiles of one of the two LDS buffers
+    static constexpr int ST = 16384 / G::TILEB >= 4 ? 4 : 16384 / G::TILEB >= 1 ? 16384 / G::TILEB : 1;
 };
 
 // chunk maxima of a row, 16 halves per group of four tiles: [hi][tile & 3][h] holds items 32 tile + 16 h + 4 hi + {0..3, 8..11}
@@ -122,14 +125,50 @@ __device__ __forceinline__ int64_t chunk_item0(int64_t c)
 }
 
 template <int D, bool F32, bool MASK, bool TOP>
-__global__ __launch_bounds__(256, 2) void wide_kernel(const void *__restrict__ P, const void *__restrict__ Qtab, const char *__restrict__ planes,
-                                                      const float *__restrict__ factor, Shape sh, const uint32_t *__restrict__ bits,
-                                                      const float *__restrict__ row_ref, int splits, float4 *__restrict__ part, uint4 *__restrict__ keys)
+struct WideLds {
+    using G = WideGeo<D, F32>;
+    __attribute__((aligned(1024))) char tile[2][G::ST * G::TILEB];
+    char bits[MASK ? 2 : 1][MASK ? 4 : 1][G::UB][512];        // a group's seen bits, 16 bytes a row of the wavefront's
+    uint32_t key[G::UB][TOP ? 4 : 1][256];                    // a group's chunk maxima, this lane's own slots
+    float all[G::UB][3][256];                                 // sums of all groups before this one, this lane's own slots
+};
+
+// the products' 16 scores of one row (register i: item (i & 3) + 8 (i >> 2) + 4 hi of the tile) into the group's sums.  SOME: bits of w mask some.
+// (Two whole versions rather than a masked copy of the scores before one: merging the copies would cost the common path 16 moves.)
+template <bool SOME, bool TOP>
+__device__ __forceinline__ void absorb(const f32x16 &acc, float f, uint32_t w, Stat &st, float ref, uint32_t *key)
+{
+    float x[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = SOME && ((w >> ((i & 3) + 8 * (i >> 2))) & 1u) ? -INFINITY : acc[i];
+    float c0 = x[0], c1 = x[8];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) { c0 = __builtin_elementwise_maximum(c0, x[i]); c1 = __builtin_elementwise_maximum(c1, x[8 + i]); }
+    const float top = __builtin_elementwise_maximum(c0, c1) * f;
+    if constexpr (TOP) *key = (uint32_t)half_bits(fmaf(c0, f, -ref)) | ((uint32_t)half_bits(fmaf(c1, f, -ref)) << 16);
+    if (__builtin_amdgcn_ballot_w64(top > st.m + kLazy) != 0ull) {
+        if (top > st.m) stat_lift(st, top);
+    }
+    float sum = 0.0f, ent = 0.0f;         // of the tile; then of the group, then of all: each sum adds up few terms
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        float t = fmaf(x[i], f, -st.m);
+        if constexpr (SOME) t = x[i] == -INFINITY ? -1.0e4f : t;
+        const float e = __builtin_amdgcn_exp2f(t);
+        sum += e;
+        ent = fmaf(e, t, ent);
+    }
+    st.sum += sum;
+    st.ent += ent;
+}
+
+template <int D, bool F32, bool MASK, bool TOP>
+__device__ __forceinline__ void wide_body(const void *__restrict__ P, const char *__restrict__ rows, const float *__restrict__ factor, const Shape &sh,
+                                          const uint32_t *__restrict__ bits, const float *__restrict__ row_ref, int splits, float4 *__restrict__ part,
+                                          uint4 *__restrict__ keys, WideLds<D, F32, MASK, TOP> &lds)
 {
     using G = WideGeo<D, F32>;
     constexpr int UB = G::UB, KS = G::KS, NP = G::NP, ST = G::ST;
-    __shared__ __attribute__((aligned(1024))) char lds[2][ST * G::TILEB];
-    __shared__ float s_all[UB][3][256];
     const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, hi = lane >> 5, l31 = lane & 31;
     const int64_t groups = (sh.items + 127) / 128;
     const int64_t g0 = groups * blockIdx.x / splits, g1 = groups * (blockIdx.x + 1) / splits;
@@ -138,7 +177,7 @@ __global__ __launch_bounds__(256, 2) void wide_kernel(const void *__restrict__ P
     // this wavefront's users: operands, scale, reference
     Frag b[UB][KS][NP];
     float rowf[UB], ref[UB];
-    Stat st[UB];                          // of the current group of tiles; of all before: s_all, this lane's own slots
+    Stat st[UB];                          // of the current group of tiles
 #pragma unroll
     for (int ub = 0; ub < UB; ++ub) {
         const int64_t r = row0 + 32 * ub + l31;
@@ -170,44 +209,62 @@ __global__ __launch_bounds__(256, 2) void wide_kernel(const void *__restrict__ P
         rowf[ub] = !ok ? 0.0f : F32 ? down : sh.scale * kLog2e;      // (fp32: scale log2 e is in the operands, the factor a power of two)
         ref[ub] = TOP && ok ? row_ref[r < sh.rows ? r : sh.rows - 1] : 0.0f;
         st[ub] = {kNone, 0.0f, 0.0f};
-        s_all[ub][0][tid] = kNone;
-        s_all[ub][1][tid] = s_all[ub][2][tid] = 0.0f;
+        lds.all[ub][0][tid] = kNone;
+        lds.all[ub][1][tid] = lds.all[ub][2][tid] = 0.0f;
     }
 
-    // copies of the next ST tiles: 1 KB a wavefront instruction, lane-linear in LDS, the swizzle in the source address
-    auto stage = [&](int64_t tile, int buf) {
+    // copies of the next ST tiles: 1 KB a wavefront instruction, lane-linear in LDS, the swizzle in the source address.  (Nothing in the loop loads into
+    // registers from memory: loads return in order, and one would wait for the next stage's copies.)
+    constexpr int NC = (ST * G::TILEB / 1024 + 3) / 4;
+    uint32_t off[NC];
 #pragma unroll
-        for (int n = 0; n < ST * G::TILEB / 4096; ++n) {
-            const int o = (n * 4 + wid) * 1024 + lane * 16, row = o / G::ROWB, c = (o % G::ROWB) / 16 ^ G::swz(row);
-            int64_t i = tile * kTile + row;
-            if constexpr (!F32) i = i < sh.items ? i : sh.items - 1;         // (the planes of fp32 tables are padded)
-            const char *src = F32 ? planes + (size_t)i * G::ROWB + 16 * c : (const char *)Qtab + (size_t)i * G::ROWB + 16 * c;
-            copy_to_lds(src, lds[buf] + (n * 4 + wid) * 1024);
+    for (int n = 0; n < NC; ++n) {
+        const int o = ((n * 4 + wid) * 1024 + lane * 16) % (ST * G::TILEB), row = o / G::ROWB, c = ((o % G::ROWB) / 16) ^ G::swz(row & 31);
+        off[n] = (uint32_t)(row * G::ROWB + 16 * c);
+    }
+    const int64_t words = mask_words(sh.items), tiles = (sh.items + kTile - 1) / kTile;
+    auto stage = [&](int64_t tile, int buf) {
+        const int64_t t = F32 || tile < tiles ? tile : tiles - 1;                // (the planes of fp32 tables are padded to groups)
+        const char *base = rows + (size_t)t * G::TILEB;
+        const int64_t left = (sh.items - t * kTile) * G::ROWB;
+#pragma unroll
+        for (int n = 0; n < NC; ++n) {
+            if ((NC * 4 - 3) * 1024 > ST * G::TILEB && (n * 4 + wid) * 1024 >= ST * G::TILEB) break;
+            uint32_t o = off[n];
+            if constexpr (!F32) o = (int64_t)o < left ? o : o % G::ROWB;          // rows behind the last item: any valid row, they are masked
+            copy_to_lds(base + o, lds.tile[buf] + (n * 4 + wid) * 1024);
+        }
+        if constexpr (MASK) {
+            if ((tile & 3) == 0) {
+#pragma unroll
+                for (int ub = 0; ub < UB; ++ub) {
+                    const int64_t r = row0 + 32 * ub + l31;
+                    if (hi == 0) copy_to_lds((const char *)(bits + (size_t)(r < sh.rows ? r : sh.rows - 1) * words + tile), lds.bits[(tile >> 2) & 1][wid][ub]);
+                }
+            }
         }
     };
-    const int64_t words = mask_words(sh.items);
-    const int sw = G::swz(l31) * 16;
+    const int hs = (16 * hi) ^ (G::swz(l31) * 16);
     if (g0 < g1) stage(4 * g0, 0);
     int buf = 0;
     for (int64_t g = g0; g < g1; ++g) {
-        uint4 seen[UB];
-        if constexpr (MASK) {
-#pragma unroll
-            for (int ub = 0; ub < UB; ++ub) {
-                const int64_t r = row0 + 32 * ub + l31;
-                seen[ub] = *reinterpret_cast<const uint4 *>(bits + (size_t)(r < sh.rows ? r : sh.rows - 1) * words + 4 * g);
-            }
-        }
-        uint32_t key[UB][4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int64_t tile = 4 * g + j;
             if (j % ST == 0) {
                 __syncthreads();         // this stage's copies have landed; everyone is done with the other buffer
+                if (TOP && j == 0 && g > g0) {        // the last group's maxima, ahead of the copies so that the next barrier finds them done
+#pragma unroll
+                    for (int ub = 0; ub < UB; ++ub) {
+                        const int64_t r = row0 + 32 * ub + l31;
+                        if (r < sh.rows)
+                            keys[(size_t)r * (2 * groups) + 2 * (g - 1) + hi] = make_uint4(lds.key[ub][0][tid], lds.key[ub][1 % (TOP ? 4 : 1)][tid], lds.key[ub][2 % (TOP ? 4 : 1)][tid], lds.key[ub][3 % (TOP ? 4 : 1)][tid]);
+                    }
+                }
                 if (j + ST < 4 || g + 1 < g1) stage(tile + ST, buf ^ 1);
                 buf ^= 1;
             }
-            const char *t0 = lds[buf ^ 1] + (j % ST) * G::TILEB + l31 * G::ROWB;
+            const char *t0 = lds.tile[buf ^ 1] + (j % ST) * G::TILEB + l31 * G::ROWB;
             f32x16 acc[UB];
 #pragma unroll
             for (int ub = 0; ub < UB; ++ub)
@@ -217,7 +274,7 @@ __global__ __launch_bounds__(256, 2) void wide_kernel(const void *__restrict__ P
             for (int s = 0; s < KS; ++s) {
                 Frag a[NP];
 #pragma unroll
-                for (int p = 0; p < NP; ++p) a[p].u = *reinterpret_cast<const uint4 *>(t0 + ((16 * (p * (D / 8) + 2 * s + hi)) ^ sw));
+                for (int p = 0; p < NP; ++p) a[p].u = *reinterpret_cast<const uint4 *>(t0 + ((p * (2 * D) + 32 * s) ^ hs));
 #pragma unroll
                 for (int ub = 0; ub < UB; ++ub) acc[ub] = mfma32<F32>(a[0], b[ub][s][0], acc[ub]);
                 if constexpr (F32) {
@@ -227,82 +284,59 @@ __global__ __launch_bounds__(256, 2) void wide_kernel(const void *__restrict__ P
                     for (int ub = 0; ub < UB; ++ub) acc[ub] = mfma32<F32>(a[1], b[ub][s][0], acc[ub]);
                 }
             }
-            // scores of row l31 (of each block): register i is item 32 tile + (i & 3) + 8 (i >> 2) + 4 hi
+            // the tile's operands are read from LDS AHEAD steps before their products
+            constexpr int AHEAD = RSX_LP_AHEAD;
+            __builtin_amdgcn_sched_group_barrier(0x100, (KS < AHEAD ? KS : AHEAD) * NP, 0);
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                __builtin_amdgcn_sched_group_barrier(0x008, (F32 ? 3 : 1) * UB, 0);
+                if (s + AHEAD < KS) __builtin_amdgcn_sched_group_barrier(0x100, NP, 0);
+            }
             const float tf = F32 ? factor[tile] : 1.0f;
             const int64_t left = sh.items - tile * kTile;
             const uint32_t none = left >= 32 ? 0u : left <= 0 ? 0xFFFFFFFFu : 0xFFFFFFFFu << left;
 #pragma unroll
             for (int ub = 0; ub < UB; ++ub) {
-                const float f = rowf[ub] * tf;
                 uint32_t w = none;
-                if constexpr (MASK) w |= j == 0 ? seen[ub].x : j == 1 ? seen[ub].y : j == 2 ? seen[ub].z : seen[ub].w;
+                if constexpr (MASK) w |= *reinterpret_cast<const uint32_t *>(lds.bits[g & 1][wid][ub] + l31 * 16 + j * 4);
                 w >>= 4 * hi;
-                const bool any = __builtin_amdgcn_ballot_w64((w & 0x0F0F0F0Fu) != 0u) != 0ull;
-                if (any) {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if ((w >> ((i & 3) + 8 * (i >> 2))) & 1u) acc[ub][i] = -INFINITY;
-                }
-                float c0 = acc[ub][0], c1 = acc[ub][8];
-#pragma unroll
-                for (int i = 1; i < 8; ++i) { c0 = fmaxf(c0, acc[ub][i]); c1 = fmaxf(c1, acc[ub][8 + i]); }
-                const float top = fmaxf(c0, c1) * f;
-                if constexpr (TOP)
-                    key[ub][j] = (uint32_t)half_bits(fmaf(c0, f, -ref[ub])) | ((uint32_t)half_bits(fmaf(c1, f, -ref[ub])) << 16);
-                if (__builtin_amdgcn_ballot_w64(top > st[ub].m + kLazy) != 0ull) {
-                    if (top > st[ub].m) stat_lift(st[ub], top);
-                }
-                const float m = st[ub].m;
-                float sum = 0.0f, ent = 0.0f;         // of the tile; then of the group, then of all: each sum adds up few terms
-                if (any) {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float t = acc[ub][i] == -INFINITY ? -1.0e4f : fmaf(acc[ub][i], f, -m);
-                        const float e = __builtin_amdgcn_exp2f(t);
-                        sum += e;
-                        ent = fmaf(e, t, ent);
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float t = fmaf(acc[ub][i], f, -m);
-                        const float e = __builtin_amdgcn_exp2f(t);
-                        sum += e;
-                        ent = fmaf(e, t, ent);
-                    }
-                }
-                st[ub].sum += sum;
-                st[ub].ent += ent;
+                uint32_t *key = &lds.key[ub][j % (TOP ? 4 : 1)][tid];
+                if (__builtin_amdgcn_ballot_w64((w & 0x0F0F0F0Fu) != 0u) == 0ull) absorb<false, TOP>(acc[ub], rowf[ub] * tf, 0u, st[ub], ref[ub], key);
+                else absorb<true, TOP>(acc[ub], rowf[ub] * tf, w, st[ub], ref[ub], key);
             }
         }
 #pragma unroll
         for (int ub = 0; ub < UB; ++ub) {
-            Stat all = {s_all[ub][0][tid], s_all[ub][1][tid], s_all[ub][2][tid]};
+            Stat all = {lds.all[ub][0][tid], lds.all[ub][1][tid], lds.all[ub][2][tid]};
             stat_lift(all, st[ub].m);
-            s_all[ub][0][tid] = all.m;
-            s_all[ub][1][tid] = all.sum + st[ub].sum;
-            s_all[ub][2][tid] = all.ent + st[ub].ent;
+            lds.all[ub][0][tid] = all.m;
+            lds.all[ub][1][tid] = all.sum + st[ub].sum;
+            lds.all[ub][2][tid] = all.ent + st[ub].ent;
             st[ub].sum = st[ub].ent = 0.0f;
-        }
-        if constexpr (TOP) {
-#pragma unroll
-            for (int ub = 0; ub < UB; ++ub) {
-                const int64_t r = row0 + 32 * ub + l31;
-                if (r < sh.rows) keys[(size_t)r * (2 * groups) + 2 * g + hi] = make_uint4(key[ub][0], key[ub][1], key[ub][2], key[ub][3]);
-            }
         }
     }
     // the two halves of a row, then the row's partial of this split
 #pragma unroll
     for (int ub = 0; ub < UB; ++ub) {
-        Stat all = {s_all[ub][0][tid], s_all[ub][1][tid], s_all[ub][2][tid]};
+        const int64_t r = row0 + 32 * ub + l31;
+        if (TOP && g1 > g0 && r < sh.rows)
+            keys[(size_t)r * (2 * groups) + 2 * (g1 - 1) + hi] = make_uint4(lds.key[ub][0][tid], lds.key[ub][1 % (TOP ? 4 : 1)][tid], lds.key[ub][2 % (TOP ? 4 : 1)][tid], lds.key[ub][3 % (TOP ? 4 : 1)][tid]);
+        Stat all = {lds.all[ub][0][tid], lds.all[ub][1][tid], lds.all[ub][2][tid]};
         Stat o = {__shfl_xor(all.m, 32, 64), __shfl_xor(all.sum, 32, 64), __shfl_xor(all.ent, 32, 64)};
         const float m = fmaxf(all.m, o.m);
         stat_lift(all, m);
         stat_lift(o, m);
-        const int64_t r = row0 + 32 * ub + l31;
         if (hi == 0 && r < sh.rows) part[(size_t)r * splits + blockIdx.x] = make_float4(m, all.sum + o.sum, all.ent + o.ent, 0.0f);
     }
+}
+
+template <int D, bool F32, bool MASK, bool TOP>
+__global__ __launch_bounds__(256, (WideGeo<D, F32>::OCC)) void wide_kernel(const void *__restrict__ P, const char *__restrict__ rows, const float *__restrict__ factor,
+                                                                           Shape sh, const uint32_t *__restrict__ bits, const float *__restrict__ row_ref, int splits,
+                                                                           float4 *__restrict__ part, uint4 *__restrict__ keys)
+{
+    __shared__ WideLds<D, F32, MASK, TOP> lds;
+    wide_body<D, F32, MASK, TOP>(P, rows, factor, sh, bits, row_ref, splits, part, keys, lds);
 }
 
 // ---- few rows ---------------------------------------------------------------------------------------------------------------------------
@@ -452,7 +486,6 @@ __global__ __launch_bounds__(256) void thin_kernel(const void *__restrict__ P, c
 }
 
 // ---- one workgroup per row: join the partials, the given items, the K best -------------------------------------------------------------
-constexpr int kFin = 256;
 constexpr int kMaxChunks = 256;                   // chunks whose items are computed again; more (ties by the thousand): the whole row is
 constexpr int kCand = 8 * kMaxChunks;
 constexpr int kListed = 4096;                     // chunks looked at more closely for that choice
@@ -461,15 +494,16 @@ static_assert(kListed * 4 <= kCand * 8 && kListed * 2 <= kCand * 4, "the list of
 // (score, id) order: larger score first, then lower id
 __device__ __forceinline__ bool before(double sa, int32_t ia, double sb, int32_t ib) { return sa > sb || (sa == sb && ia < ib); }
 
+template <int NT>
 __device__ void sort_candidates(double *s, int32_t *id, int n)          // descending; n <= kCand entries, padded here to a power of two
 {
     int n2 = 1;
     while (n2 < n) n2 <<= 1;
-    for (int t = n + threadIdx.x; t < n2; t += kFin) { s[t] = -INFINITY; id[t] = 0x7FFFFFFF; }
+    for (int t = n + threadIdx.x; t < n2; t += NT) { s[t] = -INFINITY; id[t] = 0x7FFFFFFF; }
     __syncthreads();
     for (int size = 2; size <= n2; size <<= 1)
         for (int stride = size >> 1; stride > 0; stride >>= 1) {
-            for (int t = threadIdx.x; t < n2 / 2; t += kFin) {
+            for (int t = threadIdx.x; t < n2 / 2; t += NT) {
                 const int lo = 2 * t - (t & (stride - 1)), hi = lo + stride;
                 const bool down = (lo & size) == 0;
                 if (before(s[hi], id[hi], s[lo], id[lo]) == down) {
@@ -481,66 +515,75 @@ __device__ void sort_candidates(double *s, int32_t *id, int n)          // desce
         }
 }
 
-template <int D, bool F32>
-__global__ __launch_bounds__(kFin) void finish_kernel(const void *__restrict__ P, const void *__restrict__ Q, Shape sh, const uint32_t *__restrict__ bits,
-                                                      const float4 *__restrict__ part, int splits, const uint16_t *__restrict__ keys,
-                                                      const int32_t *__restrict__ given, int T, int K, float *__restrict__ logp, float *__restrict__ lse_out,
-                                                      float *__restrict__ ent_out, int32_t *__restrict__ top_idx, float *__restrict__ top_logp)
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ half2v max2(half2v a, half2v b) { return __builtin_elementwise_max(a, b); }      // (NaN: the other)
+__device__ __forceinline__ half2v as_half2(uint32_t w) { return __builtin_bit_cast(half2v, w); }
+__device__ __forceinline__ uint32_t half_order(_Float16 v)                                                  // halves -> ordered integers
 {
-    constexpr int LPI = F32 ? D / 4 : D / 8, EPL = F32 ? 4 : 8, IPP = kFin / LPI;      // lanes an item's row takes, elements a lane, items a pass
-    __shared__ double c_s[kCand];
-    __shared__ int32_t c_id[kCand];
-    __shared__ double s_lse;
-    __shared__ double s_red[3][4];
-    __shared__ uint16_t s_max[kFin];
-    __shared__ int32_t s_list[kMaxChunks];
+    const uint32_t h = __builtin_bit_cast(uint16_t, v);
+    return (h & 0x8000u) ? (~h & 0xFFFFu) : (h | 0x8000u);
+}
+__device__ __forceinline__ float half_value(uint32_t order)
+{
+    const uint16_t h = (uint16_t)((order & 0x8000u) ? order & 0x7FFFu : ~order);
+    return (float)__builtin_bit_cast(_Float16, h);
+}
+
+// sum over groups of LPI neighbouring lanes, in their last one
+template <int LPI>
+__device__ __forceinline__ float group_sum(float v)
+{
+#define RSX_DPP_ADD(ctrl_) v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), ctrl_, 0xF, 0xF, true))
+    RSX_DPP_ADD(0x111);                                       // row_shr:1
+    RSX_DPP_ADD(0x112);
+    if constexpr (LPI >= 8) RSX_DPP_ADD(0x114);
+    if constexpr (LPI >= 16) RSX_DPP_ADD(0x118);
+#undef RSX_DPP_ADD
+    if constexpr (LPI >= 32) v += __shfl_up(v, 16, 64);
+    if constexpr (LPI >= 64) v += __shfl_up(v, 32, 64);
+    return v;
+}
+
+// NT threads a row: 1024 where rows are few and one row's chain of loads is the time, 256 where many rows share a CU
+template <int D, bool F32, int NT>
+__global__ __launch_bounds__(NT) void finish_kernel(const void *__restrict__ P, const void *__restrict__ Q, Shape sh, const uint32_t *__restrict__ bits,
+                                                    const float4 *__restrict__ part, int splits, const uint16_t *__restrict__ keys,
+                                                    const float *__restrict__ row_ref, const int32_t *__restrict__ given, int T, int K, float *__restrict__ logp,
+                                                    float *__restrict__ lse_out, float *__restrict__ ent_out, int32_t *__restrict__ top_idx, float *__restrict__ top_logp)
+{
+    constexpr int LPI = F32 ? D / 4 : D / 8, EPL = F32 ? 4 : 8, IPP = NT / LPI;        // lanes an item's row takes, elements a lane, items a pass
+    constexpr int NW = NT / 64, KR = NT == 1024 ? 16 : 8, FL = 8;                               // wavefronts; 16-byte loads of maxima a thread keeps; item rows on the way together
+    __shared__ __attribute__((aligned(16))) double c_s[kCand];
+    __shared__ __attribute__((aligned(16))) int32_t c_id[kCand];
+    __shared__ double s_red[3][NW];
+    __shared__ __attribute__((aligned(16))) uint16_t s_max[256];
+    __shared__ int32_t s_list[kMaxChunks], s_item[kMaxChunks];
     __shared__ int s_n, s_count;
     __shared__ uint32_t s_tau;
     const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
     const int64_t r = blockIdx.x;
     const int32_t u = sh.user_ids[r];
     if (!row_ok(u, sh.users)) {                    // no row: nothing is probable, nothing has a log-probability
-        for (int t = tid; t < T; t += kFin) logp[r * T + t] = 0.0f;
-        for (int t = tid; t < K; t += kFin) { top_idx[r * K + t] = -1; top_logp[r * K + t] = -INFINITY; }
+        for (int t = tid; t < T; t += NT) logp[r * T + t] = 0.0f;
+        for (int t = tid; t < K; t += NT) { top_idx[r * K + t] = -1; top_logp[r * K + t] = -INFINITY; }
         if (tid == 0) { if (lse_out) lse_out[r] = -INFINITY; if (ent_out) ent_out[r] = 0.0f; }
         return;
     }
-    // the partials, in 64 bits
-    double m = kNone, sum = 0.0, ent = 0.0;
-    for (int s = tid; s < splits; s += kFin) m = fmax(m, (double)part[r * splits + s].x);
+    // everything that is known to be needed is asked for at once: the maxima of the chunks, the user's row, the partials
+    const int64_t chunks = (sh.items + 127) / 128 * 16;
+    const uint16_t *key = keys + (size_t)r * chunks;
+    uint4 kept[KR];
+    auto fetch = [&](int64_t base) {               // maxima base + 8 (tid + NT n) ..
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m = fmax(m, __shfl_xor(m, o, 64));
-    if (lane == 0) s_red[0][wid] = m;
-    __syncthreads();
-    m = fmax(fmax(s_red[0][0], s_red[0][1]), fmax(s_red[0][2], s_red[0][3]));
-    for (int s = tid; s < splits; s += kFin) {
-        const float4 p = part[r * splits + s];
-        if (p.y == 0.0f) continue;                 // (met nothing; NaN sums are kept)
-        const double w = exp2((double)p.x - m);
-        sum += w * p.y;
-        ent += w * ((double)p.z + (double)p.y * ((double)p.x - m));
-    }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) { sum += __shfl_xor(sum, o, 64); ent += __shfl_xor(ent, o, 64); }
-    if (lane == 0) { s_red[1][wid] = sum; s_red[2][wid] = ent; }
-    __syncthreads();
-    if (tid == 0) {
-        sum = s_red[1][0] + s_red[1][1] + s_red[1][2] + s_red[1][3];
-        ent = s_red[2][0] + s_red[2][1] + s_red[2][2] + s_red[2][3];
-        const double l2 = log2(sum);
-        const double lse = sum == 0.0 ? -INFINITY : kLn2 * (m + l2);
-        s_lse = lse;
-        if (lse_out) lse_out[r] = (float)lse;
-        if (ent_out) ent_out[r] = sum == 0.0 ? 0.0f : (float)(kLn2 * (l2 - ent / sum));
-    }
-    __syncthreads();
-    const double lse = s_lse;
-
-    // a lane's elements of the row's user, and its share of an item's product in 64 bits
+        for (int n = 0; n < KR; ++n) {
+            const int64_t c = base + 8 * ((int64_t)tid + NT * n);
+            kept[n] = c < chunks ? *reinterpret_cast<const uint4 *>(key + c) : make_uint4(0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u);
+        }
+    };
+    if (K > 0) fetch(0);
     const int li = tid % LPI;
     double p[EPL];
-    auto elements = [&](const void *t, int64_t row, double *x) {
-        const uint4 v = *reinterpret_cast<const uint4 *>((const char *)t + (size_t)row * (D * (F32 ? 4 : 2)) + li * 16);
+    auto widen = [](const uint4 &v, double *x) {
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -548,177 +591,292 @@ __global__ __launch_bounds__(kFin) void finish_kernel(const void *__restrict__ P
             else { x[2 * j] = (double)__uint_as_float(w[j] << 16); x[2 * j + 1] = (double)__uint_as_float(w[j] & 0xFFFF0000u); }
         }
     };
-    elements(P, u, p);
+    widen(*reinterpret_cast<const uint4 *>((const char *)P + (size_t)u * (D * (F32 ? 4 : 2)) + li * 16), p);
+
+    float pf[EPL];
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) pf[j] = (float)p[j];
+
+    // the partials, in 64 bits
+    float4 mine = make_float4(kNone, 0.f, 0.f, 0.f);
+    if (tid < splits) mine = part[r * splits + tid];
+    double m = mine.x, sum = 0.0, ent = 0.0;
+    for (int s = tid + NT; s < splits; s += NT) m = fmax(m, (double)part[r * splits + s].x);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = fmax(m, __shfl_xor(m, o, 64));
+    if (lane == 0) s_red[0][wid] = m;
+    if (tid == 0) s_n = 0;
+    __syncthreads();
+    m = s_red[0][0];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) m = fmax(m, s_red[0][w]);
+    for (int s = tid; s < splits; s += NT) {
+        const float4 q = s == tid ? mine : part[r * splits + s];
+        if (q.y == 0.0f) continue;                 // (met nothing; NaN sums are kept)
+        const double w = exp2((double)q.x - m);
+        sum += w * q.y;
+        ent += w * ((double)q.z + (double)q.y * ((double)q.x - m));
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) { sum += __shfl_xor(sum, o, 64); ent += __shfl_xor(ent, o, 64); }
+    if (lane == 0) { s_red[1][wid] = sum; s_red[2][wid] = ent; }
+    __syncthreads();
+    sum = ent = 0.0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) { sum += s_red[1][w]; ent += s_red[2][w]; }
+    const double l2 = log2(sum);
+    const double lse = sum == 0.0 ? -INFINITY : kLn2 * (m + l2);
+    if (tid == 0) {
+        if (lse_out) lse_out[r] = (float)lse;
+        if (ent_out) ent_out[r] = sum == 0.0 ? 0.0f : (float)(kLn2 * (l2 - ent / sum));
+    }
+
     const int64_t words = mask_words(sh.items);
     const uint32_t *seen = bits ? bits + (size_t)r * words : nullptr;
     auto masked = [&](int32_t i) { return seen != nullptr && ((seen[i >> 5] >> (i & 31)) & 1u); };
-    // four items at a time: their rows are on the way together
-    auto dots = [&](const int64_t (&i)[4], double (&z)[4]) {
-        double q[4][EPL];
+    // FL items at a time
+    auto dots = [&](const int32_t (&i)[FL], double (&z)[FL]) {
+        uint4 v[FL];
 #pragma unroll
-        for (int n = 0; n < 4; ++n) elements(Q, i[n], q[n]);
+        for (int n = 0; n < FL; ++n) v[n] = *reinterpret_cast<const uint4 *>((const char *)Q + (size_t)i[n] * (D * (F32 ? 4 : 2)) + li * 16);
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
+        for (int n = 0; n < FL; ++n) {
+            double q[EPL];
+            widen(v[n], q);
             z[n] = 0.0;
 #pragma unroll
-            for (int j = 0; j < EPL; ++j) z[n] = fma(p[j], q[n][j], z[n]);
+            for (int j = 0; j < EPL; ++j) z[n] = fma(p[j], q[j], z[n]);
         }
 #pragma unroll
         for (int o = LPI / 2; o > 0; o >>= 1)
 #pragma unroll
-            for (int n = 0; n < 4; ++n) z[n] += __shfl_xor(z[n], o, LPI);
+            for (int n = 0; n < FL; ++n) z[n] += __shfl_xor(z[n], o, LPI);
 #pragma unroll
-        for (int n = 0; n < 4; ++n) z[n] *= (double)sh.scale;
+        for (int n = 0; n < FL; ++n) z[n] *= (double)sh.scale;
     };
-    for (int t0 = tid / LPI; t0 < T; t0 += 4 * IPP) {
-        int64_t i[4];
-        double z[4];
-        bool ok[4];
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-            const int t = t0 + n * IPP;
-            i[n] = t < T ? given[r * T + t] : -1;
-            ok[n] = i[n] >= 0 && i[n] < sh.items;
-            i[n] = ok[n] ? i[n] : 0;
-        }
-        dots(i, z);
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-            const int t = t0 + n * IPP;
-            if (li == 0 && t < T) logp[r * T + t] = !ok[n] ? 0.0f : masked((int32_t)i[n]) ? -INFINITY : (float)(z[n] - lse);
-        }
-    }
-    if (K == 0) return;
 
-    // K + 8 chunks with the largest maxima, and all that equal the last of them: a lower bound of that maximum comes from 256 threads' own
-    const int64_t chunks = (sh.items + 127) / 128 * 16;
-    const uint16_t *key = keys + (size_t)r * chunks;
-    auto order = [](uint32_t h) { return (h & 0x8000u) ? (~h & 0xFFFFu) : (h | 0x8000u); };      // halves -> ordered integers (NaN above all)
-    const uint32_t lowest = order(0xFC00u);                                                         // -inf: nothing in the chunk
-    uint32_t mine = 0;
-    auto walk = [&](auto f) {            // every chunk once, 8 at a time where there are many
-        if (chunks > 16 * kFin) {
-            for (int64_t c = 8 * tid; c < chunks; c += 8 * kFin) {
-                const uint4 v = *reinterpret_cast<const uint4 *>(key + c);
-                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    // K + 8 chunks with the largest maxima and all that equal the last of them.  First a lower bound of that maximum: the K + 8-th largest of the
+    // threads' own (no fewer chunks can be above it); then the chunks from the bound up, and among them the ones with fewer than K + 8 above
+    int n = 0;                                     // entries: T given items, then 8 for each chosen chunk
+    float cut = -INFINITY;                         // a score that K items reach, by the stored maxima
+    bool whole = false;                            // too many ties: every item of the row is computed
+    if (K > 0) {
+        const half2v none = as_half2(0xFC00FC00u);                                                  // -inf: nothing in the chunk
+        const uint32_t lowest = half_order(none[0]);
+        half2v top8 = none;
+        for (int64_t base = 0; base < chunks; base += 8ll * NT * KR) {
+            if (base > 0) fetch(base);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) { f(order(w[j] & 0xFFFFu), c + 2 * j); f(order(w[j] >> 16), c + 2 * j + 1); }
-            }
-        } else {
-            for (int64_t c = tid; c < chunks; c += kFin) f(order(key[c]), c);
+            for (int n_ = 0; n_ < KR; ++n_)
+                top8 = max2(top8, max2(max2(as_half2(kept[n_].x), as_half2(kept[n_].y)), max2(as_half2(kept[n_].z), as_half2(kept[n_].w))));
         }
-    };
-    walk([&](uint32_t k, int64_t) { mine = k > mine ? k : mine; });
-    s_max[tid] = (uint16_t)mine;
-    if (tid == 0) { s_n = 0; s_tau = lowest + 1; }
-    __syncthreads();
-    int above = 0;
-    for (int t = 0; t < kFin; ++t) above += s_max[t] > mine || (s_max[t] == mine && t < tid);
-    if (above == K + 7 && mine > lowest) s_tau = mine;
-    __syncthreads();
-    // the chunks from that bound up, with their maxima (in the candidates' memory); where the bound was loose -- the best items' chunks were
-    // few threads' -- the K + 8-th largest maximum among them is found bit by bit
-    int32_t *const l_chunk = reinterpret_cast<int32_t *>(c_s);
-    uint16_t *const l_key = reinterpret_cast<uint16_t *>(c_id);
-    const uint32_t bound = s_tau;
-    walk([&](uint32_t k, int64_t c) {
-        if (k >= bound) {
-            const int at = atomicAdd(&s_n, 1);
-            if (at < kListed) { l_chunk[at] = (int32_t)c; l_key[at] = (uint16_t)k; }
-        }
-    });
-    __syncthreads();
-    const int listed = s_n;
-    __syncthreads();                     // (s_n is counted anew below)
-    uint32_t tau = bound;
-    if (listed > kMaxChunks && listed <= kListed) {
-        tau = 0;
-        for (int bit = 15; bit >= 0; --bit) {
-            const uint32_t t = tau | (1u << bit);
-            if (tid == 0) s_count = 0;
-            __syncthreads();
-            int c = 0;
-            for (int q = tid; q < listed; q += kFin) c += l_key[q] >= t;
-            if (c) atomicAdd(&s_count, c);
-            __syncthreads();
-            if (s_count >= K + 8) tau = t;
-            __syncthreads();
-        }
-    }
-    if (tid == 0) s_n = listed <= kListed ? 0 : listed;
-    __syncthreads();
-    if (listed <= kListed) {
-        for (int q = tid; q < listed; q += kFin)
-            if (l_key[q] >= tau) {
-                const int at = atomicAdd(&s_n, 1);
-                if (at < kMaxChunks) s_list[at] = l_chunk[q];
-            }
-    }
-    __syncthreads();
-    int n;
-    if (s_n <= kMaxChunks) {
-        n = 8 * s_n;
-        for (int q0 = tid / LPI; q0 < n; q0 += 4 * IPP) {
-            int64_t i[4];
-            double z[4];
-            bool ok[4];
+        uint32_t best = half_order(top8[0]);
+        { const uint32_t x = half_order(top8[1]); best = x > best ? x : best; }
+        if constexpr (NT > 256) {                  // 256 maxima, of NT / 256 threads each
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int q = q0 + k * IPP;
-                i[k] = q < n ? chunk_item0(s_list[q >> 3]) + (q & 3) + 2 * (q & 4) : sh.items;
-                ok[k] = i[k] < sh.items;
-                i[k] = ok[k] ? i[k] : 0;
-            }
-            dots(i, z);
+            for (int o = 1; o < NT / 256; o <<= 1) { const uint32_t x = __shfl_xor(best, o, 64); best = x > best ? x : best; }
+        }
+        if (tid % (NT / 256) == 0) s_max[tid / (NT / 256)] = (uint16_t)best;
+        __syncthreads();
+        if (wid == 0) {                            // the K + 8-th largest of 256, bit by bit, in one wavefront
+            const uint2 v = reinterpret_cast<const uint2 *>(s_max)[lane];
+            const uint32_t x[4] = {v.x & 0xFFFFu, v.x >> 16, v.y & 0xFFFFu, v.y >> 16};
+            uint32_t t = 0;
+            for (int bit = 15; bit >= 0; --bit) {
+                const uint32_t u_ = t | (1u << bit);
+                int c = 0;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int q = q0 + k * IPP;
-                if (li == 0 && q < n) {
-                    const bool in = ok[k] && z[k] == z[k] && !masked((int32_t)i[k]);
-                    c_s[q] = in ? z[k] : -INFINITY;
-                    c_id[q] = in ? (int32_t)i[k] : 0x7FFFFFFF;
+                for (int j = 0; j < 4; ++j) c += __builtin_popcountll(__builtin_amdgcn_ballot_w64(x[j] >= u_));
+                if (c >= K + 8) t = u_;
+            }
+            if (lane == 0) s_tau = t > lowest ? t : lowest + 1;
+        }
+        __syncthreads();
+        int32_t *const l_chunk = reinterpret_cast<int32_t *>(c_s);
+        uint16_t *const l_key = reinterpret_cast<uint16_t *>(c_id);
+        const uint32_t bound = s_tau;
+        const _Float16 bound_h = (_Float16)half_value(bound);
+        for (int64_t base = 0; base < chunks; base += 8ll * NT * KR) {
+            if (chunks > 8ll * NT * KR) fetch(base);
+#pragma unroll
+            for (int n_ = 0; n_ < KR; ++n_) {
+                const half2v m2 = max2(max2(as_half2(kept[n_].x), as_half2(kept[n_].y)), max2(as_half2(kept[n_].z), as_half2(kept[n_].w)));
+                if (m2[0] < bound_h && m2[1] < bound_h) continue;
+                const uint32_t w[4] = {kept[n_].x, kept[n_].y, kept[n_].z, kept[n_].w};
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const uint32_t k = half_order(as_half2(w[j / 2])[j & 1]);
+                    if (k >= bound) {
+                        const int at = atomicAdd(&s_n, 1);
+                        if (at < kListed) { l_chunk[at] = (int32_t)(base + 8 * ((int64_t)tid + NT * n_) + j); l_key[at] = (uint16_t)k; }
+                    }
                 }
             }
         }
         __syncthreads();
-        sort_candidates(c_s, c_id, n);
+        const int listed = s_n;
+        __syncthreads();                           // (s_n is counted anew below)
+        if (tid == 0) { s_n = listed <= kListed ? 0 : listed; s_tau = 0xFFFFu; }
+        if (tid < 8 && listed <= 1024) l_key[listed + tid] = 0;              // (read eight at a time)
+        __syncthreads();
+        if (listed <= 1024) {
+            for (int q = tid; q < listed; q += NT) {
+                const uint32_t k = l_key[q];
+                int over = 0;
+                for (int t = 0; t < listed; t += 8) {
+                    const uint4 v = *reinterpret_cast<const uint4 *>(l_key + t);
+                    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) over += ((w[j] & 0xFFFFu) > k) + ((w[j] >> 16) > k);
+                }
+                if (over < K + 8) {
+                    const int at = atomicAdd(&s_n, 1);
+                    if (at < kMaxChunks) s_list[at] = l_chunk[q];
+                    if (over < K) atomicMin(&s_tau, k);                  // the K-th largest maximum, from above
+                }
+            }
+        } else if (listed <= kListed) {            // (the best items' chunks were few threads': the K + 8-th bit by bit)
+            uint32_t tau = 0;
+            for (int bit = 15; bit >= 0; --bit) {
+                const uint32_t t = tau | (1u << bit);
+                if (tid == 0) s_count = 0;
+                __syncthreads();
+                int c = 0;
+                for (int q = tid; q < listed; q += NT) c += l_key[q] >= t;
+                if (c) atomicAdd(&s_count, c);
+                __syncthreads();
+                if (s_count >= K + 8) tau = t;
+                __syncthreads();
+            }
+            for (int q = tid; q < listed; q += NT)
+                if (l_key[q] >= tau) {
+                    const int at = atomicAdd(&s_n, 1);
+                    if (at < kMaxChunks) s_list[at] = l_chunk[q];
+                }
+            if (tid == 0) s_tau = tau;
+        }
+        __syncthreads();
+        whole = s_n > kMaxChunks;
+        n = whole ? 0 : 8 * s_n;
+        // K items reach the K-th maximum; it is a rounded half of a fast product, and taken a little lower here.  (How much does not matter: if fewer
+        // than K scores certainly reach `cut`, nothing is left out.)
+        if (!whole && s_n >= K) {
+            const float h = half_value(s_tau), ref = row_ref[r];
+            cut = (ref + h - (fabsf(h) * 0.002f + fabsf(ref) * 1e-5f + 0.01f)) * (float)kLn2;
+        }
+        __syncthreads();
+        if (tid == 0) s_n = s_count = 0;
+        __syncthreads();
+    }
+    // The items of the chosen chunks in fp32 with a bound of what that is off: those that can reach `cut` are computed in 64 bits.  If K of them
+    // certainly do, the K best are among them.
+    int reach = 0;
+    if (n > 0) {
+        for (int q0 = tid / LPI; q0 < n; q0 += FL * IPP) {
+            int32_t i[FL];
+            uint4 v[FL];
+#pragma unroll
+            for (int k = 0; k < FL; ++k) {
+                const int e = q0 + k * IPP;
+                const int64_t at = e < n ? chunk_item0(s_list[e >> 3]) + (e & 3) + 2 * (e & 4) : sh.items;
+                i[k] = at < sh.items ? (int32_t)at : -1;
+                v[k] = *reinterpret_cast<const uint4 *>((const char *)Q + (size_t)(i[k] < 0 ? 0 : i[k]) * (D * (F32 ? 4 : 2)) + li * 16);
+            }
+#pragma unroll
+            for (int k = 0; k < FL; ++k) {
+                const uint32_t w[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+                float z = 0.0f, size = 0.0f;
+#pragma unroll
+                for (int j = 0; j < EPL; ++j) {
+                    const float y = F32 ? __uint_as_float(w[j % 4]) : __uint_as_float(j & 1 ? w[j / 2] & 0xFFFF0000u : w[j / 2] << 16);
+                    z = fmaf(pf[j], y, z);
+                    size = fmaf(fabsf(pf[j]), fabsf(y), size);
+                }
+                z = group_sum<LPI>(z) * sh.scale;
+                const float err = group_sum<LPI>(size) * (sh.scale * (D + 8) * 0x1p-24f) + fabsf(cut) * 0x1p-22f;
+                if (li == LPI - 1 && i[k] >= 0 && z + err >= cut && !masked(i[k])) {
+                    const int at = atomicAdd(&s_n, 1);
+                    if (at < kMaxChunks) s_item[at] = i[k];
+                    if (z - err >= cut) atomicAdd(&s_count, 1);
+                }
+            }
+        }
+        __syncthreads();
+        reach = s_n;
+        if (s_count < K || reach > kMaxChunks) reach = 0;      // no: all of them in 64 bits
+    }
+    const int all = reach > 0 ? reach : n;
+    for (int q0 = tid / LPI; q0 < T + all; q0 += FL * IPP) {
+        int32_t i[FL];
+        double z[FL];
+        bool ok[FL];
+#pragma unroll
+        for (int k = 0; k < FL; ++k) {
+            const int q = q0 + k * IPP, e = q - T;
+            const int64_t at = q < T ? given[r * T + q] : e >= all ? -1 : reach > 0 ? s_item[e] : chunk_item0(s_list[e >> 3]) + (e & 3) + 2 * (e & 4);
+            ok[k] = at >= 0 && at < sh.items;
+            i[k] = ok[k] ? (int32_t)at : 0;
+        }
+        dots(i, z);
+        if (li == 0) {
+#pragma unroll
+            for (int k = 0; k < FL; ++k) {
+                const int q = q0 + k * IPP;
+                if (q >= T + all) continue;
+                const bool out = ok[k] && masked(i[k]);
+                if (q < T) logp[r * T + q] = !ok[k] ? 0.0f : out ? -INFINITY : (float)(z[k] - lse);
+                else { c_s[q - T] = ok[k] && !out && z[k] == z[k] ? z[k] : -INFINITY; c_id[q - T] = i[k]; }
+            }
+        }
+    }
+    if (K == 0) return;
+    __syncthreads();
+    if (reach > 0) {
+        for (int q = tid; q < reach; q += NT) {      // each one's place is the number of those before it
+            const double z = c_s[q];
+            const int32_t id = c_id[q];
+            int place = 0;
+            for (int t = 0; t < reach; ++t) place += before(c_s[t], c_id[t], z, id);
+            if (place < K) { top_idx[r * K + place] = id; top_logp[r * K + place] = (float)(z - lse); }
+        }
+        return;
+    }
+    if (!whole) {
+        sort_candidates<NT>(c_s, c_id, n);
     } else {
         // the row in blocks of half the list: what exceeds the K-th best so far is added, and the list cut to K when it is half full
-        __shared__ int s_m;
-        if (tid == 0) s_m = 0;
-        double floor_ = -INFINITY;
-        __syncthreads();
+        double least = -INFINITY;
         for (int64_t base = 0; base < sh.items; base += kCand / 2) {
             const int64_t end = base + kCand / 2 < sh.items ? base + kCand / 2 : sh.items;
-            for (int64_t q0 = base + tid / LPI; q0 < base + kCand / 2; q0 += 4 * IPP) {      // (whole groups of lanes stay together)
-                int64_t i[4];
-                double z[4];
+            for (int64_t q0 = base + tid / LPI; q0 < base + kCand / 2; q0 += FL * IPP) {      // (whole groups of lanes stay together)
+                int32_t i[FL];
+                double z[FL];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) i[k] = q0 + k * IPP < end ? q0 + k * IPP : 0;
+                for (int k = 0; k < FL; ++k) i[k] = q0 + k * IPP < end ? (int32_t)(q0 + k * IPP) : 0;
                 dots(i, z);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    if (li == 0 && q0 + k * IPP < end && z[k] > floor_ && !masked((int32_t)i[k])) {
-                        const int at = atomicAdd(&s_m, 1);
+                for (int k = 0; k < FL; ++k) {
+                    if (li == 0 && q0 + k * IPP < end && z[k] > least && !masked(i[k])) {
+                        const int at = atomicAdd(&s_n, 1);
                         c_s[at] = z[k];
-                        c_id[at] = (int32_t)i[k];
+                        c_id[at] = i[k];
                     }
                 }
             }
             __syncthreads();
-            const int have = s_m;
+            const int have = s_n;
             __syncthreads();
             if (have > kCand / 2 || end == sh.items) {
-                sort_candidates(c_s, c_id, have);
-                if (have >= K) floor_ = c_s[K - 1];
-                if (tid == 0) s_m = have < K ? have : K;
+                sort_candidates<NT>(c_s, c_id, have);
+                if (have >= K) least = c_s[K - 1];
+                if (tid == 0) s_n = have < K ? have : K;
                 __syncthreads();
             }
         }
-        n = s_m;
+        n = s_n;
     }
-    for (int t = tid; t < K; t += kFin) {
-        const bool in = t < n && c_id[t] != 0x7FFFFFFF;
+    for (int t = tid; t < K; t += NT) {
+        const bool in = t < n && c_s[t] > -INFINITY;
         top_idx[r * K + t] = in ? c_id[t] : -1;
         top_logp[r * K + t] = in ? (float)(c_s[t] - lse) : -INFINITY;
     }
@@ -747,11 +905,11 @@ struct Ws {
     int64_t pass, bytes;      // rows of one pass over the catalog
 };
 
-int wide_users(int d, int dtype) { return d * (dtype == RSX_F32 ? 2 : 1) <= 256 ? 256 : 128; }
+int wide_users(int d, int dtype) { return 128 * RSX_LP_UB(d, dtype == RSX_F32); }
 
 int64_t wide_splits(int64_t rows, int64_t items, int d, int dtype)
 {
-    const int64_t slots = 2 * (int64_t)rsx_num_cus(), ut = (rows + wide_users(d, dtype) - 1) / wide_users(d, dtype), groups = (items + 127) / 128;
+    const int64_t slots = RSX_LP_OCC(d, dtype == RSX_F32) * (int64_t)rsx_num_cus(), ut = (rows + wide_users(d, dtype) - 1) / wide_users(d, dtype), groups = (items + 127) / 128;
     const int64_t s = slots / ut;
     return s < 1 ? 1 : s > groups ? groups : s;
 }
@@ -776,7 +934,7 @@ Ws carve(void *ws, int64_t rows, int64_t items, int d, int dtype, bool mask, int
     w.pass = pass_rows(rows, items);
     const int64_t parts = thin ? thin_groups(items) : wide_splits(w.pass, items, d, dtype);
     // (the last, shorter pass takes more splits over fewer rows: rows x splits never exceeds this)
-    const int64_t cells = thin ? rows * parts : w.pass * parts + 2 * (int64_t)rsx_num_cus() * wide_users(d, dtype);
+    const int64_t cells = thin ? rows * parts : w.pass * parts + RSX_LP_OCC(d, dtype == RSX_F32) * (int64_t)rsx_num_cus() * wide_users(d, dtype);
     w.planes = take(!thin && dtype == RSX_F32 ? tiles4 * kTile * (int64_t)d * 4 : 0);
     w.factor = (float *)take(!thin && dtype == RSX_F32 ? tiles4 * 4 : 0);
     w.bits = (uint32_t *)take(mask ? w.pass * mask_words(items) * 4 : 0);
@@ -819,10 +977,8 @@ void run(const Call &c, const Ws &w, hipStream_t st)
         Shape sh = c.sh;
         sh.user_ids += r0;
         sh.rows = c.sh.rows - r0 < w.pass ? c.sh.rows - r0 : w.pass;
-        if (c.indptr) launch_clear_bits(sh.rows, items, w.bits, st);
-        if (c.indptr || c.K)
-            hipLaunchKernelGGL((row_prep_kernel<D, F32>), dim3((unsigned)((sh.rows + 3) / 4)), dim3(256), 0, st, c.P, c.Q, sh, c.indptr, c.indices, w.bits,
-                               c.K ? w.ref : (float *)nullptr);
+        if (c.indptr) hipLaunchKernelGGL(seen_bits_kernel, dim3((unsigned)sh.rows), dim3(256), 0, st, sh.user_ids, sh.users, c.indptr, c.indices, items, w.bits);
+        if (c.K) hipLaunchKernelGGL((reference_kernel<D, F32>), dim3((unsigned)((sh.rows + 3) / 4)), dim3(256), 0, st, c.P, c.Q, sh, w.ref);
         int parts;
         if (thin) {
             parts = thin_groups(items);
@@ -835,14 +991,16 @@ void run(const Call &c, const Ws &w, hipStream_t st)
         } else {
             parts = (int)wide_splits(sh.rows, items, D, F32 ? RSX_F32 : RSX_BF16);
             const dim3 grid((unsigned)parts, (unsigned)((sh.rows + WideGeo<D, F32>::WGU - 1) / WideGeo<D, F32>::WGU));
-#define RSX_LP_WIDE(M_, T_) hipLaunchKernelGGL((wide_kernel<D, F32, M_, T_>), grid, dim3(256), 0, st, c.P, c.Q, w.planes, w.factor, sh, w.bits, w.ref, parts, w.part, (uint4 *)w.keys)
+#define RSX_LP_WIDE(M_, T_) hipLaunchKernelGGL((wide_kernel<D, F32, M_, T_>), grid, dim3(256), 0, st, c.P, F32 ? w.planes : (const char *)c.Q, w.factor, sh, w.bits, w.ref, parts, w.part, (uint4 *)w.keys)
             if (c.indptr) { if (c.K) RSX_LP_WIDE(true, true); else RSX_LP_WIDE(true, false); }
             else { if (c.K) RSX_LP_WIDE(false, true); else RSX_LP_WIDE(false, false); }
 #undef RSX_LP_WIDE
         }
-        hipLaunchKernelGGL((finish_kernel<D, F32>), dim3((unsigned)sh.rows), dim3(kFin), 0, st, c.P, c.Q, sh, c.indptr ? w.bits : (const uint32_t *)nullptr, w.part,
-                           parts, w.keys, c.given + (c.T ? r0 * c.T : 0), c.T, c.K, c.logp + (c.T ? r0 * c.T : 0), c.lse ? c.lse + r0 : nullptr,
-                           c.ent ? c.ent + r0 : nullptr, c.top_idx + (c.K ? r0 * c.K : 0), c.top_logp + (c.K ? r0 * c.K : 0));
+#define RSX_LP_FINISH(NT_) hipLaunchKernelGGL((finish_kernel<D, F32, NT_>), dim3((unsigned)sh.rows), dim3(NT_), 0, st, c.P, c.Q, sh, c.indptr ? w.bits : (const uint32_t *)nullptr, \
+                                              w.part, parts, w.keys, w.ref, c.given + (c.T ? r0 * c.T : 0), c.T, c.K, c.logp + (c.T ? r0 * c.T : 0), \
+                                              c.lse ? c.lse + r0 : nullptr, c.ent ? c.ent + r0 : nullptr, c.top_idx + (c.K ? r0 * c.K : 0), c.top_logp + (c.K ? r0 * c.K : 0))
+        if (sh.rows <= rsx_num_cus()) RSX_LP_FINISH(1024); else RSX_LP_FINISH(256);
+#undef RSX_LP_FINISH
     }
 }
 

@@ -28,6 +28,7 @@ using namespace lp;
 
 constexpr float kFar = 1.0e30f;           // log-normaliser of a row without probabilities: every p is 0
 constexpr float kLift = 4096.0f;          // dz of fp32 tables is held times 2^12
+constexpr int kTopFactor = 16;            // where the largest item factor is kept among the scalars ([0]: the largest w |P| of a pass)
 
 struct Args {
     const void *P, *Q;
@@ -38,83 +39,96 @@ struct Args {
     float scale;
 };
 
-// per tile of 32 positions: [0] factor of its scores, [1] lse in log2, [2] [3] dz = p (A + B log2 p), the rest unused: 1 KB, one wavefront copy
+// per tile of 32 positions: [0] factor of its scores, [1] lse in log2, [2] [3] dz = p (A + B log2 p), [4] .. [7] the first four named items (as
+// integers; -1: none): 1 KB, one wavefront's copy
+constexpr int kHeld = 4;
 struct Prm {
-    float v[8][kTile];
+    float v[4 + kHeld][kTile];
 };
 
 // ---- what the passes need -------------------------------------------------------------------------------------------------------------
-// one wavefront per position (padded to 128): coefficients, named items with theirs, seen bits; the largest w |P| of all
+// one wavefront per position (padded to 128), positions dealt round: coefficients, named items with theirs, the largest w |P| (one atomic a
+// workgroup: a thousand on one word take 12 us).  The first workgroup also finds the largest item factor.
 template <int D, bool F32>
-__global__ __launch_bounds__(256) void rows_kernel(Args a, const int64_t *__restrict__ indptr, const int32_t *__restrict__ indices, uint32_t *__restrict__ bits,
-                                                   int64_t padded, Prm *__restrict__ prm, float *__restrict__ weight, int32_t *__restrict__ named,
-                                                   float *__restrict__ coef, uint32_t *__restrict__ largest)
+__global__ __launch_bounds__(256) void rows_kernel(Args a, const uint32_t *__restrict__ bits, int64_t padded, Prm *__restrict__ prm, float *__restrict__ weight, int32_t *__restrict__ named,
+                                                   float *__restrict__ coef, uint32_t *__restrict__ scalars, const float *__restrict__ item_factor, int64_t item_tiles)
 {
-    const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
-    if (r >= padded) return;
-    const int32_t u = r < a.rows ? a.user_ids[r] : -1;
-    const bool ok = row_ok(u, a.users);
-    if (indptr != nullptr && r < a.rows) {
-        uint32_t *row = bits + r * mask_words(a.cat);
-        if (ok) set_seen_bits(u, indptr, indices, a.cat, row);
-        else for (int64_t k = lane; k < mask_words(a.cat); k += 64) row[k] = 0xFFFFFFFFu;      // nobody's row: nothing of it counts, whatever the products are
+    __shared__ float s_max[4];
+    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+    if (F32 && blockIdx.x == 0) {
+        float m = 0.0f;
+        for (int64_t t = threadIdx.x; t < item_tiles; t += 256) m = fmaxf(m, item_factor[t]);
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+        if (lane == 0) s_max[wid] = m;
+        __syncthreads();
+        if (threadIdx.x == 0) scalars[kTopFactor] = __float_as_uint(fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3])));
+        __syncthreads();
     }
-    auto listed = [&](int32_t i) {           // is item i among the row's seen items?  (the bits are still being set: the list itself)
-        bool hit = false;
-        for (int64_t p = indptr[u] + lane; p < indptr[u + 1]; p += 64) hit |= indices[p] == i;
-        return __builtin_amdgcn_ballot_w64(hit) != 0ull;
-    };
-    // the row's weight: one order of summation, every lane the same
-    double sum = 0.0, mag = 0.0;
-    for (int t = 0; t < a.T && r < a.rows; ++t) {
-        const int32_t i = a.items[r * a.T + t];
-        const bool in = ok && i >= 0 && i < a.cat && !(indptr != nullptr && listed(i));
-        const float g = in ? a.g[r * a.T + t] : 0.0f;
-        sum += g;
-        mag += fabs((double)g);
-        if (lane == 0) { named[r * a.T + t] = in ? i : -1; coef[r * a.T + t] = g; }
-    }
-    const float h = ok && a.h != nullptr ? a.h[r] : 0.0f;
-    const float lse = ok ? a.lse[r] : -INFINITY;
-    const bool live = ok && lse != -INFINITY;
-    const float w = F32 ? (float)(mag + fabs((double)h)) : 1.0f;
-    const float inv = w > 0.0f ? 1.0f / w : w == w ? 0.0f : w;              // (NaN weights stay NaN)
-    float big = 0.0f, factor = live ? F32 ? 1.0f : a.scale * kLog2e : 0.0f;
-    if (ok && lane < D / 8) {
+    float most = 0.0f;
+    for (int64_t r = (int64_t)blockIdx.x * 4 + wid; r < padded; r += (int64_t)gridDim.x * 4) {
+        const int32_t u = r < a.rows ? a.user_ids[r] : -1;
+        const bool ok = row_ok(u, a.users);
+        auto listed = [&](int32_t i) { return (bits[r * mask_words(a.cat) + (i >> 5)] >> (i & 31)) & 1u; };        // is item i among the row's seen items?
+        Prm &out = prm[r / kTile];
+        const int c = (int)(r % kTile);
+        // the row's weight: one order of summation, every lane the same
+        double sum = 0.0, mag = 0.0;
+        for (int t = 0; t < a.T; ++t) {
+            const int32_t i = r < a.rows ? a.items[r * a.T + t] : -1;
+            const bool in = ok && i >= 0 && i < a.cat && !(bits != nullptr && listed(i));
+            const float g = in ? a.g[r * a.T + t] : 0.0f;
+            sum += g;
+            mag += fabs((double)g);
+            if (lane == 0) {
+                if (r < a.rows) named[r * a.T + t] = in ? i : -1;
+                if (t < kHeld) out.v[4 + t][c] = __int_as_float(in ? i : -1);
+            }
+        }
+        const float h = ok && a.h != nullptr ? a.h[r] : 0.0f;
+        const float lse = ok ? a.lse[r] : -INFINITY;
+        const bool live = ok && lse != -INFINITY;
+        const float w = F32 ? (float)(mag + fabs((double)h)) : 1.0f;
+        const float inv = w > 0.0f ? 1.0f / w : w == w ? 0.0f : w;              // (NaN weights stay NaN)
+        float big = 0.0f, factor = live ? F32 ? 1.0f : a.scale * kLog2e : 0.0f;
         if constexpr (F32) {
-            const float4 *p = reinterpret_cast<const float4 *>((const float *)a.P + (int64_t)u * D + 8 * lane);
-            const float4 x = p[0], y = p[1];
-            big = fmaxf(fmaxf(fmaxf(finite_abs(x.x), finite_abs(x.y)), fmaxf(finite_abs(x.z), finite_abs(x.w))),
-                        fmaxf(fmaxf(finite_abs(y.x), finite_abs(y.y)), fmaxf(finite_abs(y.z), finite_abs(y.w))));
+            if (ok && lane < D / 8) {
+                const float4 *p = reinterpret_cast<const float4 *>((const float *)a.P + (int64_t)u * D + 8 * lane);
+                const float4 x = p[0], y = p[1];
+                big = fmaxf(fmaxf(fmaxf(finite_abs(x.x), finite_abs(x.y)), fmaxf(finite_abs(x.z), finite_abs(x.w))),
+                            fmaxf(fmaxf(finite_abs(y.x), finite_abs(y.y)), fmaxf(finite_abs(y.z), finite_abs(y.w))));
+            }
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor(big, o, 64));
+            float up, down;
+            scale_for(big * (a.scale * kLog2e), &up, &down);
+            factor *= down;
+            most = fmaxf(most, finite_abs(big * w));
+            for (int t = lane; t < a.T && r < a.rows; t += 64) {
+                const int32_t i = a.items[r * a.T + t];
+                coef[r * a.T + t] = ok && i >= 0 && i < a.cat ? a.g[r * a.T + t] * inv : 0.0f;        // (a masked item is not looked up)
+            }
+        } else {
+            for (int t = lane; t < a.T && r < a.rows; t += 64) coef[r * a.T + t] = a.g[r * a.T + t];
+        }
+        // lse in log2 is rounded to fp32 (half a step at 24 is 1e-6 of every p): what that changes goes into the coefficients
+        const double lse2 = (double)lse * 1.4426950408889634074;
+        const float l2 = (float)lse2;
+        const double fix = exp2((double)l2 - lse2) * inv;
+        if (lane == 0) {
+            out.v[0][c] = factor;
+            out.v[1][c] = live ? l2 : kFar;
+            out.v[2][c] = live ? (float)(-(sum + (double)h * (a.ent != nullptr ? a.ent[r] : 0.0f)) * fix) : 0.0f;
+            out.v[3][c] = live ? (float)(-(double)h * kLn2 * fix) : 0.0f;
+            for (int k = a.T; k < kHeld; ++k) out.v[4 + k][c] = __int_as_float(-1);
+            weight[r] = live ? w : 0.0f;
         }
     }
     if constexpr (F32) {
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor(big, o, 64));
-        float up, down;
-        scale_for(big * (a.scale * kLog2e), &up, &down);
-        factor *= down;
-        if (lane == 0) atomicMax(largest, __float_as_uint(finite_abs(big * w)));
+        if (lane == 0) s_max[wid] = most;
+        __syncthreads();
+        if (threadIdx.x == 0) atomicMax(scalars, __float_as_uint(fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]))));
     }
-    // lse in log2 is rounded to fp32 (half a step at 24 is 1e-6 of every p): what that changes goes into the coefficients
-    const double lse2 = (double)lse * 1.4426950408889634074;
-    const float l2 = (float)lse2;
-    const double fix = exp2((double)l2 - lse2) * inv;
-    if (lane == 0) {
-        Prm &t = prm[r / kTile];
-        const int c = (int)(r % kTile);
-        t.v[0][c] = factor;
-        t.v[1][c] = live ? l2 : kFar;
-        t.v[2][c] = live ? (float)(-(sum + (double)h * (a.ent != nullptr ? a.ent[r] : 0.0f)) * fix) : 0.0f;
-        t.v[3][c] = live ? (float)(-(double)h * kLn2 * fix) : 0.0f;
-#pragma unroll
-        for (int k = 4; k < 8; ++k) t.v[k][c] = 0.0f;
-        weight[r] = live ? w : 0.0f;
-    }
-    if constexpr (F32)
-        for (int t = 0; t < a.T && r < a.rows; ++t)
-            if (lane == 0) coef[r * a.T + t] *= inv;
 }
 
 // element order of a transposed tile: [plane][block of 32 columns][half of the rows][lane][8]: lane l, element j is column 32 kb + (l & 31) of
@@ -126,7 +140,7 @@ __device__ __forceinline__ int tile_row(int half, int hi, int j) { const int i =
 // power of two in the row-major planes, times its weight and one common scale in the transposed ones.  Items: the tile's scale in both.
 template <int D, bool F32, bool USERS>
 __global__ __launch_bounds__(256) void tiles_kernel(Args a, const float *__restrict__ weight, const uint32_t *__restrict__ largest, uint4 *__restrict__ rowm,
-                                                    uint4 *__restrict__ tr, float *__restrict__ factor, uint32_t *__restrict__ top_factor)
+                                                    uint4 *__restrict__ tr, float *__restrict__ factor)
 {
     constexpr int TPR = D / 8, LD = D + 1;
     using S = typename std::conditional<F32, float, uint16_t>::type;
@@ -185,7 +199,7 @@ __global__ __launch_bounds__(256) void tiles_kernel(Args a, const float *__restr
     if constexpr (F32 && !USERS) {
         float up, down;
         scale_for(fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3])), &up, &down);
-        if (tid == 0) { factor[tile] = down; atomicMax(top_factor, __float_as_uint(down)); }
+        if (tid == 0) factor[tile] = down;
         if (tid < kTile) s_mul[tid] = up;
         for (int t = tid; t < kTile * TPR; t += 256) {
             const int r = t / TPR, c = 8 * (t % TPR);
@@ -243,18 +257,25 @@ struct Pass {
     int64_t positions;                    // rows of named / coef / bits
     int64_t cat;
     int T;
-    int splits;
-    float *part;                          // [splits][padded rows that stay][d]
+    float *part;                          // [segments][padded rows that stay][d]
     int64_t part_rows;
 };
+
+// The work of a pass is a line of (block of 128 columns, streaming tile) cut into equal pieces, one per workgroup of a full device: no ragged last
+// round (782 item blocks on 512 slots were two rounds for 1.53).  A block's pieces are its segments, numbered from the first.
+__host__ __device__ __forceinline__ int64_t piece_begin(int64_t total, int pieces, int64_t w) { return total * w / pieces; }
+// the piece that holds position x of the line: the largest w with piece_begin(w) <= x
+__host__ __device__ __forceinline__ int64_t piece_of(int64_t total, int pieces, int64_t x) { return ((x + 1) * pieces - 1) / total; }
 
 template <int D, bool F32>
 struct GradGeo : Geo<D, F32> {
     using G = Geo<D, F32>;
     static constexpr int KB = D / 32;
     static constexpr int ST = 16384 / G::TILEB >= 4 ? 4 : 16384 / G::TILEB >= 1 ? 16384 / G::TILEB : 1;       // tiles of one LDS buffer
-    static constexpr int STAGE = ST * (2 * G::TILEB + 1024);
-    static constexpr int WGS = 2 * STAGE > 81920 ? 1 : 2;                                                      // workgroups a CU holds
+    // a buffer: row-major tiles, transposed tiles, parameter blocks, and 1 KB of seen bits a tile
+    static constexpr int PRM = 2 * ST * G::TILEB, BITS = PRM + ST * 1024, STAGE = BITS + ST * 1024;
+    // workgroups a CU holds: the sums of 256 columns alone are half of a lane's registers at two
+    static constexpr int WGS = D == 256 ? 1 : 2;
 };
 
 template <int D, bool F32, bool ITEMS_STAY, bool MASK, bool ENT>
@@ -263,33 +284,14 @@ __device__ __forceinline__ void grad_body(const Pass &a, char (*lds)[GradGeo<D, 
     using G = GradGeo<D, F32>;
     constexpr int KS = G::KS, NP = G::NP, ST = G::ST, KB = G::KB;
     const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, hi = lane >> 5, l31 = lane & 31;
-    const int64_t t0 = a.flow_tiles * blockIdx.x / a.splits, t1 = a.flow_tiles * (blockIdx.x + 1) / a.splits;
-    const int64_t col = (int64_t)blockIdx.y * 128 + wid * 32 + l31;            // this lane's column
-    const int64_t colc = col < a.stay_rows ? col : a.stay_rows - 1;
-
-    Frag b[KS][NP];
-#pragma unroll
-    for (int s = 0; s < KS; ++s)
-#pragma unroll
-        for (int p = 0; p < NP; ++p) b[s][p].u = *reinterpret_cast<const uint4 *>(a.stay + (size_t)colc * G::ROWB + 16 * (p * (D / 8) + 2 * s + hi));
-    f32x16 out[KB];
-#pragma unroll
-    for (int k = 0; k < KB; ++k)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) out[k][i] = 0.0f;
-    float sf = 0.0f, slse = 0.0f, sA = 0.0f, sB = 0.0f, my_factor = 1.0f;      // users stay: this lane's row; items stay: its tile's factor
+    const int64_t total = a.part_rows / 128 * a.flow_tiles;
+    int64_t at = piece_begin(total, gridDim.x, blockIdx.x);
+    const int64_t end = piece_begin(total, gridDim.x, blockIdx.x + 1);
     const float top = F32 ? __uint_as_float(*a.top_factor) : 1.0f;
-    if constexpr (!ITEMS_STAY) {
-        const Prm &p = a.prm[colc / kTile];
-        const int c = (int)(colc % kTile);
-        sf = p.v[0][c]; slse = p.v[1][c]; sA = p.v[2][c]; sB = p.v[3][c];
-    } else if constexpr (F32) {
-        my_factor = a.tile_factor[colc / kTile];
-    }
     const int64_t words = mask_words(a.cat);
-    const int32_t my_block = (int32_t)(((int64_t)blockIdx.y * 128 + wid * 32) / kTile);       // items stay: the block of 32 this wavefront holds
+    const int sw = G::swz(l31) * 16;
 
-    auto stage = [&](int64_t tile, int buf) {
+    auto stage = [&](int64_t tile, int buf, int64_t block, int64_t colc) {
 #pragma unroll
         for (int n = 0; n < (ST * (2 * G::TILEB / 1024 + 1) + 3) / 4; ++n) {
             const int k = n * 4 + wid;                                           // 1 KB piece of the stage: ST row-major tiles, ST transposed, ST parameter blocks
@@ -313,24 +315,60 @@ __device__ __forceinline__ void grad_body(const Pass &a, char (*lds)[GradGeo<D, 
                 copy_to_lds((const char *)(a.prm + t) + lane * 16, dst);
             }
         }
+        if constexpr (MASK) {
+            if constexpr (ITEMS_STAY) {              // four words of each of the tile's 32 positions: the workgroup's blocks (both halves of a wavefront the same)
+                if (wid < ST) {
+                    int64_t r = (tile + wid) * kTile + l31;
+                    r = r < a.positions ? r : a.positions - 1;
+                    if (hi == 0) copy_to_lds((const char *)(a.bits + (size_t)r * words + 4 * block), lds[buf] + G::BITS + wid * 1024);
+                }
+            } else {                                  // this wavefront's columns, a word a tile
+#pragma unroll
+                for (int j = 0; j < ST; ++j) {
+                    const int64_t t = tile + j < words ? tile + j : words - 1;
+                    copy4_to_lds((const char *)(a.bits + (size_t)(colc < a.positions ? colc : a.positions - 1) * words + t), lds[buf] + G::BITS + j * 1024 + wid * 256);
+                }
+            }
+        }
     };
-    const int sw = G::swz(l31) * 16;
-    if (t0 < t1) stage(t0, 0);
     int buf = 0;
+    while (at < end) {
+    const int64_t block = at / a.flow_tiles, t0 = at - block * a.flow_tiles;                        // this segment: tiles [t0, t1) of a block
+    const int64_t t1 = end - at < a.flow_tiles - t0 ? t0 + (end - at) : a.flow_tiles;
+    const int64_t segment = blockIdx.x - piece_of(total, gridDim.x, block * a.flow_tiles);
+    const int64_t col = block * 128 + wid * 32 + l31;                                                // this lane's column
+    const int64_t colc = col < a.stay_rows ? col : a.stay_rows - 1;
+    const int32_t my_block = (int32_t)(block * 4 + wid);                                             // items stay: the block of 32 this wavefront holds
+    __syncthreads();                      // (the last segment's tiles are read)
+    stage(t0, buf, block, colc);
+    Frag b[KS][NP];
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int p = 0; p < NP; ++p) b[s][p].u = *reinterpret_cast<const uint4 *>(a.stay + (size_t)colc * G::ROWB + 16 * (p * (D / 8) + 2 * s + hi));
+    f32x16 out[KB];
+#pragma unroll
+    for (int k = 0; k < KB; ++k)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) out[k][i] = 0.0f;
+    float sf = 0.0f, slse = 0.0f, sA = 0.0f, sB = 0.0f, my_factor = 1.0f;                          // users stay: this lane's row; items stay: its tile's factor
+    if constexpr (!ITEMS_STAY) {
+        const Prm &p = a.prm[colc / kTile];
+        const int c = (int)(colc % kTile);
+        sf = p.v[0][c]; slse = p.v[1][c]; sA = p.v[2][c]; sB = p.v[3][c];
+    } else if constexpr (F32) {
+        my_factor = a.tile_factor[colc / kTile];
+    }
     for (int64_t s0 = t0; s0 < t1; s0 += ST) {
         __syncthreads();
-        if (s0 + ST < t1) stage(s0 + ST, buf ^ 1);
+        if (s0 + ST < t1) stage(s0 + ST, buf ^ 1, block, colc);
         for (int j = 0; j < ST && s0 + j < t1; ++j) {
             const int64_t tile = s0 + j;
-            // what the tile's epilogue needs from memory, asked for early
+            // (nothing in this loop loads into registers from memory: loads return in order, and one would wait for the next stage's copies)
             uint32_t seen = 0u;
             if constexpr (MASK) {
-                if constexpr (ITEMS_STAY) {
-                    const int64_t r = tile * kTile + l31;
-                    seen = r < a.positions && my_block < words ? a.bits[(size_t)r * words + my_block] : 0xFFFFFFFFu;
-                } else {
-                    seen = a.bits[(size_t)(colc < a.positions ? colc : a.positions - 1) * words + tile];
-                }
+                const char *sb = lds[buf] + G::BITS + j * 1024;
+                seen = ITEMS_STAY ? *reinterpret_cast<const uint32_t *>(sb + l31 * 16 + wid * 4) : *reinterpret_cast<const uint32_t *>(sb + wid * 256 + lane * 4);
             }
             const float tf = !ITEMS_STAY && F32 ? a.tile_factor[tile] : my_factor;
             const char *rm = lds[buf] + j * G::TILEB + l31 * G::ROWB;
@@ -369,7 +407,8 @@ __device__ __forceinline__ void grad_body(const Pass &a, char (*lds)[GradGeo<D, 
                     v[i] = ENT ? p * fmaf(sB, t, sA) : p * sA;
                 }
             } else {
-                const Prm *prm = reinterpret_cast<const Prm *>(lds[buf] + 2 * ST * G::TILEB + j * 1024);
+                const Prm *prm = reinterpret_cast<const Prm *>(lds[buf] + G::PRM + j * 1024);
+                if (MASK && tile * kTile + l31 >= a.positions) seen = 0xFFFFFFFFu;            // nobody's rows behind the last
                 const bool any = MASK && __builtin_amdgcn_ballot_w64(seen != 0u) != 0ull;
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
@@ -394,8 +433,8 @@ __device__ __forceinline__ void grad_body(const Pass &a, char (*lds)[GradGeo<D, 
                 // named items of the tile's positions that are in this wavefront's block.
                 for (int t = 0; t < a.T; ++t) {
                     const int64_t r = tile * kTile + l31;
-                    const int32_t it = r < a.positions ? a.named[r * a.T + t] : -1;
-                    const bool mine = hi == 0 && it >= 0 && it / kTile == my_block;
+                    const int32_t it = t < kHeld ? __float_as_int(prm->v[4 + t][l31]) : r < a.positions ? a.named[r * a.T + t] : -1;
+                    const bool mine = hi == 0 && (it >> 5) == my_block;          // (-1 >> 5 is nobody's block)
                     unsigned long long hits = __builtin_amdgcn_ballot_w64(mine);
                     if (hits == 0ull) continue;
                     const float c = mine ? a.coef[r * a.T + t] * (F32 ? kLift : 1.0f) : 0.0f;
@@ -436,12 +475,14 @@ __device__ __forceinline__ void grad_body(const Pass &a, char (*lds)[GradGeo<D, 
         }
         buf ^= 1;
     }
-    float *dst = a.part + ((size_t)blockIdx.x * a.part_rows + col) * D + 4 * hi;
+    float *dst = a.part + ((size_t)segment * a.part_rows + col) * D + 4 * hi;
 #pragma unroll
     for (int k = 0; k < KB; ++k)
 #pragma unroll
         for (int q = 0; q < 4; ++q)
             *reinterpret_cast<float4 *>(dst + 32 * k + 8 * q) = make_float4(out[k][4 * q], out[k][4 * q + 1], out[k][4 * q + 2], out[k][4 * q + 3]);
+    at += t1 - t0;
+    }
 }
 
 template <int D, bool F32, bool ITEMS_STAY, bool MASK, bool ENT>
@@ -451,17 +492,26 @@ __global__ __launch_bounds__(256, (GradGeo<D, F32>::WGS)) void grad_kernel(Pass 
     grad_body<D, F32, ITEMS_STAY, MASK, ENT>(a, lds);
 }
 
+// segments of a block of 128 columns
+__device__ __forceinline__ int segments_of(int64_t block, int64_t flow_tiles, int pieces, int64_t part_rows)
+{
+    const int64_t total = part_rows / 128 * flow_tiles;
+    return (int)(piece_of(total, pieces, (block + 1) * flow_tiles - 1) - piece_of(total, pieces, block * flow_tiles)) + 1;
+}
+
 // ---- the partial sums -> the gradients ------------------------------------------------------------------------------------------------------
 // GP: four elements a thread; the partials in order, the row's weight, the named rows of Q
 template <int D, bool F32>
-__global__ __launch_bounds__(256) void join_rows_kernel(Args a, const float *__restrict__ part, int splits, int64_t part_rows, const float *__restrict__ weight,
+__global__ __launch_bounds__(256) void join_rows_kernel(Args a, const float *__restrict__ part, int64_t flow_tiles, int pieces, int64_t part_rows, const float *__restrict__ weight,
                                                         const uint32_t *__restrict__ top_factor, const int32_t *__restrict__ named, void *__restrict__ GP)
 {
     const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x, r = t / (D / 4);
     const int c = 4 * (int)(t % (D / 4));
     if (r >= a.rows) return;
     float s[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int k = 0; k < splits && weight[r] != 0.0f; ++k) {          // (no weight, no gradient, whatever the products were)
+    const int segments = weight[r] != 0.0f ? segments_of(r / 128, flow_tiles, pieces, part_rows) : 0;         // (no weight, no gradient, whatever the products were)
+#pragma unroll 8
+    for (int k = 0; k < segments; ++k) {
         const float4 p = *reinterpret_cast<const float4 *>(part + ((size_t)k * part_rows + r) * D + c);
         s[0] += p.x; s[1] += p.y; s[2] += p.z; s[3] += p.w;
     }
@@ -484,18 +534,29 @@ __global__ __launch_bounds__(256) void join_rows_kernel(Args a, const float *__r
     else *reinterpret_cast<ushort4 *>((uint16_t *)GP + r * D + c) = make_ushort4(f32_bf16(s[0] * a.scale), f32_bf16(s[1] * a.scale), f32_bf16(s[2] * a.scale), f32_bf16(s[3] * a.scale));
 }
 
+// GQ: the passes' sums in order, each with its own scale of the positions' rows
+struct Passes {
+    int64_t flow_tiles, last_tiles;       // streaming tiles of a pass, of the last one
+    int passes, pieces, last_pieces;
+    int64_t stride;                       // elements of a pass' partial sums
+};
 template <int D, bool F32>
-__global__ __launch_bounds__(256) void join_items_kernel(int64_t cat, const float *__restrict__ part, int splits, int64_t part_rows, const float *__restrict__ factor,
-                                                         int factor_every, float scale, void *__restrict__ GQ)
+__global__ __launch_bounds__(256) void join_items_kernel(int64_t cat, const float *__restrict__ part, Passes ps, int64_t part_rows, const float *__restrict__ factor,
+                                                         float scale, void *__restrict__ GQ)
 {
     const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x, r = t / (D / 4);
     const int c = 4 * (int)(t % (D / 4));
     if (r >= cat) return;
     float s[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int k = 0; k < splits; ++k) {
-        const float4 p = *reinterpret_cast<const float4 *>(part + ((size_t)k * part_rows + r) * D + c);
-        const float f = F32 ? factor[k / factor_every] * (scale / kLift) : scale;        // (a pass has its own scale of the positions' rows)
-        s[0] = fmaf(p.x, f, s[0]); s[1] = fmaf(p.y, f, s[1]); s[2] = fmaf(p.z, f, s[2]); s[3] = fmaf(p.w, f, s[3]);
+    for (int pass = 0; pass < ps.passes; ++pass) {
+        const bool last = pass + 1 == ps.passes;
+        const int segments = segments_of(r / 128, last ? ps.last_tiles : ps.flow_tiles, last ? ps.last_pieces : ps.pieces, part_rows);
+        const float f = F32 ? factor[pass] * (scale / kLift) : scale;
+#pragma unroll 4
+        for (int k = 0; k < segments; ++k) {
+            const float4 p = *reinterpret_cast<const float4 *>(part + (size_t)pass * ps.stride + ((size_t)k * part_rows + r) * D + c);
+            s[0] = fmaf(p.x, f, s[0]); s[1] = fmaf(p.y, f, s[1]); s[2] = fmaf(p.z, f, s[2]); s[3] = fmaf(p.w, f, s[3]);
+        }
     }
     if constexpr (F32) *reinterpret_cast<float4 *>((float *)GQ + r * D + c) = make_float4(s[0], s[1], s[2], s[3]);
     else *reinterpret_cast<ushort4 *>((uint16_t *)GQ + r * D + c) = make_ushort4(f32_bf16(s[0]), f32_bf16(s[1]), f32_bf16(s[2]), f32_bf16(s[3]));
@@ -536,8 +597,6 @@ __global__ __launch_bounds__(256) void add_rows_kernel(float *__restrict__ T, in
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------------------------
-constexpr int kTopFactor = 16;
-
 struct Ws {
     char *user_rm, *user_t, *item_rm, *item_t;
     float *tile_factor, *user_factor, *weight, *coef, *part_p, *part_q;
@@ -545,15 +604,23 @@ struct Ws {
     Prm *prm;
     int32_t *named;
     uint32_t *bits;
-    int64_t pass, passes, splits_p, splits_q, pad_p, pad_q, bytes;
+    int64_t pass, passes, seg_q, pad_p, pad_q, bytes;
+    int wgs, st;
 };
 
 int64_t pad128(int64_t n) { return (n + 127) / 128 * 128; }
 
-int64_t grad_splits(int64_t stay, int64_t flow_tiles, int wgs, int st)
+// pieces of a pass: a full device's workgroups, but pieces of at least `st` tiles; and the segments a block may have then
+int grad_pieces(int64_t stay, int64_t flow_tiles, int wgs, int st)
 {
-    const int64_t slots = (int64_t)wgs * rsx_num_cus(), s = slots / (pad128(stay) / 128), most = (flow_tiles + st - 1) / st;
-    return s < 1 ? 1 : s > most ? most : s;
+    const int64_t slots = (int64_t)wgs * rsx_num_cus(), most = (pad128(stay) / 128 * flow_tiles + st - 1) / st;
+    return (int)(most < slots ? most : slots);
+}
+int64_t grad_segments(int64_t stay, int64_t flow_tiles, int pieces)
+{
+    const int64_t per = pad128(stay) / 128 * flow_tiles / pieces;            // tiles of a piece, at least
+    const int64_t s = (flow_tiles + per - 1) / per + 1;
+    return s < pieces ? s : pieces;
 }
 
 // geometry the host needs of GradGeo
@@ -561,7 +628,7 @@ void grad_geo(int d, bool f32, int *wgs, int *st)
 {
     const int tileb = kTile * d * (f32 ? 4 : 2), s = 16384 / tileb;
     *st = s >= 4 ? 4 : s >= 1 ? s : 1;
-    *wgs = 2 * *st * (2 * tileb + 1024) > 81920 ? 1 : 2;
+    *wgs = d == 256 ? 1 : 2;
 }
 
 Ws carve(void *ws, int64_t rows, int64_t cat, int d, int dtype, bool mask, int T)
@@ -572,8 +639,7 @@ Ws carve(void *ws, int64_t rows, int64_t cat, int d, int dtype, bool mask, int T
     auto take = [&](int64_t n) { char *q = base + off; off += a256(n); return q; };
     const bool f32 = dtype == RSX_F32;
     const int rowb = d * (f32 ? 4 : 2);
-    int wgs, st;
-    grad_geo(d, f32, &wgs, &st);
+    grad_geo(d, f32, &w.wgs, &w.st);
     // a pass' bits are held to 1 GB (without a mask: one pass)
     int64_t most = (1ll << 30) / (mask_words(cat) * 4) / 128 * 128;
     most = most < 128 ? 128 : most;
@@ -582,8 +648,13 @@ Ws carve(void *ws, int64_t rows, int64_t cat, int d, int dtype, bool mask, int T
     w.pad_p = pad128(w.pass);
     w.pad_q = pad128(cat);
     const int64_t item_tiles = w.pad_q / kTile, user_tiles = w.pad_p / kTile;
-    w.splits_p = grad_splits(w.pass, item_tiles, wgs, st);
-    w.splits_q = grad_splits(cat, user_tiles, wgs, st);
+    const int64_t flow = (cat + kTile - 1) / kTile;
+    // (the last, shorter pass: fewer tiles in no fewer pieces, so a block has no more segments of items; of users it may have more, over fewer blocks)
+    const int64_t tail = rows - (w.passes - 1) * w.pass;
+    auto cells_p = [&](int64_t n) { return grad_segments(n, flow, grad_pieces(n, flow, w.wgs, w.st)) * pad128(n); };
+    auto seg_q = [&](int64_t n) { return grad_segments(cat, pad128(n) / kTile, grad_pieces(cat, pad128(n) / kTile, w.wgs, w.st)); };
+    const int64_t cells = cells_p(w.pass) > cells_p(tail) ? cells_p(w.pass) : cells_p(tail);
+    w.seg_q = seg_q(w.pass) > seg_q(tail) ? seg_q(w.pass) : seg_q(tail);
     w.user_rm = take(w.pad_p * rowb);
     w.user_t = take(w.pad_p * rowb);
     w.item_rm = take(f32 ? w.pad_q * rowb : 0);
@@ -596,16 +667,16 @@ Ws carve(void *ws, int64_t rows, int64_t cat, int d, int dtype, bool mask, int T
     w.prm = (Prm *)take(user_tiles * (int64_t)sizeof(Prm));
     w.scalars = (uint32_t *)take(256);
     w.bits = (uint32_t *)take(mask ? w.pass * mask_words(cat) * 4 : 0);
-    w.part_p = (float *)take(w.splits_p * w.pad_p * d * 4);
-    w.part_q = (float *)take(w.passes * w.splits_q * w.pad_q * d * 4);
+    w.part_p = (float *)take(cells * d * 4);
+    w.part_q = (float *)take(w.passes * w.seg_q * w.pad_q * d * 4);
     w.bytes = off;
     return w;
 }
 
 template <int D, bool F32, bool ITEMS_STAY>
-void launch_pass(const Pass &p, bool mask, bool ent, hipStream_t st)
+void launch_pass(const Pass &p, int pieces, bool mask, bool ent, hipStream_t st)
 {
-    const dim3 grid((unsigned)p.splits, (unsigned)(p.part_rows / 128));
+    const dim3 grid((unsigned)pieces);
 #define RSX_GRAD(M_, E_) hipLaunchKernelGGL((grad_kernel<D, F32, ITEMS_STAY, M_, E_>), grid, dim3(256), 0, st, p)
     if (mask) { if (ent) RSX_GRAD(true, true); else RSX_GRAD(true, false); }
     else { if (ent) RSX_GRAD(false, true); else RSX_GRAD(false, false); }
@@ -617,9 +688,10 @@ void run(const Args &all, const int64_t *indptr, const int32_t *indices, const W
 {
     const int64_t item_tiles = w.pad_q / kTile;
     const int es = F32 ? 4 : 2;
+    Passes ps{0, 0, (int)w.passes, 0, 0, w.seg_q * w.pad_q * D};
     hipLaunchKernelGGL(fill_u32_kernel, dim3(1), dim3(256), 0, st, (uint4 *)w.scalars, 16, 0u);
     hipLaunchKernelGGL((tiles_kernel<D, F32, false>), dim3((unsigned)item_tiles), dim3(256), 0, st, all, (const float *)nullptr, (const uint32_t *)nullptr,
-                       (uint4 *)w.item_rm, (uint4 *)w.item_t, w.tile_factor, w.scalars + kTopFactor);
+                       (uint4 *)w.item_rm, (uint4 *)w.item_t, w.tile_factor);
     for (int64_t k = 0; k < w.passes; ++k) {
         Args a = all;
         const int64_t r0 = k * w.pass;
@@ -629,26 +701,31 @@ void run(const Args &all, const int64_t *indptr, const int32_t *indices, const W
         if (a.h) a.h += r0;
         const int64_t pad = pad128(a.rows), user_tiles = pad / kTile;
         if (k > 0) hipLaunchKernelGGL(fill_u32_kernel, dim3(1), dim3(256), 0, st, (uint4 *)w.scalars, 1, 0u);
-        if (indptr) launch_clear_bits(a.rows, a.cat, w.bits, st);
-        hipLaunchKernelGGL((rows_kernel<D, F32>), dim3((unsigned)(pad / 4)), dim3(256), 0, st, a, indptr, indices, w.bits, pad, w.prm, w.weight, w.named, w.coef, w.scalars);
+        if (indptr) hipLaunchKernelGGL(seen_bits_kernel, dim3((unsigned)a.rows), dim3(256), 0, st, a.user_ids, a.users, indptr, indices, a.cat, w.bits);
+        const int64_t row_wgs = pad / 4 < 2 * (int64_t)rsx_num_cus() ? pad / 4 : 2 * (int64_t)rsx_num_cus();
+        hipLaunchKernelGGL((rows_kernel<D, F32>), dim3((unsigned)row_wgs), dim3(256), 0, st, a, indptr ? w.bits : (const uint32_t *)nullptr, pad, w.prm, w.weight, w.named, w.coef, w.scalars,
+                           w.tile_factor, item_tiles);
         hipLaunchKernelGGL((tiles_kernel<D, F32, true>), dim3((unsigned)user_tiles), dim3(256), 0, st, a, w.weight, w.scalars, (uint4 *)w.user_rm, (uint4 *)w.user_t,
-                           w.user_factor + k, (uint32_t *)nullptr);
+                           w.user_factor + k);
         Pass p;
         p.tile_factor = w.tile_factor; p.top_factor = w.scalars + kTopFactor; p.prm = w.prm; p.bits = w.bits; p.named = w.named; p.coef = w.coef;
         p.positions = a.rows; p.cat = a.cat; p.T = a.T;
         p.stay = w.user_rm; p.flow = F32 ? w.item_rm : (const char *)a.Q; p.flow_t = w.item_t;
         p.stay_rows = pad; p.flow_tiles = (a.cat + kTile - 1) / kTile; p.flow_valid = a.cat;
-        p.splits = (int)w.splits_p; p.part = w.part_p; p.part_rows = pad;
-        launch_pass<D, F32, false>(p, indptr != nullptr, a.h != nullptr, st);
-        hipLaunchKernelGGL((join_rows_kernel<D, F32>), dim3((unsigned)((a.rows * (D / 4) + 255) / 256)), dim3(256), 0, st, a, w.part_p, p.splits, pad, w.weight, w.scalars + kTopFactor,
-                           w.named, (char *)GP + r0 * D * es);
+        p.part = w.part_p; p.part_rows = pad;
+        const int pieces_p = grad_pieces(a.rows, p.flow_tiles, w.wgs, w.st);
+        launch_pass<D, F32, false>(p, pieces_p, indptr != nullptr, a.h != nullptr, st);
+        hipLaunchKernelGGL((join_rows_kernel<D, F32>), dim3((unsigned)((a.rows * (D / 4) + 255) / 256)), dim3(256), 0, st, a, w.part_p, p.flow_tiles, pieces_p, pad, w.weight,
+                           w.scalars + kTopFactor, w.named, (char *)GP + r0 * D * es);
         p.stay = F32 ? w.item_rm : (const char *)a.Q; p.flow = w.user_rm; p.flow_t = w.user_t;
         p.stay_rows = F32 ? w.pad_q : a.cat; p.flow_tiles = user_tiles; p.flow_valid = a.rows;
-        p.splits = (int)w.splits_q; p.part = w.part_q + (size_t)k * w.splits_q * w.pad_q * D; p.part_rows = w.pad_q;
-        launch_pass<D, F32, true>(p, indptr != nullptr, a.h != nullptr, st);
+        p.part = w.part_q + (size_t)k * w.seg_q * w.pad_q * D; p.part_rows = w.pad_q;
+        const int pieces_q = grad_pieces(a.cat, user_tiles, w.wgs, w.st);
+        launch_pass<D, F32, true>(p, pieces_q, indptr != nullptr, a.h != nullptr, st);
+        if (k == 0) { ps.flow_tiles = user_tiles; ps.pieces = pieces_q; }
+        ps.last_tiles = user_tiles; ps.last_pieces = pieces_q;
     }
-    hipLaunchKernelGGL((join_items_kernel<D, F32>), dim3((unsigned)((all.cat * (D / 4) + 255) / 256)), dim3(256), 0, st, all.cat, w.part_q, (int)(w.passes * w.splits_q), w.pad_q,
-                       w.user_factor, (int)w.splits_q, all.scale, GQ);
+    hipLaunchKernelGGL((join_items_kernel<D, F32>), dim3((unsigned)((all.cat * (D / 4) + 255) / 256)), dim3(256), 0, st, all.cat, w.part_q, ps, w.pad_q, w.user_factor, all.scale, GQ);
 }
 
 }  // namespace
