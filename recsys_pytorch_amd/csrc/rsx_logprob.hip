@@ -546,13 +546,13 @@ __device__ __forceinline__ float group_sum(float v)
 
 // NT threads a row: 1024 where rows are few and one row's chain of loads is the time, 256 where many rows share a CU
 template <int D, bool F32, int NT>
-__global__ __launch_bounds__(NT) void finish_kernel(const void *__restrict__ P, const void *__restrict__ Q, Shape sh, const uint32_t *__restrict__ bits,
+__global__ __launch_bounds__(NT, (NT == 1024 ? 4 : 5)) void finish_kernel(const void *__restrict__ P, const void *__restrict__ Q, Shape sh, const uint32_t *__restrict__ bits,
                                                     const float4 *__restrict__ part, int splits, const uint16_t *__restrict__ keys,
                                                     const float *__restrict__ row_ref, const int32_t *__restrict__ given, int T, int K, float *__restrict__ logp,
                                                     float *__restrict__ lse_out, float *__restrict__ ent_out, int32_t *__restrict__ top_idx, float *__restrict__ top_logp)
 {
     constexpr int LPI = F32 ? D / 4 : D / 8, EPL = F32 ? 4 : 8, IPP = NT / LPI;        // lanes an item's row takes, elements a lane, items a pass
-    constexpr int NW = NT / 64, KR = NT == 1024 ? 16 : 8, FL = 8;                               // wavefronts; 16-byte loads of maxima a thread keeps; item rows on the way together
+    constexpr int NW = NT / 64, KR = NT == 1024 ? 16 : 8, FL = NT == 1024 ? 8 : 4;                               // wavefronts; 16-byte loads of maxima a thread keeps; item rows on the way together
     __shared__ __attribute__((aligned(16))) double c_s[kCand];
     __shared__ __attribute__((aligned(16))) int32_t c_id[kCand];
     __shared__ double s_red[3][NW];

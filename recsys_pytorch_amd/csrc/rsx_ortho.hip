@@ -14,6 +14,8 @@
 //   gram_reduce    partials in a fixed order -> G
 //   ns_*           the iteration in [d x d]
 //   project_kernel rows times M (fp32 MFMA), with the weight update of the optimizer step
+#include <type_traits>
+
 #include "rsx_common.h"
 
 namespace {
@@ -21,27 +23,12 @@ namespace {
 typedef double f64x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-constexpr int kGramWaves = 4;
-
-__device__ __forceinline__ float bf16_f32(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
 // round to nearest even; NaN stays NaN
 __device__ __forceinline__ uint16_t f32_bf16(float v)
 {
     const uint32_t u = __float_as_uint(v);
     if ((u & 0x7FFFFFFFu) > 0x7F800000u) return (uint16_t)((u >> 16) | 0x40u);
     return (uint16_t)((u + 0x7FFFu + ((u >> 16) & 1u)) >> 16);
-}
-
-// four consecutive elements of a row, in fp32
-template <typename T>
-__device__ __forceinline__ float4 load4(const T *p);
-template <>
-__device__ __forceinline__ float4 load4<float>(const float *p) { return *reinterpret_cast<const float4 *>(p); }
-template <>
-__device__ __forceinline__ float4 load4<uint16_t>(const uint16_t *p)
-{
-    const ushort4 h = *reinterpret_cast<const ushort4 *>(p);
-    return make_float4(bf16_f32(h.x), bf16_f32(h.y), bf16_f32(h.z), bf16_f32(h.w));
 }
 
 // what is orthogonalised: X itself, or the optimizer's momentum (M <- mu M + G, U = G + mu M or M)
@@ -51,18 +38,34 @@ struct Rows {
     float *M;         // MUON: the momentum
     float mu;
     int nesterov;
-    // UPDATE: this is the pass that advances M (it reads the old one and stores the new one)
-    template <bool UPDATE>
-    __device__ __forceinline__ float4 get(int64_t at) const
+};
+
+// four elements of it, asked for early and used late
+template <typename T, bool MUON>
+struct Piece {
+    typename std::conditional<sizeof(T) == 2, uint2, uint4>::type x;
+    float4 m;
+    __device__ __forceinline__ void load(const Rows<T, MUON> &in, int64_t at, int64_t end)
     {
-        float4 g = load4<T>(X + at);
+        if (at >= end) return;
+        x = *reinterpret_cast<const decltype(x) *>(in.X + at);
+        if constexpr (MUON) m = *reinterpret_cast<const float4 *>(in.M + at);
+    }
+    // UPDATE: this is the pass that advances M
+    template <bool UPDATE>
+    __device__ __forceinline__ float4 take(const Rows<T, MUON> &in, int64_t at, int64_t end)
+    {
+        if (at >= end) return make_float4(0.f, 0.f, 0.f, 0.f);
+        float4 g;
+        if constexpr (sizeof(T) == 2) g = make_float4(__uint_as_float(x.x << 16), __uint_as_float(x.x & 0xFFFF0000u), __uint_as_float(x.y << 16), __uint_as_float(x.y & 0xFFFF0000u));
+        else g = make_float4(__uint_as_float(x.x), __uint_as_float(x.y), __uint_as_float(x.z), __uint_as_float(x.w));
         if constexpr (MUON) {
-            float4 m = *reinterpret_cast<const float4 *>(M + at);
+            const float mu = in.mu;
             if constexpr (UPDATE) {
                 m = make_float4(fmaf(mu, m.x, g.x), fmaf(mu, m.y, g.y), fmaf(mu, m.z, g.z), fmaf(mu, m.w, g.w));
-                *reinterpret_cast<float4 *>(M + at) = m;
+                *reinterpret_cast<float4 *>(in.M + at) = m;
             }
-            if (!nesterov) return m;
+            if (!in.nesterov) return m;
             g = make_float4(fmaf(mu, m.x, g.x), fmaf(mu, m.y, g.y), fmaf(mu, m.z, g.z), fmaf(mu, m.w, g.w));
         }
         return g;
@@ -70,165 +73,124 @@ struct Rows {
 };
 
 // ---- the Gram matrix -------------------------------------------------------------------------------------------------------------
-// Column groups of 16: group b = 4 q + j of a row holds the columns 64 q + 4 m + j, m = 0..15 (d = 32: 8-lane halves, see below) -- what
-// one float4 load per lane and 64 columns delivers, without a transpose.  group_col maps (group, m) back to the column.
+// Column groups of 16: what a lane's 16-byte (d = 32: 8-byte) piece of a row holds for m = lane & 15 -- no transpose.  group_col maps (group, m) back.
 __host__ __device__ constexpr int n_groups(int D) { return D / 16; }
-__device__ __forceinline__ int group_col(int D, int b, int m) { return D == 32 ? 4 * (m & 7) + 2 * (m >> 3) + b : 64 * (b >> 2) + 4 * m + (b & 3); }
+__device__ __forceinline__ int group_col(int D, int b, int m) { return D == 32 ? 2 * m + b : 64 * (b >> 2) + 4 * m + (b & 3); }
 __host__ __device__ constexpr int n_blocks(int D) { return n_groups(D) * (n_groups(D) + 1) / 2; }
 __host__ __device__ constexpr int block_at(int D, int p, int q) { return p * n_groups(D) - p * (p - 1) / 2 + (q - p); }   // q >= p
 
-// one wavefront, rows r0 + (lane >> 4), all blocks: D <= 128 (36 blocks of 8 registers at D = 128, one wavefront per SIMD).
-// Bound by the fp64 matrix rate: 36 instructions of 64 cycles per four rows.  Row loads of the next four rows fly under them.
-template <int D, typename T, bool MUON>
-__global__ __launch_bounds__(64 * kGramWaves, 1) void gram_kernel(Rows<T, MUON> in, int64_t rows, double *__restrict__ part)
+// Eight wavefronts; the 16 x 16 blocks of the upper triangle are dealt to SETS of them (8 registers a block: 72 at d = 128, 136 at d = 256, so that two
+// wavefronts share a SIMD), the rows of a tile to the 8 / SETS wavefronts of a set.  16 KB tiles pass through LDS; two tiles of G and M are on their way
+// in registers (64 KB a CU: what HBM's latency takes).  Bound by HBM with the momentum (1M x 128: 1.5 GB in 0.34 ms), by the fp64 matrix
+// rate without (36 instructions of 64 cycles per four rows: 0.27 ms).
+template <int D>
+struct Gram {
+    static constexpr int SETS = D == 256 ? 8 : D == 128 ? 4 : 1, KSPLIT = 8 / SETS, TR = 4096 / D, NB = n_blocks(D), PER = (NB + SETS - 1) / SETS;
+};
+
+template <int D, int SET, typename F>
+__device__ __forceinline__ void set_blocks(F f)          // f(index of the accumulator, block, column group p, column group q)
 {
-    constexpr int NG = n_groups(D), NB = n_blocks(D), NQ = D < 64 ? 1 : D / 64;
-    constexpr int RPI = D == 32 ? 8 : 4;            // rows a wavefront's load instruction covers (D = 32: 8 lanes of float4 a row)
-    __shared__ __attribute__((aligned(16))) double red[NB * 256];
-    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
-    f64x4 acc[NB];
+    int a = 0, n = 0;
 #pragma unroll
-    for (int b = 0; b < NB; ++b) acc[b] = f64x4{0.0, 0.0, 0.0, 0.0};
-    const int64_t stride = (int64_t)gridDim.x * kGramWaves * RPI;
-    const int64_t first = ((int64_t)blockIdx.x * kGramWaves + wid) * RPI;
-    const int lrow = D == 32 ? lane >> 3 : lane >> 4, lcol = D == 32 ? 4 * (lane & 7) : 4 * (lane & 15);
-    float4 nxt[NQ];
-    auto fetch = [&](int64_t r0) {
-        const int64_t r = r0 + lrow;
+    for (int p = 0; p < n_groups(D); ++p)
 #pragma unroll
-        for (int q = 0; q < NQ; ++q)
-            nxt[q] = r < rows ? in.template get<true>(r * D + 64 * q + lcol) : make_float4(0.f, 0.f, 0.f, 0.f);
-    };
-    if (first < rows) fetch(first);
-    for (int64_t r0 = first; r0 < rows; r0 += stride) {
-        float4 cur[NQ];
-#pragma unroll
-        for (int q = 0; q < NQ; ++q) cur[q] = nxt[q];
-        if (r0 + stride < rows) fetch(r0 + stride);
-        if constexpr (D == 32) {
-            // lane l holds columns 4 (l & 7) .. + 3 of row l >> 3.  The instruction wants 16 columns of four rows: lane l of the fragment is
-            // (m = l & 15, k = l >> 4) -> row k (then k + 4) is lanes 8 k .., column pair by m >> 3.
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int src = 8 * ((lane >> 4) + 4 * h) + (lane & 7);
-                const bool up = (lane >> 3) & 1;
-                const float x0 = __shfl(cur[0].x, src, 64), x1 = __shfl(cur[0].y, src, 64), x2 = __shfl(cur[0].z, src, 64), x3 = __shfl(cur[0].w, src, 64);
-                const double v[2] = {(double)(up ? x2 : x0), (double)(up ? x3 : x1)};
-#pragma unroll
-                for (int p = 0; p < NG; ++p)
-#pragma unroll
-                    for (int q = p; q < NG; ++q)
-                        acc[block_at(D, p, q)] = __builtin_amdgcn_mfma_f64_16x16x4f64(v[p], v[q], acc[block_at(D, p, q)], 0, 0, 0);
-            }
-        } else {
-            double v[NG];
-#pragma unroll
-            for (int q = 0; q < NQ; ++q) { v[4 * q] = cur[q].x; v[4 * q + 1] = cur[q].y; v[4 * q + 2] = cur[q].z; v[4 * q + 3] = cur[q].w; }
-#pragma unroll
-            for (int p = 0; p < NG; ++p)
-#pragma unroll
-                for (int q = p; q < NG; ++q)
-                    acc[block_at(D, p, q)] = __builtin_amdgcn_mfma_f64_16x16x4f64(v[p], v[q], acc[block_at(D, p, q)], 0, 0, 0);
-        }
-    }
-    // the four wavefronts' sums, one after the other (a fixed order), then the workgroup's partial
-    // (f64 result layout: register pair i of lane l is row 4 i + (l >> 4), column l & 15)
-    for (int w = 0; w < kGramWaves; ++w) {
-        if (wid == w) {
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    double *cell = red + b * 256 + (4 * i + (lane >> 4)) * 16 + (lane & 15);
-                    *cell = w == 0 ? acc[b][i] : *cell + acc[b][i];
-                }
-        }
-        __syncthreads();
-    }
-    double *dst = part + (size_t)blockIdx.x * (NB * 256);
-    for (int t = threadIdx.x; t < NB * 256; t += 64 * kGramWaves) dst[t] = red[t];
+        for (int q = p; q < n_groups(D); ++q, ++n)
+            if (n / Gram<D>::PER == SET) f(a++, n, p, q);
 }
 
-// D = 256: 136 blocks are four wavefronts' registers.  The workgroup stages 16 rows in LDS; wavefronts 0..2 take two 64 x 64 squares off
-// the diagonal each (32 blocks), wavefront 3 the four on it (40 blocks).
-template <int JOB, typename F>
-__device__ __forceinline__ void gram256_blocks(F f)     // f(index of the accumulator, column group p, column group q)
+template <int D, int SET, typename T, bool MUON>
+__device__ __forceinline__ void gram_body(const Rows<T, MUON> &in, int64_t rows, double *__restrict__ part, char *lds)
 {
-    constexpr int sq[3][2][2] = {{{0, 1}, {0, 2}}, {{0, 3}, {1, 3}}, {{1, 2}, {2, 3}}};
-    if constexpr (JOB < 3) {
+    using C = Gram<D>;
+    constexpr int LW = D == 32 ? 2 : 4;                                 // elements of a lane's piece
+    const int tid = threadIdx.x, lane = tid & 63, ks = (tid >> 6) % C::KSPLIT;
+    f64x4 acc[C::PER];
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
+    for (int b = 0; b < C::PER; ++b) acc[b] = f64x4{0.0, 0.0, 0.0, 0.0};
+    const int64_t stride = (int64_t)gridDim.x * C::TR, first = (int64_t)blockIdx.x * C::TR;
+    Piece<T, MUON> a[2], b[2];                                          // this thread's two pieces of the next tile, and of the one after
+    auto at = [&](int64_t r0, int n) { return r0 * D + 4 * (tid + 512 * n); };
+    auto fetch = [&](Piece<T, MUON> (&p)[2], int64_t r0) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) f(s * 16 + i * 4 + j, 4 * sq[JOB][s][0] + i, 4 * sq[JOB][s][1] + j);
-    } else {
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            int n = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = i; j < 4; ++j) f(s * 10 + n++, 4 * s + i, 4 * s + j);
-        }
-    }
-}
-
-constexpr int kG256Rows = 16;
-
-template <int JOB, typename T, bool MUON>
-__device__ __forceinline__ void gram256_body(const Rows<T, MUON> &in, int64_t rows, double *__restrict__ part, float (*tile)[kG256Rows * 256])
-{
-    constexpr int NA = JOB < 3 ? 32 : 40;
-    const int tid = threadIdx.x, lane = tid & 63;
-    f64x4 acc[NA];
-#pragma unroll
-    for (int b = 0; b < NA; ++b) acc[b] = f64x4{0.0, 0.0, 0.0, 0.0};
-    const int64_t stride = (int64_t)gridDim.x * kG256Rows, first = (int64_t)blockIdx.x * kG256Rows;
-    float4 nxt[4];
-    auto fetch = [&](int64_t r0) {
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-            const int64_t r = r0 + 4 * n + (tid >> 6);
-            nxt[n] = r < rows ? in.template get<true>(r * 256 + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
+        for (int n = 0; n < 2; ++n) p[n].load(in, at(r0, n), rows * D);
     };
-    if (first < rows) fetch(first);
-    int par = 0;
-    for (int64_t r0 = first; r0 < rows; r0 += stride, par ^= 1) {
-        float *t = tile[par];               // (two tiles: a slow wavefront still reads the last one while this one is filled)
+    auto tile = [&](Piece<T, MUON> (&p)[2], int64_t r0, float *t) {     // pieces of tile r0 -> LDS, then the next but one is asked for
 #pragma unroll
-        for (int n = 0; n < 4; ++n) *reinterpret_cast<float4 *>(t + (4 * n + (tid >> 6)) * 256 + 4 * lane) = nxt[n];
-        __syncthreads();
-        if (r0 + stride < rows) fetch(r0 + stride);
+        for (int n = 0; n < 2; ++n) *reinterpret_cast<float4 *>(t + 4 * (tid + 512 * n)) = p[n].template take<true>(in, at(r0, n), rows * D);
+        fetch(p, r0 + 2 * stride);
+        __syncthreads();                                                // (two tiles: a slow wavefront still reads the last one)
 #pragma unroll 1
-        for (int k = 0; k < kG256Rows; k += 4) {
-            double v[16];
+        for (int k = 4 * ks; k < C::TR; k += 4 * C::KSPLIT) {
+            const float *row = t + (k + (lane >> 4)) * D + LW * (lane & 15);
+            double v[n_groups(D)];
+            if constexpr (D == 32) {
+                const float2 x = *reinterpret_cast<const float2 *>(row);
+                v[0] = x.x; v[1] = x.y;
+            } else {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const float4 x = *reinterpret_cast<const float4 *>(t + (k + (lane >> 4)) * 256 + 64 * q + 4 * (lane & 15));
-                v[4 * q] = x.x; v[4 * q + 1] = x.y; v[4 * q + 2] = x.z; v[4 * q + 3] = x.w;
+                for (int q = 0; q < D / 64; ++q) {
+                    const float4 x = *reinterpret_cast<const float4 *>(row + 64 * q);
+                    v[4 * q] = x.x; v[4 * q + 1] = x.y; v[4 * q + 2] = x.z; v[4 * q + 3] = x.w;
+                }
             }
-            gram256_blocks<JOB>([&](int a, int p, int q) { acc[a] = __builtin_amdgcn_mfma_f64_16x16x4f64(v[p], v[q], acc[a], 0, 0, 0); });
+            set_blocks<D, SET>([&](int i, int, int p, int q) { acc[i] = __builtin_amdgcn_mfma_f64_16x16x4f64(v[p], v[q], acc[i], 0, 0, 0); });
+        }
+    };
+    fetch(a, first);
+    fetch(b, first + stride);
+    float *const t0 = reinterpret_cast<float *>(lds), *const t1 = t0 + 4096;
+    for (int64_t r0 = first; r0 < rows; r0 += 2 * stride) {             // (every wavefront of the workgroup runs the same rounds and barriers)
+        tile(a, r0, t0);
+        if (r0 + stride < rows) tile(b, r0 + stride, t1);
+    }
+    // the KSPLIT wavefronts of a set one after the other (a fixed order), through LDS four blocks a set at a time; then the workgroup's partial
+    // (f64 result layout: register pair i of lane l is row 4 i + (l >> 4), column l & 15)
+    double *dst = part + (size_t)blockIdx.x * (C::NB * 256);
+    auto cell = [&](int i) { return (4 * i + (lane >> 4)) * 16 + (lane & 15); };
+    if constexpr (C::KSPLIT == 1) {
+        set_blocks<D, SET>([&](int i, int n, int, int) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) dst[n * 256 + cell(e)] = acc[i][e];
+        });
+    } else {
+        double *red = reinterpret_cast<double *>(lds) + SET * 4 * 256;  // (SETS x 4 blocks of 2 KB: 32 KB at most)
+#pragma unroll
+        for (int i0 = 0; i0 < C::PER; i0 += 4) {
+            for (int w = 0; w < C::KSPLIT; ++w) {
+                __syncthreads();
+                if (ks != w) continue;
+                set_blocks<D, SET>([&](int i, int n, int, int) {
+                    if (i < i0 || i >= i0 + 4) return;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        double *c = red + (i - i0) * 256 + cell(e);
+                        const double v = w == 0 ? acc[i][e] : *c + acc[i][e];
+                        if (w + 1 < C::KSPLIT) *c = v; else dst[n * 256 + cell(e)] = v;
+                    }
+                });
+            }
         }
     }
-    double *dst = part + (size_t)blockIdx.x * (n_blocks(256) * 256);
-    gram256_blocks<JOB>([&](int a, int p, int q) {
-        double *blk = dst + (size_t)block_at(256, p, q) * 256;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) blk[(4 * i + (lane >> 4)) * 16 + (lane & 15)] = acc[a][i];
-    });
 }
 
-template <typename T, bool MUON>
-__global__ __launch_bounds__(256, 1) void gram256_kernel(Rows<T, MUON> in, int64_t rows, double *__restrict__ part)
+template <int D, typename T, bool MUON>
+__global__ __launch_bounds__(512, (D == 256 ? 2 : 4)) void gram_kernel(Rows<T, MUON> in, int64_t rows, double *__restrict__ part)
 {
-    __shared__ __attribute__((aligned(16))) float tile[2][kG256Rows * 256];
-    switch (__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) {      // (every wavefront runs the same number of rounds and barriers)
-    case 0: gram256_body<0, T, MUON>(in, rows, part, tile); break;
-    case 1: gram256_body<1, T, MUON>(in, rows, part, tile); break;
-    case 2: gram256_body<2, T, MUON>(in, rows, part, tile); break;
-    default: gram256_body<3, T, MUON>(in, rows, part, tile); break;
+    using C = Gram<D>;
+    __shared__ __attribute__((aligned(16))) char lds[32768];
+    const int set = __builtin_amdgcn_readfirstlane((threadIdx.x >> 6) / C::KSPLIT);
+    if (set == 0) gram_body<D, 0, T, MUON>(in, rows, part, lds);
+    if constexpr (C::SETS >= 4) {
+        if (set == 1) gram_body<D, 1, T, MUON>(in, rows, part, lds);
+        if (set == 2) gram_body<D, 2, T, MUON>(in, rows, part, lds);
+        if (set == 3) gram_body<D, 3, T, MUON>(in, rows, part, lds);
+    }
+    if constexpr (C::SETS >= 8) {
+        if (set == 4) gram_body<D, 4, T, MUON>(in, rows, part, lds);
+        if (set == 5) gram_body<D, 5, T, MUON>(in, rows, part, lds);
+        if (set == 6) gram_body<D, 6, T, MUON>(in, rows, part, lds);
+        if (set == 7) gram_body<D, 7, T, MUON>(in, rows, part, lds);
     }
 }
 
@@ -365,54 +327,85 @@ __global__ __launch_bounds__(256) void ns_next_kernel(const double *__restrict__
     ns_store<D>(A2, p, q, ns_block<D>([&](int r, int c) { return W[(size_t)r * D + c]; }, t, p, q, red));
 }
 
-// d <= 64: the whole iteration in one workgroup, the four matrices in LDS (128 KB at d = 64), one 16 x 16 block per wavefront.
-// Odd rows swap neighbouring groups of 16 columns: the two rows of a half-wavefront's read fall on different halves of the banks.
+// d <= 64: the whole iteration in one workgroup, the four matrices in LDS (128 KB at d = 64).  Blocks of the upper triangles are dealt to 16 wavefronts
+// (M T and A T together: 20 blocks, five a SIMD); both triangles are written.  Bound by one CU's fp64 matrix rate.
+// Columns are XORed by row: the two rows of a half-wavefront's read lie in different halves of the 256 bytes the LDS delivers a cycle, and the 16 rows
+// of a transposed store in eight different places.
 template <int D>
-__global__ __launch_bounds__(64 * (D / 16) * (D / 16)) void ns_small_kernel(const double *__restrict__ G, float *__restrict__ out, int steps, Coeffs k)
+__global__ __launch_bounds__(1024) void ns_small_kernel(const double *__restrict__ G, float *__restrict__ out, int steps, Coeffs k)
 {
-    constexpr int NG = D / 16, N = 64 * NG * NG;
+    constexpr int NB = n_blocks(D);
     __shared__ __attribute__((aligned(16))) double A[D * D], T[D * D], W[D * D], M[D * D];
     __shared__ double s_norm;
-    auto el = [](int r, int c) { return r * D + (c ^ ((r & 1) << 4)); };
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, p = w / NG, q = w % NG;
+    auto el = [](int r, int c) { return r * D + (c ^ (((r & 1) << 4) | ((r & 6) << 1))); };
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     const double s = norm_scale(G, D, k.eps, &s_norm);
-    for (int t = tid; t < D * D; t += N) {
+    for (int t = tid; t < D * D; t += 1024) {
         const int r = t / D, c = t % D;
         A[el(r, c)] = s * s * G[t];
         M[el(r, c)] = r == c ? s : 0.0;
     }
     __syncthreads();
-    auto mul = [&](const double *x, const double *y) {
+    auto mul = [&](const double *x, const double *y, int p, int q) {
         f64x4 acc = {0.0, 0.0, 0.0, 0.0};
-#pragma unroll 4
-        for (int i = 0; i < D; i += 4)
-            acc = __builtin_amdgcn_mfma_f64_16x16x4f64(x[el(i + (lane >> 4), 16 * p + (lane & 15))], y[el(i + (lane >> 4), 16 * q + (lane & 15))], acc, 0, 0, 0);
+#pragma unroll
+        for (int h = 0; h < D / 32; ++h) {                                // (eight steps' operands on their way before the first product)
+            double fx[8], fy[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int kk = 32 * h + 4 * i + (lane >> 4);
+                fx[i] = x[el(kk, 16 * p + (lane & 15))]; fy[i] = y[el(kk, 16 * q + (lane & 15))];
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) acc = __builtin_amdgcn_mfma_f64_16x16x4f64(fx[i], fy[i], acc, 0, 0, 0);
+        }
         return acc;
     };
-    auto at = [&](int i) { return el(16 * p + 4 * i + (lane >> 4), 16 * q + (lane & 15)); };
+    auto put = [&](double *x, int p, int q, int i, double v) {           // (on the diagonal one of (r, c) and (c, r) stands for both)
+        const int r = 16 * p + 4 * i + (lane >> 4), c = 16 * q + (lane & 15);
+        if (r > c) return;
+        x[el(r, c)] = v;
+        x[el(c, r)] = v;
+    };
+    int p, q, p2[2], q2[2];                                                // this wavefront's block of one product, and its two of a pair
+    ns_pq<D>(w < NB ? w : 0, &p, &q);
+#pragma unroll
+    for (int n = 0; n < 2; ++n) ns_pq<D>((w + 16 * n) % NB, &p2[n], &q2[n]);
     for (int step = 0; step < steps; ++step) {
-        const f64x4 sq = mul(A, A);
+        const bool last = step + 1 == steps;
+        if (w < NB) {
+            const f64x4 sq = mul(A, A, p, q);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = 16 * p + 4 * i + (lane >> 4), c = 16 * q + (lane & 15);
-            T[at(i)] = fma(k.c, sq[i], fma(k.b, A[at(i)], r == c ? k.a : 0.0));
+            for (int i = 0; i < 4; ++i) {
+                const int r = 16 * p + 4 * i + (lane >> 4), c = 16 * q + (lane & 15);
+                put(T, p, q, i, fma(k.c, sq[i], fma(k.b, A[el(r, c)], r == c ? k.a : 0.0)));
+            }
         }
         __syncthreads();
-        const f64x4 m = mul(M, T);
-        f64x4 x = {0.0, 0.0, 0.0, 0.0};
-        if (step + 1 < steps) x = mul(A, T);
-        __syncthreads();
+        f64x4 x[2];                                                        // blocks w and w + 16 of A T, then M T
 #pragma unroll
-        for (int i = 0; i < 4; ++i) { M[at(i)] = m[i]; W[at(i)] = x[i]; }
-        __syncthreads();
-        if (step + 1 < steps) {
-            const f64x4 y = mul(W, T);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) A[at(i)] = y[i];      // (A was last read before the barrier above)
-            __syncthreads();
+        for (int n = 0; n < 2; ++n) {
+            const int b = w + 16 * n;
+            if (b >= 2 * NB || (last && b < NB)) continue;
+            x[n] = mul(b < NB ? A : M, T, p2[n], q2[n]);
         }
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            const int b = w + 16 * n;
+            if (b >= 2 * NB || (last && b < NB)) continue;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) put(b < NB ? W : M, p2[n], q2[n], i, x[n][i]);
+        }
+        __syncthreads();
+        if (!last && w < NB) {
+            const f64x4 y = mul(W, T, p, q);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) put(A, p, q, i, y[i]);             // (A was last read before the barrier above)
+        }
+        __syncthreads();
     }
-    for (int t = tid; t < D * D; t += N) out[t] = (float)M[el(t / D, t % D)];
+    for (int t = tid; t < D * D; t += 1024) out[t] = (float)M[el(t / D, t % D)];
 }
 
 template <int D>
@@ -425,33 +418,49 @@ __global__ __launch_bounds__(256) void ns_identity_kernel(const double *__restri
 
 // ---- rows times the [d x d] result ---------------------------------------------------------------------------------------------------
 // v_mfma_f32_32x32x2_f32, exact fp32 products.  A wavefront owns 32 output columns and keeps its 32 columns of the [d x d] matrix in registers
-// (d / 2 of them) for all its rows; rows pass through LDS.  The contraction index is permuted so that a lane reads its row four
-// elements at a time: step 4 j + e multiplies k = 8 j + 4 (lane >> 5) + e.
+// (d / 2 of them) for all its rows; rows pass through LDS, and so does the result, so that every access to memory is 16 bytes a lane.  The rows of the
+// next tile and the weights of this one are on their way during the products.  The contraction index is permuted so that a lane
+// reads its row four elements at a time: step 4 j + e multiplies k = 8 j + 4 (lane >> 5) + e.  Bound by HBM (optimizer step, 1M x 128: 2.6 GB).
 template <int D>
 struct Proj {
-    static constexpr int WAVES = D == 256 ? 8 : 4, CG = D / 32, RG = WAVES / CG, TR = 32 * RG, LD = D + 4;
+    static constexpr int WAVES = D == 256 ? 8 : 4, CG = D / 32, RG = WAVES / CG, TR = 32 * RG, LD = D + 4, NT = 64 * WAVES, NP = TR * D / 4 / NT;
 };
 
 template <int D, typename T, bool MUON>
-__global__ __launch_bounds__(64 * Proj<D>::WAVES) void project_kernel(Rows<T, MUON> in, T *__restrict__ out, float *__restrict__ W, int64_t rows,
-                                                                        const float *__restrict__ Mt, float keep, float step)
+__global__ __launch_bounds__(Proj<D>::NT) void project_kernel(Rows<T, MUON> in, T *__restrict__ out, float *__restrict__ W, int64_t rows,
+                                                              const float *__restrict__ Mt, float keep, float step)
 {
     using C = Proj<D>;
-    __shared__ __attribute__((aligned(16))) float tile[C::TR * C::LD];
+    __shared__ __attribute__((aligned(16))) float tile[C::TR * C::LD], res[C::TR * C::LD];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, cg = w % C::CG, rg = w / C::CG, hi = lane >> 5, l31 = lane & 31;
+    const int64_t stride = (int64_t)gridDim.x * C::TR, first = (int64_t)blockIdx.x * C::TR, end = rows * D;
+    Piece<T, MUON> p[C::NP];
+    float4 wt[MUON ? C::NP : 1];
+    auto spot = [&](int n) { const int t = tid + C::NT * n; return (t / (D / 4)) * C::LD + 4 * (t % (D / 4)); };
+    auto at = [&](int64_t r0, int n) { return r0 * D + 4 * (int64_t)(tid + C::NT * n); };
+    auto fetch = [&](int64_t r0) {
+#pragma unroll
+        for (int n = 0; n < C::NP; ++n) p[n].load(in, at(r0, n), end);
+    };
+    auto weights = [&](int64_t r0) {
+        if constexpr (MUON) {
+#pragma unroll
+            for (int n = 0; n < C::NP; ++n)
+                if (at(r0, n) < end) wt[n] = *reinterpret_cast<const float4 *>(W + at(r0, n));
+        }
+    };
+    fetch(first);
+    weights(first);
     float b[D / 2];
 #pragma unroll
     for (int j = 0; j < D / 8; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) b[4 * j + e] = Mt[(8 * j + 4 * hi + e) * D + 32 * cg + l31];
-    for (int64_t r0 = (int64_t)blockIdx.x * C::TR; r0 < rows; r0 += (int64_t)gridDim.x * C::TR) {
+    for (int64_t r0 = first; r0 < rows; r0 += stride) {
 #pragma unroll
-        for (int t = tid; t < C::TR * (D / 4); t += 64 * C::WAVES) {
-            const int r = t / (D / 4), c = 4 * (t % (D / 4));
-            const float4 v = r0 + r < rows ? in.template get<false>((r0 + r) * D + c) : make_float4(0.f, 0.f, 0.f, 0.f);
-            *reinterpret_cast<float4 *>(tile + r * C::LD + c) = v;
-        }
+        for (int n = 0; n < C::NP; ++n) *reinterpret_cast<float4 *>(tile + spot(n)) = p[n].template take<false>(in, at(r0, n), end);
         __syncthreads();
+        fetch(r0 + stride);
         f32x16 acc;
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[i] = 0.0f;
@@ -464,21 +473,25 @@ __global__ __launch_bounds__(64 * Proj<D>::WAVES) void project_kernel(Rows<T, MU
             acc = __builtin_amdgcn_mfma_f32_32x32x2f32(x.z, b[4 * j + 2], acc, 0, 0, 0);
             acc = __builtin_amdgcn_mfma_f32_32x32x2f32(x.w, b[4 * j + 3], acc, 0, 0, 0);
         }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) res[(32 * rg + (i & 3) + 8 * (i >> 2) + 4 * hi) * C::LD + 32 * cg + l31] = acc[i];
         __syncthreads();                // (every wavefront has read its rows, also before any of them is written where out == X)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int64_t r = r0 + 32 * rg + (i & 3) + 8 * (i >> 2) + 4 * hi;
-            if (r >= rows) continue;
-            const int64_t at = r * D + 32 * cg + l31;
+        for (int n = 0; n < C::NP; ++n) {
+            if (at(r0, n) >= end) continue;
+            const float4 o = *reinterpret_cast<const float4 *>(res + spot(n));
             if constexpr (MUON) {
-                W[at] = fmaf(-step, acc[i], keep * W[at]);
-                out[at] = (T)0;         // out is the gradient: zero for the next step
+                *reinterpret_cast<float4 *>(W + at(r0, n)) = make_float4(fmaf(-step, o.x, keep * wt[n].x), fmaf(-step, o.y, keep * wt[n].y), fmaf(-step, o.z, keep * wt[n].z),
+                                                                         fmaf(-step, o.w, keep * wt[n].w));
+                if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2 *>(out + at(r0, n)) = make_uint2(0u, 0u);      // out is the gradient: zero for the next step
+                else *reinterpret_cast<float4 *>(out + at(r0, n)) = make_float4(0.f, 0.f, 0.f, 0.f);
             } else if constexpr (sizeof(T) == 2) {
-                out[at] = f32_bf16(acc[i]);
+                *reinterpret_cast<ushort4 *>(out + at(r0, n)) = make_ushort4(f32_bf16(o.x), f32_bf16(o.y), f32_bf16(o.z), f32_bf16(o.w));
             } else {
-                out[at] = acc[i];
+                *reinterpret_cast<float4 *>(out + at(r0, n)) = o;
             }
         }
+        weights(r0 + stride);
     }
 }
 
@@ -490,11 +503,10 @@ struct OrthoWs {
     int64_t bytes;
 };
 
-int gram_groups(int64_t rows, int d)
+int gram_groups(int64_t rows, int d)             // a workgroup for every two tiles of 4096 / d rows, at most two per CU (d = 256: one, by its registers)
 {
-    // a workgroup for every 64 rows, at most one per CU (the accumulators are one wavefront per SIMD)
-    const int64_t per = d == 256 ? kG256Rows : kGramWaves * (d == 32 ? 8 : 4), want = (rows + 4 * per - 1) / (4 * per);
-    return (int)(want < 1 ? 1 : want > 256 ? 256 : want);
+    const int64_t per = 2 * (4096 / d), want = (rows + per - 1) / per;
+    return (int)(want < 1 ? 1 : want > (d == 256 ? 256 : 512) ? (d == 256 ? 256 : 512) : want);
 }
 
 OrthoWs ortho_carve(void *ws, int64_t rows, int d)
@@ -518,7 +530,7 @@ void newton_schulz(const OrthoWs &w, int steps, const Coeffs &k, hipStream_t st)
 {
     if (steps == 0) { hipLaunchKernelGGL(ns_identity_kernel<D>, dim3(1), dim3(256), 0, st, w.G, w.T, k.eps); return; }
     if constexpr (D <= 64) {
-        hipLaunchKernelGGL(ns_small_kernel<D>, dim3(1), dim3(64 * (D / 16) * (D / 16)), 0, st, w.G, w.T, steps, k);
+        hipLaunchKernelGGL(ns_small_kernel<D>, dim3(1), dim3(1024), 0, st, w.G, w.T, steps, k);
     } else {
         constexpr int NB = n_blocks(D);
         double *A = w.A, *A2 = w.A2, *M = w.M, *M2 = w.M2;
@@ -541,16 +553,13 @@ void newton_schulz(const OrthoWs &w, int steps, const Coeffs &k, hipStream_t st)
 template <int D, typename T, bool MUON>
 void orthogonalize_d(const Rows<T, MUON> &in, T *out, float *W, int64_t rows, int steps, const Coeffs &k, float keep, float step, const OrthoWs &w, hipStream_t st)
 {
-    if constexpr (D == 256)
-        hipLaunchKernelGGL((gram256_kernel<T, MUON>), dim3(w.n_part), dim3(256), 0, st, in, rows, w.part);
-    else
-        hipLaunchKernelGGL((gram_kernel<D, T, MUON>), dim3(w.n_part), dim3(64 * kGramWaves), 0, st, in, rows, w.part);
+    hipLaunchKernelGGL((gram_kernel<D, T, MUON>), dim3(w.n_part), dim3(512), 0, st, in, rows, w.part);
     hipLaunchKernelGGL(gram_reduce_kernel<D>, dim3(n_blocks(D) * 16), dim3(256), 0, st, w.part, w.n_part, w.G);
     newton_schulz<D>(w, steps, k, st);
     using C = Proj<D>;
     const int64_t tiles = (rows + C::TR - 1) / C::TR;
-    const int64_t most = (int64_t)rsx_num_cus() * (D == 256 ? 2 : 4);
-    hipLaunchKernelGGL((project_kernel<D, T, MUON>), dim3((unsigned)(tiles < most ? tiles : most)), dim3(64 * C::WAVES), 0, st, in, out, W, rows, w.T, keep, step);
+    const int64_t most = (int64_t)rsx_num_cus() * (D == 256 ? 2 : 3);
+    hipLaunchKernelGGL((project_kernel<D, T, MUON>), dim3((unsigned)(tiles < most ? tiles : most)), dim3(C::NT), 0, st, in, out, W, rows, w.T, keep, step);
 }
 
 template <typename T, bool MUON>
