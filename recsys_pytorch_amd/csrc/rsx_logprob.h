@@ -76,15 +76,19 @@ __device__ __forceinline__ float opaque(float v)
     return v;
 }
 
-// eight scaled floats -> the two planes' fragments
+// eight scaled floats -> the two planes' fragments, two at a time (v_cvt_pk_f16_f32, to nearest)
+typedef float float2v __attribute__((ext_vector_type(2)));
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void split8(const float *x, Frag *hi, Frag *lo)
 {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const float v = opaque(x[j]);
-        const _Float16 h = (_Float16)v;
-        hi->h[j] = h;
-        lo->h[j] = (_Float16)(v - (float)h);
+    for (int j = 0; j < 8; j += 2) {
+        const float2v v = {opaque(x[j]), opaque(x[j + 1])};
+        const half2v h = __builtin_convertvector(v, half2v);
+        const float2v r = {v[0] - (float)h[0], v[1] - (float)h[1]};
+        const half2v l = __builtin_convertvector(r, half2v);
+        hi->h[j] = h[0]; hi->h[j + 1] = h[1];
+        lo->h[j] = l[0]; lo->h[j + 1] = l[1];
     }
 }
 

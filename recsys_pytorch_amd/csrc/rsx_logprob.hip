@@ -515,7 +515,6 @@ __device__ void sort_candidates(double *s, int32_t *id, int n)          // desce
         }
 }
 
-typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ half2v max2(half2v a, half2v b) { return __builtin_elementwise_max(a, b); }      // (NaN: the other)
 __device__ __forceinline__ half2v as_half2(uint32_t w) { return __builtin_bit_cast(half2v, w); }
 __device__ __forceinline__ uint32_t half_order(_Float16 v)                                                  // halves -> ordered integers

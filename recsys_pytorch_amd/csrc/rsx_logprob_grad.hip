@@ -39,7 +39,7 @@ struct Args {
     float scale;
 };
 
-// per tile of 32 positions: [0] factor of its scores, [1] lse in log2, [2] [3] dz = p (A + B log2 p), [4] .. [7] the first four named items (as
+// per tile of 32 positions: [0] factor of its scores, [1] what is added to them (-lse in log2; fp32 without the entropy: and 12), [2] [3] dz = p (A + B log2 p), [4] .. [7] the first four named items (as
 // integers; -1: none): 1 KB, one wavefront's copy
 constexpr int kHeld = 4;
 struct Prm {
@@ -117,7 +117,7 @@ __global__ __launch_bounds__(256) void rows_kernel(Args a, const uint32_t *__res
         const double fix = exp2((double)l2 - lse2) * inv;
         if (lane == 0) {
             out.v[0][c] = factor;
-            out.v[1][c] = live ? l2 : kFar;
+            out.v[1][c] = live ? (F32 && a.h == nullptr ? 12.0f - l2 : -l2) : -kFar;
             out.v[2][c] = live ? (float)(-(sum + (double)h * (a.ent != nullptr ? a.ent[r] : 0.0f)) * fix) : 0.0f;
             out.v[3][c] = live ? (float)(-(double)h * kLn2 * fix) : 0.0f;
             for (int k = a.T; k < kHeld; ++k) out.v[4 + k][c] = __int_as_float(-1);
@@ -291,33 +291,36 @@ __device__ __forceinline__ void grad_body(const Pass &a, char (*lds)[GradGeo<D, 
     const int64_t words = mask_words(a.cat);
     const int sw = G::swz(l31) * 16;
 
-    auto stage = [&](int64_t tile, int buf, int64_t block, int64_t colc) {
+    // Copies of the next ST tiles, 1 KB a wavefront instruction: uniform bases and lane offsets that stay (an address computed per copy
+    // would be half of the loop's vector instructions)
+    constexpr int NC = ST * G::TILEB / 4096;
+    uint32_t off[NC];
 #pragma unroll
-        for (int n = 0; n < (ST * (2 * G::TILEB / 1024 + 1) + 3) / 4; ++n) {
-            const int k = n * 4 + wid;                                           // 1 KB piece of the stage: ST row-major tiles, ST transposed, ST parameter blocks
-            if (k >= ST * (2 * G::TILEB / 1024 + 1)) break;
-            constexpr int per = G::TILEB / 1024;
-            char *dst = lds[buf] + k * 1024;
-            if (k < ST * per) {
-                const int o = k * 1024 + lane * 16, row = o / G::ROWB, c = (o % G::ROWB) / 16 ^ G::swz(row & 31);
-                int64_t i = tile * kTile + row;
-                const int64_t most = ITEMS_STAY || F32 ? a.flow_tiles * kTile - 1 : a.flow_valid - 1;    // (bf16 item rows are the table itself)
-                i = i < most ? i : most;
-                copy_to_lds(a.flow + (size_t)i * G::ROWB + 16 * c, dst);
-            } else if (k < 2 * ST * per) {
-                const int64_t last = a.flow_tiles * G::TILEB - 16;
-                int64_t o = tile * G::TILEB + (k - ST * per) * 1024 + lane * 16;
-                o = o < last ? o : last;
-                copy_to_lds(a.flow_t + o, dst);
-            } else if (ITEMS_STAY) {
-                int64_t t = tile + k - 2 * ST * per;
-                t = t < a.flow_tiles ? t : a.flow_tiles - 1;
-                copy_to_lds((const char *)(a.prm + t) + lane * 16, dst);
-            }
+    for (int n = 0; n < NC; ++n) {
+        const int o = (n * 4 + wid) * 1024 + lane * 16, row = o / G::ROWB, c = ((o % G::ROWB) / 16) ^ G::swz(row & 31);
+        off[n] = (uint32_t)(row * G::ROWB + 16 * c);
+    }
+    const uint32_t lane16 = (uint32_t)(lane * 16);
+    constexpr bool TABLE = !ITEMS_STAY && !F32;                  // bf16 item rows are the table itself: its last tile may be short
+    auto stage = [&](int64_t tile, int buf, int64_t block, int64_t colc) {
+        const char *rows = a.flow + (size_t)tile * G::TILEB, *turned = a.flow_t + (size_t)tile * G::TILEB;
+        const int64_t tiles = a.flow_tiles - tile;
+        const int64_t left = (a.flow_valid - tile * kTile) * G::ROWB;
+#pragma unroll
+        for (int n = 0; n < NC; ++n) {
+            const int k = n * 4 + wid;
+            if (ST > 1 && k * 1024 / G::TILEB >= tiles) continue;
+            uint32_t o = off[n];
+            if constexpr (TABLE) o = (int64_t)o < left ? o : o % G::ROWB;           // (rows behind the last item: any valid row, they are masked)
+            copy_to_lds(rows + o, lds[buf] + k * 1024);
+            copy_to_lds(turned + k * 1024 + lane16, lds[buf] + ST * G::TILEB + k * 1024);
+        }
+        if constexpr (ITEMS_STAY) {
+            if (wid < ST && wid < tiles) copy_to_lds((const char *)(a.prm + tile + wid) + lane16, lds[buf] + G::PRM + wid * 1024);
         }
         if constexpr (MASK) {
             if constexpr (ITEMS_STAY) {              // four words of each of the tile's 32 positions: the workgroup's blocks (both halves of a wavefront the same)
-                if (wid < ST) {
+                if (wid < ST && wid < tiles) {
                     int64_t r = (tile + wid) * kTile + l31;
                     r = r < a.positions ? r : a.positions - 1;
                     if (hi == 0) copy_to_lds((const char *)(a.bits + (size_t)r * words + 4 * block), lds[buf] + G::BITS + wid * 1024);
@@ -398,36 +401,51 @@ __device__ __forceinline__ void grad_body(const Pass &a, char (*lds)[GradGeo<D, 
                 const float f = sf * tf;
                 // items of a tile whose scale is below the largest count less by that: the tile's sums are over planes of its own scale
                 const float lift = F32 ? (float)(12 + (int)(__float_as_uint(tf) >> 23) - (int)(__float_as_uint(top) >> 23)) : 0.0f;
-                const float off = ENT ? -slse : lift - slse;             // (without the entropy's part log2 p itself is not needed)
+                const float off = F32 && !ENT ? slse + (lift - 12.0f) : slse;             // (without the entropy's part log2 p itself is not needed)
+                float t[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) t[i] = fmaf(acc[i], f, off);
+                if (any) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) t[i] = (w >> ((i & 3) + 8 * (i >> 2))) & 1u ? -1.0e4f : t[i];
+                }
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    float t = fmaf(acc[i], f, off);
-                    if (any && ((w >> ((i & 3) + 8 * (i >> 2))) & 1u)) t = -1.0e4f;
-                    const float p = __builtin_amdgcn_exp2f(F32 && ENT ? t + lift : t);
-                    v[i] = ENT ? p * fmaf(sB, t, sA) : p * sA;
+                    const float p = __builtin_amdgcn_exp2f(F32 && ENT ? t[i] + lift : t[i]);
+                    v[i] = ENT ? p * fmaf(sB, t[i], sA) : p * sA;
                 }
             } else {
                 const Prm *prm = reinterpret_cast<const Prm *>(lds[buf] + G::PRM + j * 1024);
                 if (MASK && tile * kTile + l31 >= a.positions) seen = 0xFFFFFFFFu;            // nobody's rows behind the last
                 const bool any = MASK && __builtin_amdgcn_ballot_w64(seen != 0u) != 0ull;
+                float t[16];
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     const int r0 = 8 * q + 4 * hi;
-                    const float4 f4 = *reinterpret_cast<const float4 *>(&prm->v[0][r0]), l4 = *reinterpret_cast<const float4 *>(&prm->v[1][r0]),
-                                 a4 = *reinterpret_cast<const float4 *>(&prm->v[2][r0]);
-                    float4 b4 = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if constexpr (ENT) b4 = *reinterpret_cast<const float4 *>(&prm->v[3][r0]);
-                    const float fs[4] = {f4.x, f4.y, f4.z, f4.w}, ls[4] = {l4.x, l4.y, l4.z, l4.w}, as[4] = {a4.x, a4.y, a4.z, a4.w}, bs[4] = {b4.x, b4.y, b4.z, b4.w};
+                    const float4 f4 = *reinterpret_cast<const float4 *>(&prm->v[0][r0]), l4 = *reinterpret_cast<const float4 *>(&prm->v[1][r0]);
+                    t[4 * q] = fmaf(acc[4 * q], f4.x * tf, l4.x);
+                    t[4 * q + 1] = fmaf(acc[4 * q + 1], f4.y * tf, l4.y);
+                    t[4 * q + 2] = fmaf(acc[4 * q + 2], f4.z * tf, l4.z);
+                    t[4 * q + 3] = fmaf(acc[4 * q + 3], f4.w * tf, l4.w);
+                }
+                if (any) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) t[i] = (__shfl(seen, (i & 3) + 8 * (i >> 2) + 4 * hi, 64) >> l31) & 1u ? -1.0e4f : t[i];
+                }
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int r0 = 8 * q + 4 * hi;
+                    const float4 a4 = *reinterpret_cast<const float4 *>(&prm->v[2][r0]);
+                    const float as[4] = {a4.x, a4.y, a4.z, a4.w};
+                    float bs[4] = {0.f, 0.f, 0.f, 0.f};
+                    if constexpr (ENT) {
+                        const float4 b4 = *reinterpret_cast<const float4 *>(&prm->v[3][r0]);
+                        bs[0] = b4.x; bs[1] = b4.y; bs[2] = b4.z; bs[3] = b4.w;
+                    }
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const int i = 4 * q + e;
-                        float t = fmaf(acc[i], fs[e] * tf, F32 && !ENT ? 12.0f - ls[e] : -ls[e]);
-                        if (any) {
-                            const uint32_t w = __shfl(seen, r0 + e, 64);
-                            if ((w >> l31) & 1u) t = -1.0e4f;
-                        }
-                        const float p = __builtin_amdgcn_exp2f(F32 && ENT ? t + 12.0f : t);
-                        v[i] = ENT ? p * fmaf(bs[e], t, as[e]) : p * as[e];
+                        const float p = __builtin_amdgcn_exp2f(F32 && ENT ? t[4 * q + e] + 12.0f : t[4 * q + e]);
+                        v[4 * q + e] = ENT ? p * fmaf(bs[e], t[4 * q + e], as[e]) : p * as[e];
                     }
                 }
                 // named items of the tile's positions that are in this wavefront's block.
