@@ -51,10 +51,19 @@ struct Geo {
     __device__ static __forceinline__ int swz(int row) { return ROWB >= 256 ? row & 15 : ROWB == 128 ? (row >> 1) & 7 : (row >> 2) & 3; }
 };
 
-// 64 lanes x 16 bytes from global memory straight into LDS (lane-linear from a wavefront-uniform base); the next barrier waits for it.
-// (a function of its own: called from a kernel's body, the builtin costs the kernel its host stub)
+// 64 lanes x 16 (or 4) bytes from global memory straight into LDS, lane-linear from a wavefront-uniform base.
+// (functions of their own: called from a kernel's body, the builtin costs the kernel its host stub)
 __device__ __forceinline__ void copy_to_lds(const char *src, char *dst) { __builtin_amdgcn_global_load_lds(src, dst, 16, 0, 0); }
-__device__ __forceinline__ void copy4_to_lds(const char *src, char *dst) { __builtin_amdgcn_global_load_lds(src, dst, 4, 0, 0); }       // 64 lanes x 4 bytes
+__device__ __forceinline__ void copy4_to_lds(const char *src, char *dst) { __builtin_amdgcn_global_load_lds(src, dst, 4, 0, 0); }
+// wait for this wavefront's copies (and other accesses to memory): vmcnt(0)
+__device__ __forceinline__ void wait_memory() { __builtin_amdgcn_s_waitcnt(0x0F70); }
+// Every wavefront's copies have landed, and everybody is done with what they will be followed by.  The wait is written out: a barrier alone orders
+// LDS and waits for the copies only where the compiler happens to have a reason to, and the others' copies are not its concern.
+__device__ __forceinline__ void barrier_after_copies()
+{
+    wait_memory();
+    __syncthreads();
+}
 
 // power of two that brings a largest magnitude m into [2^13, 2^14), and its inverse.  Below 2^-40 as for 2^-40: the product of two such
 // inverses stays a normal number, and what is lost there moves no score by 2^-40

@@ -252,7 +252,7 @@ __device__ __forceinline__ void wide_body(const void *__restrict__ P, const char
         for (int j = 0; j < 4; ++j) {
             const int64_t tile = 4 * g + j;
             if (j % ST == 0) {
-                __syncthreads();         // this stage's copies have landed; everyone is done with the other buffer
+                barrier_after_copies();  // this stage's tiles are there; everyone is done with the other buffer
                 if (TOP && j == 0 && g > g0) {        // the last group's maxima, ahead of the copies so that the next barrier finds them done
 #pragma unroll
                     for (int ub = 0; ub < UB; ++ub) {

@@ -246,8 +246,7 @@ __global__ __launch_bounds__(256) void tiles_kernel(Args a, const float *__restr
 struct Pass {
     const char *stay, *flow;              // row-major planes of what stays in registers and of what streams
     const char *flow_t;                   // transposed tiles of what streams
-    const float *tile_factor;             // fp32: factor of an item tile
-    const uint32_t *top_factor;           // ... and the largest of them
+    const uint32_t *top_factor;           // fp32: the largest factor of an item tile
     const Prm *prm;
     const uint32_t *bits;
     const int32_t *named;
@@ -274,16 +273,18 @@ struct GradGeo : Geo<D, F32> {
     static constexpr int ST = 16384 / G::TILEB >= 4 ? 4 : 16384 / G::TILEB >= 1 ? 16384 / G::TILEB : 1;       // tiles of one LDS buffer
     // a buffer: row-major tiles, transposed tiles, parameter blocks, and 1 KB of seen bits a tile
     static constexpr int PRM = 2 * ST * G::TILEB, BITS = PRM + ST * 1024, STAGE = BITS + ST * 1024;
-    // workgroups a CU holds: the sums of 256 columns alone are half of a lane's registers at two
-    static constexpr int WGS = D == 256 ? 1 : 2;
+    // Workgroups a CU holds, and wavefronts that share 32 columns.  d = 256: the sums of 256 elements are half of a lane's registers at two wavefronts a
+    // SIMD.  bf16: two wavefronts take 128 each, and both form the scores (24 products a tile and wavefront instead of 32, two on a SIMD:
+    // 1000 x 50021 GP 104 -> RSX_T1, GQ 175 -> RSX_T2 us); fp32, whose operands take another 128 registers: one a SIMD.
+    static constexpr int WGS = D == 256 ? 1 : 2, HS = D == 256 && !F32 ? 2 : 1, NW = 4 * HS, NT = 64 * NW;
 };
 
 template <int D, bool F32, bool ITEMS_STAY, bool MASK, bool ENT>
-__device__ __forceinline__ void grad_body(const Pass &a, char (*lds)[GradGeo<D, F32>::STAGE])
+__device__ __forceinline__ void grad_body(const Pass &a, const float *__restrict__ tile_factor, char *lds0, char *lds1)
 {
     using G = GradGeo<D, F32>;
-    constexpr int KS = G::KS, NP = G::NP, ST = G::ST, KB = G::KB;
-    const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, hi = lane >> 5, l31 = lane & 31;
+    constexpr int KS = G::KS, NP = G::NP, ST = G::ST, KB = G::KB / G::HS;              // KB: this wavefront's blocks of 32 elements
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wid = wave & 3, half = wave >> 2, hi = lane >> 5, l31 = lane & 31;
     const int64_t total = a.part_rows / 128 * a.flow_tiles;
     int64_t at = piece_begin(total, gridDim.x, blockIdx.x);
     const int64_t end = piece_begin(total, gridDim.x, blockIdx.x + 1);
@@ -293,48 +294,47 @@ __device__ __forceinline__ void grad_body(const Pass &a, char (*lds)[GradGeo<D, 
 
     // Copies of the next ST tiles, 1 KB a wavefront instruction: uniform bases and lane offsets that stay (an address computed per copy
     // would be half of the loop's vector instructions)
-    constexpr int NC = ST * G::TILEB / 4096;
+    constexpr int NC = ST * G::TILEB / (1024 * G::NW);
     uint32_t off[NC];
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
-        const int o = (n * 4 + wid) * 1024 + lane * 16, row = o / G::ROWB, c = ((o % G::ROWB) / 16) ^ G::swz(row & 31);
+        const int o = (n * G::NW + wave) * 1024 + lane * 16, row = o / G::ROWB, c = ((o % G::ROWB) / 16) ^ G::swz(row & 31);
         off[n] = (uint32_t)(row * G::ROWB + 16 * c);
     }
     const uint32_t lane16 = (uint32_t)(lane * 16);
     constexpr bool TABLE = !ITEMS_STAY && !F32;                  // bf16 item rows are the table itself: its last tile may be short
-    auto stage = [&](int64_t tile, int buf, int64_t block, int64_t colc) {
+    auto stage = [&](int64_t tile, char *lds, int64_t block, int64_t colc) __attribute__((always_inline)) {
         const char *rows = a.flow + (size_t)tile * G::TILEB, *turned = a.flow_t + (size_t)tile * G::TILEB;
         const int64_t tiles = a.flow_tiles - tile;
         const int64_t left = (a.flow_valid - tile * kTile) * G::ROWB;
 #pragma unroll
         for (int n = 0; n < NC; ++n) {
-            const int k = n * 4 + wid;
+            const int k = n * G::NW + wave;
             if (ST > 1 && k * 1024 / G::TILEB >= tiles) continue;
             uint32_t o = off[n];
             if constexpr (TABLE) o = (int64_t)o < left ? o : o % G::ROWB;           // (rows behind the last item: any valid row, they are masked)
-            copy_to_lds(rows + o, lds[buf] + k * 1024);
-            copy_to_lds(turned + k * 1024 + lane16, lds[buf] + ST * G::TILEB + k * 1024);
+            copy_to_lds(rows + o, lds + k * 1024);
+            copy_to_lds(turned + k * 1024 + lane16, lds + ST * G::TILEB + k * 1024);
         }
         if constexpr (ITEMS_STAY) {
-            if (wid < ST && wid < tiles) copy_to_lds((const char *)(a.prm + tile + wid) + lane16, lds[buf] + G::PRM + wid * 1024);
+            if (wave < ST && wave < tiles) copy_to_lds((const char *)(a.prm + tile + wave) + lane16, lds + G::PRM + wave * 1024);
         }
         if constexpr (MASK) {
             if constexpr (ITEMS_STAY) {              // four words of each of the tile's 32 positions: the workgroup's blocks (both halves of a wavefront the same)
-                if (wid < ST && wid < tiles) {
-                    int64_t r = (tile + wid) * kTile + l31;
+                if (wave < ST && wave < tiles) {
+                    int64_t r = (tile + wave) * kTile + l31;
                     r = r < a.positions ? r : a.positions - 1;
-                    if (hi == 0) copy_to_lds((const char *)(a.bits + (size_t)r * words + 4 * block), lds[buf] + G::BITS + wid * 1024);
+                    if (hi == 0) copy_to_lds((const char *)(a.bits + (size_t)r * words + 4 * block), lds + G::BITS + wave * 1024);
                 }
-            } else {                                  // this wavefront's columns, a word a tile
+            } else if (half == 0) {                                  // this wavefront's columns, a word a tile
 #pragma unroll
                 for (int j = 0; j < ST; ++j) {
                     const int64_t t = tile + j < words ? tile + j : words - 1;
-                    copy4_to_lds((const char *)(a.bits + (size_t)(colc < a.positions ? colc : a.positions - 1) * words + t), lds[buf] + G::BITS + j * 1024 + wid * 256);
+                    copy4_to_lds((const char *)(a.bits + (size_t)(colc < a.positions ? colc : a.positions - 1) * words + t), lds + G::BITS + j * 1024 + wid * 256);
                 }
             }
         }
     };
-    int buf = 0;
     while (at < end) {
     const int64_t block = at / a.flow_tiles, t0 = at - block * a.flow_tiles;                        // this segment: tiles [t0, t1) of a block
     const int64_t t1 = end - at < a.flow_tiles - t0 ? t0 + (end - at) : a.flow_tiles;
@@ -343,7 +343,7 @@ __device__ __forceinline__ void grad_body(const Pass &a, char (*lds)[GradGeo<D, 
     const int64_t colc = col < a.stay_rows ? col : a.stay_rows - 1;
     const int32_t my_block = (int32_t)(block * 4 + wid);                                             // items stay: the block of 32 this wavefront holds
     __syncthreads();                      // (the last segment's tiles are read)
-    stage(t0, buf, block, colc);
+    stage(t0, lds0, block, colc);
     Frag b[KS][NP];
 #pragma unroll
     for (int s = 0; s < KS; ++s)
@@ -360,22 +360,23 @@ __device__ __forceinline__ void grad_body(const Pass &a, char (*lds)[GradGeo<D, 
         const int c = (int)(colc % kTile);
         sf = p.v[0][c]; slse = p.v[1][c]; sA = p.v[2][c]; sB = p.v[3][c];
     } else if constexpr (F32) {
-        my_factor = a.tile_factor[colc / kTile];
+        my_factor = tile_factor[colc / kTile];
     }
-    for (int64_t s0 = t0; s0 < t1; s0 += ST) {
-        __syncthreads();
-        if (s0 + ST < t1) stage(s0 + ST, buf ^ 1, block, colc);
+    wait_memory();                        // (the operands' loads end here: left to their first use, that wait would stand in the loop, for every stage's copies)
+    auto step = [&](int64_t s0, const char *lds, char *next) __attribute__((always_inline)) {
+        barrier_after_copies();
+        if (s0 + ST < t1) stage(s0 + ST, next, block, colc);
         for (int j = 0; j < ST && s0 + j < t1; ++j) {
             const int64_t tile = s0 + j;
             // (nothing in this loop loads into registers from memory: loads return in order, and one would wait for the next stage's copies)
             uint32_t seen = 0u;
             if constexpr (MASK) {
-                const char *sb = lds[buf] + G::BITS + j * 1024;
+                const char *sb = lds + G::BITS + j * 1024;
                 seen = ITEMS_STAY ? *reinterpret_cast<const uint32_t *>(sb + l31 * 16 + wid * 4) : *reinterpret_cast<const uint32_t *>(sb + wid * 256 + lane * 4);
             }
-            const float tf = !ITEMS_STAY && F32 ? a.tile_factor[tile] : my_factor;
-            const char *rm = lds[buf] + j * G::TILEB + l31 * G::ROWB;
-            const char *tr = lds[buf] + ST * G::TILEB + j * G::TILEB + lane * 16;
+            const float tf = !ITEMS_STAY && F32 ? tile_factor[tile] : my_factor;
+            const char *rm = lds + j * G::TILEB + l31 * G::ROWB;
+            const char *tr = lds + ST * G::TILEB + j * G::TILEB + lane * 16;
             f32x16 acc;
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[i] = 0.0f;
@@ -415,7 +416,7 @@ __device__ __forceinline__ void grad_body(const Pass &a, char (*lds)[GradGeo<D, 
                     v[i] = ENT ? p * fmaf(sB, t[i], sA) : p * sA;
                 }
             } else {
-                const Prm *prm = reinterpret_cast<const Prm *>(lds[buf] + G::PRM + j * 1024);
+                const Prm *prm = reinterpret_cast<const Prm *>(lds + G::PRM + j * 1024);
                 if (MASK && tile * kTile + l31 >= a.positions) seen = 0xFFFFFFFFu;            // nobody's rows behind the last
                 const bool any = MASK && __builtin_amdgcn_ballot_w64(seen != 0u) != 0ull;
                 float t[16];
@@ -449,13 +450,11 @@ __device__ __forceinline__ void grad_body(const Pass &a, char (*lds)[GradGeo<D, 
                     }
                 }
                 // named items of the tile's positions that are in this wavefront's block.
-                for (int t = 0; t < a.T; ++t) {
-                    const int64_t r = tile * kTile + l31;
-                    const int32_t it = t < kHeld ? __float_as_int(prm->v[4 + t][l31]) : r < a.positions ? a.named[r * a.T + t] : -1;
+                auto name = [&](int32_t it, int t) __attribute__((always_inline)) {
                     const bool mine = hi == 0 && (it >> 5) == my_block;          // (-1 >> 5 is nobody's block)
                     unsigned long long hits = __builtin_amdgcn_ballot_w64(mine);
-                    if (hits == 0ull) continue;
-                    const float c = mine ? a.coef[r * a.T + t] * (F32 ? kLift : 1.0f) : 0.0f;
+                    if (hits == 0ull) return;
+                    const float c = mine ? a.coef[(tile * kTile + l31) * a.T + t] * (F32 ? kLift : 1.0f) : 0.0f;
                     while (hits) {
                         const int row = __builtin_ctzll(hits);
                         hits &= hits - 1;
@@ -466,6 +465,11 @@ __device__ __forceinline__ void grad_body(const Pass &a, char (*lds)[GradGeo<D, 
 #pragma unroll
                         for (int i = 0; i < 16; ++i) v[i] += here && i == reg ? add : 0.0f;
                     }
+                };
+                for (int t = 0; t < a.T && t < kHeld; ++t) name(__float_as_int(prm->v[4 + t][l31]), t);
+                for (int t = kHeld; t < a.T; ++t) {
+                    const int64_t r = tile * kTile + l31;
+                    name(r < a.positions ? a.named[r * a.T + t] : -1, t);
                 }
             }
             // second product: registers 8 h .. 8 h + 7 are the operand of its half h
@@ -482,7 +486,7 @@ __device__ __forceinline__ void grad_body(const Pass &a, char (*lds)[GradGeo<D, 
                 for (int k = 0; k < KB; ++k) {
                     Frag y[NP];
 #pragma unroll
-                    for (int p = 0; p < NP; ++p) y[p].u = *reinterpret_cast<const uint4 *>(tr + ((p * KB + k) * 2 + h) * 1024);
+                    for (int p = 0; p < NP; ++p) y[p].u = *reinterpret_cast<const uint4 *>(tr + ((p * G::KB + half * KB + k) * 2 + h) * 1024);
                     out[k] = mfma32<F32>(y[0], z[0], out[k]);
                     if constexpr (F32) {
                         out[k] = mfma32<F32>(y[0], z[NP - 1], out[k]);
@@ -491,9 +495,22 @@ __device__ __forceinline__ void grad_body(const Pass &a, char (*lds)[GradGeo<D, 
                 }
             }
         }
-        buf ^= 1;
+    };
+    // Written out for both buffers, as objects of their own: where one buffer is read and the other filled through the same pointer, the compiler may
+    // wait for the copies before it reads.  (fp32 rows of 256: the second copy would spill, and it does not wait there.)
+    if constexpr (F32 && D == 256) {
+        char *cur = lds0, *next = lds1;
+        for (int64_t s0 = t0; s0 < t1; s0 += ST) {
+            step(s0, cur, next);
+            char *x = cur; cur = next; next = x;
+        }
+    } else {
+        for (int64_t s0 = t0; s0 < t1; s0 += 2 * ST) {
+            step(s0, lds0, lds1);
+            if (s0 + ST < t1) step(s0 + ST, lds1, lds0);
+        }
     }
-    float *dst = a.part + ((size_t)segment * a.part_rows + col) * D + 4 * hi;
+    float *dst = a.part + ((size_t)segment * a.part_rows + col) * D + 32 * KB * half + 4 * hi;
 #pragma unroll
     for (int k = 0; k < KB; ++k)
 #pragma unroll
@@ -504,10 +521,10 @@ __device__ __forceinline__ void grad_body(const Pass &a, char (*lds)[GradGeo<D, 
 }
 
 template <int D, bool F32, bool ITEMS_STAY, bool MASK, bool ENT>
-__global__ __launch_bounds__(256, (GradGeo<D, F32>::WGS)) void grad_kernel(Pass a)
+__global__ __launch_bounds__((GradGeo<D, F32>::NT), (GradGeo<D, F32>::WGS * GradGeo<D, F32>::HS)) void grad_kernel(Pass a, const float *__restrict__ tile_factor)
 {
-    __shared__ __attribute__((aligned(1024))) char lds[2][GradGeo<D, F32>::STAGE];
-    grad_body<D, F32, ITEMS_STAY, MASK, ENT>(a, lds);
+    __shared__ __attribute__((aligned(1024))) char lds0[GradGeo<D, F32>::STAGE], lds1[GradGeo<D, F32>::STAGE];
+    grad_body<D, F32, ITEMS_STAY, MASK, ENT>(a, tile_factor, lds0, lds1);
 }
 
 // segments of a block of 128 columns
@@ -692,10 +709,10 @@ Ws carve(void *ws, int64_t rows, int64_t cat, int d, int dtype, bool mask, int T
 }
 
 template <int D, bool F32, bool ITEMS_STAY>
-void launch_pass(const Pass &p, int pieces, bool mask, bool ent, hipStream_t st)
+void launch_pass(const Pass &p, const float *tile_factor, int pieces, bool mask, bool ent, hipStream_t st)
 {
     const dim3 grid((unsigned)pieces);
-#define RSX_GRAD(M_, E_) hipLaunchKernelGGL((grad_kernel<D, F32, ITEMS_STAY, M_, E_>), grid, dim3(256), 0, st, p)
+#define RSX_GRAD(M_, E_) hipLaunchKernelGGL((grad_kernel<D, F32, ITEMS_STAY, M_, E_>), grid, dim3(GradGeo<D, F32>::NT), 0, st, p, tile_factor)
     if (mask) { if (ent) RSX_GRAD(true, true); else RSX_GRAD(true, false); }
     else { if (ent) RSX_GRAD(false, true); else RSX_GRAD(false, false); }
 #undef RSX_GRAD
@@ -726,20 +743,20 @@ void run(const Args &all, const int64_t *indptr, const int32_t *indices, const W
         hipLaunchKernelGGL((tiles_kernel<D, F32, true>), dim3((unsigned)user_tiles), dim3(256), 0, st, a, w.weight, w.scalars, (uint4 *)w.user_rm, (uint4 *)w.user_t,
                            w.user_factor + k);
         Pass p;
-        p.tile_factor = w.tile_factor; p.top_factor = w.scalars + kTopFactor; p.prm = w.prm; p.bits = w.bits; p.named = w.named; p.coef = w.coef;
+        p.top_factor = w.scalars + kTopFactor; p.prm = w.prm; p.bits = w.bits; p.named = w.named; p.coef = w.coef;
         p.positions = a.rows; p.cat = a.cat; p.T = a.T;
         p.stay = w.user_rm; p.flow = F32 ? w.item_rm : (const char *)a.Q; p.flow_t = w.item_t;
         p.stay_rows = pad; p.flow_tiles = (a.cat + kTile - 1) / kTile; p.flow_valid = a.cat;
         p.part = w.part_p; p.part_rows = pad;
         const int pieces_p = grad_pieces(a.rows, p.flow_tiles, w.wgs, w.st);
-        launch_pass<D, F32, false>(p, pieces_p, indptr != nullptr, a.h != nullptr, st);
+        launch_pass<D, F32, false>(p, w.tile_factor, pieces_p, indptr != nullptr, a.h != nullptr, st);
         hipLaunchKernelGGL((join_rows_kernel<D, F32>), dim3((unsigned)((a.rows * (D / 4) + 255) / 256)), dim3(256), 0, st, a, w.part_p, p.flow_tiles, pieces_p, pad, w.weight,
                            w.scalars + kTopFactor, w.named, (char *)GP + r0 * D * es);
         p.stay = F32 ? w.item_rm : (const char *)a.Q; p.flow = w.user_rm; p.flow_t = w.user_t;
         p.stay_rows = F32 ? w.pad_q : a.cat; p.flow_tiles = user_tiles; p.flow_valid = a.rows;
         p.part = w.part_q + (size_t)k * w.seg_q * w.pad_q * D; p.part_rows = w.pad_q;
         const int pieces_q = grad_pieces(a.cat, user_tiles, w.wgs, w.st);
-        launch_pass<D, F32, true>(p, pieces_q, indptr != nullptr, a.h != nullptr, st);
+        launch_pass<D, F32, true>(p, w.tile_factor, pieces_q, indptr != nullptr, a.h != nullptr, st);
         if (k == 0) { ps.flow_tiles = user_tiles; ps.pieces = pieces_q; }
         ps.last_tiles = user_tiles; ps.last_pieces = pieces_q;
     }
