@@ -25,13 +25,11 @@ namespace {
 using namespace lp;
 
 constexpr int kMaxK = 128;
-#ifndef RSX_LP_UB
-#define RSX_LP_UB(D_, F_) ((D_) * ((F_) ? 2 : 1) <= 256 ? 2 : 1)
-#define RSX_LP_OCC(D_, F_) 2
-#endif
-#ifndef RSX_LP_AHEAD
-#define RSX_LP_AHEAD 2
-#endif
+// Blocks of 32 users a wavefront holds: two in bf16, where an item operand read from LDS then serves two products; one in fp32, where it
+// serves two of the three products anyway, twice the workgroups fill the chip better, and a wavefront leaves registers to spare (1024 x 100K x
+// 128 fp32: 182 us with two, 166 with one; 8192 x 100K x 128 bf16: 493 with two, 520 with one and twice the wavefronts a SIMD)
+constexpr int users_block(bool f32) { return f32 ? 1 : 2; }
+constexpr int kWaves = 2;                // wavefronts a SIMD that the registers are cut for (three: 169 us in fp32)
 constexpr float kNone = -3.0e38f;        // reference of a row that has met no score yet
 constexpr float kLazy = 16.0f;           // a tile's maximum may exceed the reference by this much before the sums are rescaled
 
@@ -113,7 +111,7 @@ template <int D, bool F32>
 struct WideGeo : Geo<D, F32> {
     using G = Geo<D, F32>;
     // 32-user blocks a wavefront holds: their operands take KS * NP * 4 registers each
-    static constexpr int UB = RSX_LP_UB(D, F32), WGU = 128 * UB, OCC = RSX_LP_OCC(D, F32);
+    static constexpr int UB = users_block(F32), WGU = 128 * UB, OCC = kWaves;
     // item tiles of one of the two LDS buffers
     static constexpr int ST = 16384 / G::TILEB >= 4 ? 4 : 16384 / G::TILEB >= 1 ? 16384 / G::TILEB : 1;
 };
@@ -285,7 +283,7 @@ __device__ __forceinline__ void wide_body(const void *__restrict__ P, const char
                 }
             }
             // the tile's operands are read from LDS AHEAD steps before their products
-            constexpr int AHEAD = RSX_LP_AHEAD;
+            constexpr int AHEAD = 2;
             __builtin_amdgcn_sched_group_barrier(0x100, (KS < AHEAD ? KS : AHEAD) * NP, 0);
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
@@ -904,11 +902,11 @@ struct Ws {
     int64_t pass, bytes;      // rows of one pass over the catalog
 };
 
-int wide_users(int d, int dtype) { return 128 * RSX_LP_UB(d, dtype == RSX_F32); }
+int wide_users(int dtype) { return 128 * users_block(dtype == RSX_F32); }
 
 int64_t wide_splits(int64_t rows, int64_t items, int d, int dtype)
 {
-    const int64_t slots = RSX_LP_OCC(d, dtype == RSX_F32) * (int64_t)rsx_num_cus(), ut = (rows + wide_users(d, dtype) - 1) / wide_users(d, dtype), groups = (items + 127) / 128;
+    const int64_t slots = kWaves * (int64_t)rsx_num_cus(), ut = (rows + wide_users(dtype) - 1) / wide_users(dtype), groups = (items + 127) / 128;
     const int64_t s = slots / ut;
     return s < 1 ? 1 : s > groups ? groups : s;
 }
@@ -933,7 +931,7 @@ Ws carve(void *ws, int64_t rows, int64_t items, int d, int dtype, bool mask, int
     w.pass = pass_rows(rows, items);
     const int64_t parts = thin ? thin_groups(items) : wide_splits(w.pass, items, d, dtype);
     // (the last, shorter pass takes more splits over fewer rows: rows x splits never exceeds this)
-    const int64_t cells = thin ? rows * parts : w.pass * parts + RSX_LP_OCC(d, dtype == RSX_F32) * (int64_t)rsx_num_cus() * wide_users(d, dtype);
+    const int64_t cells = thin ? rows * parts : w.pass * parts + kWaves * (int64_t)rsx_num_cus() * wide_users(dtype);
     w.planes = take(!thin && dtype == RSX_F32 ? tiles4 * kTile * (int64_t)d * 4 : 0);
     w.factor = (float *)take(!thin && dtype == RSX_F32 ? tiles4 * 4 : 0);
     w.bits = (uint32_t *)take(mask ? w.pass * mask_words(items) * 4 : 0);
