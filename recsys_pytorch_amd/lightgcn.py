@@ -21,7 +21,7 @@ import torch
 import torch.nn as nn
 
 from .data import csr_to_device
-from .mf import BaseModel, IdsToHost, _get, _pad_dim, device_mask, end_of_epoch, kept_for_matrix
+from .mf import BaseModel, IdsToHost, _get, _pad_dim, device_mask, end_of_epoch, kept_for_matrix, logprobs_in_passes
 
 
 def normalized_adjacency(train_csr):
@@ -218,6 +218,13 @@ class LightGCN(BaseModel):
             S = self._k.score(self._out[:U], self._out[U:], self._idx(batch_users), mask=mask)
             pred_matrix[batch_users] = S.cpu().numpy()
         return pred_matrix
+
+    def predict_logprobs(self, user_ids, items=None, eval_pos=None, K=0, test_batch_size=8192):
+        """as MF.predict_logprobs, of the propagated tables"""
+        if not self._fresh:
+            self.update_lightgcn_embedding()
+        U = self.num_users
+        return logprobs_in_passes(self, self._out[:U], self._out[U:], user_ids, items, eval_pos, K, test_batch_size)
 
     topk_reuse_host = True          # predict_topk takes reuse_host (evaluator.py)
 

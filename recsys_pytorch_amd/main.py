@@ -29,7 +29,8 @@ def main(argv=None):
     ap.add_argument("--model", default="MF", choices=["MF", "LightGCN"])
     ap.add_argument("--hidden-dim", type=int, default=50)           # conf/MF.yaml
     ap.add_argument("--num-layers", type=int, default=2)            # conf/LightGCN.yaml
-    ap.add_argument("--optimizer", default="sgd", choices=["sgd", "adam"])
+    ap.add_argument("--optimizer", default="sgd", choices=["sgd", "adam", "muon"])
+    ap.add_argument("--listwise", action="store_true", help="MF: softmax over the whole catalog instead of BPR")
     ap.add_argument("--lr", type=float, default=None)
     ap.add_argument("--batch-size", type=int, default=256)          # config.py:39
     ap.add_argument("--num-epochs", type=int, default=10)           # config.py:38
@@ -50,7 +51,7 @@ def main(argv=None):
     evaluator = pkg.Evaluator(dataset.valid_input, dataset.valid_target, protocol=dataset.protocol, ks=args.ks)
     if args.model == "MF":
         hparams = {"hidden_dim": args.hidden_dim, "pointwise": False, "loss_func": "ce", "optimizer": args.optimizer,
-                   "seed": args.seed}
+                   "listwise": args.listwise, "seed": args.seed}
     else:
         hparams = {"emb_dim": args.hidden_dim, "num_layers": args.num_layers, "node_dropout": 0.0, "split": False,
                    "num_folds": 100, "reg": 1e-4, "graph_dir": "graph", "seed": args.seed}

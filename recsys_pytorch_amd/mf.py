@@ -13,6 +13,8 @@ storage.  There is no CPU fallback.
 Divergences from the reference, all documented in DESIGN.md:
   * optimizer: hparams['optimizer'] = 'sgd' (default, north star; lr default 0.05) or 'adam'
     (the reference's dense Adam, MF.py:30, reference-exact; lr default 1e-3).
+    or 'muon': one orthogonalised momentum step a table (include/rsx.h: rsx_muon_apply; lr default 0.02), every singular direction of
+    the gradient at the same length; works with every branch below, one GPU.
   * triplets: sampled on the device every step (include/rsx.h:rsx_bpr_sample), true
     BPR sampling, instead of PairwiseGenerator's once-per-fit host sampling with its
     quirks (data/generators.py:165,182-185).  `train_step` replays explicit triplets.
@@ -28,6 +30,11 @@ Divergences from the reference, all documented in DESIGN.md:
     105-130: batch_size interactions of a per-epoch permutation PLUS one uniformly drawn negative, rating 0, for EVERY
     user of the matrix -- its sample_negatives ignores the batch it is handed), assembled on the device; the gradient
     of a batch is rsx_pointwise_grad, the update the as-shipped Adam or the SGD sweep.
+  * hparams['listwise'] = True: the loss of a (user, positive) pair is -log softmax over the WHOLE catalog instead of BPR against one
+    sampled negative, with its exact gradient and without storing a score (include/rsx.h: rsx_score_logprobs, rsx_score_logprobs_grad;
+    BPREngine.listwise_step).  Pairs come from the same sampler, its negatives unused.  Any optimizer; a batch costs
+    4 * batch * items * width multiply-adds in the gradient and that many over four in the loss.
+  * predict_logprobs: the log-probabilities of given items and the K most probable ones, under the same softmax.
   * hparams['chunks'] (default 0 = off): > 1 runs the SGD step as a pipeline over that many item ranges when the blocked
     layout engages (include/rsx.h: "item chunks"; BPREngine.set_chunks): the apply -- and, user-sharded, the exchange --
     of a range travels under the rest of the step kernel; negatives come from the range of the sampled positive.  Which items
@@ -132,6 +139,27 @@ class IdsToHost:
         return self.buf[:self.n].numpy()
 
 
+def logprobs_in_passes(model, P, Q, user_ids, items, eval_pos, K, test_batch_size):
+    """rsx.score_logprobs over a long list of users, `test_batch_size` at a time: its namedtuple with numpy arrays.  items: [n] or
+    [n x T] ids (logp comes in the same shape); eval_pos: the items to leave out of the catalog, by user"""
+    user_ids = np.asarray(user_ids)
+    n = len(user_ids)
+    if items is not None:
+        items = np.asarray(items)
+        if items.ndim not in (1, 2) or items.shape[0] != n:
+            raise ValueError(f"items must be [{n}] or [{n} x T] ids")
+    shape = None if items is None else items.shape
+    mask = device_mask(model, eval_pos)
+    users_dev = model._idx(user_ids)
+    items_dev = None if items is None else model._idx(items.reshape(n, -1) if n else items.reshape(0, 1))
+    parts, step = [], max(1, int(test_batch_size))
+    for s in range(0, max(n, 1), step):
+        parts.append(model._k.score_logprobs(P, Q, users_dev[s:s + step], items_dev[s:s + step] if items_dev is not None else None, K=K, mask=mask))
+    make = type(parts[0])
+    r = make(*(None if f[0] is None else torch.cat(f).cpu().numpy() for f in zip(*parts)))
+    return r if shape is None else r._replace(logp=r.logp.reshape(shape))
+
+
 def _pad_dim(d):
     """the kernels are instantiated for rows of 32, 64, 128 and 256 floats; any other hidden_dim (the reference takes any,
     models/MF.py:19,23-24; conf/MF.yaml ships 50) is stored with zero columns behind it, which provably stay zero"""
@@ -157,6 +185,9 @@ class MF(BaseModel):
         self.num_items = dataset.num_items
         self.hidden_dim = int(hparams["hidden_dim"])
         self.pointwise = bool(hparams["pointwise"])
+        self.listwise = bool(_get(hparams, "listwise", False))
+        if self.listwise and self.pointwise:
+            raise ValueError("pointwise and listwise are two losses: set one")
         self.loss_func = "mse" if _get(hparams, "loss_func", "ce") == "mse" else "ce"          # models/MF.py:21
         opt = _get(hparams, "optimizer", None)
         if opt is None:
@@ -167,10 +198,10 @@ class MF(BaseModel):
                 MF._said_default_optimizer = True
                 print(f"recsys_pytorch_amd.MF: hparams has no 'optimizer' key -> SGD, lr {float(_get(hparams, 'lr', 0.05))} (the MI355X step kernel; "
                       "the reference's own models/MF.py:30 is dense Adam, lr 1e-3: pass hparams['optimizer'] = 'adam' for that)", flush=True)
-        if opt not in ("sgd", "adam"):
-            raise ValueError("optimizer must be 'sgd' (north star) or 'adam' (as shipped, models/MF.py:30)")
+        if opt not in ("sgd", "adam", "muon"):
+            raise ValueError("optimizer must be 'sgd' (north star), 'adam' (as shipped, models/MF.py:30) or 'muon'")
         self.optimizer_name = opt
-        self.lr = float(_get(hparams, "lr", 0.05 if opt == "sgd" else 1e-3))
+        self.lr = float(_get(hparams, "lr", {"sgd": 0.05, "adam": 1e-3, "muon": 0.02}[opt]))
         self.seed = int(_get(hparams, "seed", 2020))
         # item block of the stratified negatives; 0 = independent uniform negatives always
         self.neg_block = int(_get(hparams, "neg_block", 8))
@@ -193,6 +224,8 @@ class MF(BaseModel):
         self.item_embedding.weight.requires_grad_(False)
         self._kernels = kernels
         self._engine = BPREngine(self._P, self._Q, self.lr, kernels=kernels, seed=self.seed, optimizer=opt)
+        if opt == "muon":
+            self._engine.muon_width = self.hidden_dim
         self._engine.redraw_ranges_every = int(_get(hparams, "redraw_ranges_every", self._engine.redraw_ranges_every))
         self._k = self._engine.k
 
@@ -222,6 +255,10 @@ class MF(BaseModel):
             acc = torch.zeros(self._k.RSX_LOSS_SLOTS, dtype=torch.float32, device=self.device)
             self._k.pointwise_grad(self._P, self._Q, None, None, u, i, y, 1.0, loss_func=self.loss_func, loss_acc=acc)
             return acc.sum() / max(1, u.numel())
+        if self.listwise:                        # (the third argument, a sampled negative, is not looked at: every item is one)
+            u = self._idx(users)
+            lp = self._k.score_logprobs(self._P, self._Q, u, self._idx(items).view(-1, 1))
+            return -lp.logp.sum() / max(1, u.numel())
         u, i, j = self._idx(users), self._idx(items), self._idx(ratings)
         acc = torch.zeros(self._k.RSX_LOSS_SLOTS, dtype=torch.float32, device=self.device)
         self._k.bpr_step(self._P, self._Q, None, u, i, j, 0.0, 1.0, loss_acc=acc, no_update=True)
@@ -233,6 +270,10 @@ class MF(BaseModel):
             u, i = self._idx(users), self._idx(pos)
             y = torch.as_tensor(neg).to(device=self.device, dtype=torch.float32).contiguous()
             acc = self._engine.pointwise_step(u, i, y, self.loss_func)
+            return acc.sum() / max(1, u.numel())
+        if self.listwise:                        # (users, positives): both may repeat
+            u = self._idx(users)
+            acc = self._engine.listwise_step(u, self._idx(pos))
             return acc.sum() / max(1, u.numel())
         u, i, j = self._idx(users), self._idx(pos), self._idx(neg)
         acc = self._engine.step(u, i, j, users_unique=users_unique)
@@ -254,7 +295,7 @@ class MF(BaseModel):
         # (data/generators.py:182-195); the last batch of an epoch is short, not dropped (:213)
         n_data = self.num_users
         num_batches = int(np.ceil(n_data / batch_size))
-        if self.optimizer_name == "sgd":     # on-chip gradient summation when batch >= 2 * items
+        if self.optimizer_name == "sgd" and not self.listwise:     # on-chip gradient summation when batch >= 2 * items
             nb = self._engine.set_neg_block(batch_size if self.neg_block > 0 else 0, max(self.neg_block, 1), self.neg_block_min)
             if self.hot_items > 0 and hasattr(self._k, "HotItems"):
                 hot_for = getattr(self, "_hot_for", None)           # (the same matrix, the same kernel family: the replica tables of the last fit stand)
@@ -266,7 +307,7 @@ class MF(BaseModel):
         scores = None
         # SGD on the HIP library: the batch loop itself is native (include/rsx.h: rsx_bpr_trainer_run),
         # Python is re-entered once per epoch (or every 50 batches when verbose, for the progress line)
-        native = self.optimizer_name == "sgd" and hasattr(self._k, "BPRTrainer")
+        native = self.optimizer_name == "sgd" and not self.listwise and hasattr(self._k, "BPRTrainer")
         acc = torch.zeros(self._k.RSX_LOSS_SLOTS, dtype=torch.float32, device=self.device)
         trainer = self._engine.native_trainer(indptr, indices, batch_size, loss_acc=acc) if native else None
         for epoch in range(1, num_epochs + 1):
@@ -298,7 +339,11 @@ class MF(BaseModel):
                     trainer = self._engine.native_trainer(indptr, indices, batch_size, loss_acc=acc)
             for b in range(num_batches if not native else 0):
                 bsz = min(batch_size, n_data - b * batch_size)
-                step_acc = self._engine.sampled_step(indptr, indices, bsz)
+                if self.listwise:
+                    u, i, _ = self._engine.sample(indptr, indices, bsz)
+                    step_acc = self._engine.listwise_step(u, i)
+                else:
+                    step_acc = self._engine.sampled_step(indptr, indices, bsz)
                 batch_loss = step_acc.sum() / bsz
                 epoch_loss += batch_loss
                 if verbose and b % 50 == 0:
@@ -378,6 +423,12 @@ class MF(BaseModel):
             S = self._k.score(self._P, self._Q, self._idx(batch_users), mask=mask)
             pred_matrix[batch_users] = S.cpu().numpy()       # rows indexed by USER ID (MF.py:128)
         return pred_matrix
+
+    # -- probabilities under the softmax over the catalog: no [U x I] matrix on either side ------------
+    def predict_logprobs(self, user_ids, items=None, eval_pos=None, K=0, test_batch_size=8192):
+        """log-probabilities of `items` ([n] or [n x T] ids, one row a user) under softmax(P Q^T) over the catalog without the user's
+        items in eval_pos, log-normaliser and entropy of every user, the K most probable items: rsx.LogProbs of numpy arrays"""
+        return logprobs_in_passes(self, self._P, self._Q, user_ids, items, eval_pos, K, test_batch_size)
 
     # -- the large-catalog twin: only [n x K] indices leave the device -----------------------------
     topk_reuse_host = True          # predict_topk takes reuse_host (evaluator.py)

@@ -153,10 +153,20 @@ class BPREngine:
         self.optimizer = optimizer
         self.GP = None              # dense user-gradient buffer: Adam, and the pointwise branch (allocated on first use)
         self._pw_t = 0              # Adam's step count on the pointwise branch
+        self._lw_t = 0              # and on the listwise one
+        self._lw = None             # scratch of the listwise branch
         if optimizer == "adam":      # the reference's shipped optimizer (models/MF.py:30): dense moments
             self.GP = torch.zeros_like(P_local)
             self.mP, self.vP = torch.zeros_like(P_local), torch.zeros_like(P_local)
             self.mQ, self.vQ = torch.zeros_like(Q), torch.zeros_like(Q)
+        elif optimizer == "muon":    # orthogonalised updates of whole tables (include/rsx.h: rsx_muon_apply): dense momentum
+            if self.sharded:
+                raise ValueError("optimizer='muon' runs on one GPU: the user table's update needs all of its rows")
+            self.GP = torch.zeros_like(P_local)
+            self.mP, self.mQ = torch.zeros_like(P_local), torch.zeros_like(Q)
+            self.muon = {"momentum": 0.95, "nesterov": True, "steps": 5, "weight_decay": 0.0}
+            self.muon_width = P_local.shape[1]       # columns in use (MF sets hidden_dim: padded ones are zero and stay so)
+            self._muon_ws = None
         elif optimizer != "sgd":
             raise ValueError(optimizer)
         # how the ranks exchange the item gradients of a step:
@@ -543,7 +553,7 @@ class BPREngine:
         if want_loss:
             loss = self._loss
             loss.zero_()
-        if self.optimizer == "adam":
+        if self.optimizer in ("adam", "muon"):
             if B > 0:
                 self.k.bpr_grad(self.P, self.Q, self.GP, self.G, u_local, i, j, 1.0 / gb, loss_acc=loss)
             if self.sharded:
@@ -551,8 +561,7 @@ class BPREngine:
                 if want_loss:
                     dist.all_reduce(loss, op=dist.ReduceOp.SUM, group=self.group)
             self.step_count += 1
-            self.k.adam_apply(self.Q, self.mQ, self.vQ, self.G, self.lr, self.step_count)
-            self.k.adam_apply(self.P, self.mP, self.vP, self.GP, self.lr, self.step_count)
+            self._apply_dense(self.step_count)
             return loss
         kw = {"hot": self.hot} if self.hot is not None else {}
         if neg_block:
@@ -613,12 +622,51 @@ class BPREngine:
         if count_step:
             self.step_count += 1
         self._pw_t += 1
+        self._apply_dense(self._pw_t)
+        return loss
+
+    def _apply_dense(self, t):
+        """the optimizer's step t over both tables from the dense gradients GP and G, which are zero after it"""
         if self.optimizer == "adam":
-            self.k.adam_apply(self.Q, self.mQ, self.vQ, self.G, self.lr, self._pw_t)
-            self.k.adam_apply(self.P, self.mP, self.vP, self.GP, self.lr, self._pw_t)
+            self.k.adam_apply(self.Q, self.mQ, self.vQ, self.G, self.lr, t)
+            self.k.adam_apply(self.P, self.mP, self.vP, self.GP, self.lr, t)
+        elif self.optimizer == "muon":
+            if self._muon_ws is None:
+                need = max(self.k.orthogonalize_workspace(*T.shape) for T in (self.P, self.Q))
+                self._muon_ws = torch.empty(need, dtype=torch.uint8, device=self.Q.device)
+            for W, M, G in ((self.Q, self.mQ, self.G), (self.P, self.mP, self.GP)):
+                self.k.muon_apply(W, M, G, self.lr, update_scale=max(1.0, W.shape[0] / self.muon_width) ** 0.5, ws=self._muon_ws, **self.muon)
         else:
             self.k.apply_item_grad(self.Q, self.G, self.lr)      # table-agnostic sweep: theta -= lr * grad; grad = 0
             self.k.apply_item_grad(self.P, self.GP, self.lr)
+
+    # -- one step of the LISTWISE branch: softmax over the whole catalog (include/rsx.h: rsx_score_logprobs) -----------
+    def listwise_step(self, u, i, count_step=True):
+        """(user, item) batch, users and items may repeat: the loss is -log softmax(P[u] Q^T)[i] against ALL items instead of one
+        sampled negative, summed into the loss slots; its gradient over both tables (every item has one), then the optimizer's step.
+        The scores are never stored.  An entry with an item outside the catalog adds nothing (a user without interactions in a sampled
+        batch).  One GPU."""
+        if self.sharded:
+            raise ValueError("the listwise branch runs on one GPU")
+        if self.GP is None:
+            self.GP = torch.zeros_like(self.P)
+        loss = self._loss
+        loss.zero_()
+        n = int(u.numel())
+        if n > 0:
+            need = max(self.k.score_logprobs_workspace(n, *self.Q.shape), self.k.score_logprobs_grad_workspace(n, *self.Q.shape))
+            if self._lw is None or self._lw["ws"].numel() < need or self._lw["rows"].shape[0] < n:
+                self._lw = None
+                self._lw = {"ws": torch.empty(need, dtype=torch.uint8, device=self.Q.device), "rows": torch.empty(n, self.P.shape[1], device=self.P.device)}
+            ws, rows, i = self._lw["ws"], self._lw["rows"][:n], i.view(n, 1)
+            lp = self.k.score_logprobs(self.P, self.Q, u, i, ws=ws)
+            loss[0] = -lp.logp.sum()
+            self.k.score_logprobs_grad(self.P, self.Q, u, i, lp.lse, torch.full_like(lp.logp, -1.0 / n), out=(rows, self.G), ws=ws)
+            self.k.add_rows(self.GP, u, rows)
+        if count_step:
+            self.step_count += 1
+        self._lw_t += 1
+        self._apply_dense(self._lw_t)
         return loss
 
     # -- one step on triplets sampled on the device from this rank's CSR rows -----------
@@ -733,7 +781,7 @@ class BPREngine:
         between kernels.  When sharded, the exchange is
         this engine's all-reduce(G) handed in as a pair of callbacks.  SGD only."""
         if self.optimizer != "sgd":
-            raise ValueError("the native loop runs the SGD step; optimizer='adam' steps through BPREngine.step")
+            raise ValueError("the native loop runs the SGD step; the others step through BPREngine.step")
         batch = min(int(batch), indptr.numel() - 1)
         native = self.sharded and self.comm is not None and self.exchange != "direct"      # the library issues the exchange itself (RCCL)
         kind = {"allreduce": 1, "scatter_gather": 2}[self.exchange] if native else 0      # RSX_EXCHANGE_*
