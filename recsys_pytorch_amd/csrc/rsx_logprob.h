@@ -116,11 +116,6 @@ __device__ __forceinline__ void split8_times(const float *x, double k, Frag *hi,
 // rows of the call: a position whose user id is outside the table names no row
 __device__ __forceinline__ bool row_ok(int32_t u, int64_t num_users) { return u >= 0 && u < num_users; }
 
-static __global__ __launch_bounds__(256) void fill_u32_kernel(uint4 *__restrict__ p, int64_t n16, uint32_t v)
-{
-    for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < n16; t += (int64_t)gridDim.x * 256) p[t] = make_uint4(v, v, v, v);
-}
-
 // words a row of the bit mask holds: four tiles of 32 items at a time
 __host__ __device__ __forceinline__ int64_t mask_words(int64_t num_items) { return (num_items + 127) / 128 * 4; }
 
@@ -147,23 +142,13 @@ __device__ __forceinline__ void write_seen_bits(int32_t u, bool ok, const int64_
     }
 }
 
-static __global__ __launch_bounds__(256) void seen_bits_kernel(const int32_t *__restrict__ user_ids, int64_t num_users, const int64_t *__restrict__ indptr,
-                                                               const int32_t *__restrict__ indices, int64_t num_items, uint32_t *__restrict__ bits)
-{
-    __shared__ __attribute__((aligned(16))) uint32_t lds[kBitWords];
-    const int32_t u = user_ids[blockIdx.x];
-    write_seen_bits(u, row_ok(u, num_users), indptr, indices, num_items, bits + (size_t)blockIdx.x * mask_words(num_items), lds);
-}
-
-// fp32 item rows -> scaled planes [tiles padded to a multiple of 4][32][hi d, lo d] and a factor per tile.  One workgroup per tile.
+// a tile of fp32 item rows -> scaled planes [tiles padded to a multiple of 4][32][hi d, lo d] and the tile's factor, by 256 threads.
 // Rows behind the last item are zero.
 template <int D>
-__global__ __launch_bounds__(256) void split_items_kernel(const float *__restrict__ Q, int64_t num_items, uint4 *__restrict__ planes, float *__restrict__ factor)
+__device__ __forceinline__ void split_items(const float *__restrict__ Q, int64_t num_items, int64_t tile, uint4 *__restrict__ planes, float *__restrict__ factor, float *s_max)
 {
     constexpr int TPR = D / 8, RPP = 256 / TPR, N = kTile / RPP > 0 ? kTile / RPP : 1;       // threads a row, rows a pass, passes
-    __shared__ float s_max[4];
     const int tid = threadIdx.x;
-    const int64_t tile = blockIdx.x;
     float x[N][8];
     float m = 0.0f;
 #pragma unroll

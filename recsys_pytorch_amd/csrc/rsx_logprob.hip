@@ -81,9 +81,8 @@ __device__ __forceinline__ void load8(const void *base, int64_t at, float *x)
 // the reference a row's chunk maxima are stored against: a score of its own, so that an offset common to a row's scores does not eat the halves'
 // eleven bits.  One wavefront per row.
 template <int D, bool F32>
-__global__ __launch_bounds__(256) void reference_kernel(const void *__restrict__ P, const void *__restrict__ Q, Shape sh, float *__restrict__ ref)
+__device__ __forceinline__ void row_reference(const void *__restrict__ P, const void *__restrict__ Q, const Shape &sh, int64_t r, float *__restrict__ ref)
 {
-    const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
     if (r >= sh.rows) return;
     const int32_t u = sh.user_ids[r];
@@ -104,6 +103,28 @@ __global__ __launch_bounds__(256) void reference_kernel(const void *__restrict__
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) d[n] += __shfl_xor(d[n], o, 64);
     if (lane == 0) ref[r] = sh.scale * kLog2e * pick_reference(d[0], d[1], d[2]);
+}
+
+// what the pass needs, in one launch: workgroups [0, tiles) split the item tiles (fp32), the next bit_rows write a row's seen bits each, the rest
+// the references of four rows each.  (As three launches: 943 x 1682 x 64 took 5 us longer, of 50.)
+template <int D, bool F32>
+__global__ __launch_bounds__(256) void prepare_kernel(const void *__restrict__ P, const void *__restrict__ Q, Shape sh, const int64_t *__restrict__ indptr,
+                                                      const int32_t *__restrict__ indices, int64_t tiles, int64_t bit_rows, uint4 *__restrict__ planes, float *__restrict__ factor,
+                                                      uint32_t *__restrict__ bits, float *__restrict__ ref)
+{
+    __shared__ __attribute__((aligned(16))) uint32_t lds[kBitWords];
+    int64_t at = blockIdx.x;
+    if (at < tiles) {
+        if constexpr (F32) split_items<D>((const float *)Q, sh.items, at, planes, factor, reinterpret_cast<float *>(lds));
+        return;
+    }
+    at -= tiles;
+    if (at < bit_rows) {
+        const int32_t u = sh.user_ids[at];
+        write_seen_bits(u, row_ok(u, sh.users), indptr, indices, sh.items, bits + (size_t)at * mask_words(sh.items), lds);
+        return;
+    }
+    row_reference<D, F32>(P, Q, sh, (at - bit_rows) * 4 + (threadIdx.x >> 6), ref);
 }
 
 // ---- many rows ------------------------------------------------------------------------------------------------------------------------
@@ -967,15 +988,15 @@ template <int D, bool F32>
 void run(const Call &c, const Ws &w, hipStream_t st)
 {
     const bool thin = c.sh.rows <= thin_rows(D, F32 ? RSX_F32 : RSX_BF16);
-    const int64_t items = c.sh.items, tiles4 = (items + 127) / 128 * 4;
-    if constexpr (F32)
-        if (!thin) hipLaunchKernelGGL(split_items_kernel<D>, dim3((unsigned)tiles4), dim3(256), 0, st, (const float *)c.Q, items, (uint4 *)w.planes, w.factor);
+    const int64_t items = c.sh.items;
     for (int64_t r0 = 0; r0 < c.sh.rows; r0 += w.pass) {
         Shape sh = c.sh;
         sh.user_ids += r0;
         sh.rows = c.sh.rows - r0 < w.pass ? c.sh.rows - r0 : w.pass;
-        if (c.indptr) hipLaunchKernelGGL(seen_bits_kernel, dim3((unsigned)sh.rows), dim3(256), 0, st, sh.user_ids, sh.users, c.indptr, c.indices, items, w.bits);
-        if (c.K) hipLaunchKernelGGL((reference_kernel<D, F32>), dim3((unsigned)((sh.rows + 3) / 4)), dim3(256), 0, st, c.P, c.Q, sh, w.ref);
+        const int64_t tiles = F32 && !thin && r0 == 0 ? (items + 127) / 128 * 4 : 0, bit_rows = c.indptr ? sh.rows : 0, refs = c.K ? (sh.rows + 3) / 4 : 0;
+        if (tiles + bit_rows + refs > 0)
+            hipLaunchKernelGGL((prepare_kernel<D, F32>), dim3((unsigned)(tiles + bit_rows + refs)), dim3(256), 0, st, c.P, c.Q, sh, c.indptr, c.indices, tiles, bit_rows,
+                               (uint4 *)w.planes, w.factor, w.bits, w.ref);
         int parts;
         if (thin) {
             parts = thin_groups(items);

@@ -3,7 +3,7 @@
 //   dz_ri = scale (sum_t g_rt [i = items_rt] - p_ri (sum_t g_rt + h_r (log p_ri + H_r))),   p_ri = exp(z_ri - lse_r)
 //   GP_r = sum_i dz_ri Q_i,   GQ_i = sum_r dz_ri P_r
 //
-// Neither the scores nor dz exist in memory.  Two launches of one kernel, each recomputing the scores it needs:
+// Neither the scores nor dz exist in memory.  Two passes of one kernel, each recomputing the scores it needs:
 //   users stay, items stream   -> GP: the p part; the T rows of Q that the positions name are added when the partial sums are joined
 //   items stay, users stream   -> GQ, with the named items inside the tile
 // A wavefront keeps 32 columns (users or items) in registers: their operands for the scores and their d sums of the gradient.  Tiles of 32
@@ -28,7 +28,7 @@ using namespace lp;
 
 constexpr float kFar = 1.0e30f;           // log-normaliser of a row without probabilities: every p is 0
 constexpr float kLift = 4096.0f;          // dz of fp32 tables is held times 2^12
-constexpr int kTopFactor = 16;            // where the largest item factor is kept among the scalars ([0]: the largest w |P| of a pass)
+constexpr int kLargest = 1;               // scalars: [0] the largest item factor, [kLargest + k] the largest w |P| of pass k
 
 struct Args {
     const void *P, *Q;
@@ -51,7 +51,7 @@ struct Prm {
 // workgroup: a thousand on one word take 12 us).  The first workgroup also finds the largest item factor.
 template <int D, bool F32>
 __global__ __launch_bounds__(256) void rows_kernel(Args a, const uint32_t *__restrict__ bits, int64_t padded, Prm *__restrict__ prm, float *__restrict__ weight, int32_t *__restrict__ named,
-                                                   float *__restrict__ coef, uint32_t *__restrict__ scalars, const float *__restrict__ item_factor, int64_t item_tiles)
+                                                   float *__restrict__ coef, uint32_t *__restrict__ top_factor, uint32_t *__restrict__ largest, const float *__restrict__ item_factor, int64_t item_tiles)
 {
     __shared__ float s_max[4];
     const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
@@ -62,7 +62,7 @@ __global__ __launch_bounds__(256) void rows_kernel(Args a, const uint32_t *__res
         for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
         if (lane == 0) s_max[wid] = m;
         __syncthreads();
-        if (threadIdx.x == 0) scalars[kTopFactor] = __float_as_uint(fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3])));
+        if (threadIdx.x == 0) *top_factor = __float_as_uint(fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3])));
         __syncthreads();
     }
     float most = 0.0f;
@@ -127,7 +127,7 @@ __global__ __launch_bounds__(256) void rows_kernel(Args a, const uint32_t *__res
     if constexpr (F32) {
         if (lane == 0) s_max[wid] = most;
         __syncthreads();
-        if (threadIdx.x == 0) atomicMax(scalars, __float_as_uint(fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]))));
+        if (threadIdx.x == 0) atomicMax(largest, __float_as_uint(fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]))));
     }
 }
 
@@ -136,18 +136,23 @@ __global__ __launch_bounds__(256) void rows_kernel(Args a, const uint32_t *__res
 template <int D>
 __device__ __forceinline__ int tile_row(int half, int hi, int j) { const int i = 8 * half + j; return (i & 3) + 8 * (i >> 2) + 4 * hi; }
 
-// one workgroup per tile of 32 rows: row-major planes and the transposed tile.  USERS: rows gathered by user id, each times scale log2 e and with its own
+// a tile of 32 rows by 256 threads: row-major planes and the transposed tile.  USERS: rows gathered by user id, each times scale log2 e and with its own
 // power of two in the row-major planes, times its weight and one common scale in the transposed ones.  Items: the tile's scale in both.
+template <int D, bool F32>
+struct TileLds {
+    typename std::conditional<F32, float, uint16_t>::type x[kTile][D + 1];
+    float max[4], mul[kTile];
+};
+
 template <int D, bool F32, bool USERS>
-__global__ __launch_bounds__(256) void tiles_kernel(Args a, const float *__restrict__ weight, const uint32_t *__restrict__ largest, uint4 *__restrict__ rowm,
-                                                    uint4 *__restrict__ tr, float *__restrict__ factor)
+__device__ __forceinline__ void lay_tile(const Args &a, int64_t tile, const float *__restrict__ weight, const uint32_t *__restrict__ largest, uint4 *__restrict__ rowm,
+                                         uint4 *__restrict__ tr, float *__restrict__ factor, TileLds<D, F32> &lds)
 {
-    constexpr int TPR = D / 8, LD = D + 1;
-    using S = typename std::conditional<F32, float, uint16_t>::type;
-    __shared__ S x[kTile][LD];
-    __shared__ float s_max[4], s_mul[kTile];
+    constexpr int TPR = D / 8;
+    auto &x = lds.x;
+    float *const s_max = lds.max, *const s_mul = lds.mul;
     const int tid = threadIdx.x;
-    const int64_t tile = blockIdx.x, n = USERS ? a.rows : a.cat;
+    const int64_t n = USERS ? a.rows : a.cat;
     float m = 0.0f;
     for (int t = tid; t < kTile * TPR; t += 256) {
         const int r = t / TPR, c = 8 * (t % TPR);
@@ -242,6 +247,32 @@ __global__ __launch_bounds__(256) void tiles_kernel(Args a, const float *__restr
     }
 }
 
+// everything before the positions' coefficients, in one launch: workgroups [0, tiles) lay out the item tiles (in the first pass, the first of them also clears
+// the maxima that rows_kernel fills), the rest write a position's seen bits each
+template <int D, bool F32>
+__global__ __launch_bounds__(256) void items_kernel(Args a, const int64_t *__restrict__ indptr, const int32_t *__restrict__ indices, int64_t tiles, uint4 *__restrict__ rowm,
+                                                    uint4 *__restrict__ tr, float *__restrict__ factor, uint32_t *__restrict__ bits, uint32_t *__restrict__ largest, int64_t passes)
+{
+    __shared__ __attribute__((aligned(16))) union { TileLds<D, F32> tile; uint32_t bits[kBitWords]; } lds;
+    const int64_t at = blockIdx.x;
+    if (at < tiles) {
+        if (at == 0)
+            for (int64_t k = threadIdx.x; k < passes; k += 256) largest[k] = 0u;
+        lay_tile<D, F32, false>(a, at, nullptr, nullptr, rowm, tr, factor, lds.tile);
+        return;
+    }
+    const int32_t u = a.user_ids[at - tiles];
+    write_seen_bits(u, row_ok(u, a.users), indptr, indices, a.cat, bits + (size_t)(at - tiles) * mask_words(a.cat), lds.bits);
+}
+
+template <int D, bool F32>
+__global__ __launch_bounds__(256) void users_kernel(Args a, const float *__restrict__ weight, const uint32_t *__restrict__ largest, uint4 *__restrict__ rowm, uint4 *__restrict__ tr,
+                                                    float *__restrict__ factor)
+{
+    __shared__ __attribute__((aligned(16))) TileLds<D, F32> lds;
+    lay_tile<D, F32, true>(a, blockIdx.x, weight, largest, rowm, tr, factor, lds);
+}
+
 // ---- the pass -------------------------------------------------------------------------------------------------------------------------
 struct Pass {
     const char *stay, *flow;              // row-major planes of what stays in registers and of what streams
@@ -258,6 +289,7 @@ struct Pass {
     int T;
     float *part;                          // [segments][padded rows that stay][d]
     int64_t part_rows;
+    int pieces;                           // workgroups of this pass
 };
 
 // The work of a pass is a line of (block of 128 columns, streaming tile) cut into equal pieces, one per workgroup of a full device: no ragged last
@@ -280,14 +312,14 @@ struct GradGeo : Geo<D, F32> {
 };
 
 template <int D, bool F32, bool ITEMS_STAY, bool MASK, bool ENT>
-__device__ __forceinline__ void grad_body(const Pass &a, const float *__restrict__ tile_factor, char *lds0, char *lds1)
+__device__ __forceinline__ void grad_body(const Pass &a, int64_t piece, const float *__restrict__ tile_factor, char *lds0, char *lds1)
 {
     using G = GradGeo<D, F32>;
     constexpr int KS = G::KS, NP = G::NP, ST = G::ST, KB = G::KB / G::HS;              // KB: this wavefront's blocks of 32 elements
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wid = wave & 3, half = wave >> 2, hi = lane >> 5, l31 = lane & 31;
     const int64_t total = a.part_rows / 128 * a.flow_tiles;
-    int64_t at = piece_begin(total, gridDim.x, blockIdx.x);
-    const int64_t end = piece_begin(total, gridDim.x, blockIdx.x + 1);
+    int64_t at = piece_begin(total, a.pieces, piece);
+    const int64_t end = piece_begin(total, a.pieces, piece + 1);
     const float top = F32 ? __uint_as_float(*a.top_factor) : 1.0f;
     const int64_t words = mask_words(a.cat);
     const int sw = G::swz(l31) * 16;
@@ -338,7 +370,7 @@ __device__ __forceinline__ void grad_body(const Pass &a, const float *__restrict
     while (at < end) {
     const int64_t block = at / a.flow_tiles, t0 = at - block * a.flow_tiles;                        // this segment: tiles [t0, t1) of a block
     const int64_t t1 = end - at < a.flow_tiles - t0 ? t0 + (end - at) : a.flow_tiles;
-    const int64_t segment = blockIdx.x - piece_of(total, gridDim.x, block * a.flow_tiles);
+    const int64_t segment = piece - piece_of(total, a.pieces, block * a.flow_tiles);
     const int64_t col = block * 128 + wid * 32 + l31;                                                // this lane's column
     const int64_t colc = col < a.stay_rows ? col : a.stay_rows - 1;
     const int32_t my_block = (int32_t)(block * 4 + wid);                                             // items stay: the block of 32 this wavefront holds
@@ -522,11 +554,13 @@ __device__ __forceinline__ void grad_body(const Pass &a, const float *__restrict
     }
 }
 
-template <int D, bool F32, bool ITEMS_STAY, bool MASK, bool ENT>
-__global__ __launch_bounds__((GradGeo<D, F32>::NT), (GradGeo<D, F32>::WGS * GradGeo<D, F32>::HS)) void grad_kernel(Pass a, const float *__restrict__ tile_factor)
+// both passes in one launch, the users' first: neither waits for the other's last workgroups (256 x 1682 x 64: 9.6 us for 17 in two)
+template <int D, bool F32, bool MASK, bool ENT>
+__global__ __launch_bounds__((GradGeo<D, F32>::NT), (GradGeo<D, F32>::WGS * GradGeo<D, F32>::HS)) void grad_kernel(Pass p, Pass q, const float *__restrict__ tile_factor)
 {
     __shared__ __attribute__((aligned(1024))) char lds0[GradGeo<D, F32>::STAGE], lds1[GradGeo<D, F32>::STAGE];
-    grad_body<D, F32, ITEMS_STAY, MASK, ENT>(a, tile_factor, lds0, lds1);
+    if ((int)blockIdx.x < p.pieces) grad_body<D, F32, false, MASK, ENT>(p, blockIdx.x, tile_factor, lds0, lds1);
+    else grad_body<D, F32, true, MASK, ENT>(q, blockIdx.x - p.pieces, tile_factor, lds0, lds1);
 }
 
 // segments of a block of 128 columns
@@ -539,10 +573,10 @@ __device__ __forceinline__ int segments_of(int64_t block, int64_t flow_tiles, in
 // ---- the partial sums -> the gradients ------------------------------------------------------------------------------------------------------
 // GP: four elements a thread; the partials in order, the row's weight, the named rows of Q
 template <int D, bool F32>
-__global__ __launch_bounds__(256) void join_rows_kernel(Args a, const float *__restrict__ part, int64_t flow_tiles, int pieces, int64_t part_rows, const float *__restrict__ weight,
+__device__ __forceinline__ void join_rows(int64_t t, const Args &a, const float *__restrict__ part, int64_t flow_tiles, int pieces, int64_t part_rows, const float *__restrict__ weight,
                                                         const uint32_t *__restrict__ top_factor, const int32_t *__restrict__ named, void *__restrict__ GP)
 {
-    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x, r = t / (D / 4);
+    const int64_t r = t / (D / 4);
     const int c = 4 * (int)(t % (D / 4));
     if (r >= a.rows) return;
     float s[4] = {0.f, 0.f, 0.f, 0.f};
@@ -578,10 +612,10 @@ struct Passes {
     int64_t stride;                       // elements of a pass' partial sums
 };
 template <int D, bool F32>
-__global__ __launch_bounds__(256) void join_items_kernel(int64_t cat, const float *__restrict__ part, Passes ps, int64_t part_rows, const float *__restrict__ factor,
-                                                         float scale, void *__restrict__ GQ)
+__device__ __forceinline__ void join_items(int64_t t, int64_t cat, const float *__restrict__ part, const Passes &ps, int64_t part_rows, const float *__restrict__ factor,
+                                           float scale, void *__restrict__ GQ)
 {
-    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x, r = t / (D / 4);
+    const int64_t r = t / (D / 4);
     const int c = 4 * (int)(t % (D / 4));
     if (r >= cat) return;
     float s[4] = {0.f, 0.f, 0.f, 0.f};
@@ -597,6 +631,16 @@ __global__ __launch_bounds__(256) void join_items_kernel(int64_t cat, const floa
     }
     if constexpr (F32) *reinterpret_cast<float4 *>((float *)GQ + r * D + c) = make_float4(s[0], s[1], s[2], s[3]);
     else *reinterpret_cast<ushort4 *>((uint16_t *)GQ + r * D + c) = make_ushort4(f32_bf16(s[0]), f32_bf16(s[1]), f32_bf16(s[2]), f32_bf16(s[3]));
+}
+
+// workgroups [0, row_wgs): GP; the rest (after the last pass): GQ
+template <int D, bool F32>
+__global__ __launch_bounds__(256) void join_kernel(Args a, Pass p, const float *__restrict__ weight, void *__restrict__ GP, int64_t row_wgs, Passes ps, const float *__restrict__ part_q,
+                                                   int64_t pad_q, const float *__restrict__ user_factor, void *__restrict__ GQ)
+{
+    const int64_t at = blockIdx.x;
+    if (at < row_wgs) join_rows<D, F32>(at * 256 + threadIdx.x, a, p.part, p.flow_tiles, p.pieces, p.part_rows, weight, p.top_factor, p.named, GP);
+    else join_items<D, F32>((at - row_wgs) * 256 + threadIdx.x, a.cat, part_q, ps, pad_q, user_factor, a.scale, GQ);
 }
 
 // ---- T[ids[r]] += R[r] in the order of r -----------------------------------------------------------------------------------------------
@@ -637,7 +681,7 @@ __global__ __launch_bounds__(256) void add_rows_kernel(float *__restrict__ T, in
 struct Ws {
     char *user_rm, *user_t, *item_rm, *item_t;
     float *tile_factor, *user_factor, *weight, *coef, *part_p, *part_q;
-    uint32_t *scalars;                    // [0] largest w |P| (per pass), [kTopFactor] largest item factor
+    uint32_t *scalars;
     Prm *prm;
     int32_t *named;
     uint32_t *bits;
@@ -702,7 +746,7 @@ Ws carve(void *ws, int64_t rows, int64_t cat, int d, int dtype, bool mask, int T
     w.coef = (float *)take(w.pass * T * 4);
     w.named = (int32_t *)take(w.pass * T * 4);
     w.prm = (Prm *)take(user_tiles * (int64_t)sizeof(Prm));
-    w.scalars = (uint32_t *)take(256);
+    w.scalars = (uint32_t *)take((kLargest + w.passes) * 4);
     w.bits = (uint32_t *)take(mask ? w.pass * mask_words(cat) * 4 : 0);
     w.part_p = (float *)take(cells * d * 4);
     w.part_q = (float *)take(w.passes * w.seg_q * w.pad_q * d * 4);
@@ -710,25 +754,11 @@ Ws carve(void *ws, int64_t rows, int64_t cat, int d, int dtype, bool mask, int T
     return w;
 }
 
-template <int D, bool F32, bool ITEMS_STAY>
-void launch_pass(const Pass &p, const float *tile_factor, int pieces, bool mask, bool ent, hipStream_t st)
-{
-    const dim3 grid((unsigned)pieces);
-#define RSX_GRAD(M_, E_) hipLaunchKernelGGL((grad_kernel<D, F32, ITEMS_STAY, M_, E_>), grid, dim3(GradGeo<D, F32>::NT), 0, st, p, tile_factor)
-    if (mask) { if (ent) RSX_GRAD(true, true); else RSX_GRAD(true, false); }
-    else { if (ent) RSX_GRAD(false, true); else RSX_GRAD(false, false); }
-#undef RSX_GRAD
-}
-
 template <int D, bool F32>
 void run(const Args &all, const int64_t *indptr, const int32_t *indices, const Ws &w, void *GP, void *GQ, hipStream_t st)
 {
-    const int64_t item_tiles = w.pad_q / kTile;
     const int es = F32 ? 4 : 2;
     Passes ps{0, 0, (int)w.passes, 0, 0, w.seg_q * w.pad_q * D};
-    hipLaunchKernelGGL(fill_u32_kernel, dim3(1), dim3(256), 0, st, (uint4 *)w.scalars, 16, 0u);
-    hipLaunchKernelGGL((tiles_kernel<D, F32, false>), dim3((unsigned)item_tiles), dim3(256), 0, st, all, (const float *)nullptr, (const uint32_t *)nullptr,
-                       (uint4 *)w.item_rm, (uint4 *)w.item_t, w.tile_factor);
     for (int64_t k = 0; k < w.passes; ++k) {
         Args a = all;
         const int64_t r0 = k * w.pass;
@@ -736,33 +766,37 @@ void run(const Args &all, const int64_t *indptr, const int32_t *indices, const W
         a.user_ids += r0; a.lse += r0; a.g += r0 * a.T; a.items += r0 * a.T;
         if (a.ent) a.ent += r0;
         if (a.h) a.h += r0;
-        const int64_t pad = pad128(a.rows), user_tiles = pad / kTile;
-        if (k > 0) hipLaunchKernelGGL(fill_u32_kernel, dim3(1), dim3(256), 0, st, (uint4 *)w.scalars, 1, 0u);
-        if (indptr) hipLaunchKernelGGL(seen_bits_kernel, dim3((unsigned)a.rows), dim3(256), 0, st, a.user_ids, a.users, indptr, indices, a.cat, w.bits);
+        uint32_t *const largest = w.scalars + kLargest;
+        const int64_t pad = pad128(a.rows), user_tiles = pad / kTile, item_tiles = k == 0 ? w.pad_q / kTile : 0, bit_rows = indptr ? a.rows : 0;
+        if (item_tiles + bit_rows > 0)
+            hipLaunchKernelGGL((items_kernel<D, F32>), dim3((unsigned)(item_tiles + bit_rows)), dim3(256), 0, st, a, indptr, indices, item_tiles, (uint4 *)w.item_rm, (uint4 *)w.item_t,
+                               w.tile_factor, w.bits, largest, w.passes);
         const int64_t row_wgs = pad / 4 < 2 * (int64_t)rsx_num_cus() ? pad / 4 : 2 * (int64_t)rsx_num_cus();
         hipLaunchKernelGGL((rows_kernel<D, F32>), dim3((unsigned)row_wgs), dim3(256), 0, st, a, indptr ? w.bits : (const uint32_t *)nullptr, pad, w.prm, w.weight, w.named, w.coef, w.scalars,
-                           w.tile_factor, item_tiles);
-        hipLaunchKernelGGL((tiles_kernel<D, F32, true>), dim3((unsigned)user_tiles), dim3(256), 0, st, a, w.weight, w.scalars, (uint4 *)w.user_rm, (uint4 *)w.user_t,
-                           w.user_factor + k);
-        Pass p;
-        p.top_factor = w.scalars + kTopFactor; p.prm = w.prm; p.bits = w.bits; p.named = w.named; p.coef = w.coef;
+                           largest + k, w.tile_factor, w.pad_q / kTile);
+        hipLaunchKernelGGL((users_kernel<D, F32>), dim3((unsigned)user_tiles), dim3(256), 0, st, a, w.weight, largest + k, (uint4 *)w.user_rm, (uint4 *)w.user_t, w.user_factor + k);
+        Pass p;                               // users stay
+        p.top_factor = w.scalars; p.prm = w.prm; p.bits = w.bits; p.named = w.named; p.coef = w.coef;
         p.positions = a.rows; p.cat = a.cat; p.T = a.T;
         p.stay = w.user_rm; p.flow = F32 ? w.item_rm : (const char *)a.Q; p.flow_t = w.item_t;
         p.stay_rows = pad; p.flow_tiles = (a.cat + kTile - 1) / kTile; p.flow_valid = a.cat;
         p.part = w.part_p; p.part_rows = pad;
-        const int pieces_p = grad_pieces(a.rows, p.flow_tiles, w.wgs, w.st);
-        launch_pass<D, F32, false>(p, w.tile_factor, pieces_p, indptr != nullptr, a.h != nullptr, st);
-        hipLaunchKernelGGL((join_rows_kernel<D, F32>), dim3((unsigned)((a.rows * (D / 4) + 255) / 256)), dim3(256), 0, st, a, w.part_p, p.flow_tiles, pieces_p, pad, w.weight,
-                           w.scalars + kTopFactor, w.named, (char *)GP + r0 * D * es);
-        p.stay = F32 ? w.item_rm : (const char *)a.Q; p.flow = w.user_rm; p.flow_t = w.user_t;
-        p.stay_rows = F32 ? w.pad_q : a.cat; p.flow_tiles = user_tiles; p.flow_valid = a.rows;
-        p.part = w.part_q + (size_t)k * w.seg_q * w.pad_q * D; p.part_rows = w.pad_q;
-        const int pieces_q = grad_pieces(a.cat, user_tiles, w.wgs, w.st);
-        launch_pass<D, F32, true>(p, w.tile_factor, pieces_q, indptr != nullptr, a.h != nullptr, st);
-        if (k == 0) { ps.flow_tiles = user_tiles; ps.pieces = pieces_q; }
-        ps.last_tiles = user_tiles; ps.last_pieces = pieces_q;
+        p.pieces = grad_pieces(a.rows, p.flow_tiles, w.wgs, w.st);
+        Pass q = p;                           // items stay
+        q.stay = F32 ? w.item_rm : (const char *)a.Q; q.flow = w.user_rm; q.flow_t = w.user_t;
+        q.stay_rows = F32 ? w.pad_q : a.cat; q.flow_tiles = user_tiles; q.flow_valid = a.rows;
+        q.part = w.part_q + (size_t)k * w.seg_q * w.pad_q * D; q.part_rows = w.pad_q;
+        q.pieces = grad_pieces(a.cat, user_tiles, w.wgs, w.st);
+#define RSX_GRAD(M_, E_) hipLaunchKernelGGL((grad_kernel<D, F32, M_, E_>), dim3((unsigned)(p.pieces + q.pieces)), dim3(GradGeo<D, F32>::NT), 0, st, p, q, w.tile_factor)
+        if (indptr) { if (a.h) RSX_GRAD(true, true); else RSX_GRAD(true, false); }
+        else { if (a.h) RSX_GRAD(false, true); else RSX_GRAD(false, false); }
+#undef RSX_GRAD
+        if (k == 0) { ps.flow_tiles = user_tiles; ps.pieces = q.pieces; }
+        ps.last_tiles = user_tiles; ps.last_pieces = q.pieces;
+        const int64_t joins = (a.rows * (D / 4) + 255) / 256, item_joins = k + 1 == w.passes ? (a.cat * (D / 4) + 255) / 256 : 0;
+        hipLaunchKernelGGL((join_kernel<D, F32>), dim3((unsigned)(joins + item_joins)), dim3(256), 0, st, a, p, w.weight, (char *)GP + r0 * D * es, joins, ps, w.part_q, w.pad_q,
+                           w.user_factor, GQ);
     }
-    hipLaunchKernelGGL((join_items_kernel<D, F32>), dim3((unsigned)((all.cat * (D / 4) + 255) / 256)), dim3(256), 0, st, all.cat, w.part_q, ps, w.pad_q, w.user_factor, all.scale, GQ);
 }
 
 }  // namespace
@@ -815,6 +849,7 @@ RSX_API int rsx_add_rows(float *T, int64_t table_rows, int d, const int32_t *ids
     RSX_CHECK_ARG(rsx_dim_ok(d), "d must be 32, 64, 128 or 256");
     RSX_CHECK_ARG(dtype == RSX_F32 || dtype == RSX_BF16, "dtype must be RSX_F32 or RSX_BF16");
     RSX_CHECK_ARG(table_rows > 0 && n >= 0, "bad shape");
+    if (n == 0) return RSX_OK;
     for (int64_t r0 = 0; r0 < n; r0 += kAddRows) {
         const int m = (int)(n - r0 < kAddRows ? n - r0 : kAddRows);
         const void *src = (const char *)R + (size_t)r0 * d * (dtype == RSX_F32 ? 4 : 2);
