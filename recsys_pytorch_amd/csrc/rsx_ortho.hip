@@ -83,9 +83,12 @@ __host__ __device__ constexpr int block_at(int D, int p, int q) { return p * n_g
 // wavefronts share a SIMD), the rows of a tile to the 8 / SETS wavefronts of a set.  16 KB tiles pass through LDS; two tiles of G and M are on their way
 // in registers (64 KB a CU: what HBM's latency takes).  Bound by HBM with the momentum (1M x 128: 1.5 GB in 0.34 ms), by the fp64 matrix
 // rate without (36 instructions of 64 cycles per four rows: 0.27 ms).
-template <int D>
+// d = 256 without the momentum (whose update one workgroup has to make): four workgroups share a row range and its blocks, two sets each, so that there
+// are a quarter of the partials (20011 rows: 37 us and 5 to add them up; 256 workgroups with all 136 blocks each: 35 and 15).
+template <int D, bool MUON>
 struct Gram {
-    static constexpr int SETS = D == 256 ? 8 : D == 128 ? 4 : 1, KSPLIT = 8 / SETS, TR = 4096 / D, NB = n_blocks(D), PER = (NB + SETS - 1) / SETS;
+    static constexpr int SHARE = D == 256 && !MUON ? 4 : 1;
+    static constexpr int SETS = D == 256 ? 8 : D == 128 ? 4 : 1, MINE = SETS / SHARE, KSPLIT = 8 / MINE, TR = 4096 / D, NB = n_blocks(D), PER = (NB + SETS - 1) / SETS;
 };
 
 template <int D, int SET, typename F>
@@ -96,19 +99,19 @@ __device__ __forceinline__ void set_blocks(F f)          // f(index of the accum
     for (int p = 0; p < n_groups(D); ++p)
 #pragma unroll
         for (int q = p; q < n_groups(D); ++q, ++n)
-            if (n / Gram<D>::PER == SET) f(a++, n, p, q);
+            if (n / Gram<D, true>::PER == SET) f(a++, n, p, q);
 }
 
 template <int D, int SET, typename T, bool MUON>
-__device__ __forceinline__ void gram_body(const Rows<T, MUON> &in, int64_t rows, double *__restrict__ part, char *lds)
+__device__ __forceinline__ void gram_body(const Rows<T, MUON> &in, int64_t rows, int piece, int pieces, double *__restrict__ part, char *lds)
 {
-    using C = Gram<D>;
+    using C = Gram<D, MUON>;
     constexpr int LW = D == 32 ? 2 : 4;                                 // elements of a lane's piece
     const int tid = threadIdx.x, lane = tid & 63, ks = (tid >> 6) % C::KSPLIT;
     f64x4 acc[C::PER];
 #pragma unroll
     for (int b = 0; b < C::PER; ++b) acc[b] = f64x4{0.0, 0.0, 0.0, 0.0};
-    const int64_t stride = (int64_t)gridDim.x * C::TR, first = (int64_t)blockIdx.x * C::TR;
+    const int64_t stride = (int64_t)pieces * C::TR, first = (int64_t)piece * C::TR;
     Piece<T, MUON> a[2], b[2];                                          // this thread's two pieces of the next tile, and of the one after
     auto at = [&](int64_t r0, int n) { return r0 * D + 4 * (tid + 512 * n); };
     auto fetch = [&](Piece<T, MUON> (&p)[2], int64_t r0) {
@@ -146,7 +149,7 @@ __device__ __forceinline__ void gram_body(const Rows<T, MUON> &in, int64_t rows,
     }
     // the KSPLIT wavefronts of a set one after the other (a fixed order), through LDS four blocks a set at a time; then the workgroup's partial
     // (f64 result layout: register pair i of lane l is row 4 i + (l >> 4), column l & 15)
-    double *dst = part + (size_t)blockIdx.x * (C::NB * 256);
+    double *dst = part + (size_t)piece * (C::NB * 256);
     auto cell = [&](int i) { return (4 * i + (lane >> 4)) * 16 + (lane & 15); };
     if constexpr (C::KSPLIT == 1) {
         set_blocks<D, SET>([&](int i, int n, int, int) {
@@ -154,7 +157,7 @@ __device__ __forceinline__ void gram_body(const Rows<T, MUON> &in, int64_t rows,
             for (int e = 0; e < 4; ++e) dst[n * 256 + cell(e)] = acc[i][e];
         });
     } else {
-        double *red = reinterpret_cast<double *>(lds) + SET * 4 * 256;  // (SETS x 4 blocks of 2 KB: 32 KB at most)
+        double *red = reinterpret_cast<double *>(lds) + SET % C::MINE * 4 * 256;  // (sets x 4 blocks of 2 KB: 32 KB at most)
 #pragma unroll
         for (int i0 = 0; i0 < C::PER; i0 += 4) {
             for (int w = 0; w < C::KSPLIT; ++w) {
@@ -177,44 +180,58 @@ __device__ __forceinline__ void gram_body(const Rows<T, MUON> &in, int64_t rows,
 template <int D, typename T, bool MUON>
 __global__ __launch_bounds__(512, (D == 256 ? 2 : 4)) void gram_kernel(Rows<T, MUON> in, int64_t rows, double *__restrict__ part)
 {
-    using C = Gram<D>;
+    using C = Gram<D, MUON>;
     __shared__ __attribute__((aligned(16))) char lds[32768];
-    const int set = __builtin_amdgcn_readfirstlane((threadIdx.x >> 6) / C::KSPLIT);
-    if (set == 0) gram_body<D, 0, T, MUON>(in, rows, part, lds);
+    // workgroups of one row range 8 apart: on one XCD, whose L2 they share
+    const int share = C::SHARE == 1 ? 0 : blockIdx.x / 8 % C::SHARE, pieces = gridDim.x / C::SHARE;
+    const int piece = C::SHARE == 1 ? blockIdx.x : blockIdx.x / (8 * C::SHARE) * 8 + blockIdx.x % 8;
+    const int set = __builtin_amdgcn_readfirstlane(share * C::MINE + (threadIdx.x >> 6) / C::KSPLIT);
+    if (set == 0) gram_body<D, 0, T, MUON>(in, rows, piece, pieces, part, lds);
     if constexpr (C::SETS >= 4) {
-        if (set == 1) gram_body<D, 1, T, MUON>(in, rows, part, lds);
-        if (set == 2) gram_body<D, 2, T, MUON>(in, rows, part, lds);
-        if (set == 3) gram_body<D, 3, T, MUON>(in, rows, part, lds);
+        if (set == 1) gram_body<D, 1, T, MUON>(in, rows, piece, pieces, part, lds);
+        if (set == 2) gram_body<D, 2, T, MUON>(in, rows, piece, pieces, part, lds);
+        if (set == 3) gram_body<D, 3, T, MUON>(in, rows, piece, pieces, part, lds);
     }
     if constexpr (C::SETS >= 8) {
-        if (set == 4) gram_body<D, 4, T, MUON>(in, rows, part, lds);
-        if (set == 5) gram_body<D, 5, T, MUON>(in, rows, part, lds);
-        if (set == 6) gram_body<D, 6, T, MUON>(in, rows, part, lds);
-        if (set == 7) gram_body<D, 7, T, MUON>(in, rows, part, lds);
+        if (set == 4) gram_body<D, 4, T, MUON>(in, rows, piece, pieces, part, lds);
+        if (set == 5) gram_body<D, 5, T, MUON>(in, rows, piece, pieces, part, lds);
+        if (set == 6) gram_body<D, 6, T, MUON>(in, rows, piece, pieces, part, lds);
+        if (set == 7) gram_body<D, 7, T, MUON>(in, rows, piece, pieces, part, lds);
     }
 }
 
-// partials -> the full symmetric matrix in column order.  16 elements x 16 slices of the partials per workgroup.
+// partials -> the full symmetric matrix in column order.  32 elements x 16 slices of the partials per workgroup, eight loads of two elements on their
+// way (512 partials of d = 128, 38 MB: 7.5 us; one element a load, as many as the compiler unrolls: 13).
 template <int D>
 __global__ __launch_bounds__(256) void gram_reduce_kernel(const double *__restrict__ part, int n_part, double *__restrict__ G)
 {
     constexpr int NB = n_blocks(D);
-    __shared__ double s[16][17];
+    __shared__ double s[16][34];
     const int e = threadIdx.x & 15, sl = threadIdx.x >> 4;
-    const int at = blockIdx.x * 16 + e;                       // element of [NB][16][16]
-    double sum = 0.0;
-    for (int p = sl; p < n_part; p += 16) sum += part[(size_t)p * (NB * 256) + at];
-    s[sl][e] = sum;
+    const int at = blockIdx.x * 32 + 2 * e;                   // element of [NB][16][16]
+    double2 sum = make_double2(0.0, 0.0);
+    for (int p0 = sl; p0 < n_part; p0 += 128) {
+        double2 v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int p = p0 + 16 * k;
+            v[k] = p < n_part ? *reinterpret_cast<const double2 *>(part + (size_t)p * (NB * 256) + at) : make_double2(0.0, 0.0);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) { sum.x += v[k].x; sum.y += v[k].y; }
+    }
+    s[sl][2 * e] = sum.x;
+    s[sl][2 * e + 1] = sum.y;
     __syncthreads();
-    if (sl == 0) {
+    if (threadIdx.x < 32) {
         double v = 0.0;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v += s[i][e];
-        const int blk = at >> 8;
+        for (int i = 0; i < 16; ++i) v += s[i][threadIdx.x];
+        const int cell = blockIdx.x * 32 + threadIdx.x, blk = cell >> 8;
         int p = 0;
         while (p + 1 < n_groups(D) && block_at(D, p + 1, p + 1) <= blk) ++p;
         const int q = p + blk - block_at(D, p, p);
-        const int r = group_col(D, p, (at >> 4) & 15), c = group_col(D, q, at & 15);
+        const int r = group_col(D, p, (cell >> 4) & 15), c = group_col(D, q, cell & 15);
         G[(size_t)r * D + c] = v;
         G[(size_t)c * D + r] = v;
     }
@@ -270,46 +287,75 @@ __device__ __forceinline__ void ns_pq(int b, int *p, int *q)
 
 // both triangles from the upper one.  (On the diagonal X Y's (r, c) and (c, r) are sums of other roundings: one of them, always the same
 // one, stands for both.)
-template <int D, typename O>
-__device__ __forceinline__ void ns_store(O *out, int p, int q, double v)
+template <int D>
+__device__ __forceinline__ void ns_store(double *out, int p, int q, double v)
 {
     const int r = 16 * p + (threadIdx.x >> 4), c = 16 * q + (threadIdx.x & 15);
     if (r > c) return;
-    out[(size_t)r * D + c] = (O)v;
-    out[(size_t)c * D + r] = (O)v;
+    out[(size_t)r * D + c] = v;
+    out[(size_t)c * D + r] = v;
 }
 
-// S = A A.  FIRST: A = s^2 G is formed here and stored
+// the result: fp32 for the fp32 products, or three bf16 planes that add up to it in the operand order of project_bf16_kernel:
+// [32 columns][16 rows][plane][lane][8]
+template <int D>
+__device__ __forceinline__ void put_result(float *out, int r, int c, double v) { out[(size_t)r * D + c] = (float)v; }
+template <int D>
+__device__ __forceinline__ void put_result(uint16_t *out, int r, int c, double v)
+{
+    float m = (float)v;
+    uint16_t *dst = out + ((((size_t)(c / 32) * (D / 16) + r / 16) * 3) * 64 + 32 * ((r % 16) / 8) + c % 32) * 8 + r % 8;
+#pragma unroll
+    for (int n = 0; n < 3; ++n) {
+        const uint16_t h = f32_bf16(m);
+        dst[n * 512] = h;
+        m -= __uint_as_float((uint32_t)h << 16);
+    }
+}
+template <int D, typename O>
+__device__ __forceinline__ void ns_result(O *out, int p, int q, double v)
+{
+    const int r = 16 * p + (threadIdx.x >> 4), c = 16 * q + (threadIdx.x & 15);
+    if (r > c) return;
+    put_result<D>(out, r, c, v);
+    put_result<D>(out, c, r, v);
+}
+
+// T = a I + b A + c A A, for the two kernels behind it.  FIRST: A = s^2 G is formed here and stored
 template <int D, bool FIRST>
-__global__ __launch_bounds__(256) void ns_square_kernel(const double *__restrict__ G, double *__restrict__ A, double *__restrict__ S, double eps)
+__global__ __launch_bounds__(256) void ns_square_kernel(const double *__restrict__ G, double *__restrict__ A, double *__restrict__ T, Coeffs k)
 {
     __shared__ double red[4][64][4], s_norm;
     int p, q;
     ns_pq<D>(blockIdx.x, &p, &q);
-    double s2 = 1.0;
-    if constexpr (FIRST) { const double s = norm_scale(G, D, eps, &s_norm); s2 = s * s; }
-    auto f = [&](int k, int c) { const double v = G[(size_t)k * D + c]; return FIRST ? s2 * v : v; };
-    const double v = ns_block<D>(f, f, p, q, red);
-    ns_store<D>(S, p, q, v);
-    if constexpr (FIRST) ns_store<D>(A, p, q, s2 * G[(size_t)(16 * p + (threadIdx.x >> 4)) * D + 16 * q + (threadIdx.x & 15)]);
+    const int r = 16 * p + (threadIdx.x >> 4), c = 16 * q + (threadIdx.x & 15);
+    double here = G[(size_t)r * D + c];
+    auto f = [&](int i, int j) { return G[(size_t)i * D + j]; };
+    double v = ns_block<D>(f, f, p, q, red);
+    if constexpr (FIRST) {
+        const double s = norm_scale(G, D, k.eps, &s_norm), s2 = s * s;
+        here *= s2;
+        v *= s2 * s2;
+        ns_store<D>(A, p, q, here);
+    }
+    ns_store<D>(T, p, q, fma(k.c, v, fma(k.b, here, r == c ? k.a : 0.0)));
 }
 
 // blockIdx.y == 0: out_m = M T (FIRST: s T, no product);  1: W = A T
 template <int D, bool FIRST, typename O>
-__global__ __launch_bounds__(256) void ns_times_t_kernel(const double *__restrict__ G, const double *__restrict__ A, const double *__restrict__ S,
-                                                         const double *__restrict__ M, O *__restrict__ out_m, double *__restrict__ W, Coeffs k)
+__global__ __launch_bounds__(256) void ns_times_t_kernel(const double *__restrict__ G, const double *__restrict__ A, const double *__restrict__ T,
+                                                         const double *__restrict__ M, O *__restrict__ out_m, double *__restrict__ W, double eps)
 {
     __shared__ double red[4][64][4], s_norm;
     int p, q;
     ns_pq<D>(blockIdx.x, &p, &q);
-    auto t = [&](int r, int c) { const size_t at = (size_t)r * D + c; return fma(k.c, S[at], fma(k.b, A[at], r == c ? k.a : 0.0)); };
+    auto t = [&](int r, int c) { return T[(size_t)r * D + c]; };
     if (blockIdx.y == 0) {
-        if constexpr (FIRST) {
-            const double s = norm_scale(G, D, k.eps, &s_norm);
-            ns_store<D>(out_m, p, q, s * t(16 * p + (threadIdx.x >> 4), 16 * q + (threadIdx.x & 15)));
-        } else {
-            ns_store<D>(out_m, p, q, ns_block<D>([&](int r, int c) { return M[(size_t)r * D + c]; }, t, p, q, red));
-        }
+        double v;
+        if constexpr (FIRST) v = norm_scale(G, D, eps, &s_norm) * t(16 * p + (threadIdx.x >> 4), 16 * q + (threadIdx.x & 15));
+        else v = ns_block<D>([&](int r, int c) { return M[(size_t)r * D + c]; }, t, p, q, red);
+        if constexpr (std::is_same<O, double>::value) ns_store<D>(out_m, p, q, v);
+        else ns_result<D>(out_m, p, q, v);
     } else {
         ns_store<D>(W, p, q, ns_block<D>([&](int r, int c) { return A[(size_t)r * D + c]; }, t, p, q, red));
     }
@@ -317,22 +363,20 @@ __global__ __launch_bounds__(256) void ns_times_t_kernel(const double *__restric
 
 // A' = W T
 template <int D>
-__global__ __launch_bounds__(256) void ns_next_kernel(const double *__restrict__ A, const double *__restrict__ S, const double *__restrict__ W,
-                                                      double *__restrict__ A2, Coeffs k)
+__global__ __launch_bounds__(256) void ns_next_kernel(const double *__restrict__ W, const double *__restrict__ T, double *__restrict__ A2)
 {
     __shared__ double red[4][64][4];
     int p, q;
     ns_pq<D>(blockIdx.x, &p, &q);
-    auto t = [&](int r, int c) { const size_t at = (size_t)r * D + c; return fma(k.c, S[at], fma(k.b, A[at], r == c ? k.a : 0.0)); };
-    ns_store<D>(A2, p, q, ns_block<D>([&](int r, int c) { return W[(size_t)r * D + c]; }, t, p, q, red));
+    ns_store<D>(A2, p, q, ns_block<D>([&](int r, int c) { return W[(size_t)r * D + c]; }, [&](int r, int c) { return T[(size_t)r * D + c]; }, p, q, red));
 }
 
 // d <= 64: the whole iteration in one workgroup, the four matrices in LDS (128 KB at d = 64).  Blocks of the upper triangles are dealt to 16 wavefronts
 // (M T and A T together: 20 blocks, five a SIMD); both triangles are written.  Bound by one CU's fp64 matrix rate.
 // Columns are XORed by row: the two rows of a half-wavefront's read lie in different halves of the 256 bytes the LDS delivers a cycle, and the 16 rows
 // of a transposed store in eight different places.
-template <int D>
-__global__ __launch_bounds__(1024) void ns_small_kernel(const double *__restrict__ G, float *__restrict__ out, int steps, Coeffs k)
+template <int D, typename O>
+__global__ __launch_bounds__(1024) void ns_small_kernel(const double *__restrict__ G, O *__restrict__ out, int steps, Coeffs k)
 {
     constexpr int NB = n_blocks(D);
     __shared__ __attribute__((aligned(16))) double A[D * D], T[D * D], W[D * D], M[D * D];
@@ -343,7 +387,6 @@ __global__ __launch_bounds__(1024) void ns_small_kernel(const double *__restrict
     for (int t = tid; t < D * D; t += 1024) {
         const int r = t / D, c = t % D;
         A[el(r, c)] = s * s * G[t];
-        M[el(r, c)] = r == c ? s : 0.0;
     }
     __syncthreads();
     auto mul = [&](const double *x, const double *y, int p, int q) {
@@ -386,17 +429,20 @@ __global__ __launch_bounds__(1024) void ns_small_kernel(const double *__restrict
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
             const int b = w + 16 * n;
-            if (b >= 2 * NB || (last && b < NB)) continue;
+            if (b >= 2 * NB || (last && b < NB) || (step == 0 && b >= NB)) continue;
             x[n] = mul(b < NB ? A : M, T, p2[n], q2[n]);
         }
         __syncthreads();
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
             const int b = w + 16 * n;
-            if (b >= 2 * NB || (last && b < NB)) continue;
+            if (b >= 2 * NB || (last && b < NB) || (step == 0 && b >= NB)) continue;
 #pragma unroll
             for (int i = 0; i < 4; ++i) put(b < NB ? W : M, p2[n], q2[n], i, x[n][i]);
         }
+        if (step == 0)                                                     // (M was s I: no product)
+#pragma unroll 1
+            for (int t = tid; t < D * D; t += 1024) M[t] = s * T[t];
         __syncthreads();
         if (!last && w < NB) {
             const f64x4 y = mul(W, T, p, q);
@@ -405,15 +451,15 @@ __global__ __launch_bounds__(1024) void ns_small_kernel(const double *__restrict
         }
         __syncthreads();
     }
-    for (int t = tid; t < D * D; t += 1024) out[t] = (float)M[el(t / D, t % D)];
+    for (int t = tid; t < D * D; t += 1024) put_result<D>(out, t / D, t % D, M[el(t / D, t % D)]);
 }
 
-template <int D>
-__global__ __launch_bounds__(256) void ns_identity_kernel(const double *__restrict__ G, float *__restrict__ out, double eps)   // steps == 0
+template <int D, typename O>
+__global__ __launch_bounds__(256) void ns_identity_kernel(const double *__restrict__ G, O *__restrict__ out, double eps)   // steps == 0
 {
     __shared__ double s_norm;
     const double s = norm_scale(G, D, eps, &s_norm);
-    for (int t = threadIdx.x; t < D * D; t += 256) out[t] = t / D == t % D ? (float)s : 0.0f;
+    for (int t = threadIdx.x; t < D * D; t += 256) put_result<D>(out, t / D, t % D, t / D == t % D ? s : 0.0);
 }
 
 // ---- rows times the [d x d] result ---------------------------------------------------------------------------------------------------
@@ -485,8 +531,6 @@ __global__ __launch_bounds__(Proj<D>::NT) void project_kernel(Rows<T, MUON> in, 
                                                                          fmaf(-step, o.w, keep * wt[n].w));
                 if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2 *>(out + at(r0, n)) = make_uint2(0u, 0u);      // out is the gradient: zero for the next step
                 else *reinterpret_cast<float4 *>(out + at(r0, n)) = make_float4(0.f, 0.f, 0.f, 0.f);
-            } else if constexpr (sizeof(T) == 2) {
-                *reinterpret_cast<ushort4 *>(out + at(r0, n)) = make_ushort4(f32_bf16(o.x), f32_bf16(o.y), f32_bf16(o.z), f32_bf16(o.w));
             } else {
                 *reinterpret_cast<float4 *>(out + at(r0, n)) = o;
             }
@@ -495,55 +539,108 @@ __global__ __launch_bounds__(Proj<D>::NT) void project_kernel(Rows<T, MUON> in, 
     }
 }
 
+// bf16 rows alone (no optimizer step): v_mfma_f32_32x32x16_bf16 with the matrix in three bf16 planes (24 bits of it: exact products, as good as fp32's; six
+// times its rate).  A wavefront holds the planes of its 32 columns (192 registers at d = 256).  20011 x 256: 14 us, 37 with fp32 products.
+template <int D>
+__global__ __launch_bounds__(Proj<D>::NT, 2) void project_bf16_kernel(const uint16_t *X, uint16_t *out, int64_t rows, const uint4 *__restrict__ Mt)
+{
+    using C = Proj<D>;
+    typedef short bf16x8 __attribute__((ext_vector_type(8)));
+    typedef __bf16 frag __attribute__((ext_vector_type(8)));
+    constexpr int LD = D + 8, KS = D / 16, NP = C::TR * D / 8 / C::NT;
+    __shared__ __attribute__((aligned(16))) uint16_t tile[C::TR * LD], res[C::TR * LD];
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, cg = w % C::CG, rg = w / C::CG, hi = lane >> 5, l31 = lane & 31;
+    const int64_t stride = (int64_t)gridDim.x * C::TR, first = (int64_t)blockIdx.x * C::TR, end = rows * D;
+    uint4 p[NP];
+    auto spot = [&](int n) { const int t = tid + C::NT * n; return (t / (D / 8)) * LD + 8 * (t % (D / 8)); };
+    auto at = [&](int64_t r0, int n) { return r0 * D + 8 * (int64_t)(tid + C::NT * n); };
+    auto fetch = [&](int64_t r0) {
+#pragma unroll
+        for (int n = 0; n < NP; ++n) p[n] = at(r0, n) < end ? *reinterpret_cast<const uint4 *>(X + at(r0, n)) : make_uint4(0u, 0u, 0u, 0u);
+    };
+    fetch(first);
+    bf16x8 b[KS][3];
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int n = 0; n < 3; ++n) b[s][n] = __builtin_bit_cast(bf16x8, Mt[((size_t)cg * KS + s) * 192 + n * 64 + lane]);
+    for (int64_t r0 = first; r0 < rows; r0 += stride) {
+#pragma unroll
+        for (int n = 0; n < NP; ++n) *reinterpret_cast<uint4 *>(tile + spot(n)) = p[n];
+        __syncthreads();
+        fetch(r0 + stride);
+        f32x16 acc;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[i] = 0.0f;
+        const uint16_t *a = tile + (32 * rg + l31) * LD + 8 * hi;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const frag x = __builtin_bit_cast(frag, *reinterpret_cast<const bf16x8 *>(a + 16 * s));
+#pragma unroll
+            for (int n = 2; n >= 0; --n) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, __builtin_bit_cast(frag, b[s][n]), acc, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) res[(32 * rg + (i & 3) + 8 * (i >> 2) + 4 * hi) * LD + 32 * cg + l31] = f32_bf16(acc[i]);
+        __syncthreads();                // (every wavefront has read its rows, also before any of them is written where out == X)
+#pragma unroll
+        for (int n = 0; n < NP; ++n)
+            if (at(r0, n) < end) *reinterpret_cast<uint4 *>(out + at(r0, n)) = *reinterpret_cast<const uint4 *>(res + spot(n));
+    }
+}
+
 // ---- host ------------------------------------------------------------------------------------------------------------------------------
 struct OrthoWs {
-    double *part, *G, *A, *A2, *S, *W, *M, *M2;
-    float *T;
+    double *part, *G, *A, *A2, *P, *W, *M, *M2;      // P: the polynomial T of a step
+    void *T;                                     // the result, float or planes (put_result)
     int n_part;
     int64_t bytes;
 };
 
-int gram_groups(int64_t rows, int d)             // a workgroup for every two tiles of 4096 / d rows, at most two per CU (d = 256: one, by its registers)
+// row ranges: one for every two tiles of 4096 / d rows, at most two workgroups per CU (d = 256: one, by its registers; shared by four: a quarter, whole
+// groups of eight)
+int gram_pieces(int64_t rows, int d, bool muon)
 {
     const int64_t per = 2 * (4096 / d), want = (rows + per - 1) / per;
-    return (int)(want < 1 ? 1 : want > (d == 256 ? 256 : 512) ? (d == 256 ? 256 : 512) : want);
+    if (d == 256 && !muon) return want >= 64 ? 64 : (int)((want + 7) / 8 * 8);
+    const int64_t most = d == 256 ? 256 : 512;
+    return (int)(want > most ? most : want);
 }
 
-OrthoWs ortho_carve(void *ws, int64_t rows, int d)
+OrthoWs ortho_carve(void *ws, int64_t rows, int d, bool muon)
 {
     OrthoWs w;
     char *base = (char *)ws;
     int64_t off = 0;
     auto take = [&](int64_t n) { char *q = base + off; off += (n + 255) / 256 * 256; return q; };
-    w.n_part = gram_groups(rows, d);
+    w.n_part = gram_pieces(rows, d, muon);
     const int64_t mat = (int64_t)d * d * 8;
     w.part = (double *)take((int64_t)w.n_part * n_blocks(d) * 2048);
-    w.G = (double *)take(mat); w.A = (double *)take(mat); w.A2 = (double *)take(mat); w.S = (double *)take(mat);
+    w.G = (double *)take(mat); w.A = (double *)take(mat); w.A2 = (double *)take(mat); w.P = (double *)take(mat);
     w.W = (double *)take(mat); w.M = (double *)take(mat); w.M2 = (double *)take(mat);
-    w.T = (float *)take(mat / 2);
+    w.T = take(mat);
     w.bytes = off;
     return w;
 }
 
-template <int D>
-void newton_schulz(const OrthoWs &w, int steps, const Coeffs &k, hipStream_t st)
+template <int D, typename O>
+void newton_schulz(const OrthoWs &w, O *out, int steps, const Coeffs &k, hipStream_t st)
 {
-    if (steps == 0) { hipLaunchKernelGGL(ns_identity_kernel<D>, dim3(1), dim3(256), 0, st, w.G, w.T, k.eps); return; }
+    if (steps == 0) { hipLaunchKernelGGL((ns_identity_kernel<D, O>), dim3(1), dim3(256), 0, st, w.G, out, k.eps); return; }
     if constexpr (D <= 64) {
-        hipLaunchKernelGGL(ns_small_kernel<D>, dim3(1), dim3(1024), 0, st, w.G, w.T, steps, k);
+        hipLaunchKernelGGL((ns_small_kernel<D, O>), dim3(1), dim3(1024), 0, st, w.G, out, steps, k);
     } else {
         constexpr int NB = n_blocks(D);
         double *A = w.A, *A2 = w.A2, *M = w.M, *M2 = w.M2;
         for (int s = 0; s < steps; ++s) {
             const bool last = s + 1 == steps;
-            if (s == 0) hipLaunchKernelGGL((ns_square_kernel<D, true>), dim3(NB), dim3(256), 0, st, w.G, A, w.S, k.eps);
-            else hipLaunchKernelGGL((ns_square_kernel<D, false>), dim3(NB), dim3(256), 0, st, A, (double *)nullptr, w.S, k.eps);
+            if (s == 0) hipLaunchKernelGGL((ns_square_kernel<D, true>), dim3(NB), dim3(256), 0, st, w.G, A, w.P, k);
+            else hipLaunchKernelGGL((ns_square_kernel<D, false>), dim3(NB), dim3(256), 0, st, A, (double *)nullptr, w.P, k);
             const dim3 grid(NB, last ? 1 : 2);
-            if (s == 0 && last) hipLaunchKernelGGL((ns_times_t_kernel<D, true, float>), grid, dim3(256), 0, st, w.G, A, w.S, M, w.T, w.W, k);
-            else if (s == 0) hipLaunchKernelGGL((ns_times_t_kernel<D, true, double>), grid, dim3(256), 0, st, w.G, A, w.S, M, M2, w.W, k);
-            else if (last) hipLaunchKernelGGL((ns_times_t_kernel<D, false, float>), grid, dim3(256), 0, st, w.G, A, w.S, M, w.T, w.W, k);
-            else hipLaunchKernelGGL((ns_times_t_kernel<D, false, double>), grid, dim3(256), 0, st, w.G, A, w.S, M, M2, w.W, k);
-            if (!last) hipLaunchKernelGGL(ns_next_kernel<D>, dim3(NB), dim3(256), 0, st, A, w.S, w.W, A2, k);
+            if (s == 0 && last) hipLaunchKernelGGL((ns_times_t_kernel<D, true, O>), grid, dim3(256), 0, st, w.G, A, w.P, M, out, w.W, k.eps);
+            else if (s == 0) hipLaunchKernelGGL((ns_times_t_kernel<D, true, double>), grid, dim3(256), 0, st, w.G, A, w.P, M, M2, w.W, k.eps);
+            else if (last) hipLaunchKernelGGL((ns_times_t_kernel<D, false, O>), grid, dim3(256), 0, st, w.G, A, w.P, M, out, w.W, k.eps);
+            else hipLaunchKernelGGL((ns_times_t_kernel<D, false, double>), grid, dim3(256), 0, st, w.G, A, w.P, M, M2, w.W, k.eps);
+            if (!last) hipLaunchKernelGGL(ns_next_kernel<D>, dim3(NB), dim3(256), 0, st, w.W, w.P, A2);
             double *x = A; A = A2; A2 = x;
             x = M; M = M2; M2 = x;
         }
@@ -553,13 +650,18 @@ void newton_schulz(const OrthoWs &w, int steps, const Coeffs &k, hipStream_t st)
 template <int D, typename T, bool MUON>
 void orthogonalize_d(const Rows<T, MUON> &in, T *out, float *W, int64_t rows, int steps, const Coeffs &k, float keep, float step, const OrthoWs &w, hipStream_t st)
 {
-    hipLaunchKernelGGL((gram_kernel<D, T, MUON>), dim3(w.n_part), dim3(512), 0, st, in, rows, w.part);
-    hipLaunchKernelGGL(gram_reduce_kernel<D>, dim3(n_blocks(D) * 16), dim3(256), 0, st, w.part, w.n_part, w.G);
-    newton_schulz<D>(w, steps, k, st);
+    hipLaunchKernelGGL((gram_kernel<D, T, MUON>), dim3(w.n_part * Gram<D, MUON>::SHARE), dim3(512), 0, st, in, rows, w.part);
+    hipLaunchKernelGGL(gram_reduce_kernel<D>, dim3(n_blocks(D) * 8), dim3(256), 0, st, w.part, w.n_part, w.G);
     using C = Proj<D>;
     const int64_t tiles = (rows + C::TR - 1) / C::TR;
-    const int64_t most = (int64_t)rsx_num_cus() * (D == 256 ? 2 : 3);
-    hipLaunchKernelGGL((project_kernel<D, T, MUON>), dim3((unsigned)(tiles < most ? tiles : most)), dim3(C::NT), 0, st, in, out, W, rows, w.T, keep, step);
+    auto grid = [&](int per_cu) { const int64_t most = (int64_t)rsx_num_cus() * per_cu; return dim3((unsigned)(tiles < most ? tiles : most)); };
+    if constexpr (sizeof(T) == 2 && !MUON) {
+        newton_schulz<D>(w, (uint16_t *)w.T, steps, k, st);
+        hipLaunchKernelGGL(project_bf16_kernel<D>, grid(D == 256 ? 1 : 3), dim3(C::NT), 0, st, in.X, out, rows, (const uint4 *)w.T);
+    } else {
+        newton_schulz<D>(w, (float *)w.T, steps, k, st);
+        hipLaunchKernelGGL((project_kernel<D, T, MUON>), grid(D == 256 ? 2 : 3), dim3(C::NT), 0, st, in, out, W, rows, (const float *)w.T, keep, step);
+    }
 }
 
 template <typename T, bool MUON>
@@ -582,7 +684,8 @@ bool finite64(double v) { return v - v == 0.0; }
 RSX_API int64_t rsx_orthogonalize_workspace(int64_t rows, int d)
 {
     if (rows < 0 || !rsx_dim_ok(d)) return RSX_E_INVALID;
-    return ortho_carve(nullptr, rows, d).bytes;
+    const int64_t a = ortho_carve(nullptr, rows < 1 ? 1 : rows, d, false).bytes, b = ortho_carve(nullptr, rows < 1 ? 1 : rows, d, true).bytes;
+    return a > b ? a : b;
 }
 
 RSX_API int rsx_orthogonalize(const void *X, void *out, int64_t rows, int d, int dtype, int steps, double a, double b, double c, double eps, void *ws,
@@ -596,7 +699,7 @@ RSX_API int rsx_orthogonalize(const void *X, void *out, int64_t rows, int d, int
     RSX_CHECK_ARG(finite64(a) && finite64(b) && finite64(c) && finite64(eps) && eps >= 0.0, "coefficients must be finite, eps >= 0");
     RSX_CHECK_ARG(aligned16(X) && aligned16(out), "rows must be 16-byte aligned");
     if (rows == 0) return RSX_OK;
-    const OrthoWs w = ortho_carve(ws, rows, d);
+    const OrthoWs w = ortho_carve(ws, rows, d, false);
     if (ws == nullptr || ws_bytes < w.bytes || (reinterpret_cast<uintptr_t>(ws) & 7)) {
         rsx_set_error("rsx_orthogonalize: workspace of %lld bytes (8-byte aligned) required, got %lld", (long long)w.bytes, (long long)ws_bytes);
         return RSX_E_WORKSPACE;
@@ -623,7 +726,7 @@ RSX_API int rsx_muon_apply(float *W, float *M, void *G, int64_t rows, int d, int
     RSX_CHECK_ARG(finite64(lr) && finite64(weight_decay) && finite64(update_scale) && momentum >= 0.0 && momentum < 1.0, "momentum must be in [0, 1), the rest finite");
     RSX_CHECK_ARG(aligned16(W) && aligned16(M) && aligned16(G), "rows must be 16-byte aligned");
     if (rows == 0) return RSX_OK;
-    const OrthoWs w = ortho_carve(ws, rows, d);
+    const OrthoWs w = ortho_carve(ws, rows, d, true);
     if (ws == nullptr || ws_bytes < w.bytes || (reinterpret_cast<uintptr_t>(ws) & 7)) {
         rsx_set_error("rsx_muon_apply: workspace of %lld bytes (8-byte aligned) required, got %lld", (long long)w.bytes, (long long)ws_bytes);
         return RSX_E_WORKSPACE;
