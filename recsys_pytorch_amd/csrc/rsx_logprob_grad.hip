@@ -39,8 +39,10 @@ struct Args {
     float scale;
 };
 
-// per tile of 32 positions: [0] factor of its scores, [1] what is added to them (-lse in log2; fp32 without the entropy: and 12), [2] [3] dz = p (A + B log2 p), [4] .. [7] the first four named items (as
-// integers; -1: none): 1 KB, one wavefront's copy
+// per tile of 32 positions: [0] factor of its scores (bf16: the same in every row), [1] what is added to them, [2] [3] dz = p (A + B log2 p), [4] .. [7] the first
+// four named items (as integers; -1: none): 1 KB, one wavefront's copy.  Without the entropy's part B = 0: [1] is log2 |A| - lse (fp32: and 12), so that the
+// exponential is |dz|, and the sign of A goes with the row's weight (GP) and into the streaming rows (GQ): the same products with one parameter of a row
+// instead of three and a multiplication less a score (1000 x 50021 x 256 bf16: 269 -> 264 us)
 constexpr int kHeld = 4;
 struct Prm {
     float v[4 + kHeld][kTile];
@@ -88,6 +90,7 @@ __global__ __launch_bounds__(256) void rows_kernel(Args a, const uint32_t *__res
         const float h = ok && a.h != nullptr ? a.h[r] : 0.0f;
         const float lse = ok ? a.lse[r] : -INFINITY;
         const bool live = ok && lse != -INFINITY;
+        const float sign = a.h == nullptr && sum > 0.0 ? -1.0f : 1.0f;
         const float w = F32 ? (float)(mag + fabs((double)h)) : 1.0f;
         const float inv = w > 0.0f ? 1.0f / w : w == w ? 0.0f : w;              // (NaN weights stay NaN)
         float big = 0.0f, factor = live ? F32 ? 1.0f : a.scale * kLog2e : 0.0f;
@@ -106,22 +109,23 @@ __global__ __launch_bounds__(256) void rows_kernel(Args a, const uint32_t *__res
             most = fmaxf(most, finite_abs(big * w));
             for (int t = lane; t < a.T && r < a.rows; t += 64) {
                 const int32_t i = a.items[r * a.T + t];
-                coef[r * a.T + t] = ok && i >= 0 && i < a.cat ? a.g[r * a.T + t] * inv : 0.0f;        // (a masked item is not looked up)
+                coef[r * a.T + t] = ok && i >= 0 && i < a.cat ? a.g[r * a.T + t] * inv * sign : 0.0f;        // (a masked item is not looked up)
             }
         } else {
-            for (int t = lane; t < a.T && r < a.rows; t += 64) coef[r * a.T + t] = a.g[r * a.T + t];
+            for (int t = lane; t < a.T && r < a.rows; t += 64) coef[r * a.T + t] = a.g[r * a.T + t] * sign;
         }
-        // lse in log2 is rounded to fp32 (half a step at 24 is 1e-6 of every p): what that changes goes into the coefficients
         const double lse2 = (double)lse * 1.4426950408889634074;
+        // with the entropy: lse in log2 is rounded to fp32 (half a step at 24 is 1e-6 of every p): what that changes goes into the coefficients
         const float l2 = (float)lse2;
         const double fix = exp2((double)l2 - lse2) * inv;
+        const double off = (F32 ? 12.0 : 0.0) - lse2 + log2(fabs(sum) * inv);
         if (lane == 0) {
             out.v[0][c] = factor;
-            out.v[1][c] = live ? (F32 && a.h == nullptr ? 12.0f - l2 : -l2) : -kFar;
+            out.v[1][c] = !live ? -kFar : a.h == nullptr ? (float)off : -l2;
             out.v[2][c] = live ? (float)(-(sum + (double)h * (a.ent != nullptr ? a.ent[r] : 0.0f)) * fix) : 0.0f;
             out.v[3][c] = live ? (float)(-(double)h * kLn2 * fix) : 0.0f;
             for (int k = a.T; k < kHeld; ++k) out.v[4 + k][c] = __int_as_float(-1);
-            weight[r] = live ? w : 0.0f;
+            weight[r] = live ? sign * w : 0.0f;
         }
     }
     if constexpr (F32) {
@@ -188,6 +192,9 @@ __device__ __forceinline__ void lay_tile(const Args &a, int64_t tile, const floa
             for (int j = 0; j < 4; ++j) { x[r][c + 2 * j] = (uint16_t)w[j]; x[r][c + 2 * j + 1] = (uint16_t)(w[j] >> 16); }
         }
     }
+    if constexpr (USERS && !F32) {
+        if (tid < kTile) s_mul[tid] = weight[tile * kTile + tid];
+    }
     if constexpr (F32) {
         if constexpr (USERS) {
             float up, down;
@@ -238,8 +245,10 @@ __device__ __forceinline__ void lay_tile(const Args &a, int64_t tile, const floa
             uint16_t v[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const uint16_t y = x[tile_row<D>(half, lane >> 5, j)][col];
+                const int r = tile_row<D>(half, lane >> 5, j);
+                const uint16_t y = x[r][col];
                 v[j] = (y & 0x7F80u) == 0x7F80u ? (uint16_t)0 : y;
+                if constexpr (USERS) v[j] ^= s_mul[r] < 0.0f ? 0x8000u : 0u;
             }
             h.u = make_uint4(v[0] | ((uint32_t)v[1] << 16), v[2] | ((uint32_t)v[3] << 16), v[4] | ((uint32_t)v[5] << 16), v[6] | ((uint32_t)v[7] << 16));
         }
@@ -287,6 +296,7 @@ struct Pass {
     int64_t positions;                    // rows of named / coef / bits
     int64_t cat;
     int T;
+    float factor;                         // bf16: scale log2 e
     float *part;                          // [segments][padded rows that stay][d]
     int64_t part_rows;
     int pieces;                           // workgroups of this pass
@@ -447,7 +457,7 @@ __device__ __forceinline__ void grad_body(const Pass &a, int64_t piece, const fl
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const float p = __builtin_amdgcn_exp2f(F32 && ENT ? t[i] + lift : t[i]);
-                    v[i] = ENT ? p * fmaf(sB, t[i], sA) : p * sA;
+                    v[i] = ENT ? p * fmaf(sB, t[i], sA) : p;
                 }
             } else {
                 const Prm *prm = reinterpret_cast<const Prm *>(lds + G::PRM + j * 1024);
@@ -457,7 +467,7 @@ __device__ __forceinline__ void grad_body(const Pass &a, int64_t piece, const fl
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     const int r0 = 8 * q + 4 * hi;
-                    const float4 f4 = *reinterpret_cast<const float4 *>(&prm->v[0][r0]), l4 = *reinterpret_cast<const float4 *>(&prm->v[1][r0]);
+                    const float4 f4 = F32 ? *reinterpret_cast<const float4 *>(&prm->v[0][r0]) : make_float4(a.factor, a.factor, a.factor, a.factor), l4 = *reinterpret_cast<const float4 *>(&prm->v[1][r0]);
                     t[4 * q] = fmaf(acc[4 * q], f4.x * tf, l4.x);
                     t[4 * q + 1] = fmaf(acc[4 * q + 1], f4.y * tf, l4.y);
                     t[4 * q + 2] = fmaf(acc[4 * q + 2], f4.z * tf, l4.z);
@@ -470,17 +480,16 @@ __device__ __forceinline__ void grad_body(const Pass &a, int64_t piece, const fl
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     const int r0 = 8 * q + 4 * hi;
-                    const float4 a4 = *reinterpret_cast<const float4 *>(&prm->v[2][r0]);
-                    const float as[4] = {a4.x, a4.y, a4.z, a4.w};
-                    float bs[4] = {0.f, 0.f, 0.f, 0.f};
+                    float as[4], bs[4];
                     if constexpr (ENT) {
-                        const float4 b4 = *reinterpret_cast<const float4 *>(&prm->v[3][r0]);
+                        const float4 a4 = *reinterpret_cast<const float4 *>(&prm->v[2][r0]), b4 = *reinterpret_cast<const float4 *>(&prm->v[3][r0]);
+                        as[0] = a4.x; as[1] = a4.y; as[2] = a4.z; as[3] = a4.w;
                         bs[0] = b4.x; bs[1] = b4.y; bs[2] = b4.z; bs[3] = b4.w;
                     }
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const float p = __builtin_amdgcn_exp2f(F32 && ENT ? t[4 * q + e] + 12.0f : t[4 * q + e]);
-                        v[4 * q + e] = ENT ? p * fmaf(bs[e], t[4 * q + e], as[e]) : p * as[e];
+                        v[4 * q + e] = ENT ? p * fmaf(bs[e], t[4 * q + e], as[e]) : p;
                     }
                 }
                 // named items of the tile's positions that are in this wavefront's block.
@@ -777,7 +786,7 @@ void run(const Args &all, const int64_t *indptr, const int32_t *indices, const W
         hipLaunchKernelGGL((users_kernel<D, F32>), dim3((unsigned)user_tiles), dim3(256), 0, st, a, w.weight, largest + k, (uint4 *)w.user_rm, (uint4 *)w.user_t, w.user_factor + k);
         Pass p;                               // users stay
         p.top_factor = w.scalars; p.prm = w.prm; p.bits = w.bits; p.named = w.named; p.coef = w.coef;
-        p.positions = a.rows; p.cat = a.cat; p.T = a.T;
+        p.positions = a.rows; p.cat = a.cat; p.T = a.T; p.factor = a.scale * kLog2e;
         p.stay = w.user_rm; p.flow = F32 ? w.item_rm : (const char *)a.Q; p.flow_t = w.item_t;
         p.stay_rows = pad; p.flow_tiles = (a.cat + kTile - 1) / kTile; p.flow_valid = a.cat;
         p.part = w.part_p; p.part_rows = pad;
