@@ -7,6 +7,7 @@ library or a non-device tensor raises.
 import ctypes as C
 import os
 from collections import namedtuple
+from contextlib import nullcontext
 
 import torch
 
@@ -305,12 +306,16 @@ def _scratch(ws, need, device):
     return ws
 
 
+_HERE = nullcontext()
+
+
 def _same_device(first, *others):
     """everything on one device, which the launch is made on whatever the caller's current one is"""
+    device = first.device
     for t in others:
-        if t is not None and t.device != first.device:
-            raise RsxError(f"tensors on {first.device} and {t.device} in one call")
-    return torch.cuda.device(first.device)
+        if t is not None and t.device != device:
+            raise RsxError(f"tensors on {device} and {t.device} in one call")
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def orthogonalize_workspace(rows, d):
