@@ -28,7 +28,7 @@ using namespace lp;
 
 constexpr float kFar = 1.0e30f;           // log-normaliser of a row without probabilities: every p is 0
 constexpr float kLift = 4096.0f;          // dz of fp32 tables is held times 2^12
-constexpr int kLargest = 1;               // scalars: [0] the largest item factor, [kLargest + k] the largest w |P| of pass k
+constexpr int kLargest = 1;               // scalars: [0] the largest item factor, [kLargest + g] the largest w |P| among the positions of rows_kernel's workgroup g
 
 struct Args {
     const void *P, *Q;
@@ -49,11 +49,12 @@ struct Prm {
 };
 
 // ---- what the passes need -------------------------------------------------------------------------------------------------------------
-// one wavefront per position (padded to 128), positions dealt round: coefficients, named items with theirs, the largest w |P| (one atomic a
-// workgroup: a thousand on one word take 12 us).  The first workgroup also finds the largest item factor.
+// one wavefront per position (padded to 128), positions dealt round: coefficients, named items with theirs, the largest w |P| of a workgroup's
+// (users_kernel takes the largest of those: an atomic maximum on one word, 512 times, was 6 us of this kernel's 11 at 2395 positions).  The first
+// workgroup also finds the largest item factor.
 template <int D, bool F32>
 __global__ __launch_bounds__(256) void rows_kernel(Args a, const uint32_t *__restrict__ bits, int64_t padded, Prm *__restrict__ prm, float *__restrict__ weight, int32_t *__restrict__ named,
-                                                   float *__restrict__ coef, uint32_t *__restrict__ top_factor, uint32_t *__restrict__ largest, const float *__restrict__ item_factor, int64_t item_tiles)
+                                                   float *__restrict__ coef, uint32_t *__restrict__ top_factor, float *__restrict__ largest, const float *__restrict__ item_factor, int64_t item_tiles)
 {
     __shared__ float s_max[4];
     const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
@@ -131,7 +132,7 @@ __global__ __launch_bounds__(256) void rows_kernel(Args a, const uint32_t *__res
     if constexpr (F32) {
         if (lane == 0) s_max[wid] = most;
         __syncthreads();
-        if (threadIdx.x == 0) atomicMax(largest, __float_as_uint(fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]))));
+        if (threadIdx.x == 0) largest[blockIdx.x] = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
     }
 }
 
@@ -149,7 +150,7 @@ struct TileLds {
 };
 
 template <int D, bool F32, bool USERS>
-__device__ __forceinline__ void lay_tile(const Args &a, int64_t tile, const float *__restrict__ weight, const uint32_t *__restrict__ largest, uint4 *__restrict__ rowm,
+__device__ __forceinline__ void lay_tile(const Args &a, int64_t tile, const float *__restrict__ weight, const float *__restrict__ largest, int groups, uint4 *__restrict__ rowm,
                                          uint4 *__restrict__ tr, float *__restrict__ factor, TileLds<D, F32> &lds)
 {
     constexpr int TPR = D / 8;
@@ -157,7 +158,9 @@ __device__ __forceinline__ void lay_tile(const Args &a, int64_t tile, const floa
     float *const s_max = lds.max, *const s_mul = lds.mul;
     const int tid = threadIdx.x;
     const int64_t n = USERS ? a.rows : a.cat;
-    float m = 0.0f;
+    float m = 0.0f;                       // items: the tile's largest element; users: the largest w |P|
+    if constexpr (USERS && F32)
+        for (int t = tid; t < groups; t += 256) m = fmaxf(m, largest[t]);
     for (int t = tid; t < kTile * TPR; t += 256) {
         const int r = t / TPR, c = 8 * (t % TPR);
         const int64_t at = tile * kTile + r;
@@ -172,7 +175,7 @@ __device__ __forceinline__ void lay_tile(const Args &a, int64_t tile, const floa
             float big = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) { v[j] = row < 0 ? 0.0f : v[j]; big = fmaxf(big, finite_abs(v[j])); x[r][c + j] = v[j]; }
-            m = fmaxf(m, big);
+            if constexpr (!USERS) m = fmaxf(m, big);
             if constexpr (USERS) {            // the row's own scale: its TPR threads are neighbours (a power of two, at most 32)
 #pragma unroll
                 for (int o = TPR / 2; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor(big, o, TPR));
@@ -196,32 +199,27 @@ __device__ __forceinline__ void lay_tile(const Args &a, int64_t tile, const floa
         if (tid < kTile) s_mul[tid] = weight[tile * kTile + tid];
     }
     if constexpr (F32) {
-        if constexpr (USERS) {
-            float up, down;
-            scale_for(__uint_as_float(*largest), &up, &down, -100);      // (weights may be small)
-            if (tid < kTile) s_mul[tid] = weight[tile * kTile + tid] * up;
-            if (tile == 0 && tid == 0) factor[0] = down;
-        } else {
 #pragma unroll
-            for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-            if ((tid & 63) == 0) s_max[tid >> 6] = m;
-        }
+        for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+        if ((tid & 63) == 0) s_max[tid >> 6] = m;
     }
     __syncthreads();
-    if constexpr (F32 && !USERS) {
+    if constexpr (F32) {
         float up, down;
-        scale_for(fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3])), &up, &down);
-        if (tid == 0) factor[tile] = down;
-        if (tid < kTile) s_mul[tid] = up;
-        for (int t = tid; t < kTile * TPR; t += 256) {
-            const int r = t / TPR, c = 8 * (t % TPR);
-            float v[8];
+        scale_for(fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3])), &up, &down, USERS ? -100 : -40);      // (weights may be small)
+        if (tid == 0 && (!USERS || tile == 0)) factor[tile] = down;
+        if (tid < kTile) s_mul[tid] = USERS ? weight[tile * kTile + tid] * up : up;
+        if constexpr (!USERS) {
+            for (int t = tid; t < kTile * TPR; t += 256) {
+                const int r = t / TPR, c = 8 * (t % TPR);
+                float v[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = x[r][c + j] * up;
-            Frag h, l;
-            split8(v, &h, &l);
-            rowm[(size_t)(tile * kTile + r) * (2 * TPR) + t % TPR] = h.u;
-            rowm[(size_t)(tile * kTile + r) * (2 * TPR) + TPR + t % TPR] = l.u;
+                for (int j = 0; j < 8; ++j) v[j] = x[r][c + j] * up;
+                Frag h, l;
+                split8(v, &h, &l);
+                rowm[(size_t)(tile * kTile + r) * (2 * TPR) + t % TPR] = h.u;
+                rowm[(size_t)(tile * kTile + r) * (2 * TPR) + TPR + t % TPR] = l.u;
+            }
         }
         __syncthreads();
     }
@@ -256,18 +254,16 @@ __device__ __forceinline__ void lay_tile(const Args &a, int64_t tile, const floa
     }
 }
 
-// everything before the positions' coefficients, in one launch: workgroups [0, tiles) lay out the item tiles (in the first pass, the first of them also clears
-// the maxima that rows_kernel fills), the rest write a position's seen bits each
+// everything before the positions' coefficients, in one launch: workgroups [0, tiles) lay out the item tiles (in the first pass), the rest write a
+// position's seen bits each
 template <int D, bool F32>
 __global__ __launch_bounds__(256) void items_kernel(Args a, const int64_t *__restrict__ indptr, const int32_t *__restrict__ indices, int64_t tiles, uint4 *__restrict__ rowm,
-                                                    uint4 *__restrict__ tr, float *__restrict__ factor, uint32_t *__restrict__ bits, uint32_t *__restrict__ largest, int64_t passes)
+                                                    uint4 *__restrict__ tr, float *__restrict__ factor, uint32_t *__restrict__ bits)
 {
     __shared__ __attribute__((aligned(16))) union { TileLds<D, F32> tile; uint32_t bits[kBitWords]; } lds;
     const int64_t at = blockIdx.x;
     if (at < tiles) {
-        if (at == 0)
-            for (int64_t k = threadIdx.x; k < passes; k += 256) largest[k] = 0u;
-        lay_tile<D, F32, false>(a, at, nullptr, nullptr, rowm, tr, factor, lds.tile);
+        lay_tile<D, F32, false>(a, at, nullptr, nullptr, 0, rowm, tr, factor, lds.tile);
         return;
     }
     const int32_t u = a.user_ids[at - tiles];
@@ -275,11 +271,11 @@ __global__ __launch_bounds__(256) void items_kernel(Args a, const int64_t *__res
 }
 
 template <int D, bool F32>
-__global__ __launch_bounds__(256) void users_kernel(Args a, const float *__restrict__ weight, const uint32_t *__restrict__ largest, uint4 *__restrict__ rowm, uint4 *__restrict__ tr,
+__global__ __launch_bounds__(256) void users_kernel(Args a, const float *__restrict__ weight, const float *__restrict__ largest, int groups, uint4 *__restrict__ rowm, uint4 *__restrict__ tr,
                                                     float *__restrict__ factor)
 {
     __shared__ __attribute__((aligned(16))) TileLds<D, F32> lds;
-    lay_tile<D, F32, true>(a, blockIdx.x, weight, largest, rowm, tr, factor, lds);
+    lay_tile<D, F32, true>(a, blockIdx.x, weight, largest, groups, rowm, tr, factor, lds);
 }
 
 // ---- the pass -------------------------------------------------------------------------------------------------------------------------
@@ -700,12 +696,24 @@ struct Ws {
 
 int64_t pad128(int64_t n) { return (n + 127) / 128 * 128; }
 
-// pieces of a pass: a full device's workgroups, but pieces of at least `st` tiles; and the segments a block may have then
+// workgroups of rows_kernel: four positions each while the chip has room (a chain of loads a position: as many at once as it holds)
+int row_groups(int64_t padded)
+{
+    const int64_t most = 4 * (int64_t)rsx_num_cus();
+    return (int)(padded / 4 < most ? padded / 4 : most);
+}
+
+// Pieces of a pass, of at least `st` tiles: each of the two passes fills the device, so that the device deals their pieces out as it gets through them; with
+// fewer than 16 tiles a piece, where a piece's start and its partial sums cost as much as its tiles, both together (315 x 8135 x 256 fp32, three
+// tiles a piece and then six: 90 -> 69 us, 1000 x 20000 x 128 bf16 71 -> 58).
 int grad_pieces(int64_t stay, int64_t flow_tiles, int wgs, int st)
 {
-    const int64_t slots = (int64_t)wgs * rsx_num_cus(), most = (pad128(stay) / 128 * flow_tiles + st - 1) / st;
+    const int64_t units = pad128(stay) / 128 * flow_tiles, most = (units + st - 1) / st;
+    int64_t slots = (int64_t)wgs * rsx_num_cus();
+    if (units < 16 * slots) slots /= 2;
     return (int)(most < slots ? most : slots);
 }
+// and the segments a block of 128 columns may have then
 int64_t grad_segments(int64_t stay, int64_t flow_tiles, int pieces)
 {
     const int64_t per = pad128(stay) / 128 * flow_tiles / pieces;            // tiles of a piece, at least
@@ -755,7 +763,7 @@ Ws carve(void *ws, int64_t rows, int64_t cat, int d, int dtype, bool mask, int T
     w.coef = (float *)take(w.pass * T * 4);
     w.named = (int32_t *)take(w.pass * T * 4);
     w.prm = (Prm *)take(user_tiles * (int64_t)sizeof(Prm));
-    w.scalars = (uint32_t *)take((kLargest + w.passes) * 4);
+    w.scalars = (uint32_t *)take((kLargest + row_groups(w.pad_p)) * 4);
     w.bits = (uint32_t *)take(mask ? w.pass * mask_words(cat) * 4 : 0);
     w.part_p = (float *)take(cells * d * 4);
     w.part_q = (float *)take(w.passes * w.seg_q * w.pad_q * d * 4);
@@ -775,15 +783,15 @@ void run(const Args &all, const int64_t *indptr, const int32_t *indices, const W
         a.user_ids += r0; a.lse += r0; a.g += r0 * a.T; a.items += r0 * a.T;
         if (a.ent) a.ent += r0;
         if (a.h) a.h += r0;
-        uint32_t *const largest = w.scalars + kLargest;
+        float *const largest = (float *)w.scalars + kLargest;
         const int64_t pad = pad128(a.rows), user_tiles = pad / kTile, item_tiles = k == 0 ? w.pad_q / kTile : 0, bit_rows = indptr ? a.rows : 0;
         if (item_tiles + bit_rows > 0)
             hipLaunchKernelGGL((items_kernel<D, F32>), dim3((unsigned)(item_tiles + bit_rows)), dim3(256), 0, st, a, indptr, indices, item_tiles, (uint4 *)w.item_rm, (uint4 *)w.item_t,
-                               w.tile_factor, w.bits, largest, w.passes);
-        const int64_t row_wgs = pad / 4 < 2 * (int64_t)rsx_num_cus() ? pad / 4 : 2 * (int64_t)rsx_num_cus();
-        hipLaunchKernelGGL((rows_kernel<D, F32>), dim3((unsigned)row_wgs), dim3(256), 0, st, a, indptr ? w.bits : (const uint32_t *)nullptr, pad, w.prm, w.weight, w.named, w.coef, w.scalars,
-                           largest + k, w.tile_factor, w.pad_q / kTile);
-        hipLaunchKernelGGL((users_kernel<D, F32>), dim3((unsigned)user_tiles), dim3(256), 0, st, a, w.weight, largest + k, (uint4 *)w.user_rm, (uint4 *)w.user_t, w.user_factor + k);
+                               w.tile_factor, w.bits);
+        const int groups = row_groups(pad);
+        hipLaunchKernelGGL((rows_kernel<D, F32>), dim3((unsigned)groups), dim3(256), 0, st, a, indptr ? w.bits : (const uint32_t *)nullptr, pad, w.prm, w.weight, w.named, w.coef, w.scalars,
+                           largest, w.tile_factor, w.pad_q / kTile);
+        hipLaunchKernelGGL((users_kernel<D, F32>), dim3((unsigned)user_tiles), dim3(256), 0, st, a, w.weight, largest, groups, (uint4 *)w.user_rm, (uint4 *)w.user_t, w.user_factor + k);
         Pass p;                               // users stay
         p.top_factor = w.scalars; p.prm = w.prm; p.bits = w.bits; p.named = w.named; p.coef = w.coef;
         p.positions = a.rows; p.cat = a.cat; p.T = a.T; p.factor = a.scale * kLog2e;
