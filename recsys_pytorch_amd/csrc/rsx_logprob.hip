@@ -562,9 +562,10 @@ __device__ __forceinline__ float group_sum(float v)
     return v;
 }
 
-// NT threads a row: 1024 where rows are few and one row's chain of loads is the time, 256 where many rows share a CU
+// NT threads a row: 1024 where rows are few and one row's chain of loads is the time, 512 up to two rows a CU, 256 where more rows share a CU (whole call,
+// 300 x 50K x 256: 144 us with 256, 130 with 512, 154 with 1024; 943 x 1682 x 64: 46 with 256, 60 with 512)
 template <int D, bool F32, int NT>
-__global__ __launch_bounds__(NT, (NT == 1024 ? 4 : 5)) void finish_kernel(const void *__restrict__ P, const void *__restrict__ Q, Shape sh, const uint32_t *__restrict__ bits,
+__global__ __launch_bounds__(NT, (NT >= 512 ? 4 : 5)) void finish_kernel(const void *__restrict__ P, const void *__restrict__ Q, Shape sh, const uint32_t *__restrict__ bits,
                                                     const float4 *__restrict__ part, int splits, const uint16_t *__restrict__ keys,
                                                     const float *__restrict__ row_ref, const int32_t *__restrict__ given, int T, int K, float *__restrict__ logp,
                                                     float *__restrict__ lse_out, float *__restrict__ ent_out, int32_t *__restrict__ top_idx, float *__restrict__ top_logp)
@@ -1017,7 +1018,7 @@ void run(const Call &c, const Ws &w, hipStream_t st)
 #define RSX_LP_FINISH(NT_) hipLaunchKernelGGL((finish_kernel<D, F32, NT_>), dim3((unsigned)sh.rows), dim3(NT_), 0, st, c.P, c.Q, sh, c.indptr ? w.bits : (const uint32_t *)nullptr, \
                                               w.part, parts, w.keys, w.ref, c.given + (c.T ? r0 * c.T : 0), c.T, c.K, c.logp + (c.T ? r0 * c.T : 0), \
                                               c.lse ? c.lse + r0 : nullptr, c.ent ? c.ent + r0 : nullptr, c.top_idx + (c.K ? r0 * c.K : 0), c.top_logp + (c.K ? r0 * c.K : 0))
-        if (sh.rows <= rsx_num_cus()) RSX_LP_FINISH(1024); else RSX_LP_FINISH(256);
+        if (sh.rows <= rsx_num_cus()) RSX_LP_FINISH(1024); else if (sh.rows <= 2 * rsx_num_cus()) RSX_LP_FINISH(512); else RSX_LP_FINISH(256);
 #undef RSX_LP_FINISH
     }
 }

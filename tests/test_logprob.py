@@ -271,3 +271,17 @@ def test_hip_logprobs_captured_on_another_stream_and_reproducible():
             eager = rsx.score_logprobs(P, Q, u, t, K=10, mask=mask)
             torch.cuda.synchronize()
             assert all(torch.equal(a, b) for a, b in zip(eager, held)), k
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("d", [32, 64, 128, 256])
+@pytest.mark.parametrize("n,tied", [(513, False), (300, True), (513, True)])
+def test_hip_logprobs_of_more_rows_than_the_chip_has_room_for_at_once(n, tied, d, bf16):
+    """the last kernel's forms for up to two rows a CU and for more; tied: every item four times, so that whole chunks tie at the border"""
+    rng = np.random.default_rng(n + d)
+    P, Q = tables(rng, 97, 640, d, bf16)
+    if tied:
+        Q = Q[:160].repeat(4, 1).reshape(640, d).contiguous()
+    users = rng.integers(-1, 98, n)
+    check(P, Q, users, rng.integers(-1, 641, (n, 2)), 30, seen_csr(rng, 97, 640, 60), 1.0)
