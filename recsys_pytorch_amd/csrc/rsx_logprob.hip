@@ -547,6 +547,26 @@ __device__ __forceinline__ float half_value(uint32_t order)
     return (float)__builtin_bit_cast(_Float16, h);
 }
 
+// EPL elements of a table row as they lie in memory
+template <bool F32, int EPL>
+struct RowPiece {
+    uint4 lo, hi;                                             // (16 bytes: lo alone)
+    __device__ __forceinline__ float at(int j) const
+    {
+        const uint32_t a[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+        return F32 ? __uint_as_float(a[j]) : __uint_as_float(j & 1 ? a[j / 2] & 0xFFFF0000u : a[j / 2] << 16);
+    }
+};
+template <bool F32, int EPL>
+__device__ __forceinline__ RowPiece<F32, EPL> load_piece(const void *base, int64_t at)
+{
+    RowPiece<F32, EPL> v{};
+    const uint4 *src = reinterpret_cast<const uint4 *>((const char *)base + at * (F32 ? 4 : 2));
+    v.lo = src[0];
+    if constexpr (F32 && EPL == 8) v.hi = src[1];
+    return v;
+}
+
 // sum over groups of LPI neighbouring lanes, in their last one
 template <int LPI>
 __device__ __forceinline__ float group_sum(float v)
@@ -570,7 +590,9 @@ __global__ __launch_bounds__(NT, (NT >= 512 ? 4 : 5)) void finish_kernel(const v
                                                     const float *__restrict__ row_ref, const int32_t *__restrict__ given, int T, int K, float *__restrict__ logp,
                                                     float *__restrict__ lse_out, float *__restrict__ ent_out, int32_t *__restrict__ top_idx, float *__restrict__ top_logp)
 {
-    constexpr int LPI = F32 ? D / 4 : D / 8, EPL = F32 ? 4 : 8, IPP = NT / LPI;        // lanes an item's row takes, elements a lane, items a pass
+    // elements of an item's row a lane takes, lanes a row, items a pass.  fp32: eight where the work of many rows is the time (fewer additions between lanes:
+    // 943 x 1682 x 64 48 -> 43 us, 600 x 50K x 256 167 -> 149), four where one row's chain is (34.1 us a call against 35.4)
+    constexpr int EPL = F32 && NT == 1024 ? 4 : 8, LPI = D / EPL, IPP = NT / LPI;
     constexpr int NW = NT / 64, KR = NT == 1024 ? 16 : 8, FL = NT == 1024 ? 8 : 4;                               // wavefronts; 16-byte loads of maxima a thread keeps; item rows on the way together
     __shared__ __attribute__((aligned(16))) double c_s[kCand];
     __shared__ __attribute__((aligned(16))) int32_t c_id[kCand];
@@ -602,16 +624,12 @@ __global__ __launch_bounds__(NT, (NT >= 512 ? 4 : 5)) void finish_kernel(const v
     if (K > 0) fetch(0);
     const int li = tid % LPI;
     double p[EPL];
-    auto widen = [](const uint4 &v, double *x) {
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    auto piece = [&](const void *base, int64_t row) { return load_piece<F32, EPL>(base, row * D + EPL * li); };
+    {
+        const RowPiece<F32, EPL> v = piece(P, u);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if constexpr (F32) x[j] = (double)__uint_as_float(w[j]);
-            else { x[2 * j] = (double)__uint_as_float(w[j] << 16); x[2 * j + 1] = (double)__uint_as_float(w[j] & 0xFFFF0000u); }
-        }
-    };
-    widen(*reinterpret_cast<const uint4 *>((const char *)P + (size_t)u * (D * (F32 ? 4 : 2)) + li * 16), p);
-
+        for (int j = 0; j < EPL; ++j) p[j] = (double)v.at(j);
+    }
     float pf[EPL];
 #pragma unroll
     for (int j = 0; j < EPL; ++j) pf[j] = (float)p[j];
@@ -655,16 +673,14 @@ __global__ __launch_bounds__(NT, (NT >= 512 ? 4 : 5)) void finish_kernel(const v
     auto masked = [&](int32_t i) { return seen != nullptr && ((seen[i >> 5] >> (i & 31)) & 1u); };
     // FL items at a time
     auto dots = [&](const int32_t (&i)[FL], double (&z)[FL]) {
-        uint4 v[FL];
+        RowPiece<F32, EPL> v[FL];
 #pragma unroll
-        for (int n = 0; n < FL; ++n) v[n] = *reinterpret_cast<const uint4 *>((const char *)Q + (size_t)i[n] * (D * (F32 ? 4 : 2)) + li * 16);
+        for (int n = 0; n < FL; ++n) v[n] = piece(Q, i[n]);
 #pragma unroll
         for (int n = 0; n < FL; ++n) {
-            double q[EPL];
-            widen(v[n], q);
             z[n] = 0.0;
 #pragma unroll
-            for (int j = 0; j < EPL; ++j) z[n] = fma(p[j], q[j], z[n]);
+            for (int j = 0; j < EPL; ++j) z[n] = fma(p[j], (double)v[n].at(j), z[n]);
         }
 #pragma unroll
         for (int o = LPI / 2; o > 0; o >>= 1)
@@ -793,31 +809,45 @@ __global__ __launch_bounds__(NT, (NT >= 512 ? 4 : 5)) void finish_kernel(const v
     if (n > 0) {
         for (int q0 = tid / LPI; q0 < n; q0 += FL * IPP) {
             int32_t i[FL];
-            uint4 v[FL];
+            RowPiece<F32, EPL> v[FL];
 #pragma unroll
             for (int k = 0; k < FL; ++k) {
                 const int e = q0 + k * IPP;
                 const int64_t at = e < n ? chunk_item0(s_list[e >> 3]) + (e & 3) + 2 * (e & 4) : sh.items;
                 i[k] = at < sh.items ? (int32_t)at : -1;
-                v[k] = *reinterpret_cast<const uint4 *>((const char *)Q + (size_t)(i[k] < 0 ? 0 : i[k]) * (D * (F32 ? 4 : 2)) + li * 16);
+                v[k] = piece(Q, i[k] < 0 ? 0 : i[k]);
             }
-#pragma unroll
-            for (int k = 0; k < FL; ++k) {
-                const uint32_t w[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
-                float z = 0.0f, size = 0.0f;
-#pragma unroll
-                for (int j = 0; j < EPL; ++j) {
-                    const float y = F32 ? __uint_as_float(w[j % 4]) : __uint_as_float(j & 1 ? w[j / 2] & 0xFFFF0000u : w[j / 2] << 16);
-                    z = fmaf(pf[j], y, z);
-                    size = fmaf(fabsf(pf[j]), fabsf(y), size);
-                }
-                z = group_sum<LPI>(z) * sh.scale;
-                const float err = group_sum<LPI>(size) * (sh.scale * (D + 8) * 0x1p-24f) + fabsf(cut) * 0x1p-22f;
+            auto reaches = [&](int k, float z, float err) {
                 if (li == LPI - 1 && i[k] >= 0 && z + err >= cut && !masked(i[k])) {
                     const int at = atomicAdd(&s_n, 1);
                     if (at < kMaxChunks) s_item[at] = i[k];
                     if (z - err >= cut) atomicAdd(&s_count, 1);
                 }
+            };
+            auto bound = [&](float size) { return group_sum<LPI>(size) * (sh.scale * (D + 8) * 0x1p-24f) + fabsf(cut) * 0x1p-22f; };
+            float size = 0.0f, err = 0.0f;   // sums of |x||y|
+            if constexpr (F32 && EPL == 8) { // (one for the FL items, with the largest of their elements in every place)
+#pragma unroll
+                for (int j = 0; j < EPL; ++j) {
+                    float most = fabsf(v[0].at(j));
+#pragma unroll
+                    for (int k = 1; k < FL; ++k) most = fmaxf(most, fabsf(v[k].at(j)));
+                    size = fmaf(fabsf(pf[j]), fminf(most, 3.0e38f), size);      // (an infinity of a masked item is not to make its neighbours' bound a NaN)
+                }
+                err = bound(size);
+            }
+#pragma unroll
+            for (int k = 0; k < FL; ++k) {
+                float z = 0.0f;
+                if constexpr (!(F32 && EPL == 8)) size = 0.0f;
+#pragma unroll
+                for (int j = 0; j < EPL; ++j) {
+                    z = fmaf(pf[j], v[k].at(j), z);
+                    if constexpr (!(F32 && EPL == 8)) size = fmaf(fabsf(pf[j]), fabsf(v[k].at(j)), size);
+                }
+                z = group_sum<LPI>(z) * sh.scale;
+                if constexpr (!(F32 && EPL == 8)) err = bound(size);
+                reaches(k, z, err);
             }
         }
         __syncthreads();

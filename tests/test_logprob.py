@@ -285,3 +285,21 @@ def test_hip_logprobs_of_more_rows_than_the_chip_has_room_for_at_once(n, tied, d
         Q = Q[:160].repeat(4, 1).reshape(640, d).contiguous()
     users = rng.integers(-1, 98, n)
     check(P, Q, users, rng.integers(-1, 641, (n, 2)), 30, seen_csr(rng, 97, 640, 60), 1.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [7, 300, 600])
+@pytest.mark.parametrize("d", [32, 128])
+def test_hip_logprobs_of_zero_elements_beside_infinities_in_masked_places(d, n):
+    """infinities and NaN in items that everybody has seen, zeros in the users' rows: 0 * inf of a masked item is no neighbour's business"""
+    rng = np.random.default_rng(n + d)
+    P, Q = tables(rng, n, 1000, d, False)
+    P[:, : d // 2] = 0.0
+    P[::3] = 0.0
+    bad = rng.permutation(1000)[:120]
+    Q[bad[:60], : d // 4] = float("inf")
+    Q[bad[60:], 1] = float("nan")
+    indptr, indices = seen_csr(rng, n, 1000, 20)
+    rows = [np.union1d(indices[indptr[u]:indptr[u + 1]], bad) for u in range(n)]
+    mask = np.concatenate([[0], np.cumsum([len(r) for r in rows])]).astype(np.int64), np.concatenate(rows).astype(np.int32)
+    check(P, Q, np.arange(n), rng.integers(0, 1000, (n, 3)), 40, mask, 1.0)
