@@ -965,12 +965,12 @@ int64_t wide_splits(int64_t rows, int64_t items, int d, int dtype)
     return s < 1 ? 1 : s > groups ? groups : s;
 }
 
-// a pass' bits and chunk maxima are held to 768 MB
+// a pass' bits and chunk maxima are held to 768 MB, its blocks of rows to what a grid's second dimension takes
 int64_t pass_rows(int64_t rows, int64_t items)
 {
     const int64_t per = mask_words(items) * 4 + (items + 127) / 128 * 32;
     int64_t most = (768ll << 20) / per / 256 * 256;
-    most = most < 256 ? 256 : most;
+    most = most < 256 ? 256 : most > (1ll << 22) ? 1ll << 22 : most;
     return rows < most ? rows : most;
 }
 

@@ -303,3 +303,23 @@ def test_hip_logprobs_of_zero_elements_beside_infinities_in_masked_places(d, n):
     rows = [np.union1d(indices[indptr[u]:indptr[u + 1]], bad) for u in range(n)]
     mask = np.concatenate([[0], np.cumsum([len(r) for r in rows])]).astype(np.int64), np.concatenate(rows).astype(np.int32)
     check(P, Q, np.arange(n), rng.integers(0, 1000, (n, 3)), 40, mask, 1.0)
+
+
+@pytest.mark.gpu
+def test_hip_logprobs_of_more_rows_than_a_grids_second_dimension_takes():
+    """nine million positions of a catalog of three"""
+    import torch
+    from recsys_pytorch_amd import rsx
+    P, Q = tables(np.random.default_rng(4), 50, 3, 32, False)
+    n = 9_000_000
+    users = torch.arange(n, dtype=torch.int32, device="cuda") % 50
+    got = rsx.score_logprobs(P, Q, users, (users % 3).view(-1, 1).contiguous(), K=2)
+    u = np.arange(150) % 50
+    logp, lse, ent, top, topv, ez = reference(P.double().cpu().numpy(), Q.double().cpu().numpy(), u, (u % 3)[:, None], 2, None, 1.0)
+    el = ez + 5e-5
+    dev = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda().view(1, 150, -1)
+    whole = lambda t: t.view(n // 150, 150, -1)
+    assert (whole(got.top_idx) == dev(top)).all()
+    for a, b, tol in ((got.lse, lse, el + 2.0 ** -24 * np.abs(lse)), (got.entropy, ent, el * (2 + ent) + ez), (got.logp, logp, el[:, None] + 2.0 ** -24 * np.abs(logp)),
+                      (got.top_logp, topv, el[:, None] + 2.0 ** -24 * np.abs(topv))):
+        assert ((whole(a).double() - dev(b)).abs() <= dev(tol)).all()
