@@ -840,6 +840,7 @@ RSX_API int rsx_score_logprobs_grad(const void *P, int64_t num_users, const int3
     RSX_CHECK_ARG(T >= 0 && (T == 0 || (items_dev && g_logp_dev)), "T items per row need their ids and gradients");
     RSX_CHECK_ARG(T > 0 || g_entropy_dev != nullptr, "nothing to differentiate");
     RSX_CHECK_ARG(aligned16(P) && aligned16(Q) && aligned16(GP_out) && aligned16(GQ_out), "table rows must be 16-byte aligned");
+    RSX_CHECK_ARG(GP_out != GQ_out && GP_out != P && GP_out != Q && GQ_out != P && GQ_out != Q, "the gradients need memory of their own");
     const Ws w = carve(ws, num_rows, num_items, d, dtype, mask_indptr_dev != nullptr, T);
     if (ws == nullptr || ws_bytes < w.bytes || !aligned16(ws)) {
         rsx_set_error("rsx_score_logprobs_grad: workspace of %lld bytes (16-byte aligned) required, got %lld", (long long)w.bytes, (long long)ws_bytes);

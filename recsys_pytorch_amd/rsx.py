@@ -1190,7 +1190,9 @@ def score_logprobs_grad(P, Q, user_ids, items, lse, g_logp, entropy=None, g_entr
     (num_users, d), num_items = P.shape, Q.shape[0]
     if (entropy is None) != (g_entropy is None):
         raise RsxError("entropy and g_entropy come together")
-    vec = lambda t, n, name: _dev(t, torch.float32, name) if t.numel() == n else _shape_error(name, n)
+    if (items is None) != (g_logp is None):
+        raise RsxError("items and g_logp come together")
+    vec = lambda t, n, name: _dev(t, torch.float32, name) if isinstance(t, torch.Tensor) and t.numel() == n else _shape_error(name, n)
     pl = vec(lse, rows, "lse")
     pg = vec(g_logp, rows * T, "g_logp") if items is not None else None
     pe, ph = (vec(entropy, rows, "entropy"), vec(g_entropy, rows, "g_entropy")) if entropy is not None else (None, None)

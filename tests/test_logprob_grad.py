@@ -124,14 +124,14 @@ def test_refusals():
         with pytest.raises(rsx.RsxError):
             call()
     L = rsx.lib()
-    good = dict(P=16, U=4, ids=16, n=2, Q=16, I=300, d=32, dt=0, mp=None, mi=None, scale=1.0, items=16, T=1, lse=16, g=16, ent=None, h=None, GP=16, GQ=16)
+    good = dict(P=16, U=4, ids=16, n=2, Q=16, I=300, d=32, dt=0, mp=None, mi=None, scale=1.0, items=16, T=1, lse=16, g=16, ent=None, h=None, GP=32, GQ=48)
 
     def call(**kw):
         k = {**good, **kw}
         return L.rsx_score_logprobs_grad(k["P"], k["U"], k["ids"], k["n"], k["Q"], k["I"], k["d"], k["dt"], k["mp"], k["mi"], k["scale"], k["items"], k["T"],
                                          k["lse"], k["g"], k["ent"], k["h"], k["GP"], k["GQ"], None, 0, None)
     for bad in (dict(P=None), dict(GQ=None), dict(GP=8), dict(lse=None), dict(n=0), dict(n=2 ** 31), dict(I=0), dict(d=100), dict(dt=3), dict(mi=16),
-                dict(scale=-1.0), dict(T=0), dict(g=None), dict(items=None), dict(ent=16), dict(h=16)):
+                dict(scale=-1.0), dict(GP=48), dict(GP=16), dict(GQ=16), dict(T=0), dict(g=None), dict(items=None), dict(ent=16), dict(h=16)):
         assert call(**bad) == -1, bad
     assert call() == -3 and b"workspace" in L.rsx_last_error() and call(T=0, items=None, g=None, ent=16, h=16) == -3
     assert L.rsx_add_rows(16, 4, 31, 16, 16, 0, 1, None) == -1 and L.rsx_add_rows(16, 0, 32, 16, 16, 0, 1, None) == -1
