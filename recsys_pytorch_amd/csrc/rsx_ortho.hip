@@ -373,33 +373,34 @@ __global__ __launch_bounds__(256) void ns_next_kernel(const double *__restrict__
 
 // d <= 64: the whole iteration in one workgroup, the four matrices in LDS (128 KB at d = 64).  Blocks of the upper triangles are dealt to 16 wavefronts
 // (M T and A T together: 20 blocks, five a SIMD); both triangles are written.  Bound by one CU's fp64 matrix rate and the
-// LDS reads before it (five steps at d = 64: 38 us, about 24 of them products).
+// LDS reads before it (five steps at d = 64: 33 us, about 22 of them products; 38 before the addresses were one place and constant offsets).
 // Columns are XORed by row: the two rows of a half-wavefront's read lie in different halves of the 256 bytes the LDS delivers a cycle, and the 16 rows
 // of a transposed store in eight different places.
+constexpr int kSmallThreads = 1024;      // (512: fewer wavefronts to cover the LDS reads, a 1682 x 64 step 54 us for 52)
 template <int D, typename O>
-__global__ __launch_bounds__(1024) void ns_small_kernel(const double *__restrict__ G, O *__restrict__ out, int steps, Coeffs k)
+__global__ __launch_bounds__(kSmallThreads) void ns_small_kernel(const double *__restrict__ G, O *__restrict__ out, int steps, Coeffs k)
 {
-    constexpr int NB = n_blocks(D);
+    constexpr int NB = n_blocks(D), NW = kSmallThreads / 64, ONE = (NB + NW - 1) / NW, TWO = (2 * NB + NW - 1) / NW;      // a wavefront's blocks of one product, of a pair
     __shared__ __attribute__((aligned(16))) double A[D * D], T[D * D], W[D * D], M[D * D];
     __shared__ double s_norm;
     auto el = [](int r, int c) { return r * D + (c ^ (((r & 1) << 4) | ((r & 6) << 1))); };
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const double s = norm_scale(G, D, k.eps, &s_norm);
-    for (int t = tid; t < D * D; t += 1024) {
+    for (int t = tid; t < D * D; t += kSmallThreads) {
         const int r = t / D, c = t % D;
         A[el(r, c)] = s * s * G[t];
     }
     __syncthreads();
+    // el(4 i + (lane >> 4), 16 p + (lane & 15)) less 4 i D: one place for the even i, one for the odd ones
+    auto place = [&](int p, int odd) { const int r = lane >> 4; return r * D + ((16 * p) ^ ((r & 1) << 4)) + ((lane & 15) ^ ((r & 2) << 1) ^ (odd << 3)); };
     auto mul = [&](const double *x, const double *y, int p, int q) {
+        const int bx[2] = {place(p, 0), place(p, 1)}, by[2] = {place(q, 0), place(q, 1)};
         f64x4 acc = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
         for (int h = 0; h < D / 32; ++h) {                                // (eight steps' operands on their way before the first product)
             double fx[8], fy[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int kk = 32 * h + 4 * i + (lane >> 4);
-                fx[i] = x[el(kk, 16 * p + (lane & 15))]; fy[i] = y[el(kk, 16 * q + (lane & 15))];
-            }
+            for (int i = 0; i < 8; ++i) { fx[i] = x[bx[i & 1] + (32 * h + 4 * i) * D]; fy[i] = y[by[i & 1] + (32 * h + 4 * i) * D]; }
 #pragma unroll
             for (int i = 0; i < 8; ++i) acc = __builtin_amdgcn_mfma_f64_16x16x4f64(fx[i], fy[i], acc, 0, 0, 0);
         }
@@ -411,13 +412,14 @@ __global__ __launch_bounds__(1024) void ns_small_kernel(const double *__restrict
         x[el(r, c)] = v;
         x[el(c, r)] = v;
     };
-    int p, q, p2[2], q2[2];                                                // this wavefront's block of one product, and its two of a pair
-    ns_pq<D>(w < NB ? w : 0, &p, &q);
-#pragma unroll
-    for (int n = 0; n < 2; ++n) ns_pq<D>((w + 16 * n) % NB, &p2[n], &q2[n]);
     for (int step = 0; step < steps; ++step) {
         const bool last = step + 1 == steps;
-        if (w < NB) {
+        f64x4 x[TWO];                                                      // (results leave the registers when everybody has read what they replace)
+        int p, q;
+#pragma unroll
+        for (int n = 0; n < ONE; ++n) {
+            if (w + NW * n >= NB) continue;
+            ns_pq<D>(w + NW * n, &p, &q);
             const f64x4 sq = mul(A, A, p, q);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -426,33 +428,41 @@ __global__ __launch_bounds__(1024) void ns_small_kernel(const double *__restrict
             }
         }
         __syncthreads();
-        f64x4 x[2];                                                        // blocks w and w + 16 of A T, then M T
+        // blocks of A T, then of M T (not of A T in the last step, nor of M T in the first: M = s I)
+        const int first = last ? NB : 0, end = step == 0 ? NB : 2 * NB;
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            const int b = w + 16 * n;
-            if (b >= 2 * NB || (last && b < NB) || (step == 0 && b >= NB)) continue;
-            x[n] = mul(b < NB ? A : M, T, p2[n], q2[n]);
+        for (int n = 0; n < TWO; ++n) {
+            const int b = first + w + NW * n;
+            if (b >= end) continue;
+            ns_pq<D>(b % NB, &p, &q);
+            x[n] = mul(b < NB ? A : M, T, p, q);
         }
         __syncthreads();
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            const int b = w + 16 * n;
-            if (b >= 2 * NB || (last && b < NB) || (step == 0 && b >= NB)) continue;
+        for (int n = 0; n < TWO; ++n) {
+            const int b = first + w + NW * n;
+            if (b >= end) continue;
+            ns_pq<D>(b % NB, &p, &q);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) put(b < NB ? W : M, p2[n], q2[n], i, x[n][i]);
+            for (int i = 0; i < 4; ++i) put(b < NB ? W : M, p, q, i, x[n][i]);
         }
-        if (step == 0)                                                     // (M was s I: no product)
+        if (step == 0)
 #pragma unroll 1
-            for (int t = tid; t < D * D; t += 1024) M[t] = s * T[t];
+            for (int t = tid; t < D * D; t += kSmallThreads) M[t] = s * T[t];
         __syncthreads();
-        if (!last && w < NB) {
-            const f64x4 y = mul(W, T, p, q);
+        if (!last) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) put(A, p, q, i, y[i]);             // (A was last read before the barrier above)
+            for (int n = 0; n < ONE; ++n) {                                // (A was last read before the barrier above)
+                if (w + NW * n >= NB) continue;
+                ns_pq<D>(w + NW * n, &p, &q);
+                const f64x4 y = mul(W, T, p, q);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) put(A, p, q, i, y[i]);
+            }
         }
         __syncthreads();
     }
-    for (int t = tid; t < D * D; t += 1024) put_result<D>(out, t / D, t % D, M[el(t / D, t % D)]);
+    for (int t = tid; t < D * D; t += kSmallThreads) put_result<D>(out, t / D, t % D, M[el(t / D, t % D)]);
 }
 
 template <int D, typename O>
@@ -628,7 +638,7 @@ void newton_schulz(const OrthoWs &w, O *out, int steps, const Coeffs &k, hipStre
 {
     if (steps == 0) { hipLaunchKernelGGL((ns_identity_kernel<D, O>), dim3(1), dim3(256), 0, st, w.G, out, k.eps); return; }
     if constexpr (D <= 64) {
-        hipLaunchKernelGGL((ns_small_kernel<D, O>), dim3(1), dim3(1024), 0, st, w.G, out, steps, k);
+        hipLaunchKernelGGL((ns_small_kernel<D, O>), dim3(1), dim3(kSmallThreads), 0, st, w.G, out, steps, k);
     } else {
         constexpr int NB = n_blocks(D);
         double *A = w.A, *A2 = w.A2, *M = w.M, *M2 = w.M2;
