@@ -254,7 +254,8 @@ int rsx_pair_score(const float *P, const float *Q, const int32_t *u_dev, const i
  * mask_indices); rows need not be sorted, ids outside the catalog are ignored.  What a masked cell's product would have been
  * (infinities, NaN) does not matter.
  * rsx_score_logprobs_grad: gradient of sum_rt g_logp[r, t] logp_rt + sum_r g_entropy[r] H_r with respect to the rows:
- *   GP[r]  = sum_i dz_ri Q[i]  [num_rows x d],   GQ[i] = sum_r dz_ri P[user_ids[r]]  [num_items x d],   both overwritten, in dtype,
+ *   GP[r]  = sum_i dz_ri Q[i]  [num_rows x d],   GQ[i] = sum_r dz_ri P[user_ids[r]]  [num_items x d],   both overwritten, in dtype, in memory of
+ *   their own (equal pointers to a table's are refused),
  *   dz_ri  = scale (sum_t g_logp[r, t] ([i = items[r, t]] - p_ri) - g_entropy[r] p_ri (log p_ri + H_r))
  *   over unmasked i and the items that are neither masked nor outside the catalog (a masked item's logp is the constant -inf).
  *   An item listed twice counts twice.  lse, entropy: what rsx_score_logprobs returned for the same arguments (entropy and

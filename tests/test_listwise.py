@@ -293,3 +293,34 @@ def test_hip_command_line_takes_them(tmp_path):
     path.write_text("".join(f"{u}\t{u + n}\t5\t{12 * u + n}\n" for u in range(30) for n in range(12)))
     ret = main.main(["--data", str(path), "--hidden-dim", "32", "--optimizer", "muon", "--listwise", "--batch-size", "8", "--num-epochs", "2"])
     assert all(np.isfinite(v) for v in ret["scores"].values())
+
+
+@pytest.mark.gpu
+def test_hip_calls_at_once_on_two_streams():
+    """the calls of two training steps side by side, workspaces their own: the same bits as one after the other"""
+    from recsys_pytorch_amd import rsx
+    rng = np.random.default_rng(9)
+    f = lambda *s: torch.from_numpy(rng.standard_normal(s).astype(np.float32)).cuda()
+    jobs = []
+    for U, I, d, n in ((300, 5000, 64, 200), (500, 3001, 128, 129)):
+        jobs.append((f(U, d), f(I, d), torch.from_numpy(rng.integers(0, U, n).astype(np.int32)).cuda(), torch.from_numpy(rng.integers(0, I, (n, 2)).astype(np.int32)).cuda(), f(n, 2)))
+
+    def step(P, Q, u, it, g):
+        P, Q, M = P.clone(), Q.clone(), torch.zeros_like(Q)
+        lp = rsx.score_logprobs(P, Q, u, it, K=10)
+        GP, GQ = rsx.score_logprobs_grad(P, Q, u, it, lp.lse, g)
+        rsx.add_rows(P, u, GP)
+        rsx.muon_apply(Q, M, GQ, 0.02)
+        return (*lp, GP, P, Q, M, rsx.orthogonalize(P))
+    want = [step(*j) for j in jobs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(4):
+        for k in range(2):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(step(*jobs[k]))
+    torch.cuda.synchronize()
+    for k in range(2):
+        for run in got[k]:
+            assert all(torch.equal(a, b) for a, b in zip(run, want[k]))
