@@ -587,7 +587,7 @@ __device__ __forceinline__ float group_sum(float v)
 // NT threads a row: 1024 where rows are few and one row's chain of loads is the time, 512 up to two rows a CU, 256 where more rows share a CU (whole call,
 // 300 x 50K x 256: 144 us with 256, 130 with 512, 154 with 1024; 943 x 1682 x 64: 46 with 256, 60 with 512)
 template <int D, bool F32, int NT>
-__global__ __launch_bounds__(NT, (NT >= 512 ? 4 : 5)) void finish_kernel(const void *__restrict__ P, const void *__restrict__ Q, Shape sh, const uint32_t *__restrict__ bits,
+__global__ __launch_bounds__(NT, (NT >= 512 ? 4 : F32 ? 5 : 6)) void finish_kernel(const void *__restrict__ P, const void *__restrict__ Q, Shape sh, const uint32_t *__restrict__ bits,
                                                     const float4 *__restrict__ part, int splits, const uint16_t *__restrict__ keys,
                                                     const float *__restrict__ row_ref, const int32_t *__restrict__ given, int T, int K, float *__restrict__ logp,
                                                     float *__restrict__ lse_out, float *__restrict__ ent_out, int32_t *__restrict__ top_idx, float *__restrict__ top_logp)
@@ -595,12 +595,16 @@ __global__ __launch_bounds__(NT, (NT >= 512 ? 4 : 5)) void finish_kernel(const v
     // elements of an item's row a lane takes, lanes a row, items a pass.  fp32: eight where the work of many rows is the time (fewer additions between lanes:
     // 943 x 1682 x 64 48 -> 43 us, 600 x 50K x 256 167 -> 149), four where one row's chain is (34.1 us a call against 35.4)
     constexpr int EPL = F32 && NT == 1024 ? 4 : 8, LPI = D / EPL, IPP = NT / LPI;
+    // the maxima from the bound up are read again, by the few threads that have any, instead of kept: a sixth wavefront a SIMD fits (4000 x 20K x 64 bf16 102 ->
+    // 97 us; fp32, whose rows take more registers, would spill: 2000 x 50K x 128 150 -> 158)
+    constexpr bool AGAIN = !F32 && NT == 256;
     constexpr int NW = NT / 64, KR = NT == 1024 ? 16 : 8, FL = NT == 1024 ? 8 : 4;                               // wavefronts; 16-byte loads of maxima a thread keeps; item rows on the way together
     __shared__ __attribute__((aligned(16))) double c_s[kCand];
     __shared__ __attribute__((aligned(16))) int32_t c_id[kCand];
     __shared__ double s_red[3][NW];
     __shared__ __attribute__((aligned(16))) uint16_t s_max[256];
-    __shared__ int32_t s_list[kMaxChunks], s_item[kMaxChunks];
+    __shared__ int32_t s_list[kMaxChunks];
+    int32_t *const s_item = c_id;                  // (item e is read where its id is written back: the same value)
     __shared__ int s_n, s_count;
     __shared__ uint32_t s_tau;
     const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
@@ -707,7 +711,7 @@ __global__ __launch_bounds__(NT, (NT >= 512 ? 4 : 5)) void finish_kernel(const v
             for (int n_ = 0; n_ < KR; ++n_)
                 top8 = max2(top8, max2(max2(as_half2(kept[n_].x), as_half2(kept[n_].y)), max2(as_half2(kept[n_].z), as_half2(kept[n_].w))));
         }
-        uint32_t best = half_order(top8[0]);
+        uint32_t best = half_order(top8[0]);       // this thread's largest (NT > 256: that of NT / 256 threads)
         { const uint32_t x = half_order(top8[1]); best = x > best ? x : best; }
         if constexpr (NT > 256) {                  // 256 maxima, of NT / 256 threads each
 #pragma unroll
@@ -734,7 +738,8 @@ __global__ __launch_bounds__(NT, (NT >= 512 ? 4 : 5)) void finish_kernel(const v
         const uint32_t bound = s_tau;
         const _Float16 bound_h = (_Float16)half_value(bound);
         for (int64_t base = 0; base < chunks; base += 8ll * NT * KR) {
-            if (chunks > 8ll * NT * KR) fetch(base);
+            if (AGAIN ? best >= bound : chunks > 8ll * NT * KR) fetch(base);
+            else if (AGAIN) continue;
 #pragma unroll
             for (int n_ = 0; n_ < KR; ++n_) {
                 const half2v m2 = max2(max2(as_half2(kept[n_].x), as_half2(kept[n_].y)), max2(as_half2(kept[n_].z), as_half2(kept[n_].w)));
