@@ -963,7 +963,7 @@ struct Ws {
 
 int wide_users(int dtype) { return 128 * users_block(dtype == RSX_F32); }
 
-int64_t wide_splits(int64_t rows, int64_t items, int d, int dtype)
+int64_t wide_splits(int64_t rows, int64_t items, int dtype)
 {
     const int64_t slots = kWaves * (int64_t)rsx_num_cus(), ut = (rows + wide_users(dtype) - 1) / wide_users(dtype), groups = (items + 127) / 128;
     const int64_t s = slots / ut;
@@ -988,7 +988,7 @@ Ws carve(void *ws, int64_t rows, int64_t items, int d, int dtype, bool mask, int
     const int64_t tiles4 = (items + 127) / 128 * 4;
     const bool thin = rows <= thin_rows(d, dtype);
     w.pass = pass_rows(rows, items);
-    const int64_t parts = thin ? thin_groups(items) : wide_splits(w.pass, items, d, dtype);
+    const int64_t parts = thin ? thin_groups(items) : wide_splits(w.pass, items, dtype);
     // (the last, shorter pass takes more splits over fewer rows: rows x splits never exceeds this)
     const int64_t cells = thin ? rows * parts : w.pass * parts + kWaves * (int64_t)rsx_num_cus() * wide_users(dtype);
     w.planes = take(!thin && dtype == RSX_F32 ? tiles4 * kTile * (int64_t)d * 4 : 0);
@@ -1045,7 +1045,7 @@ void run(const Call &c, const Ws &w, hipStream_t st)
                 else if constexpr (MOST >= 4) launch_thin<D, F32, 4>(c, sh, w, parts, st);
             }
         } else {
-            parts = (int)wide_splits(sh.rows, items, D, F32 ? RSX_F32 : RSX_BF16);
+            parts = (int)wide_splits(sh.rows, items, F32 ? RSX_F32 : RSX_BF16);
             const dim3 grid((unsigned)parts, (unsigned)((sh.rows + WideGeo<D, F32>::WGU - 1) / WideGeo<D, F32>::WGU));
 #define RSX_LP_WIDE(M_, T_) hipLaunchKernelGGL((wide_kernel<D, F32, M_, T_>), grid, dim3(256), 0, st, c.P, F32 ? w.planes : (const char *)c.Q, w.factor, sh, w.bits, w.ref, parts, w.part, (uint4 *)w.keys)
             if (c.indptr) { if (c.K) RSX_LP_WIDE(true, true); else RSX_LP_WIDE(true, false); }
