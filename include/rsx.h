@@ -247,7 +247,7 @@ int rsx_pair_score(const float *P, const float *Q, const int32_t *u_dev, const i
  *   logp_out[r, t]  = z_r,items[r, t] - lse[r]                (T per row, T = 0: none; -inf for a masked item)
  *   topk_idx_out / topk_logp_out [num_rows x K]: the K most probable items in descending order and their log-probabilities
  *                     (K = 0: none; K <= 128).  Ties go to the lowest id.  The order is that of the products in 64 bits.
- *                     Fewer than K unmasked items: -1 and -inf.
+ *                     Fewer than K unmasked items with a score above -inf: -1 and -inf.
  * The scores are never stored.  P, Q: dtype RSX_F32 or RSX_BF16, both [. x d]; sums in fp32 and 64 bits.
  * A position whose user id is outside [0, num_users) names no row (a padded batch): lse -inf, entropy 0, logp 0, no top items.
  * An item id outside [0, num_items) names no item: its logp is 0.  mask_indptr: int64 [num_users + 1] (nullable with

@@ -10,7 +10,7 @@
 // scores of ONE row (items are the matrix instruction's rows, users its columns): all of this is lane-local.
 //
 // Top-K: the pass also stores the largest score of every 8 items as a half (relative to a score of the same row, so that halves
-// resolve it).  The K best items lie in chunks whose maximum is at least the K-th largest maximum; finish_kernel takes K + 8 chunks
+// resolve it; -inf only where all 8 are masked).  The K best items lie in chunks whose maximum is at least the K-th largest maximum; finish_kernel takes K + 8 chunks
 // and every tie, computes their items' products again in 64 bits and orders those.  What the fast products' rounding could swap is
 // decided by the 64-bit ones.
 //
@@ -62,7 +62,9 @@ __device__ __forceinline__ float pick_reference(float a, float b, float c)
     return fabsf(m) < 1.0e30f ? m : 0.0f;
 }
 
-__device__ __forceinline__ uint16_t half_bits(float v) { const _Float16 h = (_Float16)v; return __builtin_bit_cast(uint16_t, h); }
+// chunk maxima as halves, two at a time.  Rounded towards zero: what lies beyond a half's range stays finite (+-65504; the ties this makes are told apart by
+// their products in 64 bits), and -inf is left to the chunks that hold nothing
+__device__ __forceinline__ uint32_t key_bits(float a, float b) { return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b)); }
 
 // eight consecutive elements of a table row in fp32
 template <bool F32>
@@ -166,7 +168,7 @@ __device__ __forceinline__ void absorb(const f32x16 &acc, float f, uint32_t w, S
 #pragma unroll
     for (int i = 1; i < 8; ++i) { c0 = __builtin_elementwise_maximum(c0, x[i]); c1 = __builtin_elementwise_maximum(c1, x[8 + i]); }
     const float top = __builtin_elementwise_maximum(c0, c1) * f;
-    if constexpr (TOP) *key = (uint32_t)half_bits(fmaf(c0, f, -ref)) | ((uint32_t)half_bits(fmaf(c1, f, -ref)) << 16);
+    if constexpr (TOP) *key = key_bits(fmaf(c0, f, -ref), fmaf(c1, f, -ref));
     if (__builtin_amdgcn_ballot_w64(top > st.m + kLazy) != 0ull) {
         if (top > st.m) stat_lift(st, top);
     }
@@ -449,7 +451,7 @@ __global__ __launch_bounds__(256) void thin_kernel(const void *__restrict__ P, c
             const float top = c * f;
             if constexpr (TOP) {
                 const int64_t r = 16 * ub + l15;
-                if (r < sh.rows) keys[(size_t)r * (16 * groups) + 16 * (tile >> 2) + 8 * (g & 1) + 2 * (tile & 3) + (g >> 1)] = half_bits(fmaf(c, f, -ref[ub]));
+                if (r < sh.rows) keys[(size_t)r * (16 * groups) + 16 * (tile >> 2) + 8 * (g & 1) + 2 * (tile & 3) + (g >> 1)] = (uint16_t)key_bits(fmaf(c, f, -ref[ub]), 0.0f);
             }
             if (__builtin_amdgcn_ballot_w64(top > st[ub].m + kLazy) != 0ull) {
                 if (top > st[ub].m) stat_lift(st[ub], top);
@@ -800,7 +802,7 @@ __global__ __launch_bounds__(NT, (NT >= 512 ? 4 : F32 ? 5 : 6)) void finish_kern
         __syncthreads();
         whole = s_n > kMaxChunks;
         n = whole ? 0 : 8 * s_n;
-        // K items reach the K-th maximum; it is a rounded half of a fast product, and taken a little lower here.  (How much does not matter: if fewer
+        // K items reach the K-th maximum; it is a half (rounded towards zero) of a fast product, and taken a little lower here.  (How much does not matter: if fewer
         // than K scores certainly reach `cut`, nothing is left out.)
         if (!whole && s_n >= K) {
             const float h = half_value(s_tau), ref = row_ref[r];

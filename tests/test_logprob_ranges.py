@@ -1,0 +1,45 @@
+"""rsx.score_logprobs where values lie far apart: scores thousands of units below a row's best, item rows of very unequal length, masked
+rows of large finite values, long sums of equal terms.
+
+Tolerances: test_logprob.py's (its `check`), whose score error counts the unmasked items only; what a test allows instead is derived at it."""
+import numpy as np
+import pytest
+
+from test_logprob import check, reference, seen_csr, tables
+
+
+def _mask_all(users, ids):
+    return np.arange(users + 1, dtype=np.int64) * len(ids), np.tile(np.asarray(ids, np.int32), users)
+
+
+# ---- the K best ------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("n", [4, 140, 300, 600])
+def test_hip_top_items_of_scores_far_apart(n, bf16):
+    """scores over hundreds of thousands of units: far below a row's reference is not the same as masked"""
+    import torch
+    rng = np.random.default_rng(n)
+    for I, K, near in ((100, 100, 1), (3000, 128, 30)):
+        P, Q = (rng.standard_normal((r, 32)).astype(np.float32) for r in (n, I))
+        P[:, 0] = rng.choice([1.0, 2.0, -1.0], n)
+        P[:2, 0] = 1.0, -1.0
+        Q[:, 0] = 0.0
+        far = rng.permutation(I)[near:]
+        Q[far, 0] = -np.linspace(1e5, 3e5, I - near)
+        P, Q = torch.from_numpy(P).cuda(), torch.from_numpy(Q).cuda()
+        P, Q = (P.bfloat16(), Q.bfloat16()) if bf16 else (P, Q)
+        mask = _mask_all(n, far[:40]) if I == 3000 else None
+        check(P, Q, np.arange(n), rng.integers(0, I, (n, 2)), K, mask, rows=np.r_[0:4, n - 4:n])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,bf16", [(4, False), (4, True), (140, True), (600, True)])
+def test_hip_top_items_beside_masked_rows_of_large_values(n, bf16):
+    """finite products of 10^20 in masked places, where a row's reference may look too"""
+    rng = np.random.default_rng(n)
+    for I, bad in ((2, [1]), (33, [0, 16]), (900, [0, 450, 899]), (900, [450, 899])):
+        P, Q = tables(rng, n, I, 64, bf16)
+        P[:, 5] = P[:, 5].abs() + 1.0
+        Q[bad, 5] = 1e20 if I != 33 else -1e20
+        check(P, Q, np.arange(n), rng.integers(0, I, (n, 2)), min(I, 20), _mask_all(n, bad), rows=np.r_[0:4, n - 4:n])
