@@ -4,7 +4,8 @@
 // x = hi + lo with hi = half(x), lo = half(x - hi) holds x to 2^-24 of itself (11 + 11 bits and a sign) as long as lo is not
 // subnormal.  x y = hi hi' + hi lo' + lo hi' (lo lo' is below 2^-24 |x y|): three instructions instead of sixteen.  A row of P, and
 // 32 rows of Q together, are scaled by a power of two that puts their largest element into [2^13, 2^14): elements down to 2^-27 of the
-// largest keep their 24 bits.  bf16 tables are multiplied as they are.
+// largest keep their 24 bits.  Where the largest elements of 32 rows of Q lie more than 2^12 apart, each has a scale of its own: a row that shares one
+// is then off by 2^-26 of its own largest element at most, whatever its neighbours are.  bf16 tables are multiplied as they are.
 #pragma once
 #include "rsx_common.h"
 
@@ -65,8 +66,8 @@ __device__ __forceinline__ void barrier_after_copies()
     __syncthreads();
 }
 
-// power of two that brings a largest magnitude m into [2^13, 2^14), and its inverse.  Below 2^-40 as for 2^-40: the product of two such
-// inverses stays a normal number, and what is lost there moves no score by 2^-40
+// power of two that brings a largest magnitude m into [2^13, 2^14), and its inverse.  Below 2^least as for 2^least; at kLeast both are still normal
+constexpr int kLeast = -112;
 __device__ __forceinline__ void scale_for(float m, float *up, float *down, int least = -40)
 {
     int e = (int)((__float_as_uint(m) >> 23) & 0xFF) - 126;      // m in [2^(e-1), 2^e)
@@ -142,15 +143,38 @@ __device__ __forceinline__ void write_seen_bits(int32_t u, bool ok, const int64_
     }
 }
 
-// a tile of fp32 item rows -> scaled planes [tiles padded to a multiple of 4][32][hi d, lo d] and the tile's factor, by 256 threads.
-// Rows behind the last item are zero.
+// rows of a tile share a scale while their largest elements lie within this; rows of zeros do not count
+constexpr float kUneven = 4096.0f;
+constexpr float kOwnScales = -1.0f;       // in place of a tile's factor: every row has its own
+
+// largest element of this thread's row (held by its TPR neighbours), and of the 32 rows the largest and smallest of those
+template <int TPR>
+__device__ __forceinline__ float row_max(float m)
+{
+#pragma unroll
+    for (int o = TPR / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, TPR));
+    return m;
+}
+__device__ __forceinline__ void tile_range(float *most, float *least, float *lds)      // by 256 threads, over their values; lds: 8 words
+{
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) { *most = fmaxf(*most, __shfl_xor(*most, o, 64)); *least = fminf(*least, __shfl_xor(*least, o, 64)); }
+    if ((threadIdx.x & 63) == 0) { lds[threadIdx.x >> 6] = *most; lds[4 + (threadIdx.x >> 6)] = *least; }
+    __syncthreads();
+    *most = fmaxf(fmaxf(lds[0], lds[1]), fmaxf(lds[2], lds[3]));
+    *least = fminf(fminf(lds[4], lds[5]), fminf(lds[6], lds[7]));
+}
+
+// a tile of fp32 item rows -> scaled planes [tiles padded to a multiple of 4][32][hi d, lo d] and the tile's factor (or kOwnScales and its rows'), by 256
+// threads.  Rows behind the last item are zero.
 template <int D>
-__device__ __forceinline__ void split_items(const float *__restrict__ Q, int64_t num_items, int64_t tile, uint4 *__restrict__ planes, float *__restrict__ factor, float *s_max)
+__device__ __forceinline__ void split_items(const float *__restrict__ Q, int64_t num_items, int64_t tile, uint4 *__restrict__ planes, float *__restrict__ factor,
+                                            float *__restrict__ row_factor, float *lds)
 {
     constexpr int TPR = D / 8, RPP = 256 / TPR, N = kTile / RPP > 0 ? kTile / RPP : 1;       // threads a row, rows a pass, passes
     const int tid = threadIdx.x;
-    float x[N][8];
-    float m = 0.0f;
+    float x[N][8], big[N];
+    float most = 0.0f, least = INFINITY;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
         const int r = n * RPP + tid / TPR;
@@ -159,21 +183,26 @@ __device__ __forceinline__ void split_items(const float *__restrict__ Q, int64_t
         const float4 *src = reinterpret_cast<const float4 *>(Q + (size_t)(live ? i : 0) * D + 8 * (tid % TPR));
         const float4 a = live ? src[0] : make_float4(0.f, 0.f, 0.f, 0.f), b = live ? src[1] : make_float4(0.f, 0.f, 0.f, 0.f);
         x[n][0] = a.x; x[n][1] = a.y; x[n][2] = a.z; x[n][3] = a.w; x[n][4] = b.x; x[n][5] = b.y; x[n][6] = b.z; x[n][7] = b.w;
+        float m = 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) m = fmaxf(m, finite_abs(x[n][j]));
+        big[n] = row_max<TPR>(m);
+        most = fmaxf(most, big[n]);
+        least = big[n] > 0.0f ? fminf(least, big[n]) : least;
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-    if ((tid & 63) == 0) s_max[tid >> 6] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
+    tile_range(&most, &least, lds);
+    const bool own = least * kUneven < most;
     float up, down;
-    scale_for(m, &up, &down);
-    if (tid == 0) factor[tile] = down;
+    scale_for(most, &up, &down, kLeast);
+    if (tid == 0) factor[tile] = own ? kOwnScales : down;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
         const int r = n * RPP + tid / TPR;
         if (r >= kTile) continue;
+        if (own) {
+            scale_for(big[n], &up, &down, kLeast);
+            if (tid % TPR == 0) row_factor[tile * kTile + r] = down;
+        }
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[n][j] *= up;
         Frag h, l;

@@ -114,12 +114,12 @@ __device__ __forceinline__ void row_reference(const void *__restrict__ P, const 
 template <int D, bool F32>
 __global__ __launch_bounds__(256) void prepare_kernel(const void *__restrict__ P, const void *__restrict__ Q, Shape sh, const int64_t *__restrict__ indptr,
                                                       const int32_t *__restrict__ indices, int64_t tiles, int64_t bit_rows, uint4 *__restrict__ planes, float *__restrict__ factor,
-                                                      uint32_t *__restrict__ bits, float *__restrict__ ref)
+                                                      float *__restrict__ row_factor, uint32_t *__restrict__ bits, float *__restrict__ ref)
 {
     __shared__ __attribute__((aligned(16))) uint32_t lds[kBitWords];
     int64_t at = blockIdx.x;
     if (at < tiles) {
-        if constexpr (F32) split_items<D>((const float *)Q, sh.items, at, planes, factor, reinterpret_cast<float *>(lds));
+        if constexpr (F32) split_items<D>((const float *)Q, sh.items, at, planes, factor, row_factor, reinterpret_cast<float *>(lds));
         return;
     }
     at -= tiles;
@@ -186,7 +186,7 @@ __device__ __forceinline__ void absorb(const f32x16 &acc, float f, uint32_t w, S
 }
 
 template <int D, bool F32, bool MASK, bool TOP>
-__device__ __forceinline__ void wide_body(const void *__restrict__ P, const char *__restrict__ rows, const float *__restrict__ factor, const Shape &sh,
+__device__ __forceinline__ void wide_body(const void *__restrict__ P, const char *__restrict__ rows, const float *__restrict__ factor, const float *__restrict__ row_factor, const Shape &sh,
                                           const uint32_t *__restrict__ bits, const float *__restrict__ row_ref, int splits, float4 *__restrict__ part,
                                           uint4 *__restrict__ keys, WideLds<D, F32, MASK, TOP> &lds)
 {
@@ -217,7 +217,7 @@ __device__ __forceinline__ void wide_body(const void *__restrict__ P, const char
 #pragma unroll
                 for (int j = 0; j < 8; ++j) m = fmaxf(m, finite_abs(x[j]));
             }
-            scale_for(fmaxf(m, __shfl_xor(m, 32, 64)) * (sh.scale * kLog2e), &up, &down);
+            scale_for(fmaxf(m, __shfl_xor(m, 32, 64)) * (sh.scale * kLog2e), &up, &down, kLeast);
         }
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
@@ -324,7 +324,14 @@ __device__ __forceinline__ void wide_body(const void *__restrict__ P, const char
                 if constexpr (MASK) w |= *reinterpret_cast<const uint32_t *>(lds.bits[g & 1][wid][ub] + l31 * 16 + j * 4);
                 w >>= 4 * hi;
                 uint32_t *key = &lds.key[ub][j % (TOP ? 4 : 1)][tid];
-                if (__builtin_amdgcn_ballot_w64((w & 0x0F0F0F0Fu) != 0u) == 0ull) absorb<false, TOP>(acc[ub], rowf[ub] * tf, 0u, st[ub], ref[ub], key);
+                if (F32 && tf < 0.0f) {       // (kOwnScales: rare, and the only loads of the loop)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const float4 v = *reinterpret_cast<const float4 *>(row_factor + tile * kTile + 8 * q + 4 * hi);
+                        acc[ub][4 * q] *= rowf[ub] * v.x; acc[ub][4 * q + 1] *= rowf[ub] * v.y; acc[ub][4 * q + 2] *= rowf[ub] * v.z; acc[ub][4 * q + 3] *= rowf[ub] * v.w;
+                    }
+                    absorb<true, TOP>(acc[ub], 1.0f, w, st[ub], ref[ub], key);
+                } else if (__builtin_amdgcn_ballot_w64((w & 0x0F0F0F0Fu) != 0u) == 0ull) absorb<false, TOP>(acc[ub], rowf[ub] * tf, 0u, st[ub], ref[ub], key);
                 else absorb<true, TOP>(acc[ub], rowf[ub] * tf, w, st[ub], ref[ub], key);
             }
         }
@@ -355,11 +362,11 @@ __device__ __forceinline__ void wide_body(const void *__restrict__ P, const char
 
 template <int D, bool F32, bool MASK, bool TOP>
 __global__ __launch_bounds__(256, (WideGeo<D, F32>::OCC)) void wide_kernel(const void *__restrict__ P, const char *__restrict__ rows, const float *__restrict__ factor,
-                                                                           Shape sh, const uint32_t *__restrict__ bits, const float *__restrict__ row_ref, int splits,
+                                                                           const float *__restrict__ row_factor, Shape sh, const uint32_t *__restrict__ bits, const float *__restrict__ row_ref, int splits,
                                                                            float4 *__restrict__ part, uint4 *__restrict__ keys)
 {
     __shared__ WideLds<D, F32, MASK, TOP> lds;
-    wide_body<D, F32, MASK, TOP>(P, rows, factor, sh, bits, row_ref, splits, part, keys, lds);
+    wide_body<D, F32, MASK, TOP>(P, rows, factor, row_factor, sh, bits, row_ref, splits, part, keys, lds);
 }
 
 // ---- few rows ---------------------------------------------------------------------------------------------------------------------------
@@ -955,7 +962,7 @@ int thin_groups(int64_t items)
 
 struct Ws {
     char *planes;
-    float *factor;
+    float *factor, *row_factor;
     uint32_t *bits;
     float *ref;
     float4 *part;
@@ -995,6 +1002,7 @@ Ws carve(void *ws, int64_t rows, int64_t items, int d, int dtype, bool mask, int
     const int64_t cells = thin ? rows * parts : w.pass * parts + kWaves * (int64_t)rsx_num_cus() * wide_users(dtype);
     w.planes = take(!thin && dtype == RSX_F32 ? tiles4 * kTile * (int64_t)d * 4 : 0);
     w.factor = (float *)take(!thin && dtype == RSX_F32 ? tiles4 * 4 : 0);
+    w.row_factor = (float *)take(!thin && dtype == RSX_F32 ? tiles4 * kTile * 4 : 0);
     w.bits = (uint32_t *)take(mask ? w.pass * mask_words(items) * 4 : 0);
     w.ref = (float *)take(w.pass * 4);
     w.part = (float4 *)take(cells * 16);
@@ -1036,7 +1044,7 @@ void run(const Call &c, const Ws &w, hipStream_t st)
         const int64_t tiles = F32 && !thin && r0 == 0 ? (items + 127) / 128 * 4 : 0, bit_rows = c.indptr ? sh.rows : 0, refs = c.K ? (sh.rows + 3) / 4 : 0;
         if (tiles + bit_rows + refs > 0)
             hipLaunchKernelGGL((prepare_kernel<D, F32>), dim3((unsigned)(tiles + bit_rows + refs)), dim3(256), 0, st, c.P, c.Q, sh, c.indptr, c.indices, tiles, bit_rows,
-                               (uint4 *)w.planes, w.factor, w.bits, w.ref);
+                               (uint4 *)w.planes, w.factor, w.row_factor, w.bits, w.ref);
         int parts;
         if (thin) {
             parts = thin_groups(items);
@@ -1049,7 +1057,7 @@ void run(const Call &c, const Ws &w, hipStream_t st)
         } else {
             parts = (int)wide_splits(sh.rows, items, F32 ? RSX_F32 : RSX_BF16);
             const dim3 grid((unsigned)parts, (unsigned)((sh.rows + WideGeo<D, F32>::WGU - 1) / WideGeo<D, F32>::WGU));
-#define RSX_LP_WIDE(M_, T_) hipLaunchKernelGGL((wide_kernel<D, F32, M_, T_>), grid, dim3(256), 0, st, c.P, F32 ? w.planes : (const char *)c.Q, w.factor, sh, w.bits, w.ref, parts, w.part, (uint4 *)w.keys)
+#define RSX_LP_WIDE(M_, T_) hipLaunchKernelGGL((wide_kernel<D, F32, M_, T_>), grid, dim3(256), 0, st, c.P, F32 ? w.planes : (const char *)c.Q, w.factor, w.row_factor, sh, w.bits, w.ref, parts, w.part, (uint4 *)w.keys)
             if (c.indptr) { if (c.K) RSX_LP_WIDE(true, true); else RSX_LP_WIDE(true, false); }
             else { if (c.K) RSX_LP_WIDE(false, true); else RSX_LP_WIDE(false, false); }
 #undef RSX_LP_WIDE

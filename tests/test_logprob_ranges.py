@@ -43,3 +43,52 @@ def test_hip_top_items_beside_masked_rows_of_large_values(n, bf16):
         P[:, 5] = P[:, 5].abs() + 1.0
         Q[bad, 5] = 1e20 if I != 33 else -1e20
         check(P, Q, np.arange(n), rng.integers(0, I, (n, 2)), min(I, 20), _mask_all(n, bad), rows=np.r_[0:4, n - 4:n])
+
+
+# ---- item rows of unequal length (fp32 rows share scales) ------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [32, 64, 128, 256])
+@pytest.mark.parametrize("size", [1e5, 1e6, 1e9, 1e12, 1e30])
+def test_hip_logprobs_beside_masked_rows_of_large_values(size, d):
+    """what a masked cell's product would have been does not matter: finite values too, however large"""
+    rng = np.random.default_rng(d)
+    n, I = 140, 500
+    P, Q = tables(rng, n, I, d, False)
+    bad = [0, 37, 250, 251, 499]
+    Q[bad] *= size
+    check(P, Q, np.arange(n), rng.integers(0, I, (n, 3)), 30, _mask_all(n, bad))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [5, 140])
+def test_hip_logprobs_beside_an_item_of_probability_zero(n):
+    """an unmasked row a million times the others whose score is -3 10^6 for everybody: the others' log-probabilities are those without it"""
+    import torch
+    from recsys_pytorch_amd import rsx
+    rng = np.random.default_rng(n)
+    I, out = 400, 70
+    P, Q = tables(rng, n, I, 64, False)
+    P[:, 0] = 3.0
+    Q[out] = 0.0
+    Q[out, 0] = -1e6
+    items = rng.integers(0, I, (n, 3))
+    items[items == out] = 0
+    dev = lambda a: torch.from_numpy(np.ascontiguousarray(a, np.int32)).cuda()
+    got = rsx.score_logprobs(P, Q, dev(np.arange(n)), dev(items), K=20)
+    logp, lse, ent, top, topv, ez = reference(P.double().cpu().numpy(), Q.double().cpu().numpy(), np.arange(n), items, 20, _mask_all(n, [out]), 1.0)
+    el = ez + 5e-5
+    err = lambda a, b: np.abs(a.double().cpu().numpy() - b)
+    assert (err(got.lse, lse) <= el + 2.0 ** -24 * np.abs(lse)).all()
+    assert (err(got.entropy, ent) <= el * (2 + ent) + ez).all()
+    assert (err(got.logp, logp) <= el[:, None] + 2.0 ** -24 * np.abs(logp)).all()
+    assert np.array_equal(got.top_idx.cpu().numpy(), top) and (err(got.top_logp, topv) <= el[:, None] + 2.0 ** -24 * np.abs(topv)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [3, 90])
+@pytest.mark.parametrize("power", [60, 80, 100])
+def test_hip_logprobs_of_tables_of_opposite_size(n, power):
+    rng = np.random.default_rng(power)
+    for up in (2.0 ** power, 2.0 ** -power):
+        P, Q = tables(rng, n, 300, 64, False)
+        check(P * up, Q / up, np.arange(n), rng.integers(0, 300, (n, 2)), 10, None)
