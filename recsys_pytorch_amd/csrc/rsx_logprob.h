@@ -66,12 +66,11 @@ __device__ __forceinline__ void barrier_after_copies()
     __syncthreads();
 }
 
-// power of two that brings a largest magnitude m into [2^13, 2^14), and its inverse.  Below 2^least as for 2^least; at kLeast both are still normal
-constexpr int kLeast = -112;
-__device__ __forceinline__ void scale_for(float m, float *up, float *down, int least = -40)
+// power of two that brings a largest magnitude m into [2^13, 2^14), and its inverse.  Below 2^-112 as for 2^-112, where both are still normal
+__device__ __forceinline__ void scale_for(float m, float *up, float *down)
 {
     int e = (int)((__float_as_uint(m) >> 23) & 0xFF) - 126;      // m in [2^(e-1), 2^e)
-    e = e < least ? least : e;
+    e = e < -112 ? -112 : e;
     *up = ldexpf(1.0f, 14 - e);
     *down = ldexpf(1.0f, e - 14);
 }
@@ -193,14 +192,14 @@ __device__ __forceinline__ void split_items(const float *__restrict__ Q, int64_t
     tile_range(&most, &least, lds);
     const bool own = least * kUneven < most;
     float up, down;
-    scale_for(most, &up, &down, kLeast);
+    scale_for(most, &up, &down);
     if (tid == 0) factor[tile] = own ? kOwnScales : down;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
         const int r = n * RPP + tid / TPR;
         if (r >= kTile) continue;
         if (own) {
-            scale_for(big[n], &up, &down, kLeast);
+            scale_for(big[n], &up, &down);
             if (tid % TPR == 0) row_factor[tile * kTile + r] = down;
         }
 #pragma unroll

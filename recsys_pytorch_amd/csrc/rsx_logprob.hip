@@ -217,7 +217,7 @@ __device__ __forceinline__ void wide_body(const void *__restrict__ P, const char
 #pragma unroll
                 for (int j = 0; j < 8; ++j) m = fmaxf(m, finite_abs(x[j]));
             }
-            scale_for(fmaxf(m, __shfl_xor(m, 32, 64)) * (sh.scale * kLog2e), &up, &down, kLeast);
+            scale_for(fmaxf(m, __shfl_xor(m, 32, 64)) * (sh.scale * kLog2e), &up, &down);
         }
 #pragma unroll
         for (int s = 0; s < KS; ++s) {

@@ -15,9 +15,12 @@
 // 8 n I d operations instead of the 6 that a stored dz would take, against 3 n I of stored and twice read halves: recomputing is the
 // cheaper side from d = 128 down (4096 x 100 000 x 128: 0.4 TFLOP against 2.4 GB).  No atomics: every sum has one order.
 //
-// fp32: three products of halves (rsx_logprob.h) on both sides; dz is a half pair too.  |dz| <= about 5 of the row's weight w_r =
-// sum |g| + |h|; it is divided by w_r, multiplied by 2^12 and its lower end is 2^-24 (a half's), 2^-36 of w_r.  w_r goes to the joined sum
-// (GP) or into the streaming rows (GQ), whose common scale is the largest of w_r |P_r|.  bf16: dz is rounded to bf16, an error of a
+// fp32: three products of halves (rsx_logprob.h) on both sides, dz is a half pair too.  A half ends at 2^-25 (half its last step), a row's sum may be
+// of probabilities near 1 or of 2^-60: every column keeps a power of two M of its own, and dz |y| / 2^M is what is split, y scaled to its row's (32 item
+// rows': rsx_logprob.h) largest element.  M follows the first terms and is raised, with the sums, where a tile exceeds it: the largest term of
+// a sum is held at 2^7 or more, the others to 2^-32 of it, whatever other columns, rows or weights are.  Rising costs a maximum of the tile's
+// exponents a score and a branch a tile that is hardly taken after the first.  A tile's shares of exponent and sign are in the row's
+// parameters: the scores' exponential delivers dz |y| / 2^M as it is.  bf16: dz is rounded to bf16, an error of a
 // term that is at most as large as that of rounding the result (the same where one term is all of it; sums of many average theirs out).
 #include <type_traits>
 
@@ -27,8 +30,12 @@ namespace {
 using namespace lp;
 
 constexpr float kFar = 1.0e30f;           // log-normaliser of a row without probabilities: every p is 0
-constexpr float kLift = 4096.0f;          // dz of fp32 tables is held times 2^12
-constexpr int kLargest = 1;               // scalars: [0] the largest item factor, [kLargest + g] the largest w |P| among the positions of rows_kernel's workgroup g
+// exponents of dz |y| / 2^M: where one is above kTop, M is raised in every column of the wavefront whose largest is above kSet, to that (six binades of room: every
+// raise multiplies the sums; kSet 12: 4096 x 100K x 128 1.21 ms, 8: 1.19).  With the entropy's part the exponent is that of p |y| alone, which has to
+// stay within fp32's (kGuard, then kGuardSet), and the products' own magnitude is looked at after it
+constexpr float kTop = 14.0f, kSet = 8.0f, kGuard = 100.0f, kGuardSet = 90.0f;
+constexpr float kNothing = -250.0f;       // exponents below it are not looked at: no sum of such terms is a number of fp32
+constexpr int kUnit = 14;                 // rows' scaled elements are in units of 2^-14 of their exponent
 
 struct Args {
     const void *P, *Q;
@@ -39,36 +46,30 @@ struct Args {
     float scale;
 };
 
-// per tile of 32 positions: [0] factor of its scores (bf16: the same in every row), [1] what is added to them, [2] [3] dz = p (A + B log2 p), [4] .. [7] the first
-// four named items (as integers; -1: none): 1 KB, one wavefront's copy.  Without the entropy's part B = 0: [1] is log2 |A| - lse (fp32: and 12), so that the
+// per tile of 32 positions: [0] factor of its scores (bf16: the same in every row), [1] what is added to them, [2] [3] dz = 2^t (A + B t), [4] .. [7] the first
+// four named items (as integers; -1: none): 1 KB, one wavefront's copy.  Without the entropy's part B = 0: [1] is log2 |A| - lse, so that the
 // exponential is |dz|, and the sign of A goes with the row's weight (GP) and into the streaming rows (GQ): the same products with one parameter of a row
-// instead of three and a multiplication less a score (4096 x 100K x 128 fp32: 1.173 -> 1.161 ms)
+// instead of three and a multiplication less a score (4096 x 100K x 128 fp32: 1.173 -> 1.161 ms).  fp32: the row's exponent is in [1], and taken out of A t.
 constexpr int kHeld = 4;
 struct Prm {
     float v[4 + kHeld][kTile];
 };
+// the same of a position that stays: without its row's exponent; w: the exponent of its weight, out of A and B (fp32 with the entropy's part)
+struct Stay {
+    float f, off, A, B, w, pad[3];
+};
+
+// e with m in [2^(e - 1), 2^e), and the one of a power of two 2^(e - kUnit) that scale_for made
+__device__ __forceinline__ int exponent_of(float m) { return (int)((__float_as_uint(m) >> 23) & 0xFF) - 126; }
+__device__ __forceinline__ float exponent_of_factor(float down) { return (float)((int)(__float_as_uint(down) >> 23) - 127 + kUnit); }
 
 // ---- what the passes need -------------------------------------------------------------------------------------------------------------
-// one wavefront per position (padded to 128), positions dealt round: coefficients, named items with theirs, the largest w |P| of a workgroup's
-// (users_kernel takes the largest of those: an atomic maximum on one word, 512 times, was 6 us of this kernel's 11 at 2395 positions).  The first
-// workgroup also finds the largest item factor.
+// one wavefront per position (padded to 128), positions dealt round: coefficients, named items with theirs
 template <int D, bool F32>
-__global__ __launch_bounds__(256) void rows_kernel(Args a, const uint32_t *__restrict__ bits, int64_t padded, Prm *__restrict__ prm, float *__restrict__ weight, int32_t *__restrict__ named,
-                                                   float *__restrict__ coef, uint32_t *__restrict__ top_factor, float *__restrict__ largest, const float *__restrict__ item_factor, int64_t item_tiles)
+__global__ __launch_bounds__(256) void rows_kernel(Args a, const uint32_t *__restrict__ bits, int64_t padded, Prm *__restrict__ prm, Stay *__restrict__ stay, float *__restrict__ weight,
+                                                   int32_t *__restrict__ named, float *__restrict__ coef)
 {
-    __shared__ float s_max[4];
     const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
-    if (F32 && blockIdx.x == 0) {
-        float m = 0.0f;
-        for (int64_t t = threadIdx.x; t < item_tiles; t += 256) m = fmaxf(m, item_factor[t]);
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-        if (lane == 0) s_max[wid] = m;
-        __syncthreads();
-        if (threadIdx.x == 0) *top_factor = __float_as_uint(fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3])));
-        __syncthreads();
-    }
-    float most = 0.0f;
     for (int64_t r = (int64_t)blockIdx.x * 4 + wid; r < padded; r += (int64_t)gridDim.x * 4) {
         const int32_t u = r < a.rows ? a.user_ids[r] : -1;
         const bool ok = row_ok(u, a.users);
@@ -92,10 +93,11 @@ __global__ __launch_bounds__(256) void rows_kernel(Args a, const uint32_t *__res
         const float lse = ok ? a.lse[r] : -INFINITY;
         const bool live = ok && lse != -INFINITY;
         const float sign = a.h == nullptr && sum > 0.0 ? -1.0f : 1.0f;
-        const float w = F32 ? (float)(mag + fabs((double)h)) : 1.0f;
-        const float inv = w > 0.0f ? 1.0f / w : w == w ? 0.0f : w;              // (NaN weights stay NaN)
-        float big = 0.0f, factor = live ? F32 ? 1.0f : a.scale * kLog2e : 0.0f;
+        const double w = mag + fabs((double)h);
+        float factor = live ? F32 ? 1.0f : a.scale * kLog2e : 0.0f;
+        int e_row = 0, e_w = 0;                // exponents of the row and (with the entropy's part) of its weight
         if constexpr (F32) {
+            float big = 0.0f;
             if (ok && lane < D / 8) {
                 const float4 *p = reinterpret_cast<const float4 *>((const float *)a.P + (int64_t)u * D + 8 * lane);
                 const float4 x = p[0], y = p[1];
@@ -107,32 +109,39 @@ __global__ __launch_bounds__(256) void rows_kernel(Args a, const uint32_t *__res
             float up, down;
             scale_for(big * (a.scale * kLog2e), &up, &down);
             factor *= down;
-            most = fmaxf(most, finite_abs(big * w));
-            for (int t = lane; t < a.T && r < a.rows; t += 64) {
-                const int32_t i = a.items[r * a.T + t];
-                coef[r * a.T + t] = ok && i >= 0 && i < a.cat ? a.g[r * a.T + t] * inv * sign : 0.0f;        // (a masked item is not looked up)
-            }
-        } else {
-            for (int t = lane; t < a.T && r < a.rows; t += 64) coef[r * a.T + t] = a.g[r * a.T + t] * sign;
+            scale_for(big, &up, &down);
+            e_row = (int)exponent_of_factor(down);
+            if (a.h != nullptr) e_w = exponent_of((float)w);
         }
+        for (int t = lane; t < a.T && r < a.rows; t += 64) {              // (a masked item is not looked up)
+            const int32_t i = a.items[r * a.T + t];
+            coef[r * a.T + t] = ok && i >= 0 && i < a.cat ? ldexpf(a.g[r * a.T + t] * sign, e_row) : 0.0f;
+        }
+        // dz = p (A + B log2 p), p = 2^(z - lse2), by t = z + off, off the rounded e - lse2: what the rounding (half a step at 24 is 1e-6 of every p) and
+        // e change goes into the coefficients
         const double lse2 = (double)lse * 1.4426950408889634074;
-        // with the entropy: lse in log2 is rounded to fp32 (half a step at 24 is 1e-6 of every p): what that changes goes into the coefficients
-        const float l2 = (float)lse2;
-        const double fix = exp2((double)l2 - lse2) * inv;
-        const double off = (F32 ? 12.0 : 0.0) - lse2 + log2(fabs(sum) * inv);
+        const double H = a.h != nullptr ? (double)h * a.ent[r < a.rows ? r : 0] : 0.0;
+        const double A = live ? ldexp(-(sum + H), -e_w) : 0.0, B = live ? ldexp(-(double)h * kLn2, -e_w) : 0.0;
+        auto params = [&](int e, float *off, float *pa, float *pb) {
+            if (!live || (a.h == nullptr && sum == 0.0)) { *off = -kFar; *pa = *pb = 0.0f; return; }
+            if (a.h == nullptr) { *off = (float)(log2(fabs(sum)) - lse2 + e); *pa = *pb = 0.0f; return; }
+            const double want = e - lse2;
+            *off = (float)want;
+            const double d = (double)*off - want, fix = exp2(-d);
+            *pa = (float)((A - B * (e + d)) * fix);
+            *pb = (float)(B * fix);
+        };
         if (lane == 0) {
+            Stay q{};
+            q.f = factor;
+            q.w = (float)e_w;
+            params(0, &q.off, &q.A, &q.B);
+            stay[r] = q;
             out.v[0][c] = factor;
-            out.v[1][c] = !live ? -kFar : a.h == nullptr ? (float)off : -l2;
-            out.v[2][c] = live ? (float)(-(sum + (double)h * (a.ent != nullptr ? a.ent[r] : 0.0f)) * fix) : 0.0f;
-            out.v[3][c] = live ? (float)(-(double)h * kLn2 * fix) : 0.0f;
+            params(e_row + e_w, &out.v[1][c], &out.v[2][c], &out.v[3][c]);
             for (int k = a.T; k < kHeld; ++k) out.v[4 + k][c] = __int_as_float(-1);
-            weight[r] = live ? sign * w : 0.0f;
+            weight[r] = live && !(w == 0.0) ? sign : 0.0f;                // (no weight, no gradient; NaN stays NaN)
         }
-    }
-    if constexpr (F32) {
-        if (lane == 0) s_max[wid] = most;
-        __syncthreads();
-        if (threadIdx.x == 0) largest[blockIdx.x] = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
     }
 }
 
@@ -142,25 +151,24 @@ template <int D>
 __device__ __forceinline__ int tile_row(int half, int hi, int j) { const int i = 8 * half + j; return (i & 3) + 8 * (i >> 2) + 4 * hi; }
 
 // a tile of 32 rows by 256 threads: row-major planes and the transposed tile.  USERS: rows gathered by user id, each times scale log2 e and with its own
-// power of two in the row-major planes, times its weight and one common scale in the transposed ones.  Items: the tile's scale in both.
+// power of two in the row-major planes, times its own and its sign (0: no weight) in the transposed ones.  Items: the tile's power of two in both, or each row's own
+// where they are too unequal (rsx_logprob.h).
 template <int D, bool F32>
 struct TileLds {
     typename std::conditional<F32, float, uint16_t>::type x[kTile][D + 1];
-    float max[4], mul[kTile];
+    float range[8], big[kTile], mul[kTile];
 };
 
 template <int D, bool F32, bool USERS>
-__device__ __forceinline__ void lay_tile(const Args &a, int64_t tile, const float *__restrict__ weight, const float *__restrict__ largest, int groups, uint4 *__restrict__ rowm,
-                                         uint4 *__restrict__ tr, float *__restrict__ factor, TileLds<D, F32> &lds)
+__device__ __forceinline__ void lay_tile(const Args &a, int64_t tile, const float *__restrict__ weight, uint4 *__restrict__ rowm, uint4 *__restrict__ tr, float *__restrict__ factor,
+                                         float *__restrict__ row_factor, TileLds<D, F32> &lds)
 {
     constexpr int TPR = D / 8;
     auto &x = lds.x;
-    float *const s_max = lds.max, *const s_mul = lds.mul;
+    float *const s_mul = lds.mul;
     const int tid = threadIdx.x;
     const int64_t n = USERS ? a.rows : a.cat;
-    float m = 0.0f;                       // items: the tile's largest element; users: the largest w |P|
-    if constexpr (USERS && F32)
-        for (int t = tid; t < groups; t += 256) m = fmaxf(m, largest[t]);
+    float most = 0.0f, least = INFINITY;  // items: the rows' largest elements, the largest and the smallest of them
     for (int t = tid; t < kTile * TPR; t += 256) {
         const int r = t / TPR, c = 8 * (t % TPR);
         const int64_t at = tile * kTile + r;
@@ -172,19 +180,22 @@ __device__ __forceinline__ void lay_tile(const Args &a, int64_t tile, const floa
             const float4 *p = reinterpret_cast<const float4 *>((const float *)src + (row < 0 ? 0 : row) * D + c);
             const float4 y = p[0], z = p[1];
             v[0] = y.x; v[1] = y.y; v[2] = y.z; v[3] = y.w; v[4] = z.x; v[5] = z.y; v[6] = z.z; v[7] = z.w;
-            float big = 0.0f;
+            float big = 0.0f, up, down;
 #pragma unroll
             for (int j = 0; j < 8; ++j) { v[j] = row < 0 ? 0.0f : v[j]; big = fmaxf(big, finite_abs(v[j])); x[r][c + j] = v[j]; }
-            if constexpr (!USERS) m = fmaxf(m, big);
-            if constexpr (USERS) {            // the row's own scale: its TPR threads are neighbours (a power of two, at most 32)
-#pragma unroll
-                for (int o = TPR / 2; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor(big, o, TPR));
-                float up, down;
+            big = row_max<TPR>(big);
+            if constexpr (USERS) {
                 scale_for(big * (a.scale * kLog2e), &up, &down);
                 Frag h, l;
                 split8_times(v, (double)a.scale * 1.4426950408889634074 * up, &h, &l);
                 rowm[(size_t)at * (2 * TPR) + t % TPR] = h.u;
                 rowm[(size_t)at * (2 * TPR) + TPR + t % TPR] = l.u;
+                scale_for(big, &up, &down);
+                if (c == 0) s_mul[r] = weight[at] * up;
+            } else {
+                most = fmaxf(most, big);
+                least = big > 0.0f ? fminf(least, big) : least;
+                if (c == 0) lds.big[r] = big;
             }
         } else {
             uint4 v = *reinterpret_cast<const uint4 *>((const uint16_t *)src + (row < 0 ? 0 : row) * D + c);
@@ -198,31 +209,29 @@ __device__ __forceinline__ void lay_tile(const Args &a, int64_t tile, const floa
     if constexpr (USERS && !F32) {
         if (tid < kTile) s_mul[tid] = weight[tile * kTile + tid];
     }
-    if constexpr (F32) {
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-        if ((tid & 63) == 0) s_max[tid >> 6] = m;
-    }
-    __syncthreads();
-    if constexpr (F32) {
-        float up, down;
-        scale_for(fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3])), &up, &down, USERS ? -100 : -40);      // (weights may be small)
-        if (tid == 0 && (!USERS || tile == 0)) factor[tile] = down;
-        if (tid < kTile) s_mul[tid] = USERS ? weight[tile * kTile + tid] * up : up;
-        if constexpr (!USERS) {
-            for (int t = tid; t < kTile * TPR; t += 256) {
-                const int r = t / TPR, c = 8 * (t % TPR);
-                float v[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = x[r][c + j] * up;
-                Frag h, l;
-                split8(v, &h, &l);
-                rowm[(size_t)(tile * kTile + r) * (2 * TPR) + t % TPR] = h.u;
-                rowm[(size_t)(tile * kTile + r) * (2 * TPR) + TPR + t % TPR] = l.u;
-            }
+    if constexpr (F32 && !USERS) {
+        tile_range(&most, &least, lds.range);
+        const bool own = least * kUneven < most;
+        if (tid < kTile) {
+            float up, down;
+            scale_for(own ? lds.big[tid] : most, &up, &down);
+            s_mul[tid] = up;
+            row_factor[tile * kTile + tid] = down;
+            if (tid == 0) factor[tile] = own ? kOwnScales : down;
         }
         __syncthreads();
+        for (int t = tid; t < kTile * TPR; t += 256) {
+            const int r = t / TPR, c = 8 * (t % TPR);
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = x[r][c + j] * s_mul[r];
+            Frag h, l;
+            split8(v, &h, &l);
+            rowm[(size_t)(tile * kTile + r) * (2 * TPR) + t % TPR] = h.u;
+            rowm[(size_t)(tile * kTile + r) * (2 * TPR) + TPR + t % TPR] = l.u;
+        }
     }
+    __syncthreads();
     // the second product multiplies by dz = 0 where a cell is masked: what is not finite is 0 there (where it is not masked, lse is NaN already)
     constexpr int NF = D / 32 * 2 * 64;
     uint4 *dst = tr + (size_t)tile * (NF * (F32 ? 2 : 1));
@@ -258,12 +267,12 @@ __device__ __forceinline__ void lay_tile(const Args &a, int64_t tile, const floa
 // position's seen bits each
 template <int D, bool F32>
 __global__ __launch_bounds__(256) void items_kernel(Args a, const int64_t *__restrict__ indptr, const int32_t *__restrict__ indices, int64_t tiles, uint4 *__restrict__ rowm,
-                                                    uint4 *__restrict__ tr, float *__restrict__ factor, uint32_t *__restrict__ bits)
+                                                    uint4 *__restrict__ tr, float *__restrict__ factor, float *__restrict__ row_factor, uint32_t *__restrict__ bits)
 {
     __shared__ __attribute__((aligned(16))) union { TileLds<D, F32> tile; uint32_t bits[kBitWords]; } lds;
     const int64_t at = blockIdx.x;
     if (at < tiles) {
-        lay_tile<D, F32, false>(a, at, nullptr, nullptr, 0, rowm, tr, factor, lds.tile);
+        lay_tile<D, F32, false>(a, at, nullptr, rowm, tr, factor, row_factor, lds.tile);
         return;
     }
     const int32_t u = a.user_ids[at - tiles];
@@ -271,19 +280,19 @@ __global__ __launch_bounds__(256) void items_kernel(Args a, const int64_t *__res
 }
 
 template <int D, bool F32>
-__global__ __launch_bounds__(256) void users_kernel(Args a, const float *__restrict__ weight, const float *__restrict__ largest, int groups, uint4 *__restrict__ rowm, uint4 *__restrict__ tr,
-                                                    float *__restrict__ factor)
+__global__ __launch_bounds__(256) void users_kernel(Args a, const float *__restrict__ weight, uint4 *__restrict__ rowm, uint4 *__restrict__ tr)
 {
     __shared__ __attribute__((aligned(16))) TileLds<D, F32> lds;
-    lay_tile<D, F32, true>(a, blockIdx.x, weight, largest, groups, rowm, tr, factor, lds);
+    lay_tile<D, F32, true>(a, blockIdx.x, weight, rowm, tr, nullptr, nullptr, lds);
 }
 
 // ---- the pass -------------------------------------------------------------------------------------------------------------------------
 struct Pass {
     const char *stay, *flow;              // row-major planes of what stays in registers and of what streams
     const char *flow_t;                   // transposed tiles of what streams
-    const uint32_t *top_factor;           // fp32: the largest factor of an item tile
+    const float *tile_factor, *row_factor;      // fp32 items: a tile's (or kOwnScales), a row's
     const Prm *prm;
+    const Stay *stay_prm;
     const uint32_t *bits;
     const int32_t *named;
     const float *coef;
@@ -318,7 +327,7 @@ struct GradGeo : Geo<D, F32> {
 };
 
 template <int D, bool F32, bool ITEMS_STAY, bool MASK, bool ENT>
-__device__ __forceinline__ void grad_body(const Pass &a, int64_t piece, const float *__restrict__ tile_factor, char *lds0, char *lds1)
+__device__ __forceinline__ void grad_body(const Pass &a, int64_t piece, char *lds0, char *lds1)
 {
     using G = GradGeo<D, F32>;
     constexpr int KS = G::KS, NP = G::NP, ST = G::ST, KB = G::KB / G::HS;              // KB: this wavefront's blocks of 32 elements
@@ -326,7 +335,6 @@ __device__ __forceinline__ void grad_body(const Pass &a, int64_t piece, const fl
     const int64_t total = a.part_rows / 128 * a.flow_tiles;
     int64_t at = piece_begin(total, a.pieces, piece);
     const int64_t end = piece_begin(total, a.pieces, piece + 1);
-    const float top = F32 ? __uint_as_float(*a.top_factor) : 1.0f;
     const int64_t words = mask_words(a.cat);
     const int sw = G::swz(l31) * 16;
 
@@ -392,27 +400,43 @@ __device__ __forceinline__ void grad_body(const Pass &a, int64_t piece, const fl
     for (int k = 0; k < KB; ++k)
 #pragma unroll
         for (int i = 0; i < 16; ++i) out[k][i] = 0.0f;
-    float sf = 0.0f, slse = 0.0f, sA = 0.0f, sB = 0.0f, my_factor = 1.0f;                          // users stay: this lane's row; items stay: its tile's factor
+    float sf = 0.0f, slse = 0.0f, sA = 0.0f, sB = 0.0f, sE = 0.0f, my_factor = 1.0f;               // users stay: this lane's row; items stay: its row's factor
     if constexpr (!ITEMS_STAY) {
-        const Prm &p = a.prm[colc / kTile];
-        const int c = (int)(colc % kTile);
-        sf = p.v[0][c]; slse = p.v[1][c]; sA = p.v[2][c]; sB = p.v[3][c];
+        const Stay &p = a.stay_prm[colc];
+        sf = p.f; slse = p.off; sA = p.A; sB = p.B; sE = p.w;
     } else if constexpr (F32) {
-        my_factor = tile_factor[colc / kTile];
+        my_factor = a.row_factor[colc];
     }
+    float M = 0.0f;                       // this column's: what dz |y| is divided by, as an exponent (a whole number; the same in both lanes of a column)
+    float limit = kNothing;               // an exponent above this changes M (until the column has met a term: any)
+    // M up by k binades, the sums down.  (fp32 rows of 256: the sums are in accumulation registers, and said to stay there; else the whole loop moves
+    // them to and fro for this branch: 1000 x 50021 512 us instead of 411)
+    auto raise = [&](float k) __attribute__((always_inline)) {
+        const float f = k > 0.0f ? ldexpf(1.0f, -(int)k) : 1.0f;       // (down only before the first term)
+#pragma unroll
+        for (int q = 0; q < KB; ++q) {
+            if constexpr (F32 && D == 256) asm volatile("" : "+a"(out[q]));
+#pragma unroll
+            for (int i = 0; i < 16; ++i) out[q][i] *= f;
+            if constexpr (F32 && D == 256) asm volatile("" : "+a"(out[q]));
+        }
+        M += k;
+    };
     wait_memory();                        // (the operands' loads end here: left to their first use, that wait would stand in the loop, for every stage's copies)
     auto step = [&](int64_t s0, const char *lds, char *next) __attribute__((always_inline)) {
         barrier_after_copies();
         if (s0 + ST < t1) stage(s0 + ST, next, block, colc);
         for (int j = 0; j < ST && s0 + j < t1; ++j) {
             const int64_t tile = s0 + j;
-            // (nothing in this loop loads into registers from memory: loads return in order, and one would wait for the next stage's copies)
+            // (hardly anything in this loop loads into registers from memory: loads return in order, and one waits for the next stage's copies.  What does: the
+            // coefficient of a named item that is found, the factors of rows with scales of their own, and, from the fifth of T on, the names: 1024 x 100K x 128
+            // fp32 381 us with T = 4, 418 with 10)
             uint32_t seen = 0u;
             if constexpr (MASK) {
                 const char *sb = lds + G::BITS + j * 1024;
                 seen = ITEMS_STAY ? *reinterpret_cast<const uint32_t *>(sb + l31 * 16 + wid * 4) : *reinterpret_cast<const uint32_t *>(sb + wid * 256 + lane * 4);
             }
-            const float tf = !ITEMS_STAY && F32 ? tile_factor[tile] : my_factor;
+            const float tf = !ITEMS_STAY && F32 ? a.tile_factor[tile] : my_factor;
             const char *rm = lds + j * G::TILEB + l31 * G::ROWB;
             const char *tr = lds + ST * G::TILEB + j * G::TILEB + lane * 16;
             __builtin_amdgcn_s_setprio(1);         // (a wavefront in its products goes first: the two of a SIMD fall into step otherwise; 1.19 -> 1.16 ms)
@@ -431,84 +455,133 @@ __device__ __forceinline__ void grad_body(const Pass &a, int64_t piece, const fl
                 }
             }
             __builtin_amdgcn_s_setprio(0);
-            // dz of this lane's column and rows (i & 3) + 8 (i >> 2) + 4 hi of the tile
+            // dz of this lane's column and rows (i & 3) + 8 (i >> 2) + 4 hi of the tile: 2^s, or with the entropy's part 2^s (A + B t)
             float v[16];
+            float s[16], t[ENT ? 16 : 1];
+            float need = 0.0f;                     // sum of the named items' |dz| |y| of this column
+            uint64_t hit = F32 ? 0 : ~0ull;        // which of the T names have one here (bit k & 63)
             if constexpr (!ITEMS_STAY) {
+                if (F32 && tf < 0.0f) {            // (kOwnScales: rare, and loads in the loop)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const float4 y = *reinterpret_cast<const float4 *>(a.row_factor + tile * kTile + 8 * q + 4 * hi);
+                        const float ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float by = exponent_of_factor(ys[e]) + sE - M;
+                            if constexpr (ENT) { t[4 * q + e] = fmaf(acc[4 * q + e], sf * ys[e], slse); s[4 * q + e] = t[4 * q + e] + by; }
+                            else s[4 * q + e] = fmaf(acc[4 * q + e], sf * ys[e], slse + by);
+                        }
+                    }
+                } else {
+                    const float f = sf * tf, by = F32 ? exponent_of_factor(tf) + sE - M : 0.0f, off = slse + by;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        if constexpr (ENT) { t[i] = fmaf(acc[i], f, slse); s[i] = t[i] + by; }
+                        else s[i] = fmaf(acc[i], f, off);
+                    }
+                }
                 const int64_t left = a.flow_valid - tile * kTile;
                 uint32_t w = left >= 32 ? 0u : 0xFFFFFFFFu << left;
                 if constexpr (MASK) w |= seen;
                 w >>= 4 * hi;
-                const bool any = __builtin_amdgcn_ballot_w64((w & 0x0F0F0F0Fu) != 0u) != 0ull;
-                const float f = sf * tf;
-                // items of a tile whose scale is below the largest count less by that: the tile's sums are over planes of its own scale
-                const float lift = F32 ? (float)(12 + (int)(__float_as_uint(tf) >> 23) - (int)(__float_as_uint(top) >> 23)) : 0.0f;
-                const float off = F32 && !ENT ? slse + (lift - 12.0f) : slse;             // (without the entropy's part log2 p itself is not needed)
-                float t[16];
+                if (__builtin_amdgcn_ballot_w64((w & 0x0F0F0F0Fu) != 0u) != 0ull) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) t[i] = fmaf(acc[i], f, off);
-                if (any) {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) t[i] = (w >> ((i & 3) + 8 * (i >> 2))) & 1u ? -1.0e4f : t[i];
-                }
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float p = __builtin_amdgcn_exp2f(F32 && ENT ? t[i] + lift : t[i]);
-                    v[i] = ENT ? p * fmaf(sB, t[i], sA) : p;
+                    for (int i = 0; i < 16; ++i) {
+                        const bool none = (w >> ((i & 3) + 8 * (i >> 2))) & 1u;
+                        s[i] = none ? -1.0e4f : s[i];
+                        if constexpr (ENT) t[i] = none ? 0.0f : t[i];
+                    }
                 }
             } else {
                 const Prm *prm = reinterpret_cast<const Prm *>(lds + G::PRM + j * 1024);
                 if (MASK && tile * kTile + l31 >= a.positions) seen = 0xFFFFFFFFu;            // nobody's rows behind the last
-                const bool any = MASK && __builtin_amdgcn_ballot_w64(seen != 0u) != 0ull;
-                float t[16];
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     const int r0 = 8 * q + 4 * hi;
                     const float4 f4 = F32 ? *reinterpret_cast<const float4 *>(&prm->v[0][r0]) : make_float4(a.factor, a.factor, a.factor, a.factor), l4 = *reinterpret_cast<const float4 *>(&prm->v[1][r0]);
-                    t[4 * q] = fmaf(acc[4 * q], f4.x * tf, l4.x);
-                    t[4 * q + 1] = fmaf(acc[4 * q + 1], f4.y * tf, l4.y);
-                    t[4 * q + 2] = fmaf(acc[4 * q + 2], f4.z * tf, l4.z);
-                    t[4 * q + 3] = fmaf(acc[4 * q + 3], f4.w * tf, l4.w);
-                }
-                if (any) {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) t[i] = (__shfl(seen, (i & 3) + 8 * (i >> 2) + 4 * hi, 64) >> l31) & 1u ? -1.0e4f : t[i];
-                }
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int r0 = 8 * q + 4 * hi;
-                    float as[4], bs[4];
-                    if constexpr (ENT) {
-                        const float4 a4 = *reinterpret_cast<const float4 *>(&prm->v[2][r0]), b4 = *reinterpret_cast<const float4 *>(&prm->v[3][r0]);
-                        as[0] = a4.x; as[1] = a4.y; as[2] = a4.z; as[3] = a4.w;
-                        bs[0] = b4.x; bs[1] = b4.y; bs[2] = b4.z; bs[3] = b4.w;
-                    }
+                    const float fs[4] = {f4.x, f4.y, f4.z, f4.w}, ls[4] = {l4.x, l4.y, l4.z, l4.w};
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const float p = __builtin_amdgcn_exp2f(F32 && ENT ? t[4 * q + e] + 12.0f : t[4 * q + e]);
-                        v[4 * q + e] = ENT ? p * fmaf(bs[e], t[4 * q + e], as[e]) : p;
+                        if constexpr (ENT) { t[4 * q + e] = fmaf(acc[4 * q + e], fs[e] * tf, ls[e]); s[4 * q + e] = F32 ? t[4 * q + e] - M : t[4 * q + e]; }
+                        else s[4 * q + e] = fmaf(acc[4 * q + e], fs[e] * tf, F32 ? ls[e] - M : ls[e]);
                     }
                 }
-                // named items of the tile's positions that are in this wavefront's block.
-                auto name = [&](int32_t it, int t) __attribute__((always_inline)) {
+                if (MASK && __builtin_amdgcn_ballot_w64(seen != 0u) != 0ull) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const bool none = (__shfl(seen, (i & 3) + 8 * (i >> 2) + 4 * hi, 64) >> l31) & 1u;
+                        s[i] = none ? -1.0e4f : s[i];
+                        if constexpr (ENT) t[i] = none ? 0.0f : t[i];
+                    }
+                }
+            }
+            // named items of the tile's positions that are in this wavefront's block: f(position in the tile, column, what is added to its dz)
+            auto named = [&](bool add, auto f) __attribute__((always_inline)) {
+                const Prm *prm = reinterpret_cast<const Prm *>(lds + G::PRM + j * 1024);
+                for (int k = 0; k < a.T; ++k) {
+                    if (F32 && add && !((hit >> (k & 63)) & 1)) continue;
+                    const int64_t r = tile * kTile + l31;
+                    const int32_t it = k < kHeld ? __float_as_int(prm->v[4 + k][l31]) : r < a.positions ? a.named[r * a.T + k] : -1;
                     const bool mine = hi == 0 && (it >> 5) == my_block;          // (-1 >> 5 is nobody's block)
                     unsigned long long hits = __builtin_amdgcn_ballot_w64(mine);
-                    if (hits == 0ull) return;
-                    const float c = mine ? a.coef[(tile * kTile + l31) * a.T + t] * (F32 ? kLift : 1.0f) : 0.0f;
+                    if (hits == 0ull) continue;
+                    hit |= 1ull << (k & 63);
+                    const float c = mine ? a.coef[r * a.T + k] : 0.0f;
                     while (hits) {
                         const int row = __builtin_ctzll(hits);
                         hits &= hits - 1;
-                        const int at = __builtin_amdgcn_readlane(it, row) & 31;
-                        const float add = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(c), row));
-                        const int reg = (row & 3) | ((row >> 3) << 2);
-                        const bool here = lane == at + 32 * ((row >> 2) & 1);
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) v[i] += here && i == reg ? add : 0.0f;
+                        f(row, __builtin_amdgcn_readlane(it, row) & 31, __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(c), row)));
                     }
-                };
-                for (int t = 0; t < a.T && t < kHeld; ++t) name(__float_as_int(prm->v[4 + t][l31]), t);
-                for (int t = kHeld; t < a.T; ++t) {
-                    const int64_t r = tile * kTile + l31;
-                    name(r < a.positions ? a.named[r * a.T + t] : -1, t);
+                }
+            };
+            if constexpr (F32) {
+                if constexpr (ITEMS_STAY) named(false, [&](int, int at, float c) { need += l31 == at ? fabsf(c) : 0.0f; });
+                float most = s[0];
+#pragma unroll
+                for (int i = 1; i < 16; ++i) most = fmaxf(most, s[i]);
+                if (need > 0.0f) most = fmaxf(most, (float)exponent_of(need) - M);
+                if (__builtin_amdgcn_ballot_w64(most > limit) != 0ull) {
+                    most = fmaxf(most, __shfl_xor(most, 32, 64));
+                    constexpr float set = ENT ? kGuardSet : kSet;
+                    const float k = most > fminf(limit, set) ? fminf(ceilf(most) - set, 600.0f) : 0.0f;
+                    if (most > kNothing) limit = ENT ? kGuard : kTop;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[i] -= k;
+                    raise(k);
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const Prm *prm = reinterpret_cast<const Prm *>(lds + G::PRM + j * 1024);
+                float4 a4 = make_float4(sA, sA, sA, sA), b4 = make_float4(sB, sB, sB, sB);
+                if constexpr (ENT && ITEMS_STAY) { a4 = *reinterpret_cast<const float4 *>(&prm->v[2][8 * q + 4 * hi]); b4 = *reinterpret_cast<const float4 *>(&prm->v[3][8 * q + 4 * hi]); }
+                const float as[4] = {a4.x, a4.y, a4.z, a4.w}, bs[4] = {b4.x, b4.y, b4.z, b4.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    v[4 * q + e] = __builtin_amdgcn_exp2f(s[4 * q + e]);
+                    if constexpr (ENT) v[4 * q + e] *= fmaf(bs[e], t[4 * q + e], as[e]);
+                }
+            }
+            if (ITEMS_STAY && hit != 0)
+                named(true, [&](int row, int at, float c) {
+                    const float add = F32 ? ldexpf(c, -(int)M) : c;
+                    const int reg = (row & 3) | ((row >> 3) << 2);
+                    const bool here = lane == at + 32 * ((row >> 2) & 1);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) v[i] += here && i == reg ? add : 0.0f;
+                });
+            if constexpr (F32 && ENT) {
+                float most = fabsf(v[0]);
+#pragma unroll
+                for (int i = 1; i < 16; ++i) most = fmaxf(most, fabsf(v[i]));
+                constexpr float over = 32768.0f;       // 2^(kTop + 1)
+                if (__builtin_amdgcn_ballot_w64(most > over) != 0ull) {
+                    most = fmaxf(most, __shfl_xor(most, 32, 64));
+                    const int e = exponent_of(most) - (int)kSet, k = e > 0 ? e : 0;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) v[i] = ldexpf(v[i], -k);
+                    raise((float)k);
                 }
             }
             // second product: registers 8 h .. 8 h + 7 are the operand of its half h
@@ -550,22 +623,23 @@ __device__ __forceinline__ void grad_body(const Pass &a, int64_t piece, const fl
         }
     }
     float *dst = a.part + ((size_t)segment * a.part_rows + col) * D + 32 * KB * half + 4 * hi;
+    const int e = F32 ? (int)M - kUnit : 0;
 #pragma unroll
     for (int k = 0; k < KB; ++k)
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-            *reinterpret_cast<float4 *>(dst + 32 * k + 8 * q) = make_float4(out[k][4 * q], out[k][4 * q + 1], out[k][4 * q + 2], out[k][4 * q + 3]);
+            *reinterpret_cast<float4 *>(dst + 32 * k + 8 * q) = make_float4(ldexpf(out[k][4 * q], e), ldexpf(out[k][4 * q + 1], e), ldexpf(out[k][4 * q + 2], e), ldexpf(out[k][4 * q + 3], e));
     at += t1 - t0;
     }
 }
 
 // both passes in one launch, the users' first: neither waits for the other's last workgroups (256 x 1682 x 64: 9.6 us for 17 in two)
 template <int D, bool F32, bool MASK, bool ENT>
-__global__ __launch_bounds__((GradGeo<D, F32>::NT), (GradGeo<D, F32>::WGS * GradGeo<D, F32>::HS)) void grad_kernel(Pass p, Pass q, const float *__restrict__ tile_factor)
+__global__ __launch_bounds__((GradGeo<D, F32>::NT), (GradGeo<D, F32>::WGS * GradGeo<D, F32>::HS)) void grad_kernel(Pass p, Pass q)
 {
     __shared__ __attribute__((aligned(1024))) char lds0[GradGeo<D, F32>::STAGE], lds1[GradGeo<D, F32>::STAGE];
-    if ((int)blockIdx.x < p.pieces) grad_body<D, F32, false, MASK, ENT>(p, blockIdx.x, tile_factor, lds0, lds1);
-    else grad_body<D, F32, true, MASK, ENT>(q, blockIdx.x - p.pieces, tile_factor, lds0, lds1);
+    if ((int)blockIdx.x < p.pieces) grad_body<D, F32, false, MASK, ENT>(p, blockIdx.x, lds0, lds1);
+    else grad_body<D, F32, true, MASK, ENT>(q, blockIdx.x - p.pieces, lds0, lds1);
 }
 
 // segments of a block of 128 columns
@@ -576,10 +650,10 @@ __device__ __forceinline__ int segments_of(int64_t block, int64_t flow_tiles, in
 }
 
 // ---- the partial sums -> the gradients ------------------------------------------------------------------------------------------------------
-// GP: four elements a thread; the partials in order, the row's weight, the named rows of Q
+// GP: four elements a thread; the partials in order, the row's sign, the named rows of Q
 template <int D, bool F32>
 __device__ __forceinline__ void join_rows(int64_t t, const Args &a, const float *__restrict__ part, int64_t flow_tiles, int pieces, int64_t part_rows, const float *__restrict__ weight,
-                                                        const uint32_t *__restrict__ top_factor, const int32_t *__restrict__ named, void *__restrict__ GP)
+                                                        const int32_t *__restrict__ named, void *__restrict__ GP)
 {
     const int64_t r = t / (D / 4);
     const int c = 4 * (int)(t % (D / 4));
@@ -591,7 +665,7 @@ __device__ __forceinline__ void join_rows(int64_t t, const Args &a, const float 
         const float4 p = *reinterpret_cast<const float4 *>(part + ((size_t)k * part_rows + r) * D + c);
         s[0] += p.x; s[1] += p.y; s[2] += p.z; s[3] += p.w;
     }
-    const float f = F32 ? __uint_as_float(*top_factor) * (1.0f / kLift) * weight[r] : weight[r];
+    const float f = weight[r];
 #pragma unroll
     for (int j = 0; j < 4; ++j) s[j] *= f;
     for (int k = 0; k < a.T; ++k) {
@@ -610,15 +684,14 @@ __device__ __forceinline__ void join_rows(int64_t t, const Args &a, const float 
     else *reinterpret_cast<ushort4 *>((uint16_t *)GP + r * D + c) = make_ushort4(f32_bf16(s[0] * a.scale), f32_bf16(s[1] * a.scale), f32_bf16(s[2] * a.scale), f32_bf16(s[3] * a.scale));
 }
 
-// GQ: the passes' sums in order, each with its own scale of the positions' rows
+// GQ: the passes' sums in order
 struct Passes {
     int64_t flow_tiles, last_tiles;       // streaming tiles of a pass, of the last one
     int passes, pieces, last_pieces;
     int64_t stride;                       // elements of a pass' partial sums
 };
 template <int D, bool F32>
-__device__ __forceinline__ void join_items(int64_t t, int64_t cat, const float *__restrict__ part, const Passes &ps, int64_t part_rows, const float *__restrict__ factor,
-                                           float scale, void *__restrict__ GQ)
+__device__ __forceinline__ void join_items(int64_t t, int64_t cat, const float *__restrict__ part, const Passes &ps, int64_t part_rows, float scale, void *__restrict__ GQ)
 {
     const int64_t r = t / (D / 4);
     const int c = 4 * (int)(t % (D / 4));
@@ -627,13 +700,14 @@ __device__ __forceinline__ void join_items(int64_t t, int64_t cat, const float *
     for (int pass = 0; pass < ps.passes; ++pass) {
         const bool last = pass + 1 == ps.passes;
         const int segments = segments_of(r / 128, last ? ps.last_tiles : ps.flow_tiles, last ? ps.last_pieces : ps.pieces, part_rows);
-        const float f = F32 ? factor[pass] * (scale / kLift) : scale;
 #pragma unroll 4
         for (int k = 0; k < segments; ++k) {
             const float4 p = *reinterpret_cast<const float4 *>(part + (size_t)pass * ps.stride + ((size_t)k * part_rows + r) * D + c);
-            s[0] = fmaf(p.x, f, s[0]); s[1] = fmaf(p.y, f, s[1]); s[2] = fmaf(p.z, f, s[2]); s[3] = fmaf(p.w, f, s[3]);
+            s[0] += p.x; s[1] += p.y; s[2] += p.z; s[3] += p.w;
         }
     }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[j] *= scale;
     if constexpr (F32) *reinterpret_cast<float4 *>((float *)GQ + r * D + c) = make_float4(s[0], s[1], s[2], s[3]);
     else *reinterpret_cast<ushort4 *>((uint16_t *)GQ + r * D + c) = make_ushort4(f32_bf16(s[0]), f32_bf16(s[1]), f32_bf16(s[2]), f32_bf16(s[3]));
 }
@@ -641,11 +715,11 @@ __device__ __forceinline__ void join_items(int64_t t, int64_t cat, const float *
 // workgroups [0, row_wgs): GP; the rest (after the last pass): GQ
 template <int D, bool F32>
 __global__ __launch_bounds__(256) void join_kernel(Args a, Pass p, const float *__restrict__ weight, void *__restrict__ GP, int64_t row_wgs, Passes ps, const float *__restrict__ part_q,
-                                                   int64_t pad_q, const float *__restrict__ user_factor, void *__restrict__ GQ)
+                                                   int64_t pad_q, void *__restrict__ GQ)
 {
     const int64_t at = blockIdx.x;
-    if (at < row_wgs) join_rows<D, F32>(at * 256 + threadIdx.x, a, p.part, p.flow_tiles, p.pieces, p.part_rows, weight, p.top_factor, p.named, GP);
-    else join_items<D, F32>((at - row_wgs) * 256 + threadIdx.x, a.cat, part_q, ps, pad_q, user_factor, a.scale, GQ);
+    if (at < row_wgs) join_rows<D, F32>(at * 256 + threadIdx.x, a, p.part, p.flow_tiles, p.pieces, p.part_rows, weight, p.named, GP);
+    else join_items<D, F32>((at - row_wgs) * 256 + threadIdx.x, a.cat, part_q, ps, pad_q, a.scale, GQ);
 }
 
 // ---- T[ids[r]] += R[r] in the order of r -----------------------------------------------------------------------------------------------
@@ -685,9 +759,9 @@ __global__ __launch_bounds__(256) void add_rows_kernel(float *__restrict__ T, in
 // ---- host ---------------------------------------------------------------------------------------------------------------------------------
 struct Ws {
     char *user_rm, *user_t, *item_rm, *item_t;
-    float *tile_factor, *user_factor, *weight, *coef, *part_p, *part_q;
-    uint32_t *scalars;
+    float *tile_factor, *row_factor, *weight, *coef, *part_p, *part_q;
     Prm *prm;
+    Stay *stay;
     int32_t *named;
     uint32_t *bits;
     int64_t pass, passes, seg_q, pad_p, pad_q, bytes;
@@ -757,13 +831,13 @@ Ws carve(void *ws, int64_t rows, int64_t cat, int d, int dtype, bool mask, int T
     w.user_t = take(w.pad_p * rowb);
     w.item_rm = take(f32 ? w.pad_q * rowb : 0);
     w.item_t = take(w.pad_q * rowb);
-    w.tile_factor = (float *)take(item_tiles * 4);
-    w.user_factor = (float *)take(w.passes * 4);
+    w.tile_factor = (float *)take(f32 ? item_tiles * 4 : 0);
+    w.row_factor = (float *)take(f32 ? w.pad_q * 4 : 0);
     w.weight = (float *)take(w.pad_p * 4);
     w.coef = (float *)take(w.pass * T * 4);
     w.named = (int32_t *)take(w.pass * T * 4);
     w.prm = (Prm *)take(user_tiles * (int64_t)sizeof(Prm));
-    w.scalars = (uint32_t *)take((kLargest + row_groups(w.pad_p)) * 4);
+    w.stay = (Stay *)take(w.pad_p * (int64_t)sizeof(Stay));
     w.bits = (uint32_t *)take(mask ? w.pass * mask_words(cat) * 4 : 0);
     w.part_p = (float *)take(cells * d * 4);
     w.part_q = (float *)take(w.passes * w.seg_q * w.pad_q * d * 4);
@@ -783,17 +857,14 @@ void run(const Args &all, const int64_t *indptr, const int32_t *indices, const W
         a.user_ids += r0; a.lse += r0; a.g += r0 * a.T; a.items += r0 * a.T;
         if (a.ent) a.ent += r0;
         if (a.h) a.h += r0;
-        float *const largest = (float *)w.scalars + kLargest;
         const int64_t pad = pad128(a.rows), user_tiles = pad / kTile, item_tiles = k == 0 ? w.pad_q / kTile : 0, bit_rows = indptr ? a.rows : 0;
         if (item_tiles + bit_rows > 0)
             hipLaunchKernelGGL((items_kernel<D, F32>), dim3((unsigned)(item_tiles + bit_rows)), dim3(256), 0, st, a, indptr, indices, item_tiles, (uint4 *)w.item_rm, (uint4 *)w.item_t,
-                               w.tile_factor, w.bits);
-        const int groups = row_groups(pad);
-        hipLaunchKernelGGL((rows_kernel<D, F32>), dim3((unsigned)groups), dim3(256), 0, st, a, indptr ? w.bits : (const uint32_t *)nullptr, pad, w.prm, w.weight, w.named, w.coef, w.scalars,
-                           largest, w.tile_factor, w.pad_q / kTile);
-        hipLaunchKernelGGL((users_kernel<D, F32>), dim3((unsigned)user_tiles), dim3(256), 0, st, a, w.weight, largest, groups, (uint4 *)w.user_rm, (uint4 *)w.user_t, w.user_factor + k);
+                               w.tile_factor, w.row_factor, w.bits);
+        hipLaunchKernelGGL((rows_kernel<D, F32>), dim3((unsigned)row_groups(pad)), dim3(256), 0, st, a, indptr ? w.bits : (const uint32_t *)nullptr, pad, w.prm, w.stay, w.weight, w.named, w.coef);
+        hipLaunchKernelGGL((users_kernel<D, F32>), dim3((unsigned)user_tiles), dim3(256), 0, st, a, w.weight, (uint4 *)w.user_rm, (uint4 *)w.user_t);
         Pass p;                               // users stay
-        p.top_factor = w.scalars; p.prm = w.prm; p.bits = w.bits; p.named = w.named; p.coef = w.coef;
+        p.tile_factor = w.tile_factor; p.row_factor = w.row_factor; p.prm = w.prm; p.stay_prm = w.stay; p.bits = w.bits; p.named = w.named; p.coef = w.coef;
         p.positions = a.rows; p.cat = a.cat; p.T = a.T; p.factor = a.scale * kLog2e;
         p.stay = w.user_rm; p.flow = F32 ? w.item_rm : (const char *)a.Q; p.flow_t = w.item_t;
         p.stay_rows = pad; p.flow_tiles = (a.cat + kTile - 1) / kTile; p.flow_valid = a.cat;
@@ -804,7 +875,7 @@ void run(const Args &all, const int64_t *indptr, const int32_t *indices, const W
         q.stay_rows = F32 ? w.pad_q : a.cat; q.flow_tiles = user_tiles; q.flow_valid = a.rows;
         q.part = w.part_q + (size_t)k * w.seg_q * w.pad_q * D; q.part_rows = w.pad_q;
         q.pieces = grad_pieces(a.cat, user_tiles, w.wgs, w.st);
-#define RSX_GRAD(M_, E_) hipLaunchKernelGGL((grad_kernel<D, F32, M_, E_>), dim3((unsigned)(p.pieces + q.pieces)), dim3(GradGeo<D, F32>::NT), 0, st, p, q, w.tile_factor)
+#define RSX_GRAD(M_, E_) hipLaunchKernelGGL((grad_kernel<D, F32, M_, E_>), dim3((unsigned)(p.pieces + q.pieces)), dim3(GradGeo<D, F32>::NT), 0, st, p, q)
         if (indptr) { if (a.h) RSX_GRAD(true, true); else RSX_GRAD(true, false); }
         else { if (a.h) RSX_GRAD(false, true); else RSX_GRAD(false, false); }
 #undef RSX_GRAD
@@ -812,7 +883,7 @@ void run(const Args &all, const int64_t *indptr, const int32_t *indices, const W
         ps.last_tiles = user_tiles; ps.last_pieces = q.pieces;
         const int64_t joins = (a.rows * (D / 4) + 255) / 256, item_joins = k + 1 == w.passes ? (a.cat * (D / 4) + 255) / 256 : 0;
         hipLaunchKernelGGL((join_kernel<D, F32>), dim3((unsigned)(joins + item_joins)), dim3(256), 0, st, a, p, w.weight, (char *)GP + r0 * D * es, joins, ps, w.part_q, w.pad_q,
-                           w.user_factor, GQ);
+                           GQ);
     }
 }
 
