@@ -113,6 +113,22 @@ __device__ __forceinline__ void split8_times(const float *x, double k, Frag *hi,
     }
 }
 
+// eight consecutive elements of a table row in fp32
+template <bool F32>
+__device__ __forceinline__ void load8(const void *base, int64_t at, float *x)
+{
+    if constexpr (F32) {
+        const float4 *p = reinterpret_cast<const float4 *>((const float *)base + at);
+        const float4 a = p[0], b = p[1];
+        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    } else {
+        const uint4 v = *reinterpret_cast<const uint4 *>((const uint16_t *)base + at);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { x[2 * j] = __uint_as_float(w[j] << 16); x[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u); }
+    }
+}
+
 // rows of the call: a position whose user id is outside the table names no row
 __device__ __forceinline__ bool row_ok(int32_t u, int64_t num_users) { return u >= 0 && u < num_users; }
 

@@ -66,22 +66,6 @@ __device__ __forceinline__ float pick_reference(float a, float b, float c)
 // their products in 64 bits), and -inf is left to the chunks that hold nothing
 __device__ __forceinline__ uint32_t key_bits(float a, float b) { return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b)); }
 
-// eight consecutive elements of a table row in fp32
-template <bool F32>
-__device__ __forceinline__ void load8(const void *base, int64_t at, float *x)
-{
-    if constexpr (F32) {
-        const float4 *p = reinterpret_cast<const float4 *>((const float *)base + at);
-        const float4 a = p[0], b = p[1];
-        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-    } else {
-        const uint4 v = *reinterpret_cast<const uint4 *>((const uint16_t *)base + at);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) { x[2 * j] = __uint_as_float(w[j] << 16); x[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u); }
-    }
-}
-
 // the reference a row's chunk maxima are stored against: a score of its own, so that an offset common to a row's scores does not eat the halves'
 // eleven bits.  One wavefront per row.
 template <int D, bool F32>

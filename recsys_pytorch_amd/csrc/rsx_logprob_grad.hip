@@ -15,15 +15,13 @@
 // 8 n I d operations instead of the 6 that a stored dz would take, against 3 n I of stored and twice read halves: recomputing is the
 // cheaper side from d = 128 down (4096 x 100 000 x 128: 0.4 TFLOP against 2.4 GB).  No atomics: every sum has one order.
 //
-// fp32: three products of halves (rsx_logprob.h) on both sides, dz is a half pair too.  A half ends at 2^-25 (half its last step), a row's sum may be
-// of probabilities near 1 or of 2^-60: every column keeps a power of two M of its own, and dz |y| / 2^M is what is split, y scaled to its row's (32 item
-// rows': rsx_logprob.h) largest element.  M follows the first terms and is raised, with the sums, where a tile exceeds it: the largest term of
-// a sum is held at 2^7 or more, the others to 2^-32 of it, whatever other columns, rows or weights are.  Rising costs a maximum of the tile's
-// exponents a score and a branch a tile that is hardly taken after the first.  A tile's shares of exponent and sign are in the row's
-// parameters: the scores' exponential delivers dz |y| / 2^M as it is.  bf16: dz is rounded to bf16, an error of a
-// term that is at most as large as that of rounding the result (the same where one term is all of it; sums of many average theirs out).
-#include <type_traits>
-
+// dz goes into the second product as halves, one (bf16 tables: 2^-11 of itself, an eighth of what rounding the result to bf16 may take; dz in bf16, as far off
+// as the result's rounding, was measured at 2.3e-3 instead of 1.7e-3 of GP) or two (fp32 tables: three products, rsx_logprob.h, on both sides).  A half ends
+// at 2^-25 (half its last step), a row's sum may be of probabilities near 1 or of 2^-60: every column keeps a power of two M of its own, and dz |y| / 2^M is
+// what is split, y scaled to its row's (32 item rows': rsx_logprob.h) largest element.  M follows the first terms and is raised, with the sums, where a tile
+// exceeds it: the largest term of a sum is held at 2^7 or more, the others to 2^-32 of it, whatever other columns, rows or weights are.  Rising costs a maximum of
+// the tile's exponents a score and a branch a tile that is hardly taken after the first.  A tile's shares of exponent and sign are in the
+// row's parameters: the scores' exponential delivers dz |y| / 2^M as it is.  bf16 rows in scaled halves are what they were down to 2^-31 of their scale.
 #include "rsx_logprob.h"
 
 namespace {
@@ -49,12 +47,12 @@ struct Args {
 // per tile of 32 positions: [0] factor of its scores (bf16: the same in every row), [1] what is added to them, [2] [3] dz = 2^t (A + B t), [4] .. [7] the first
 // four named items (as integers; -1: none): 1 KB, one wavefront's copy.  Without the entropy's part B = 0: [1] is log2 |A| - lse, so that the
 // exponential is |dz|, and the sign of A goes with the row's weight (GP) and into the streaming rows (GQ): the same products with one parameter of a row
-// instead of three and a multiplication less a score (4096 x 100K x 128 fp32: 1.173 -> 1.161 ms).  fp32: the row's exponent is in [1], and taken out of A t.
+// instead of three and a multiplication less a score (4096 x 100K x 128 fp32: 1.173 -> 1.161 ms).  The row's exponent is in [1], and taken out of A t.
 constexpr int kHeld = 4;
 struct Prm {
     float v[4 + kHeld][kTile];
 };
-// the same of a position that stays: without its row's exponent; w: the exponent of its weight, out of A and B (fp32 with the entropy's part)
+// the same of a position that stays: without its row's exponent; w: the exponent of its weight, out of A and B (with the entropy's part)
 struct Stay {
     float f, off, A, B, w, pad[3];
 };
@@ -96,23 +94,22 @@ __global__ __launch_bounds__(256) void rows_kernel(Args a, const uint32_t *__res
         const double w = mag + fabs((double)h);
         float factor = live ? F32 ? 1.0f : a.scale * kLog2e : 0.0f;
         int e_row = 0, e_w = 0;                // exponents of the row and (with the entropy's part) of its weight
-        if constexpr (F32) {
-            float big = 0.0f;
-            if (ok && lane < D / 8) {
-                const float4 *p = reinterpret_cast<const float4 *>((const float *)a.P + (int64_t)u * D + 8 * lane);
-                const float4 x = p[0], y = p[1];
-                big = fmaxf(fmaxf(fmaxf(finite_abs(x.x), finite_abs(x.y)), fmaxf(finite_abs(x.z), finite_abs(x.w))),
-                            fmaxf(fmaxf(finite_abs(y.x), finite_abs(y.y)), fmaxf(finite_abs(y.z), finite_abs(y.w))));
-            }
+        float big = 0.0f, up, down;
+        if (ok && lane < D / 8) {
+            float x[8];
+            load8<F32>(a.P, (int64_t)u * D + 8 * lane, x);
 #pragma unroll
-            for (int o = 32; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor(big, o, 64));
-            float up, down;
+            for (int j = 0; j < 8; ++j) big = fmaxf(big, finite_abs(x[j]));
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor(big, o, 64));
+        if constexpr (F32) {
             scale_for(big * (a.scale * kLog2e), &up, &down);
             factor *= down;
-            scale_for(big, &up, &down);
-            e_row = (int)exponent_of_factor(down);
-            if (a.h != nullptr) e_w = exponent_of((float)w);
         }
+        scale_for(big, &up, &down);
+        e_row = (int)exponent_of_factor(down);
+        if (a.h != nullptr) e_w = exponent_of((float)w);
         for (int t = lane; t < a.T && r < a.rows; t += 64) {              // (a masked item is not looked up)
             const int32_t i = a.items[r * a.T + t];
             coef[r * a.T + t] = ok && i >= 0 && i < a.cat ? ldexpf(a.g[r * a.T + t] * sign, e_row) : 0.0f;
@@ -150,18 +147,18 @@ __global__ __launch_bounds__(256) void rows_kernel(Args a, const uint32_t *__res
 template <int D>
 __device__ __forceinline__ int tile_row(int half, int hi, int j) { const int i = 8 * half + j; return (i & 3) + 8 * (i >> 2) + 4 * hi; }
 
-// a tile of 32 rows by 256 threads: row-major planes and the transposed tile.  USERS: rows gathered by user id, each times scale log2 e and with its own
+// a tile of 32 rows by 256 threads: row-major planes (bf16 items: the table is that) and the transposed tile.  USERS: rows gathered by user id, each times scale log2 e and with its own
 // power of two in the row-major planes, times its own and its sign (0: no weight) in the transposed ones.  Items: the tile's power of two in both, or each row's own
 // where they are too unequal (rsx_logprob.h).
-template <int D, bool F32>
+template <int D>
 struct TileLds {
-    typename std::conditional<F32, float, uint16_t>::type x[kTile][D + 1];
+    float x[kTile][D + 1];
     float range[8], big[kTile], mul[kTile];
 };
 
 template <int D, bool F32, bool USERS>
 __device__ __forceinline__ void lay_tile(const Args &a, int64_t tile, const float *__restrict__ weight, uint4 *__restrict__ rowm, uint4 *__restrict__ tr, float *__restrict__ factor,
-                                         float *__restrict__ row_factor, TileLds<D, F32> &lds)
+                                         float *__restrict__ row_factor, TileLds<D> &lds)
 {
     constexpr int TPR = D / 8;
     auto &x = lds.x;
@@ -175,41 +172,32 @@ __device__ __forceinline__ void lay_tile(const Args &a, int64_t tile, const floa
         int64_t row = at < n ? at : -1;
         if constexpr (USERS) { const int32_t u = row >= 0 ? a.user_ids[row] : -1; row = row_ok(u, a.users) ? u : -1; }
         const void *src = USERS ? a.P : a.Q;
-        if constexpr (F32) {
-            float v[8];
-            const float4 *p = reinterpret_cast<const float4 *>((const float *)src + (row < 0 ? 0 : row) * D + c);
-            const float4 y = p[0], z = p[1];
-            v[0] = y.x; v[1] = y.y; v[2] = y.z; v[3] = y.w; v[4] = z.x; v[5] = z.y; v[6] = z.z; v[7] = z.w;
-            float big = 0.0f, up, down;
+        float v[8], big = 0.0f, up, down;
+        load8<F32>(src, (row < 0 ? 0 : row) * D + c, v);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) { v[j] = row < 0 ? 0.0f : v[j]; big = fmaxf(big, finite_abs(v[j])); x[r][c + j] = v[j]; }
-            big = row_max<TPR>(big);
-            if constexpr (USERS) {
+        for (int j = 0; j < 8; ++j) { v[j] = row < 0 ? 0.0f : v[j]; big = fmaxf(big, finite_abs(v[j])); x[r][c + j] = v[j]; }
+        big = row_max<TPR>(big);
+        if constexpr (USERS) {
+            if constexpr (F32) {
                 scale_for(big * (a.scale * kLog2e), &up, &down);
                 Frag h, l;
                 split8_times(v, (double)a.scale * 1.4426950408889634074 * up, &h, &l);
                 rowm[(size_t)at * (2 * TPR) + t % TPR] = h.u;
                 rowm[(size_t)at * (2 * TPR) + TPR + t % TPR] = l.u;
-                scale_for(big, &up, &down);
-                if (c == 0) s_mul[r] = weight[at] * up;
             } else {
-                most = fmaxf(most, big);
-                least = big > 0.0f ? fminf(least, big) : least;
-                if (c == 0) lds.big[r] = big;
+                uint4 y = *reinterpret_cast<const uint4 *>((const uint16_t *)src + (row < 0 ? 0 : row) * D + c);
+                if (row < 0) y = make_uint4(0u, 0u, 0u, 0u);
+                rowm[(size_t)at * TPR + t % TPR] = y;
             }
+            scale_for(big, &up, &down);
+            if (c == 0) s_mul[r] = weight[at] * up;
         } else {
-            uint4 v = *reinterpret_cast<const uint4 *>((const uint16_t *)src + (row < 0 ? 0 : row) * D + c);
-            if (row < 0) v = make_uint4(0u, 0u, 0u, 0u);
-            if constexpr (USERS) rowm[(size_t)at * TPR + t % TPR] = v;
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) { x[r][c + 2 * j] = (uint16_t)w[j]; x[r][c + 2 * j + 1] = (uint16_t)(w[j] >> 16); }
+            most = fmaxf(most, big);
+            least = big > 0.0f ? fminf(least, big) : least;
+            if (c == 0) lds.big[r] = big;
         }
     }
-    if constexpr (USERS && !F32) {
-        if (tid < kTile) s_mul[tid] = weight[tile * kTile + tid];
-    }
-    if constexpr (F32 && !USERS) {
+    if constexpr (!USERS) {
         tile_range(&most, &least, lds.range);
         const bool own = least * kUneven < most;
         if (tid < kTile) {
@@ -220,7 +208,7 @@ __device__ __forceinline__ void lay_tile(const Args &a, int64_t tile, const floa
             if (tid == 0) factor[tile] = own ? kOwnScales : down;
         }
         __syncthreads();
-        for (int t = tid; t < kTile * TPR; t += 256) {
+        for (int t = tid; F32 && t < kTile * TPR; t += 256) {
             const int r = t / TPR, c = 8 * (t % TPR);
             float v[8];
 #pragma unroll
@@ -238,27 +226,15 @@ __device__ __forceinline__ void lay_tile(const Args &a, int64_t tile, const floa
     for (int t = tid; t < NF; t += 256) {
         const int lane = t & 63, half = (t >> 6) & 1, kb = t >> 7, col = 32 * kb + (lane & 31);
         Frag h, l;
-        if constexpr (F32) {
-            float v[8];
+        float v[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int r = tile_row<D>(half, lane >> 5, j);
-                const float y = x[r][col];
-                v[j] = (fabsf(y) < INFINITY ? y : 0.0f) * s_mul[r];
-            }
-            split8(v, &h, &l);
-            dst[NF + t] = l.u;
-        } else {
-            uint16_t v[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int r = tile_row<D>(half, lane >> 5, j);
-                const uint16_t y = x[r][col];
-                v[j] = (y & 0x7F80u) == 0x7F80u ? (uint16_t)0 : y;
-                if constexpr (USERS) v[j] ^= s_mul[r] < 0.0f ? 0x8000u : 0u;
-            }
-            h.u = make_uint4(v[0] | ((uint32_t)v[1] << 16), v[2] | ((uint32_t)v[3] << 16), v[4] | ((uint32_t)v[5] << 16), v[6] | ((uint32_t)v[7] << 16));
+        for (int j = 0; j < 8; ++j) {
+            const int r = tile_row<D>(half, lane >> 5, j);
+            const float y = x[r][col];
+            v[j] = (fabsf(y) < INFINITY ? y : 0.0f) * s_mul[r];
         }
+        split8(v, &h, &l);
+        if constexpr (F32) dst[NF + t] = l.u;
         dst[t] = h.u;
     }
 }
@@ -269,7 +245,7 @@ template <int D, bool F32>
 __global__ __launch_bounds__(256) void items_kernel(Args a, const int64_t *__restrict__ indptr, const int32_t *__restrict__ indices, int64_t tiles, uint4 *__restrict__ rowm,
                                                     uint4 *__restrict__ tr, float *__restrict__ factor, float *__restrict__ row_factor, uint32_t *__restrict__ bits)
 {
-    __shared__ __attribute__((aligned(16))) union { TileLds<D, F32> tile; uint32_t bits[kBitWords]; } lds;
+    __shared__ __attribute__((aligned(16))) union { TileLds<D> tile; uint32_t bits[kBitWords]; } lds;
     const int64_t at = blockIdx.x;
     if (at < tiles) {
         lay_tile<D, F32, false>(a, at, nullptr, rowm, tr, factor, row_factor, lds.tile);
@@ -282,7 +258,7 @@ __global__ __launch_bounds__(256) void items_kernel(Args a, const int64_t *__res
 template <int D, bool F32>
 __global__ __launch_bounds__(256) void users_kernel(Args a, const float *__restrict__ weight, uint4 *__restrict__ rowm, uint4 *__restrict__ tr)
 {
-    __shared__ __attribute__((aligned(16))) TileLds<D, F32> lds;
+    __shared__ __attribute__((aligned(16))) TileLds<D> lds;
     lay_tile<D, F32, true>(a, blockIdx.x, weight, rowm, tr, nullptr, nullptr, lds);
 }
 
@@ -290,7 +266,7 @@ __global__ __launch_bounds__(256) void users_kernel(Args a, const float *__restr
 struct Pass {
     const char *stay, *flow;              // row-major planes of what stays in registers and of what streams
     const char *flow_t;                   // transposed tiles of what streams
-    const float *tile_factor, *row_factor;      // fp32 items: a tile's (or kOwnScales), a row's
+    const float *tile_factor, *row_factor;      // items: a tile's scale (or kOwnScales), a row's
     const Prm *prm;
     const Stay *stay_prm;
     const uint32_t *bits;
@@ -436,7 +412,7 @@ __device__ __forceinline__ void grad_body(const Pass &a, int64_t piece, char *ld
                 const char *sb = lds + G::BITS + j * 1024;
                 seen = ITEMS_STAY ? *reinterpret_cast<const uint32_t *>(sb + l31 * 16 + wid * 4) : *reinterpret_cast<const uint32_t *>(sb + wid * 256 + lane * 4);
             }
-            const float tf = !ITEMS_STAY && F32 ? a.tile_factor[tile] : my_factor;
+            const float tf = ITEMS_STAY ? my_factor : a.tile_factor[tile];
             const char *rm = lds + j * G::TILEB + l31 * G::ROWB;
             const char *tr = lds + ST * G::TILEB + j * G::TILEB + lane * 16;
             __builtin_amdgcn_s_setprio(1);         // (a wavefront in its products goes first: the two of a SIMD fall into step otherwise; 1.19 -> 1.16 ms)
@@ -459,9 +435,9 @@ __device__ __forceinline__ void grad_body(const Pass &a, int64_t piece, char *ld
             float v[16];
             float s[16], t[ENT ? 16 : 1];
             float need = 0.0f;                     // sum of the named items' |dz| |y| of this column
-            uint64_t hit = F32 ? 0 : ~0ull;        // which of the T names have one here (bit k & 63)
+            uint64_t hit = 0;                      // which of the T names have one here (bit k & 63)
             if constexpr (!ITEMS_STAY) {
-                if (F32 && tf < 0.0f) {            // (kOwnScales: rare, and loads in the loop)
+                if (tf < 0.0f) {                   // (kOwnScales: rare, and loads in the loop)
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
                         const float4 y = *reinterpret_cast<const float4 *>(a.row_factor + tile * kTile + 8 * q + 4 * hi);
@@ -469,12 +445,13 @@ __device__ __forceinline__ void grad_body(const Pass &a, int64_t piece, char *ld
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const float by = exponent_of_factor(ys[e]) + sE - M;
-                            if constexpr (ENT) { t[4 * q + e] = fmaf(acc[4 * q + e], sf * ys[e], slse); s[4 * q + e] = t[4 * q + e] + by; }
-                            else s[4 * q + e] = fmaf(acc[4 * q + e], sf * ys[e], slse + by);
+                            const float f = F32 ? sf * ys[e] : sf;
+                            if constexpr (ENT) { t[4 * q + e] = fmaf(acc[4 * q + e], f, slse); s[4 * q + e] = t[4 * q + e] + by; }
+                            else s[4 * q + e] = fmaf(acc[4 * q + e], f, slse + by);
                         }
                     }
                 } else {
-                    const float f = sf * tf, by = F32 ? exponent_of_factor(tf) + sE - M : 0.0f, off = slse + by;
+                    const float f = F32 ? sf * tf : sf, by = exponent_of_factor(tf) + sE - M, off = slse + by;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         if constexpr (ENT) { t[i] = fmaf(acc[i], f, slse); s[i] = t[i] + by; }
@@ -503,8 +480,8 @@ __device__ __forceinline__ void grad_body(const Pass &a, int64_t piece, char *ld
                     const float fs[4] = {f4.x, f4.y, f4.z, f4.w}, ls[4] = {l4.x, l4.y, l4.z, l4.w};
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        if constexpr (ENT) { t[4 * q + e] = fmaf(acc[4 * q + e], fs[e] * tf, ls[e]); s[4 * q + e] = F32 ? t[4 * q + e] - M : t[4 * q + e]; }
-                        else s[4 * q + e] = fmaf(acc[4 * q + e], fs[e] * tf, F32 ? ls[e] - M : ls[e]);
+                        if constexpr (ENT) { t[4 * q + e] = fmaf(acc[4 * q + e], fs[e] * tf, ls[e]); s[4 * q + e] = t[4 * q + e] - M; }
+                        else s[4 * q + e] = fmaf(acc[4 * q + e], fs[e] * tf, ls[e] - M);
                     }
                 }
                 if (MASK && __builtin_amdgcn_ballot_w64(seen != 0u) != 0ull) {
@@ -520,7 +497,7 @@ __device__ __forceinline__ void grad_body(const Pass &a, int64_t piece, char *ld
             auto named = [&](bool add, auto f) __attribute__((always_inline)) {
                 const Prm *prm = reinterpret_cast<const Prm *>(lds + G::PRM + j * 1024);
                 for (int k = 0; k < a.T; ++k) {
-                    if (F32 && add && !((hit >> (k & 63)) & 1)) continue;
+                    if (add && !((hit >> (k & 63)) & 1)) continue;
                     const int64_t r = tile * kTile + l31;
                     const int32_t it = k < kHeld ? __float_as_int(prm->v[4 + k][l31]) : r < a.positions ? a.named[r * a.T + k] : -1;
                     const bool mine = hi == 0 && (it >> 5) == my_block;          // (-1 >> 5 is nobody's block)
@@ -535,7 +512,7 @@ __device__ __forceinline__ void grad_body(const Pass &a, int64_t piece, char *ld
                     }
                 }
             };
-            if constexpr (F32) {
+            {
                 if constexpr (ITEMS_STAY) named(false, [&](int, int at, float c) { need += l31 == at ? fabsf(c) : 0.0f; });
                 float most = s[0];
 #pragma unroll
@@ -565,13 +542,13 @@ __device__ __forceinline__ void grad_body(const Pass &a, int64_t piece, char *ld
             }
             if (ITEMS_STAY && hit != 0)
                 named(true, [&](int row, int at, float c) {
-                    const float add = F32 ? ldexpf(c, -(int)M) : c;
+                    const float add = ldexpf(c, -(int)M);
                     const int reg = (row & 3) | ((row >> 3) << 2);
                     const bool here = lane == at + 32 * ((row >> 2) & 1);
 #pragma unroll
                     for (int i = 0; i < 16; ++i) v[i] += here && i == reg ? add : 0.0f;
                 });
-            if constexpr (F32 && ENT) {
+            if constexpr (ENT) {
                 float most = fabsf(v[0]);
 #pragma unroll
                 for (int i = 1; i < 16; ++i) most = fmaxf(most, fabsf(v[i]));
@@ -592,17 +569,21 @@ __device__ __forceinline__ void grad_body(const Pass &a, int64_t piece, char *ld
                     split8(v + 8 * h, &z[0], &z[NP - 1]);
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) z[0].b[e] = (__bf16)v[8 * h + e];
+                    for (int e = 0; e < 8; e += 2) {
+                        const float2v w = {v[8 * h + e], v[8 * h + e + 1]};
+                        const half2v y = __builtin_convertvector(w, half2v);
+                        z[0].h[e] = y[0]; z[0].h[e + 1] = y[1];
+                    }
                 }
 #pragma unroll
                 for (int k = 0; k < KB; ++k) {
                     Frag y[NP];
 #pragma unroll
                     for (int p = 0; p < NP; ++p) y[p].u = *reinterpret_cast<const uint4 *>(tr + ((p * G::KB + half * KB + k) * 2 + h) * 1024);
-                    out[k] = mfma32<F32>(y[0], z[0], out[k]);
+                    out[k] = mfma32<true>(y[0], z[0], out[k]);
                     if constexpr (F32) {
-                        out[k] = mfma32<F32>(y[0], z[NP - 1], out[k]);
-                        out[k] = mfma32<F32>(y[NP - 1], z[0], out[k]);
+                        out[k] = mfma32<true>(y[0], z[NP - 1], out[k]);
+                        out[k] = mfma32<true>(y[NP - 1], z[0], out[k]);
                     }
                 }
             }
@@ -623,7 +604,7 @@ __device__ __forceinline__ void grad_body(const Pass &a, int64_t piece, char *ld
         }
     }
     float *dst = a.part + ((size_t)segment * a.part_rows + col) * D + 32 * KB * half + 4 * hi;
-    const int e = F32 ? (int)M - kUnit : 0;
+    const int e = (int)M - kUnit;
 #pragma unroll
     for (int k = 0; k < KB; ++k)
 #pragma unroll
@@ -831,8 +812,8 @@ Ws carve(void *ws, int64_t rows, int64_t cat, int d, int dtype, bool mask, int T
     w.user_t = take(w.pad_p * rowb);
     w.item_rm = take(f32 ? w.pad_q * rowb : 0);
     w.item_t = take(w.pad_q * rowb);
-    w.tile_factor = (float *)take(f32 ? item_tiles * 4 : 0);
-    w.row_factor = (float *)take(f32 ? w.pad_q * 4 : 0);
+    w.tile_factor = (float *)take(item_tiles * 4);
+    w.row_factor = (float *)take(w.pad_q * 4);
     w.weight = (float *)take(w.pad_p * 4);
     w.coef = (float *)take(w.pass * T * 4);
     w.named = (int32_t *)take(w.pass * T * 4);

@@ -87,7 +87,7 @@ def test_hip_gradient_of_probabilities_far_below_one(d, entropy):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("entropy", [False, True])
-@pytest.mark.parametrize("bf16", [False])
+@pytest.mark.parametrize("bf16", [False, True])
 @pytest.mark.parametrize("size", [1e4, 1e6, 1e9, 1e25])
 def test_hip_gradient_beside_masked_rows_of_large_values(size, bf16, entropy):
     rng = np.random.default_rng(7)
@@ -104,7 +104,7 @@ def test_hip_gradient_beside_masked_rows_of_large_values(size, bf16, entropy):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("entropy", [False, True])
-@pytest.mark.parametrize("bf16", [False])
+@pytest.mark.parametrize("bf16", [False, True])
 def test_hip_gradient_beside_an_item_of_probability_zero(bf16, entropy):
     """one unmasked row a million times the others, its score -3 10^6 for everybody"""
     rng = np.random.default_rng(3)
@@ -120,7 +120,7 @@ def test_hip_gradient_beside_an_item_of_probability_zero(bf16, entropy):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("entropy", [False, True])
-@pytest.mark.parametrize("bf16", [False])
+@pytest.mark.parametrize("bf16", [False, True])
 def test_hip_gradient_of_weights_and_rows_of_many_sizes(bf16, entropy):
     """weights from 10^-12 to 1 and user rows from 10^-3 to 1 in one batch, item rows from 10^-6 to 1 side by side"""
     import torch
@@ -134,3 +134,14 @@ def test_hip_gradient_of_weights_and_rows_of_many_sizes(bf16, entropy):
     w = 10.0 ** rng.uniform(-12, 0, n)
     within(P, Q, rng.permutation(n), rng.integers(0, I, (n, 5)), rng.standard_normal((n, 5)) * w[:, None], rng.standard_normal(n) * w if entropy else None,
            seen_csr(rng, n, I, 20))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [32, 64, 128, 256])
+@pytest.mark.parametrize("n,I,T,masked,entropy", [(6, 300, 1, False, False), (200, 900, 7, True, False), (70, 130, 3, True, True)])
+def test_hip_gradient_of_bf16_tables_to_the_results_rounding(n, I, T, masked, entropy, d):
+    """dz is not rounded to bf16 on its way: sums that cancel show it"""
+    rng = np.random.default_rng(n + d)
+    P, Q = tables(rng, n, I, d, True)
+    within(P, Q, rng.permutation(n), rng.integers(0, I, (n, T)), rng.standard_normal((n, T)) / n, rng.standard_normal(n) / n if entropy else None,
+           seen_csr(rng, n, I, 30) if masked else None)
