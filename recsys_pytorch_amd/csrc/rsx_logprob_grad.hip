@@ -110,24 +110,30 @@ __global__ __launch_bounds__(256) void rows_kernel(Args a, const uint32_t *__res
         scale_for(big, &up, &down);
         e_row = (int)exponent_of_factor(down);
         if (a.h != nullptr) e_w = exponent_of((float)w);
-        for (int t = lane; t < a.T && r < a.rows; t += 64) {              // (a masked item is not looked up)
-            const int32_t i = a.items[r * a.T + t];
-            coef[r * a.T + t] = ok && i >= 0 && i < a.cat ? ldexpf(a.g[r * a.T + t] * sign, e_row) : 0.0f;
-        }
-        // dz = p (A + B log2 p), p = 2^(z - lse2), by t = z + off, off the rounded e - lse2: what the rounding (half a step at 24 is 1e-6 of every p) and
-        // e change goes into the coefficients
+        // dz = p (A + B log2 p), p = 2^(z - lse2).  Without the entropy's part |dz| = 2^(z + off), off = log2 |A| - lse2 in whole 2^-15, to which whole exponents
+        // add exactly; what is left (`fix`) goes where the sign goes.  With it, by t = z + off, off the rounded e - lse2: what the rounding (half a
+        // step at 24 is 1e-6 of every p) and e change goes into the coefficients
         const double lse2 = (double)lse * 1.4426950408889634074;
         const double H = a.h != nullptr ? (double)h * a.ent[r < a.rows ? r : 0] : 0.0;
         const double A = live ? ldexp(-(sum + H), -e_w) : 0.0, B = live ? ldexp(-(double)h * kLn2, -e_w) : 0.0;
+        const bool none = !live || (a.h == nullptr && sum == 0.0);
+        const double exact = log2(fabs(sum)) - lse2;
+        const float near = (float)(rint(exact * 32768.0) * 0x1p-15);
+        const double fix = a.h == nullptr && !none ? exp2(exact - (double)near) : 1.0;
         auto params = [&](int e, float *off, float *pa, float *pb) {
-            if (!live || (a.h == nullptr && sum == 0.0)) { *off = -kFar; *pa = *pb = 0.0f; return; }
-            if (a.h == nullptr) { *off = (float)(log2(fabs(sum)) - lse2 + e); *pa = *pb = 0.0f; return; }
+            *off = none ? -kFar : near + (float)e;
+            *pa = *pb = 0.0f;
+            if (a.h == nullptr || none) return;
             const double want = e - lse2;
             *off = (float)want;
-            const double d = (double)*off - want, fix = exp2(-d);
-            *pa = (float)((A - B * (e + d)) * fix);
-            *pb = (float)(B * fix);
+            const double d = (double)*off - want, turn = exp2(-d);
+            *pa = (float)((A - B * (e + d)) * turn);
+            *pb = (float)(B * turn);
         };
+        for (int t = lane; t < a.T && r < a.rows; t += 64) {              // (a masked item is not looked up)
+            const int32_t i = a.items[r * a.T + t];
+            coef[r * a.T + t] = ok && i >= 0 && i < a.cat ? (float)ldexp((double)a.g[r * a.T + t] * sign / fix, e_row) : 0.0f;
+        }
         if (lane == 0) {
             Stay q{};
             q.f = factor;
@@ -137,7 +143,7 @@ __global__ __launch_bounds__(256) void rows_kernel(Args a, const uint32_t *__res
             out.v[0][c] = factor;
             params(e_row + e_w, &out.v[1][c], &out.v[2][c], &out.v[3][c]);
             for (int k = a.T; k < kHeld; ++k) out.v[4 + k][c] = __int_as_float(-1);
-            weight[r] = live && !(w == 0.0) ? sign : 0.0f;                // (no weight, no gradient; NaN stays NaN)
+            weight[r] = live && !(w == 0.0) ? sign * (float)fix : 0.0f;   // (no weight, no gradient; NaN stays NaN)
         }
     }
 }
@@ -631,7 +637,7 @@ __device__ __forceinline__ int segments_of(int64_t block, int64_t flow_tiles, in
 }
 
 // ---- the partial sums -> the gradients ------------------------------------------------------------------------------------------------------
-// GP: four elements a thread; the partials in order, the row's sign, the named rows of Q
+// GP: four elements a thread; the partials in order, the row's sign (and what its exponent was rounded by), the named rows of Q
 template <int D, bool F32>
 __device__ __forceinline__ void join_rows(int64_t t, const Args &a, const float *__restrict__ part, int64_t flow_tiles, int pieces, int64_t part_rows, const float *__restrict__ weight,
                                                         const int32_t *__restrict__ named, void *__restrict__ GP)

@@ -145,3 +145,25 @@ def test_hip_gradient_of_bf16_tables_to_the_results_rounding(n, I, T, masked, en
     P, Q = tables(rng, n, I, d, True)
     within(P, Q, rng.permutation(n), rng.integers(0, I, (n, T)), rng.standard_normal((n, T)) / n, rng.standard_normal(n) / n if entropy else None,
            seen_csr(rng, n, I, 30) if masked else None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("weight", [1.0, -3.0])
+def test_hip_gradient_of_one_probability(weight):
+    """one item, scores of 64 to 127 binades: scale = ln 2, so that the operands (x scale log2 e in 22 bits) are exact to 2^-28 and z log2 e to 2^-21.  p = exp(z - lse) of
+    the lse that is handed in: the exponent's half step where it is below 1 is 2^-25, the exponential is off by 2^-23, the half pair by 2^-22, the row by 2^-22,
+    z by 2^-21: 1.1e-6; nothing of the normaliser's own size (half a step at 127 is 2.6e-6 of p)"""
+    import torch
+    from recsys_pytorch_amd import rsx
+    n, d, scale = 64, 32, float(np.float32(np.log(2)))
+    rng = np.random.default_rng(1)
+    P, Q = torch.zeros(n, d), torch.zeros(1, d)
+    P[:, 0], Q[0, 0], Q[0, 1] = torch.arange(64, 64 + n) / 8.0, 8.0, 1.0
+    z = (P[:, 0] * 8.0).double().numpy() * scale
+    lse = np.float32(z + rng.uniform(0.0, 0.01, n))
+    p = np.exp(z - lse.astype(np.float64))
+    dev = lambda a, t=np.float32: torch.from_numpy(np.ascontiguousarray(a, t)).cuda()
+    GP, GQ = rsx.score_logprobs_grad(P.cuda(), Q.cuda(), dev(np.arange(n), np.int32), dev(np.zeros((n, 1)), np.int32), dev(lse), dev(np.full((n, 1), weight)), scale=scale)
+    # 1 - p of two numbers near 1: their own roundings (2^-24 each) and the result's beside p's
+    want, tol = weight * scale * (1 - p), abs(weight) * scale * (1.1e-6 + 2.0 ** -23)
+    assert (np.abs(GP[:, 1].double().cpu().numpy() - want) <= tol).all()
