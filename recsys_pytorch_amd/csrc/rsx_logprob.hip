@@ -581,7 +581,7 @@ __device__ __forceinline__ float group_sum(float v)
 // 300 x 50K x 256: 144 us with 256, 130 with 512, 154 with 1024; 943 x 1682 x 64: 46 with 256, 60 with 512)
 template <int D, bool F32, int NT>
 __global__ __launch_bounds__(NT, (NT >= 512 ? 4 : F32 ? 5 : 6)) void finish_kernel(const void *__restrict__ P, const void *__restrict__ Q, Shape sh, const uint32_t *__restrict__ bits,
-                                                    const float4 *__restrict__ part, int splits, const uint16_t *__restrict__ keys,
+                                                    const float4 *__restrict__ part, int splits, double skew, const uint16_t *__restrict__ keys,
                                                     const float *__restrict__ row_ref, const int32_t *__restrict__ given, int T, int K, float *__restrict__ logp,
                                                     float *__restrict__ lse_out, float *__restrict__ ent_out, int32_t *__restrict__ top_idx, float *__restrict__ top_logp)
 {
@@ -661,7 +661,9 @@ __global__ __launch_bounds__(NT, (NT >= 512 ? 4 : F32 ? 5 : 6)) void finish_kern
 #pragma unroll
     for (int w = 0; w < NW; ++w) { sum += s_red[1][w]; ent += s_red[2][w]; }
     const double l2 = log2(sum);
-    const double lse = sum == 0.0 ? -INFINITY : kLn2 * (m + l2);
+    // the pass multiplied by a factor that is off by `skew` of itself: to first order (skew^2 is 2^-46) the normaliser is off by that of the mean score
+    const double mean = m + ent / sum, late = mean - mean == 0.0 ? skew * mean : 0.0;
+    const double lse = sum == 0.0 ? -INFINITY : kLn2 * (m + l2 - late);
     if (tid == 0) {
         if (lse_out) lse_out[r] = (float)lse;
         if (ent_out) ent_out[r] = sum == 0.0 ? 0.0f : (float)(kLn2 * (l2 - ent / sum));
@@ -1021,6 +1023,7 @@ void run(const Call &c, const Ws &w, hipStream_t st)
 {
     const bool thin = c.sh.rows <= thin_rows(D, F32 ? RSX_F32 : RSX_BF16);
     const int64_t items = c.sh.items;
+    const double off_by = (double)(c.sh.scale * kLog2e) / (c.sh.scale * 1.4426950408889634074) - 1.0;      // of the fp32 factor scale log2 e
     for (int64_t r0 = 0; r0 < c.sh.rows; r0 += w.pass) {
         Shape sh = c.sh;
         sh.user_ids += r0;
@@ -1030,6 +1033,7 @@ void run(const Call &c, const Ws &w, hipStream_t st)
             hipLaunchKernelGGL((prepare_kernel<D, F32>), dim3((unsigned)(tiles + bit_rows + refs)), dim3(256), 0, st, c.P, c.Q, sh, c.indptr, c.indices, tiles, bit_rows,
                                (uint4 *)w.planes, w.factor, w.row_factor, w.bits, w.ref);
         int parts;
+        double skew;
         if (thin) {
             parts = thin_groups(items);
             constexpr int MOST = F32 ? 256 / D : 512 / D;
@@ -1038,7 +1042,9 @@ void run(const Call &c, const Ws &w, hipStream_t st)
                 if (sh.rows <= 32) launch_thin<D, F32, 2>(c, sh, w, parts, st);
                 else if constexpr (MOST >= 4) launch_thin<D, F32, 4>(c, sh, w, parts, st);
             }
+            skew = off_by;
         } else {
+            skew = F32 ? 0.0 : off_by;          // (fp32: scale log2 e is in the operands)
             parts = (int)wide_splits(sh.rows, items, F32 ? RSX_F32 : RSX_BF16);
             const dim3 grid((unsigned)parts, (unsigned)((sh.rows + WideGeo<D, F32>::WGU - 1) / WideGeo<D, F32>::WGU));
 #define RSX_LP_WIDE(M_, T_) hipLaunchKernelGGL((wide_kernel<D, F32, M_, T_>), grid, dim3(256), 0, st, c.P, F32 ? w.planes : (const char *)c.Q, w.factor, w.row_factor, sh, w.bits, w.ref, parts, w.part, (uint4 *)w.keys)
@@ -1047,7 +1053,7 @@ void run(const Call &c, const Ws &w, hipStream_t st)
 #undef RSX_LP_WIDE
         }
 #define RSX_LP_FINISH(NT_) hipLaunchKernelGGL((finish_kernel<D, F32, NT_>), dim3((unsigned)sh.rows), dim3(NT_), 0, st, c.P, c.Q, sh, c.indptr ? w.bits : (const uint32_t *)nullptr, \
-                                              w.part, parts, w.keys, w.ref, c.given + (c.T ? r0 * c.T : 0), c.T, c.K, c.logp + (c.T ? r0 * c.T : 0), \
+                                              w.part, parts, skew, w.keys, w.ref, c.given + (c.T ? r0 * c.T : 0), c.T, c.K, c.logp + (c.T ? r0 * c.T : 0), \
                                               c.lse ? c.lse + r0 : nullptr, c.ent ? c.ent + r0 : nullptr, c.top_idx + (c.K ? r0 * c.K : 0), c.top_logp + (c.K ? r0 * c.K : 0))
         if (sh.rows <= rsx_num_cus()) RSX_LP_FINISH(1024); else if (sh.rows <= 2 * rsx_num_cus()) RSX_LP_FINISH(512); else RSX_LP_FINISH(256);
 #undef RSX_LP_FINISH

@@ -92,3 +92,28 @@ def test_hip_logprobs_of_tables_of_opposite_size(n, power):
     for up in (2.0 ** power, 2.0 ** -power):
         P, Q = tables(rng, n, 300, 64, False)
         check(P * up, Q / up, np.arange(n), rng.integers(0, 300, (n, 2)), 10, None)
+
+
+# ---- the normaliser's last bits --------------------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("n", [2, 200])
+def test_hip_normaliser_of_one_item_is_its_score(n, bf16):
+    """one item: lse = z, exact products.  2^(t - m) is 2^r with r what the reference's rounding left (the fused multiply-add is exact to 2^-24 of
+    it): 2^-22 for exponential and logarithm, half a step of the result below 16 (2^-24 16): together 7.2e-7 on scores up to 16.  Many fp32 rows: the operand is x scale log2 e as two halves (2^-24 of it), two products are
+    added up in fp32 (2^-24 of the score each): 3 2^-24 16 = 2.9e-6 more"""
+    import torch
+    from recsys_pytorch_amd import rsx
+    two = np.log2(np.e)
+    scales = np.arange(1, 4000, dtype=np.float32) / np.float32(2500)
+    scale = float(scales[np.argmax(np.abs((scales * np.float32(two)).astype(np.float64) / (scales.astype(np.float64) * two) - 1))])       # rounds worst
+    x = np.arange(1, 1 + n) % 128 + 128.0                          # eight bits
+    y = np.float32(15.9 / 255 / scale)
+    y = float(torch.tensor(y).bfloat16())
+    P, Q = torch.zeros(n, 32), torch.zeros(1, 32)
+    P[:, 3], Q[:, 3] = torch.from_numpy(x.astype(np.float32)), y
+    P, Q = (P.bfloat16().cuda(), Q.bfloat16().cuda()) if bf16 else (P.cuda(), Q.cuda())
+    got = rsx.score_logprobs(P, Q, torch.arange(n, dtype=torch.int32, device="cuda"), scale=scale)
+    want = x * y * float(np.float32(scale))
+    assert want.max() < 16.0
+    assert np.abs(got.lse.double().cpu().numpy() - want).max() <= 7.2e-7 + (2.9e-6 if n > 64 and not bf16 else 0.0)
