@@ -41,17 +41,23 @@ struct Shape {
     float scale;
 };
 
-// running sums of one row, in units of log2
-struct Stat {
-    float m, sum, ent;
+// running sums of one row, in units of log2: in fp32 over a tile or a group of tiles, in 64 bits over those (equal terms round the same way: a
+// few hundred groups in fp32 were off by 3e-6)
+template <typename T>
+struct StatOf {
+    float m;
+    T sum, ent;
 };
+typedef StatOf<float> Stat;
+typedef StatOf<double> LongStat;
 
-__device__ __forceinline__ void stat_lift(Stat &s, float top)      // new reference max(m, top)
+template <typename T>
+__device__ __forceinline__ void stat_lift(StatOf<T> &s, float top)      // new reference max(m, top)
 {
     const float m = fmaxf(s.m, top);
     const float r = __builtin_amdgcn_exp2f(s.m - m);
-    s.ent = s.sum > 0.0f ? r * fmaf(s.sum, s.m - m, s.ent) : s.ent;      // (0 * inf for a row that has met nothing: skipped.  NaN sums: kept)
-    s.sum = s.sum * r;
+    s.ent = s.sum > 0 ? (T)r * fma(s.sum, (T)(s.m - m), s.ent) : s.ent;      // (0 * inf for a row that has met nothing: skipped.  NaN sums: kept)
+    s.sum = s.sum * (T)r;
     s.m = m;
 }
 
@@ -137,7 +143,8 @@ struct WideLds {
     __attribute__((aligned(1024))) char tile[2][G::ST * G::TILEB];
     char bits[MASK ? 2 : 1][MASK ? 4 : 1][G::UB][512];        // a group's seen bits, 16 bytes a row of the wavefront's
     uint32_t key[G::UB][TOP ? 4 : 1][256];                    // a group's chunk maxima, this lane's own slots
-    float all[G::UB][3][256];                                 // sums of all groups before this one, this lane's own slots
+    float top[G::UB][256];                                    // reference and sums of all groups before this one, this lane's own slots
+    double sum[G::UB][256], ent[G::UB][256];
 };
 
 // the products' 16 scores of one row (register i: item (i & 3) + 8 (i >> 2) + 4 hi of the tile) into the group's sums.  SOME: bits of w mask some.
@@ -156,7 +163,7 @@ __device__ __forceinline__ void absorb(const f32x16 &acc, float f, uint32_t w, S
     if (__builtin_amdgcn_ballot_w64(top > st.m + kLazy) != 0ull) {
         if (top > st.m) stat_lift(st, top);
     }
-    float sum = 0.0f, ent = 0.0f;         // of the tile; then of the group, then of all: each sum adds up few terms
+    float sum = 0.0f, ent = 0.0f;         // of the tile; then of the group, then (in 64 bits) of all
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
         float t = fmaf(x[i], f, -st.m);
@@ -216,8 +223,8 @@ __device__ __forceinline__ void wide_body(const void *__restrict__ P, const char
         rowf[ub] = !ok ? 0.0f : F32 ? down : sh.scale * kLog2e;      // (fp32: scale log2 e is in the operands, the factor a power of two)
         ref[ub] = TOP && ok ? row_ref[r < sh.rows ? r : sh.rows - 1] : 0.0f;
         st[ub] = {kNone, 0.0f, 0.0f};
-        lds.all[ub][0][tid] = kNone;
-        lds.all[ub][1][tid] = lds.all[ub][2][tid] = 0.0f;
+        lds.top[ub][tid] = kNone;
+        lds.sum[ub][tid] = lds.ent[ub][tid] = 0.0;
     }
 
     // copies of the next ST tiles: 1 KB a wavefront instruction, lane-linear in LDS, the swizzle in the source address.  (Nothing in the loop loads into
@@ -321,11 +328,11 @@ __device__ __forceinline__ void wide_body(const void *__restrict__ P, const char
         }
 #pragma unroll
         for (int ub = 0; ub < UB; ++ub) {
-            Stat all = {lds.all[ub][0][tid], lds.all[ub][1][tid], lds.all[ub][2][tid]};
-            stat_lift(all, st[ub].m);
-            lds.all[ub][0][tid] = all.m;
-            lds.all[ub][1][tid] = all.sum + st[ub].sum;
-            lds.all[ub][2][tid] = all.ent + st[ub].ent;
+            LongStat all = {lds.top[ub][tid], lds.sum[ub][tid], lds.ent[ub][tid]};
+            if (__builtin_amdgcn_ballot_w64(st[ub].m > all.m) != 0ull) stat_lift(all, st[ub].m);
+            lds.top[ub][tid] = all.m;
+            lds.sum[ub][tid] = all.sum + (double)st[ub].sum;
+            lds.ent[ub][tid] = all.ent + (double)st[ub].ent;
             st[ub].sum = st[ub].ent = 0.0f;
         }
     }
@@ -335,12 +342,12 @@ __device__ __forceinline__ void wide_body(const void *__restrict__ P, const char
         const int64_t r = row0 + 32 * ub + l31;
         if (TOP && g1 > g0 && r < sh.rows)
             keys[(size_t)r * (2 * groups) + 2 * (g1 - 1) + hi] = make_uint4(lds.key[ub][0][tid], lds.key[ub][1 % (TOP ? 4 : 1)][tid], lds.key[ub][2 % (TOP ? 4 : 1)][tid], lds.key[ub][3 % (TOP ? 4 : 1)][tid]);
-        Stat all = {lds.all[ub][0][tid], lds.all[ub][1][tid], lds.all[ub][2][tid]};
-        Stat o = {__shfl_xor(all.m, 32, 64), __shfl_xor(all.sum, 32, 64), __shfl_xor(all.ent, 32, 64)};
+        LongStat all = {lds.top[ub][tid], lds.sum[ub][tid], lds.ent[ub][tid]};
+        LongStat o = {__shfl_xor(all.m, 32, 64), __shfl_xor(all.sum, 32, 64), __shfl_xor(all.ent, 32, 64)};
         const float m = fmaxf(all.m, o.m);
         stat_lift(all, m);
         stat_lift(o, m);
-        if (hi == 0 && r < sh.rows) part[(size_t)r * splits + blockIdx.x] = make_float4(m, all.sum + o.sum, all.ent + o.ent, 0.0f);
+        if (hi == 0 && r < sh.rows) part[(size_t)r * splits + blockIdx.x] = make_float4(m, (float)(all.sum + o.sum), (float)(all.ent + o.ent), 0.0f);
     }
 }
 
@@ -369,7 +376,7 @@ __global__ __launch_bounds__(256) void thin_kernel(const void *__restrict__ P, c
     auto load = [&](const void *t, int64_t row, int n) { return *reinterpret_cast<const u32x4 *>((const char *)t + (size_t)row * (D * (F32 ? 4 : 2)) + n * 64 + g * 16); };
     u32x4 b[UB][NL];
     float rowf[UB], ref[UB];
-    Stat st[UB];
+    LongStat st[UB];
 #pragma unroll
     for (int ub = 0; ub < UB; ++ub) {
         const int64_t r = 16 * ub + l15;
@@ -455,8 +462,8 @@ __global__ __launch_bounds__(256) void thin_kernel(const void *__restrict__ P, c
                 sum += e;
                 ent = fmaf(e, t, ent);
             }
-            st[ub].sum += sum;
-            st[ub].ent += ent;
+            st[ub].sum += (double)sum;
+            st[ub].ent += (double)ent;
         }
     }
     // four lanes and four wavefronts hold a row
@@ -464,14 +471,14 @@ __global__ __launch_bounds__(256) void thin_kernel(const void *__restrict__ P, c
     for (int ub = 0; ub < UB; ++ub) {
 #pragma unroll
         for (int o = 16; o <= 32; o <<= 1) {
-            Stat q = {__shfl_xor(st[ub].m, o, 64), __shfl_xor(st[ub].sum, o, 64), __shfl_xor(st[ub].ent, o, 64)};
+            LongStat q = {__shfl_xor(st[ub].m, o, 64), __shfl_xor(st[ub].sum, o, 64), __shfl_xor(st[ub].ent, o, 64)};
             const float m = fmaxf(st[ub].m, q.m);
             stat_lift(st[ub], m);
             stat_lift(q, m);
             st[ub].sum += q.sum;
             st[ub].ent += q.ent;
         }
-        if (g == 0) s_part[wid][16 * ub + l15] = make_float4(st[ub].m, st[ub].sum, st[ub].ent, 0.f);
+        if (g == 0) s_part[wid][16 * ub + l15] = make_float4(st[ub].m, (float)st[ub].sum, (float)st[ub].ent, 0.f);
     }
     __syncthreads();
     if (tid < 16 * UB && tid < sh.rows) {

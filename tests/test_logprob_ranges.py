@@ -117,3 +117,41 @@ def test_hip_normaliser_of_one_item_is_its_score(n, bf16):
     want = x * y * float(np.float32(scale))
     assert want.max() < 16.0
     assert np.abs(got.lse.double().cpu().numpy() - want).max() <= 7.2e-7 + (2.9e-6 if n > 64 and not bf16 else 0.0)
+
+
+def _sum_in_fp32(e, groups):
+    """a lane's sum of 64 equal terms a group, groups added one to the next, all in fp32; relative to the exact one"""
+    e = np.float32(e)
+    tile = np.float32(0)
+    for _ in range(16):
+        tile = np.float32(tile + e)
+    group = np.float32(0)
+    for _ in range(4):
+        group = np.float32(group + tile)
+    total = np.float32(0)
+    for _ in range(groups):
+        total = np.float32(total + group)
+    return float(total) / (64.0 * groups * float(e)) - 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bf16", [False, True])
+def test_hip_normaliser_of_a_long_sum_of_equal_terms(bf16):
+    """30 000 equal scores under one that is larger, in one piece of the catalog: the groups' sums must not pile up fp32 roundings (equal terms round
+    the same way).  Exponential 2^-22, 20 additions of a group 20 2^-24, half a step of a result below 16: 1.9e-6"""
+    import torch
+    from recsys_pytorch_amd import rsx
+    n, I = 70_000, 30_000
+    steps = np.arange(1, 128) / 128.0
+    off = [abs(_sum_in_fp32(np.exp2(np.float32(np.log2(np.e)) * -s), I // 128)) for s in steps]
+    gap = float(steps[int(np.argmax(off))])
+    assert max(off) > 3e-6
+    P, Q = torch.zeros(n, 32), torch.zeros(I, 32)
+    P[:, 0], Q[:, 0], Q[7, 0] = 1.0, -gap, 0.0
+    P, Q = (P.bfloat16().cuda(), Q.bfloat16().cuda()) if bf16 else (P.cuda(), Q.cuda())
+    got = rsx.score_logprobs(P, Q, torch.arange(n, dtype=torch.int32, device="cuda"))
+    p = (I - 1) * np.exp(-gap)
+    want = np.log1p(p)
+    assert np.abs(got.lse.double().cpu().numpy() - want).max() <= 1.9e-6
+    # H = lse - E z, E z = -gap p / (1 + p): twice the terms' roundings, and half a step of the result
+    assert np.abs(got.entropy.double().cpu().numpy() - (want + gap * p / (1 + p))).max() <= 4e-6
