@@ -1090,7 +1090,8 @@ def _mask_ptrs(mask):
     if mask is None:
         return None, None
     indptr, indices = mask
-    return _dev(indptr, torch.int64, "mask indptr"), _dev(indices, torch.int32, "mask indices")
+    ptrs = _dev(indptr, torch.int64, "mask indptr"), _dev(indices, torch.int32, "mask indices")
+    return ptrs if indices.numel() > 0 else (None, None)       # (a tensor without elements has no address; it masks nothing)
 
 
 def score(P, Q, user_ids, mask=None, out=None):

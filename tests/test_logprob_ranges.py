@@ -155,3 +155,31 @@ def test_hip_normaliser_of_a_long_sum_of_equal_terms(bf16):
     assert np.abs(got.lse.double().cpu().numpy() - want).max() <= 1.9e-6
     # H = lse - E z, E z = -gap p / (1 + p): twice the terms' roundings, and half a step of the result
     assert np.abs(got.entropy.double().cpu().numpy() - (want + gap * p / (1 + p))).max() <= 4e-6
+
+
+# ---- a mask of nothing -----------------------------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [3, 140])
+def test_hip_a_mask_without_entries_masks_nothing(n):
+    import scipy.sparse as sp
+    import torch
+    import recsys_pytorch_amd as pkg
+    from recsys_pytorch_amd import rsx
+    rng = np.random.default_rng(n)
+    P, Q = tables(rng, n, 300, 64, False)
+    dev = lambda a, t=np.int32: torch.from_numpy(np.ascontiguousarray(a, t)).cuda()
+    u, it = dev(np.arange(n)), dev(rng.integers(0, 300, (n, 2)))
+    empty = torch.zeros(n + 1, dtype=torch.int64, device="cuda"), torch.zeros(0, dtype=torch.int32, device="cuda")
+    want, got = rsx.score_logprobs(P, Q, u, it, K=7), rsx.score_logprobs(P, Q, u, it, K=7, mask=empty)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    g = dev(rng.standard_normal((n, 2)), np.float32)
+    for a, b in zip(rsx.score_logprobs_grad(P, Q, u, it, want.lse, g), rsx.score_logprobs_grad(P, Q, u, it, want.lse, g, mask=empty)):
+        assert torch.equal(a, b)
+    assert torch.equal(rsx.score(P, Q, u), rsx.score(P, Q, u, mask=empty)) and torch.equal(rsx.score_topk(P, Q, u, 7), rsx.score_topk(P, Q, u, 7, mask=empty))
+    with pytest.raises(rsx.RsxError, match="indptr"):                # (its shape is still looked at)
+        rsx.score_logprobs(P, Q, u, it, mask=(empty[0][:-1], empty[1]))
+    ds = pkg.InteractionData(sp.random(n, 300, 0.1, random_state=1, data_rvs=np.ones).tocsr())
+    m = pkg.MF(ds, {"hidden_dim": 64, "pointwise": False, "loss_func": "ce", "optimizer": "sgd"}, "cuda")
+    nothing = sp.csr_matrix((n, 300))
+    for a, b in zip(m.predict_logprobs(np.arange(n), np.arange(n), K=5), m.predict_logprobs(np.arange(n), np.arange(n), eval_pos=nothing, K=5)):
+        assert np.array_equal(a, b)
