@@ -484,7 +484,7 @@ struct Proj {
 };
 
 template <int D, typename T, bool MUON>
-__global__ __launch_bounds__(Proj<D>::NT) void project_kernel(Rows<T, MUON> in, T *__restrict__ out, float *__restrict__ W, int64_t rows,
+__global__ __launch_bounds__(Proj<D>::NT) void project_kernel(Rows<T, MUON> in, T *out, float *__restrict__ W, int64_t rows,      // (out may be in.X)
                                                               const float *__restrict__ Mt, float keep, float step)
 {
     using C = Proj<D>;
