@@ -214,7 +214,7 @@ int rsx_adam_apply(float *W, float *M, float *V, float *G, int64_t n, double lr,
  *   M = momentum M + G;  U = nesterov ? G + momentum M : M;
  *   W = (1 - lr weight_decay) W - lr update_scale orthogonalize(U);   G = 0
  *   W, M fp32; G of g_dtype.  update_scale is the caller's, sqrt(max(1, rows / width)) by custom.
- * ws: rsx_orthogonalize_workspace(rows, d) bytes of scratch, contents irrelevant, one per concurrent call.  Rows 16-byte aligned.
+ * ws: rsx_orthogonalize_workspace(rows, d) bytes of scratch, contents irrelevant, one per concurrent call.  Rows and ws 16-byte aligned.
  * No host synchronisation: the calls can be captured into a graph.                                                              */
 int64_t rsx_orthogonalize_workspace(int64_t rows, int d);
 int rsx_orthogonalize(const void *X, void *out, int64_t rows, int d, int dtype, int steps, double a, double b, double c,

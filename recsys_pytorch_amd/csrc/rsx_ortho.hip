@@ -711,8 +711,8 @@ RSX_API int rsx_orthogonalize(const void *X, void *out, int64_t rows, int d, int
     RSX_CHECK_ARG(aligned16(X) && aligned16(out), "rows must be 16-byte aligned");
     if (rows == 0) return RSX_OK;
     const OrthoWs w = ortho_carve(ws, rows, d, false);
-    if (ws == nullptr || ws_bytes < w.bytes || (reinterpret_cast<uintptr_t>(ws) & 7)) {
-        rsx_set_error("rsx_orthogonalize: workspace of %lld bytes (8-byte aligned) required, got %lld", (long long)w.bytes, (long long)ws_bytes);
+    if (ws == nullptr || ws_bytes < w.bytes || !aligned16(ws)) {
+        rsx_set_error("rsx_orthogonalize: workspace of %lld bytes (16-byte aligned) required, got %lld", (long long)w.bytes, (long long)ws_bytes);
         return RSX_E_WORKSPACE;
     }
     const Coeffs k{a, b, c, eps};
@@ -738,8 +738,8 @@ RSX_API int rsx_muon_apply(float *W, float *M, void *G, int64_t rows, int d, int
     RSX_CHECK_ARG(aligned16(W) && aligned16(M) && aligned16(G), "rows must be 16-byte aligned");
     if (rows == 0) return RSX_OK;
     const OrthoWs w = ortho_carve(ws, rows, d, true);
-    if (ws == nullptr || ws_bytes < w.bytes || (reinterpret_cast<uintptr_t>(ws) & 7)) {
-        rsx_set_error("rsx_muon_apply: workspace of %lld bytes (8-byte aligned) required, got %lld", (long long)w.bytes, (long long)ws_bytes);
+    if (ws == nullptr || ws_bytes < w.bytes || !aligned16(ws)) {
+        rsx_set_error("rsx_muon_apply: workspace of %lld bytes (16-byte aligned) required, got %lld", (long long)w.bytes, (long long)ws_bytes);
         return RSX_E_WORKSPACE;
     }
     const Coeffs k{a, b, c, eps};

@@ -71,6 +71,16 @@ def test_refusals():
     assert muon() == -3 and muon(rows=0) == 0
 
 
+def test_a_workspace_between_16_byte_lines_is_refused():
+    """the kernels read it 16 bytes at a time"""
+    from recsys_pytorch_amd import build, rsx
+    build.build()
+    L = rsx.lib()
+    for ws in (8, 4104):
+        assert L.rsx_orthogonalize(16, 16, 4, 32, 0, 5, 1.0, 0.0, 0.0, 0.0, ws, 1 << 30, None) == -3 and b"16-byte" in L.rsx_last_error()
+        assert L.rsx_muon_apply(16, 32, 48, 4, 32, 0, 0.1, 0.9, 1, 5, 1.0, 0.0, 0.0, 0.0, 0.0, 1.0, ws, 1 << 30, None) == -3 and b"16-byte" in L.rsx_last_error()
+
+
 def test_the_polynomial_is_the_iteration():
     """the bound's M against the iteration itself, and the Gram-space form against it (64 bits, CPU)"""
     rng = np.random.default_rng(0)
