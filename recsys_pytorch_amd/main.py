@@ -38,6 +38,8 @@ def main(argv=None):
     ap.add_argument("--seed", type=int, default=2020)               # config.py:46
     ap.add_argument("--test-step", type=int, default=1)
     args = ap.parse_args(argv)
+    if args.model != "MF" and (args.listwise or args.optimizer == "muon"):
+        ap.error(f"{args.model} has neither --listwise nor --optimizer muon")
 
     np.random.seed(args.seed)
     torch.manual_seed(args.seed)

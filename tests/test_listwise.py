@@ -159,6 +159,14 @@ def test_predict_logprobs_on_plain_kernels():
     assert m.predict_logprobs([], np.zeros((0, 3)), K=2).logp.shape == (0, 3)
 
 
+@pytest.mark.parametrize("argv", [["--listwise"], ["--optimizer", "muon"]])
+def test_command_line_refuses_what_a_model_lacks(argv, capsys):
+    from recsys_pytorch_amd import main
+    with pytest.raises(SystemExit) as stop:
+        main.main(["--data", "nowhere.npz", "--model", "LightGCN", *argv])
+    assert stop.value.code == 2 and "LightGCN" in capsys.readouterr().err
+
+
 # ---- on the GPU ------------------------------------------------------------------------------------------------------------------
 def _engine(U, I, d, optimizer="sgd", lr=0.5, seed=5):
     from recsys_pytorch_amd.sharded import BPREngine
