@@ -150,8 +150,9 @@ def logprobs_in_passes(model, P, Q, user_ids, items, eval_pos, K, test_batch_siz
             raise ValueError(f"items must be [{n}] or [{n} x T] ids")
     shape = None if items is None else items.shape
     mask = device_mask(model, eval_pos)
-    users_dev = model._idx(user_ids)
-    items_dev = None if items is None else model._idx(items.reshape(n, -1) if n else items.reshape(0, 1))
+    named = lambda ids, most: model._idx(np.where((ids >= 0) & (ids < most), ids, -1))       # (before they are cut to 32 bits)
+    users_dev = named(user_ids, P.shape[0])
+    items_dev = None if items is None else named(items.reshape(n, -1) if n else items.reshape(0, 1), Q.shape[0])
     parts, step = [], max(1, int(test_batch_size))
     for s in range(0, max(n, 1), step):
         parts.append(model._k.score_logprobs(P, Q, users_dev[s:s + step], items_dev[s:s + step] if items_dev is not None else None, K=K, mask=mask))

@@ -159,6 +159,18 @@ def test_predict_logprobs_on_plain_kernels():
     assert m.predict_logprobs([], np.zeros((0, 3)), K=2).logp.shape == (0, 3)
 
 
+def test_predict_logprobs_of_ids_beyond_32_bits():
+    """an id that names nothing names nothing, whatever its lower half is"""
+    import recsys_pytorch_amd as pkg
+    mat = _matrix()
+    m = pkg.MF(_dataset(mat), dict(HP, optimizer="sgd"), "cpu", kernels=_plain_kernels())
+    far = 2 ** 32
+    r = m.predict_logprobs([5, far + 5, -far], np.array([[1, far + 1], [1, 2], [3, 4]]), K=3)
+    want = m.predict_logprobs([5, -1, -1], np.array([[1, -1], [1, 2], [3, 4]]), K=3)
+    assert all(np.array_equal(a, b) for a, b in zip(r, want))
+    assert r.logp[0, 1] == 0.0 and r.lse[1] == -np.inf and (r.top_idx[1:] == -1).all()
+
+
 @pytest.mark.parametrize("argv", [["--listwise"], ["--optimizer", "muon"]])
 def test_command_line_refuses_what_a_model_lacks(argv, capsys):
     from recsys_pytorch_amd import main
