@@ -154,7 +154,6 @@ class BPREngine:
         self.GP = None              # dense user-gradient buffer: Adam, and the pointwise branch (allocated on first use)
         self._pw_t = 0              # Adam's step count on the pointwise branch
         self._lw_t = 0              # and on the listwise one
-        self._lw = None             # scratch of the listwise branch
         if optimizer == "adam":      # the reference's shipped optimizer (models/MF.py:30): dense moments
             self.GP = torch.zeros_like(P_local)
             self.mP, self.vP = torch.zeros_like(P_local), torch.zeros_like(P_local)
@@ -654,11 +653,9 @@ class BPREngine:
         loss.zero_()
         n = int(u.numel())
         if n > 0:
+            # (scratch of this call alone: one that was kept and grew would be taken from under a captured step that still writes to it)
             need = max(self.k.score_logprobs_workspace(n, *self.Q.shape), self.k.score_logprobs_grad_workspace(n, *self.Q.shape))
-            if self._lw is None or self._lw["ws"].numel() < need or self._lw["rows"].shape[0] < n:
-                self._lw = None
-                self._lw = {"ws": torch.empty(need, dtype=torch.uint8, device=self.Q.device), "rows": torch.empty(n, self.P.shape[1], device=self.P.device)}
-            ws, rows, i = self._lw["ws"], self._lw["rows"][:n], i.view(n, 1)
+            ws, rows, i = torch.empty(need, dtype=torch.uint8, device=self.Q.device), torch.empty(n, self.P.shape[1], device=self.P.device), i.view(n, 1)
             lp = self.k.score_logprobs(self.P, self.Q, u, i, ws=ws)
             loss[0] = -lp.logp.sum()
             self.k.score_logprobs_grad(self.P, self.Q, u, i, lp.lse, torch.full_like(lp.logp, -1.0 / n), out=(rows, self.G), ws=ws)

@@ -344,3 +344,30 @@ def test_hip_calls_at_once_on_two_streams():
     for k in range(2):
         for run in got[k]:
             assert all(torch.equal(a, b) for a, b in zip(run, want[k]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("optimizer", ["sgd", "muon"])
+def test_hip_captured_listwise_step_outlives_larger_eager_ones(optimizer):
+    """a step of 60 pairs replayed from its graph after an eager step of 700 and other work in the memory between: the same bits as eager steps"""
+    rng = np.random.default_rng(4)
+    dev = lambda n, top: torch.from_numpy(rng.integers(0, top, n).astype(np.int32)).cuda()
+    (eng, *_), (twin, *_) = _engine(200, 900, 64, optimizer), _engine(200, 900, 64, optimizer)
+    u, i, many_u, many_i = dev(60, 200), dev(60, 900), dev(700, 200), dev(700, 900)
+    for e in (eng, twin):
+        e.listwise_step(u, i)
+    torch.cuda.synchronize()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+        eng.listwise_step(u, i)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for e in (eng, twin):
+            e.listwise_step(many_u, many_i)
+        others = [torch.full((1 << 18,), 7.0, device="cuda") for _ in range(40)]
+        torch.cuda.synchronize()
+        graph.replay()
+        twin.listwise_step(u, i)
+        torch.cuda.synchronize()
+        assert torch.equal(eng.P, twin.P) and torch.equal(eng.Q, twin.Q) and all(bool((o == 7.0).all()) for o in others)
