@@ -111,15 +111,15 @@ __global__ __launch_bounds__(256) void rows_kernel(Args a, const uint32_t *__res
         e_row = (int)exponent_of_factor(down);
         if (a.h != nullptr) e_w = exponent_of((float)w);
         // dz = p (A + B log2 p), p = 2^(z - lse2).  Without the entropy's part |dz| = 2^(z + off), off = log2 |A| - lse2 in whole 2^-15, to which whole exponents
-        // add exactly; what is left (`fix`) goes where the sign goes.  With it, by t = z + off, off the rounded e - lse2: what the rounding (half a
+        // add exactly; what is left (`fix`) goes where the sign goes (bf16 rows stay as they are: rounded to fp32 is enough there).  With it, by t = z + off, off the rounded e - lse2: what the rounding (half a
         // step at 24 is 1e-6 of every p) and e change goes into the coefficients
         const double lse2 = (double)lse * 1.4426950408889634074;
         const double H = a.h != nullptr ? (double)h * a.ent[r < a.rows ? r : 0] : 0.0;
         const double A = live ? ldexp(-(sum + H), -e_w) : 0.0, B = live ? ldexp(-(double)h * kLn2, -e_w) : 0.0;
         const bool none = !live || (a.h == nullptr && sum == 0.0);
         const double exact = log2(fabs(sum)) - lse2;
-        const float near = (float)(rint(exact * 32768.0) * 0x1p-15);
-        const double fix = a.h == nullptr && !none ? exp2(exact - (double)near) : 1.0;
+        const float near = (float)(F32 ? rint(exact * 32768.0) * 0x1p-15 : exact);
+        const double fix = F32 && a.h == nullptr && !none ? exp2(exact - (double)near) : 1.0;
         auto params = [&](int e, float *off, float *pa, float *pb) {
             *off = none ? -kFar : near + (float)e;
             *pa = *pb = 0.0f;
