@@ -258,6 +258,7 @@ int rsx_pair_score(const float *P, const float *Q, const int32_t *u_dev, const i
  *   their own (equal pointers to a table's are refused),
  *   dz_ri  = scale (sum_t g_logp[r, t] ([i = items[r, t]] - p_ri) - g_entropy[r] p_ri (log p_ri + H_r))
  *   over unmasked i and the items that are neither masked nor outside the catalog (a masked item's logp is the constant -inf).
+ *   dz is held to 2^-22 of itself (bf16 tables: 2^-11), down to 2^-32 of the largest term of the row's own sum; sums in fp32.
  *   An item listed twice counts twice.  lse, entropy: what rsx_score_logprobs returned for the same arguments (entropy and
  *   g_entropy nullable together).  GP is per POSITION: add the rows of a user that stands in the batch more than once
  *   (rsx_add_rows).  A position that names no row has a zero row.  Bit-reproducible (no floating atomics).

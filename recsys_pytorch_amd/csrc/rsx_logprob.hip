@@ -19,7 +19,7 @@
 //                bf16: 256 MB in 42 us)
 //   wide_kernel  many rows: item tiles through LDS (asynchronous copies, two buffers), users' operands held in registers for the whole
 //                pass (up to 128 registers a lane), bound by the matrix cores (fp32: three f16 products, rsx_logprob.h) or, for bf16
-//                rows of 128, by the five vector instructions a score needs after its product (8192 x 100K: 0.37 ms, 0.16 of it
+//                rows of 128, by the five vector instructions a score needs after its product (8192 x 100K: 0.34 ms, 0.16 of it
 //                products; 1024 x 100K fp32: 94 us, 55 of it products)
 #include "rsx_logprob.h"
 
@@ -507,7 +507,8 @@ __global__ __launch_bounds__(256) void thin_kernel(const void *__restrict__ P, c
 }
 
 // ---- one workgroup per row: join the partials, the given items, the K best -------------------------------------------------------------
-constexpr int kMaxChunks = 256;                   // chunks whose items are computed again; more (ties by the thousand): the whole row is
+constexpr int kMaxChunks = 256;                   // chunks whose items are computed again; more (a row of zeros, ties by the thousand): the whole row is, by its one
+                                                  // workgroup (100K x 128: 1.5 ms, ten times what 1024 rows without such a one take)
 constexpr int kCand = 8 * kMaxChunks;
 constexpr int kListed = 4096;                     // chunks looked at more closely for that choice
 static_assert(kListed * 4 <= kCand * 8 && kListed * 2 <= kCand * 4, "the list of chunks lies in the candidates' memory");

@@ -81,7 +81,7 @@ __host__ __device__ constexpr int block_at(int D, int p, int q) { return p * n_g
 
 // Eight wavefronts; the 16 x 16 blocks of the upper triangle are dealt to SETS of them (8 registers a block: 72 at d = 128, 136 at d = 256, so that two
 // wavefronts share a SIMD), the rows of a tile to the 8 / SETS wavefronts of a set.  16 KB tiles pass through LDS; two tiles of G and M are on their way
-// in registers (64 KB a CU: what HBM's latency takes).  Bound by HBM with the momentum (1M x 128: 1.5 GB in 0.37 ms), by the fp64 matrix
+// in registers (64 KB a CU: what HBM's latency takes).  Bound by HBM with the momentum (1M x 128: 1.5 GB in 0.39 ms), by the fp64 matrix
 // rate without (36 instructions of 64 cycles per four rows: 0.27 ms).
 // d = 256 without the momentum (whose update one workgroup has to make): four workgroups share a row range and its blocks, two sets each, so that there
 // are a quarter of the partials (20011 rows: 37 us and 5 to add them up; 256 workgroups with all 136 blocks each: 35 and 15).
@@ -477,7 +477,7 @@ __global__ __launch_bounds__(256) void ns_identity_kernel(const double *__restri
 // v_mfma_f32_32x32x2_f32, exact fp32 products.  A wavefront owns 32 output columns and keeps its 32 columns of the [d x d] matrix in registers
 // (d / 2 of them) for all its rows; rows pass through LDS, and so does the result, so that every access to memory is 16 bytes a lane.  The rows of the
 // next tile and the weights of this one are on their way during the products.  The contraction index is permuted so that a lane
-// reads its row four elements at a time: step 4 j + e multiplies k = 8 j + 4 (lane >> 5) + e.  Bound by HBM (optimizer step, 1M x 128: 2.6 GB in 0.48 ms).
+// reads its row four elements at a time: step 4 j + e multiplies k = 8 j + 4 (lane >> 5) + e.  Bound by HBM (optimizer step, 1M x 128: 2.6 GB in 0.47 ms).
 template <int D>
 struct Proj {
     static constexpr int WAVES = D == 256 ? 8 : 4, CG = D / 32, RG = WAVES / CG, TR = 32 * RG, LD = D + 4, NT = 64 * WAVES, NP = TR * D / 4 / NT;
