@@ -10,9 +10,9 @@
 // scores of ONE row (items are the matrix instruction's rows, users its columns): all of this is lane-local.
 //
 // Top-K: the pass also stores the largest score of every 8 items as a half (relative to a score of the same row, so that halves
-// resolve it; -inf only where all 8 are masked).  The K best items lie in chunks whose maximum is at least the K-th largest maximum; finish_kernel takes K + 8 chunks
-// and every tie, computes their items' products again in 64 bits and orders those.  What the fast products' rounding could swap is
-// decided by the 64-bit ones.
+// resolve it; -inf only where all 8 are masked).  The K best items lie in chunks whose maximum is at least the K-th largest maximum, less what halves and fast
+// products are off by; finish_kernel takes the chunks from there up, computes their items' products again in 64 bits and orders those.  What the fast
+// products' rounding could swap is decided by the 64-bit ones.
 //
 // Two forms of the pass:
 //   thin_kernel  few rows: the catalog is read once, straight into registers (v_mfma_f32_16x16x4_f32 / 16x16x32_bf16), bound by HBM (16 rows, 1M x 128
@@ -73,15 +73,16 @@ __device__ __forceinline__ float pick_reference(float a, float b, float c)
 __device__ __forceinline__ uint32_t key_bits(float a, float b) { return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b)); }
 
 // the reference a row's chunk maxima are stored against: a score of its own, so that an offset common to a row's scores does not eat the halves'
-// eleven bits.  One wavefront per row.
+// eleven bits; and how far apart two of its fast products may be off: twice 3 (d + 1) 2^-24 sum |x||y|, of the middle one of the same three items (a
+// bound that no roundings reach, with room for items a few times as long).  One wavefront per row.
 template <int D, bool F32>
-__device__ __forceinline__ void row_reference(const void *__restrict__ P, const void *__restrict__ Q, const Shape &sh, int64_t r, float *__restrict__ ref)
+__device__ __forceinline__ void row_reference(const void *__restrict__ P, const void *__restrict__ Q, const Shape &sh, int64_t r, float *__restrict__ ref, float *__restrict__ slack)
 {
     const int lane = threadIdx.x & 63;
     if (r >= sh.rows) return;
     const int32_t u = sh.user_ids[r];
     if (!row_ok(u, sh.users)) return;
-    float d[3] = {0.0f, 0.0f, 0.0f};
+    float d[3] = {0.0f, 0.0f, 0.0f}, size[3] = {0.0f, 0.0f, 0.0f};
     if (lane < D / 8) {
         float x[8], q[8];
         load8<F32>(P, (int64_t)u * D + 8 * lane, x);
@@ -89,14 +90,17 @@ __device__ __forceinline__ void row_reference(const void *__restrict__ P, const 
         for (int n = 0; n < 3; ++n) {
             load8<F32>(Q, (n == 0 ? 0 : n == 1 ? sh.items / 2 : sh.items - 1) * D + 8 * lane, q);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) d[n] = fmaf(x[j], q[j], d[n]);
+            for (int j = 0; j < 8; ++j) { d[n] = fmaf(x[j], q[j], d[n]); size[n] = fmaf(fabsf(x[j]), fabsf(q[j]), size[n]); }
         }
     }
 #pragma unroll
     for (int n = 0; n < 3; ++n)
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) d[n] += __shfl_xor(d[n], o, 64);
-    if (lane == 0) ref[r] = sh.scale * kLog2e * pick_reference(d[0], d[1], d[2]);
+        for (int o = 16; o > 0; o >>= 1) { d[n] += __shfl_xor(d[n], o, 64); size[n] += __shfl_xor(size[n], o, 64); }
+    if (lane == 0) {
+        ref[r] = sh.scale * kLog2e * pick_reference(d[0], d[1], d[2]);
+        slack[r] = sh.scale * kLog2e * (6 * (D + 1) * 0x1p-24f) * pick_reference(size[0], size[1], size[2]);
+    }
 }
 
 // what the pass needs, in one launch: workgroups [0, tiles) split the item tiles (fp32), the next bit_rows write a row's seen bits each, the rest
@@ -104,7 +108,7 @@ __device__ __forceinline__ void row_reference(const void *__restrict__ P, const 
 template <int D, bool F32>
 __global__ __launch_bounds__(256) void prepare_kernel(const void *__restrict__ P, const void *__restrict__ Q, Shape sh, const int64_t *__restrict__ indptr,
                                                       const int32_t *__restrict__ indices, int64_t tiles, int64_t bit_rows, uint4 *__restrict__ planes, float *__restrict__ factor,
-                                                      float *__restrict__ row_factor, uint32_t *__restrict__ bits, float *__restrict__ ref)
+                                                      float *__restrict__ row_factor, uint32_t *__restrict__ bits, float *__restrict__ ref, float *__restrict__ slack)
 {
     __shared__ __attribute__((aligned(16))) uint32_t lds[kBitWords];
     int64_t at = blockIdx.x;
@@ -118,7 +122,7 @@ __global__ __launch_bounds__(256) void prepare_kernel(const void *__restrict__ P
         write_seen_bits(u, row_ok(u, sh.users), indptr, indices, sh.items, bits + (size_t)at * mask_words(sh.items), lds);
         return;
     }
-    row_reference<D, F32>(P, Q, sh, (at - bit_rows) * 4 + (threadIdx.x >> 6), ref);
+    row_reference<D, F32>(P, Q, sh, (at - bit_rows) * 4 + (threadIdx.x >> 6), ref, slack);
 }
 
 // ---- many rows ------------------------------------------------------------------------------------------------------------------------
@@ -550,6 +554,9 @@ __device__ __forceinline__ float half_value(uint32_t order)
     return (float)__builtin_bit_cast(_Float16, h);
 }
 
+// a stored maximum less what it may be off by: a half's last place twice (the maximum's, and the bound's own) and the fast products
+__device__ __forceinline__ float surely_above(float h, float slack) { return h - (fabsf(h) * 0.003f + 0x1p-23f + slack); }
+
 // EPL elements of a table row as they lie in memory
 template <bool F32, int EPL>
 struct RowPiece {
@@ -590,7 +597,7 @@ __device__ __forceinline__ float group_sum(float v)
 template <int D, bool F32, int NT>
 __global__ __launch_bounds__(NT, (NT >= 512 ? 4 : F32 ? 5 : 6)) void finish_kernel(const void *__restrict__ P, const void *__restrict__ Q, Shape sh, const uint32_t *__restrict__ bits,
                                                     const float4 *__restrict__ part, int splits, double skew, const uint16_t *__restrict__ keys,
-                                                    const float *__restrict__ row_ref, const int32_t *__restrict__ given, int T, int K, float *__restrict__ logp,
+                                                    const float *__restrict__ row_ref, const float *__restrict__ row_slack, const int32_t *__restrict__ given, int T, int K, float *__restrict__ logp,
                                                     float *__restrict__ lse_out, float *__restrict__ ent_out, int32_t *__restrict__ top_idx, float *__restrict__ top_logp)
 {
     // elements of an item's row a lane takes, lanes a row, items a pass.  fp32: eight where the work of many rows is the time (fewer additions between lanes:
@@ -699,8 +706,8 @@ __global__ __launch_bounds__(NT, (NT >= 512 ? 4 : F32 ? 5 : 6)) void finish_kern
         for (int n = 0; n < FL; ++n) z[n] *= (double)sh.scale;
     };
 
-    // K + 8 chunks with the largest maxima and all that equal the last of them.  First a lower bound of that maximum: the K + 8-th largest of the
-    // threads' own (no fewer chunks can be above it); then the chunks from the bound up, and among them the ones with fewer than K + 8 above
+    // The chunks whose maximum may be among the K largest: those from a little below the K-th largest up.  First a lower bound of that maximum: the K-th largest of the
+    // threads' own (no fewer chunks can be above it); then the chunks from a little below the bound up, the K-th largest among them, and those from there up
     int n = 0;                                     // entries: T given items, then 8 for each chosen chunk
     float cut = -INFINITY;                         // a score that K items reach, by the stored maxima
     bool whole = false;                            // too many ties: every item of the row is computed
@@ -722,7 +729,13 @@ __global__ __launch_bounds__(NT, (NT >= 512 ? 4 : F32 ? 5 : 6)) void finish_kern
         }
         if (tid % (NT / 256) == 0) s_max[tid / (NT / 256)] = (uint16_t)best;
         __syncthreads();
-        if (wid == 0) {                            // the K + 8-th largest of 256, bit by bit, in one wavefront
+        const float slack = row_slack[r];
+        // a maximum's order -> that of the smallest one that may belong to a larger score (-inf, a chunk with nothing in it, never does)
+        auto from = [&](uint32_t order) {
+            const uint32_t low = half_order((_Float16)__builtin_bit_cast(half2v, key_bits(surely_above(half_value(order), slack), 0.0f))[0]);
+            return order <= lowest || low <= lowest ? lowest + 1 : low < order ? low : order;        // (NaN and infinities: themselves)
+        };
+        if (wid == 0) {                            // the K-th largest of 256, bit by bit, in one wavefront
             const uint2 v = reinterpret_cast<const uint2 *>(s_max)[lane];
             const uint32_t x[4] = {v.x & 0xFFFFu, v.x >> 16, v.y & 0xFFFFu, v.y >> 16};
             uint32_t t = 0;
@@ -731,9 +744,9 @@ __global__ __launch_bounds__(NT, (NT >= 512 ? 4 : F32 ? 5 : 6)) void finish_kern
                 int c = 0;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) c += __builtin_popcountll(__builtin_amdgcn_ballot_w64(x[j] >= u_));
-                if (c >= K + 8) t = u_;
+                if (c >= K) t = u_;
             }
-            if (lane == 0) s_tau = t > lowest ? t : lowest + 1;
+            if (lane == 0) s_tau = from(t);
         }
         __syncthreads();
         int32_t *const l_chunk = reinterpret_cast<int32_t *>(c_s);
@@ -774,13 +787,9 @@ __global__ __launch_bounds__(NT, (NT >= 512 ? 4 : F32 ? 5 : 6)) void finish_kern
 #pragma unroll
                     for (int j = 0; j < 4; ++j) over += ((w[j] & 0xFFFFu) > k) + ((w[j] >> 16) > k);
                 }
-                if (over < K + 8) {
-                    const int at = atomicAdd(&s_n, 1);
-                    if (at < kMaxChunks) s_list[at] = l_chunk[q];
-                    if (over < K) atomicMin(&s_tau, k);                  // the K-th largest maximum, from above
-                }
+                if (over < K) atomicMin(&s_tau, k);                      // the K-th largest maximum, from above
             }
-        } else if (listed <= kListed) {            // (the best items' chunks were few threads': the K + 8-th bit by bit)
+        } else if (listed <= kListed) {            // (the best items' chunks were few threads': the K-th bit by bit)
             uint32_t tau = 0;
             for (int bit = 15; bit >= 0; --bit) {
                 const uint32_t t = tau | (1u << bit);
@@ -790,25 +799,25 @@ __global__ __launch_bounds__(NT, (NT >= 512 ? 4 : F32 ? 5 : 6)) void finish_kern
                 for (int q = tid; q < listed; q += NT) c += l_key[q] >= t;
                 if (c) atomicAdd(&s_count, c);
                 __syncthreads();
-                if (s_count >= K + 8) tau = t;
+                if (s_count >= K) tau = t;
                 __syncthreads();
             }
+            if (tid == 0) s_tau = tau;
+        }
+        __syncthreads();
+        if (listed <= kListed) {
+            const uint32_t least = from(s_tau);
             for (int q = tid; q < listed; q += NT)
-                if (l_key[q] >= tau) {
+                if (l_key[q] >= least) {
                     const int at = atomicAdd(&s_n, 1);
                     if (at < kMaxChunks) s_list[at] = l_chunk[q];
                 }
-            if (tid == 0) s_tau = tau;
         }
         __syncthreads();
         whole = s_n > kMaxChunks;
         n = whole ? 0 : 8 * s_n;
-        // K items reach the K-th maximum; it is a half (rounded towards zero) of a fast product, and taken a little lower here.  (How much does not matter: if fewer
-        // than K scores certainly reach `cut`, nothing is left out.)
-        if (!whole && s_n >= K) {
-            const float h = half_value(s_tau), ref = row_ref[r];
-            cut = (ref + h - (fabsf(h) * 0.002f + fabsf(ref) * 1e-5f + 0.01f)) * (float)kLn2;
-        }
+        // K items reach the K-th maximum.  (How much lower the cut is taken does not matter: if fewer than K scores certainly reach it, nothing is left out.)
+        if (!whole && s_n >= K) cut = (row_ref[r] + surely_above(half_value(s_tau), slack)) * (float)kLn2;
         __syncthreads();
         if (tid == 0) s_n = s_count = 0;
         __syncthreads();
@@ -958,7 +967,7 @@ struct Ws {
     char *planes;
     float *factor, *row_factor;
     uint32_t *bits;
-    float *ref;
+    float *ref, *slack;
     float4 *part;
     uint16_t *keys;
     int64_t pass, bytes;      // rows of one pass over the catalog
@@ -999,6 +1008,7 @@ Ws carve(void *ws, int64_t rows, int64_t items, int d, int dtype, bool mask, int
     w.row_factor = (float *)take(!thin && dtype == RSX_F32 ? tiles4 * kTile * 4 : 0);
     w.bits = (uint32_t *)take(mask ? w.pass * mask_words(items) * 4 : 0);
     w.ref = (float *)take(w.pass * 4);
+    w.slack = (float *)take(w.pass * 4);
     w.part = (float4 *)take(cells * 16);
     w.keys = (uint16_t *)take(K > 0 ? w.pass * ((items + 127) / 128) * 32 : 0);
     w.bytes = off;
@@ -1039,7 +1049,7 @@ void run(const Call &c, const Ws &w, hipStream_t st)
         const int64_t tiles = F32 && !thin && r0 == 0 ? (items + 127) / 128 * 4 : 0, bit_rows = c.indptr ? sh.rows : 0, refs = c.K ? (sh.rows + 3) / 4 : 0;
         if (tiles + bit_rows + refs > 0)
             hipLaunchKernelGGL((prepare_kernel<D, F32>), dim3((unsigned)(tiles + bit_rows + refs)), dim3(256), 0, st, c.P, c.Q, sh, c.indptr, c.indices, tiles, bit_rows,
-                               (uint4 *)w.planes, w.factor, w.row_factor, w.bits, w.ref);
+                               (uint4 *)w.planes, w.factor, w.row_factor, w.bits, w.ref, w.slack);
         int parts;
         double skew;
         if (thin) {
@@ -1061,7 +1071,7 @@ void run(const Call &c, const Ws &w, hipStream_t st)
 #undef RSX_LP_WIDE
         }
 #define RSX_LP_FINISH(NT_) hipLaunchKernelGGL((finish_kernel<D, F32, NT_>), dim3((unsigned)sh.rows), dim3(NT_), 0, st, c.P, c.Q, sh, c.indptr ? w.bits : (const uint32_t *)nullptr, \
-                                              w.part, parts, skew, w.keys, w.ref, c.given + (c.T ? r0 * c.T : 0), c.T, c.K, c.logp + (c.T ? r0 * c.T : 0), \
+                                              w.part, parts, skew, w.keys, w.ref, w.slack, c.given + (c.T ? r0 * c.T : 0), c.T, c.K, c.logp + (c.T ? r0 * c.T : 0), \
                                               c.lse ? c.lse + r0 : nullptr, c.ent ? c.ent + r0 : nullptr, c.top_idx + (c.K ? r0 * c.K : 0), c.top_logp + (c.K ? r0 * c.K : 0))
         if (sh.rows <= rsx_num_cus()) RSX_LP_FINISH(1024); else if (sh.rows <= 2 * rsx_num_cus()) RSX_LP_FINISH(512); else RSX_LP_FINISH(256);
 #undef RSX_LP_FINISH

@@ -183,3 +183,33 @@ def test_hip_a_mask_without_entries_masks_nothing(n):
     nothing = sp.csr_matrix((n, 300))
     for a, b in zip(m.predict_logprobs(np.arange(n), np.arange(n), K=5), m.predict_logprobs(np.arange(n), np.arange(n), eval_pos=nothing, K=5)):
         assert np.array_equal(a, b)
+
+
+# ---- scores closer than the fast products' rounding ---------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [3, 140, 600])
+@pytest.mark.parametrize("I", [700, 1900, 9000])
+def test_hip_top_items_among_items_that_are_nearly_equal(I, n):
+    """item rows that differ in their last bits: the order of the scores is that of their products in 64 bits all the same"""
+    import torch
+    rng = np.random.default_rng(I + n)
+    P = torch.from_numpy(rng.standard_normal((n, 64)).astype(np.float32)).cuda()
+    base = rng.standard_normal(64)
+    Q = torch.from_numpy((base + 3e-7 * rng.standard_normal((I, 64))).astype(np.float32)).cuda()
+    check(P, Q, np.arange(n), rng.integers(0, I, (n, 2)), 20, None, rows=np.r_[0:3, n - 3:n])
+    Q[::5] += 0.5                                             # ... and half a unit above the others a fifth of them
+    check(P, Q, np.arange(n), rng.integers(0, I, (n, 2)), 20, _mask_all(n, [5, 10, 200]), rows=np.r_[0:3, n - 3:n])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [3, 140])
+@pytest.mark.parametrize("size", [1e-4, 1.0, 100.0])
+def test_hip_top_items_of_scores_whose_terms_cancel(size, n):
+    """products of size^2 whose sums are thousands of times smaller, and tables whose scores differ by 10^-8 of one"""
+    import torch
+    rng = np.random.default_rng(n)
+    half = rng.standard_normal((n, 32))
+    P = torch.from_numpy((np.concatenate([half, -half], 1) * size).astype(np.float32)).cuda()
+    twin = rng.standard_normal((3000, 32))
+    Q = torch.from_numpy((np.concatenate([twin, twin + 1e-4 * rng.standard_normal(twin.shape)], 1) * size).astype(np.float32)).cuda()
+    check(P, Q, np.arange(n), rng.integers(0, 3000, (n, 2)), 20, None, rows=np.r_[0:3, n - 3:n])
