@@ -88,11 +88,11 @@ def test_hip_gradient_of_probabilities_far_below_one(d, entropy):
 @pytest.mark.gpu
 @pytest.mark.parametrize("entropy", [False, True])
 @pytest.mark.parametrize("bf16", [False, True])
-@pytest.mark.parametrize("size", [1e4, 1e6, 1e9, 1e25])
-def test_hip_gradient_beside_masked_rows_of_large_values(size, bf16, entropy):
+@pytest.mark.parametrize("size,d", [(1e4, 64), (1e6, 64), (1e9, 64), (1e25, 64), (1e9, 32), (1e9, 128), (1e9, 256)])
+def test_hip_gradient_beside_masked_rows_of_large_values(size, d, bf16, entropy):
     rng = np.random.default_rng(7)
     n, I = 150, 700
-    P, Q = tables(rng, n, I, 64, bf16)
+    P, Q = tables(rng, n, I, d, bf16)
     bad = [0, 3, 350, 699]
     Q[bad] *= size
     mask = (np.arange(n + 1, dtype=np.int64) * len(bad), np.tile(np.asarray(bad, np.int32), n))
@@ -121,12 +121,13 @@ def test_hip_gradient_beside_an_item_of_probability_zero(bf16, entropy):
 @pytest.mark.gpu
 @pytest.mark.parametrize("entropy", [False, True])
 @pytest.mark.parametrize("bf16", [False, True])
-def test_hip_gradient_of_weights_and_rows_of_many_sizes(bf16, entropy):
+@pytest.mark.parametrize("d", [32, 64, 128, 256])
+def test_hip_gradient_of_weights_and_rows_of_many_sizes(d, bf16, entropy):
     """weights from 10^-12 to 1 and user rows from 10^-3 to 1 in one batch, item rows from 10^-6 to 1 side by side"""
     import torch
     rng = np.random.default_rng(5)
     n, I = 130, 600
-    P, Q = tables(rng, n, I, 64, bf16)
+    P, Q = tables(rng, n, I, d, bf16)
     f = lambda a: torch.from_numpy(a.astype(np.float32)).cuda()
     P = (P.float() * f(np.logspace(-3, 0.3, n))[:, None]).to(P.dtype)
     Q = (Q.float() * f(10.0 ** rng.uniform(-6, 0, (I, 1)))).to(Q.dtype)
