@@ -168,3 +168,18 @@ def test_hip_gradient_of_one_probability(weight):
     # 1 - p of two numbers near 1: their own roundings (2^-24 each) and the result's beside p's
     want, tol = weight * scale * (1 - p), abs(weight) * scale * (1.1e-6 + 2.0 ** -23)
     assert (np.abs(GP[:, 1].double().cpu().numpy() - want) <= tol).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("entropy", [False, True])
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("d", [32, 256])
+def test_hip_gradient_of_many_named_items(d, bf16, entropy):
+    """70 names a position, one item up to all 70 times: their sum in one cell stays within a half"""
+    rng = np.random.default_rng(d)
+    n, I, T = 45, 140, 70
+    P, Q = tables(rng, n, I, d, bf16)
+    items = rng.integers(0, I, (n, T))
+    items[:5] = 33
+    items[5:9, ::2] = rng.integers(0, 3, (4, 35))
+    within(P, Q, rng.permutation(n), items, rng.standard_normal((n, T)) + 0.7, rng.standard_normal(n) if entropy else None, seen_csr(rng, n, I, 6))
